@@ -312,21 +312,18 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
         return t;
     };
 
-    // ---- CHAIN mode: tickets, table entries, completion counters.  Wave 0 does all of it with SCALAR instructions; the other waves learn the
-    // outcome from LDS behind a barrier.  Nothing here may touch the vector-memory queue: vmcnt retires in order, so a value loaded there is
-    // only readable once every row piece and weight fragment requested before it has returned -- the first version (vector atomic for the
-    // ticket, nine flag loads) stalled wave 0 for 2.9 k cycles per tile at its two consumption points.  s_atomic_add ... glc returns to an
-    // SGPR and is counted by lgkmcnt (tools/ubench_chain.hip: one counter for all 8 XCDs, coherent read-back by adding 0).  Issue and use
-    // are a chunk apart, so the result lands in a MAILBOX register the compiler never allocates: s100 / s101 (hipcc's allocatable range on
-    // gfx950 ends at s99; tests/test_isa_hygiene.py holds it to that -- a compiler-visible destination could be copied or spilled before the
-    // value has arrived).
+    // ---- CHAIN mode: tickets, table entries, completion counters.  Wave 0 does all of it; the other waves learn the outcome from LDS behind
+    // a barrier.  vmcnt retires in order, so a value requested from memory inside a tile is only readable once every row piece and weight
+    // fragment requested before it has returned: a first version (ticket and nine flag loads consumed under the chunk bodies) stalled wave 0
+    // for 2.9 k cycles per tile.  The next ticket (a returning vector atomic) and the pending tile's row word (a device-coherent load) are
+    // therefore requested where a tile ends, in front of the s_waitcnt vmcnt(0) that the tile's stores need before it is published: both
+    // have arrived behind that wait and are kept as plain scalars, ticket_v and rows_v, until they are used a chunk or a tile later.
     // Completion is counted per (layer, image, tile row) in ONE word per row that also carries its two neighbours: a finished tile of row y
     // adds 1 << 10 to word y, 1 to word y-1 and 1 << 20 to word y+1, so tile (l, n, y, x) may start when word y of (l-1, n) reads
     // tiles_x in every field whose row exists -- one scalar read per poll.
     int* chs = (int*)((float*)lds_raw + 32);             // spare words of wave 0's bias area: [0] pending ticket, [1] its state (0 none left, 1 ready, 2 not ready yet, 3 aborted)
     u32x4* ltab = ttab + TT * 4;                         // [L][4]: the layers resolved (see chain_entry)
     const int chain_total = CHAIN ? ch.L * ntiles : 0;   // < 2^24 (host)
-    const unsigned long long ws64 = (unsigned long long)ch.ws;
     // The lane index, recomputed where it is used (two v_mbcnt): OPAQUE, so a lane test is never merged with another test of the lane index
     // across a barrier (tools/ubench_chain.hip: hipcc threaded two `tid == 0` blocks round a loop and split wave 0 at the barriers), and
     // never a long-lived register -- a copy kept for the whole kernel was spilled, and its reload is a scratch load + s_waitcnt vmcnt(0):
@@ -336,11 +333,18 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
         asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
         return l;
     };
-#define CHAIN_SADD(REG, BYTEOFF, VAL) asm volatile("s_mov_b32 " REG ", %2\n\ts_atomic_add " REG ", %0, %1 glc" :: "s"(ws64), "s"(BYTEOFF), "s"(VAL) : "memory", REG)
-#define CHAIN_STAKE(REG, OUT) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 %0, " REG : "=s"(OUT) :: "memory")
-#define CHAIN_SSET(REG, VAL) asm volatile("s_mov_b32 " REG ", %0" :: "s"(VAL) : REG)
-    auto chain_ticket_issue = [&]() __attribute__((always_inline)) { CHAIN_SADD("s100", 0, 1); };
-    auto chain_ticket_take = [&]() __attribute__((always_inline)) { int tk; CHAIN_STAKE("s100", tk); return tk; };
+    int ticket_v = 0, rows_v = 0;                        // the last ticket drawn, the row word last read (wave 0; uniform)
+    // (inc32, not a fetch-add: hipcc's atomic optimiser turns a uniform add into one lane's add and a broadcast, with s_waitcnt vmcnt(0) right
+    // behind the request; a wrapping increment by one is the same counter and is left alone)
+    auto chain_ticket_request = [&]() __attribute__((always_inline)) {        // lane 0 of the result
+        int v = 0;
+        if (lane_now() == 0) v = (int)__builtin_amdgcn_atomic_inc32(ch.ws, 0xffffffffu, __ATOMIC_RELAXED, "agent");
+        return v;
+    };
+    auto chain_word = [&](int word) __attribute__((always_inline)) {
+        return (int)__hip_atomic_load(ch.ws + word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    auto uni = [](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(v); };
     int pr_row = -1, pr_ty = 0;                          // of the tile last decoded: its own row word in the layer before (-1: layer 0), its tile row
     int e_row = 0;                                       // ... its own row word (what it adds to when it is finished)
     int dec_tk = -1, dec_l = 0, dec_r = 0;               // the last ticket decoded: tickets only grow, so (layer, tile) advance by the difference -- no division
@@ -374,18 +378,12 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
         if (jl < 5 || jl == 6) *(unsigned long long*)(ent + wr) = v64;
         if (jl == 5) ((u32x4*)ent)[3] = u32x4{(unsigned)ty | ((unsigned)tx << 16), q[3], (unsigned)a.Cout_g, (unsigned)e_row};      // [3]: the tile's own completion word
     };
-    // the pending tile's row word of the layer before -> mailbox s101 (layer 0: the expected value at once)
+    // the pending tile's row word of the layer before (layer 0: the expected value at once)
     auto chain_rows_want = [&]() __attribute__((always_inline)) {
         return (pr_ty + 1 < tiles_y ? a.tiles_x : 0) | (a.tiles_x << 10) | (pr_ty > 0 ? a.tiles_x << 20 : 0);
     };
-    auto chain_rows_issue = [&]() __attribute__((always_inline)) {
-        if (pr_row >= 0) CHAIN_SADD("s101", (64 + pr_row) * 4, 0); else CHAIN_SSET("s101", chain_rows_want());
-    };
-    auto chain_rows_take = [&]() __attribute__((always_inline)) {
-        int c1;
-        CHAIN_STAKE("s101", c1);
-        return c1 == chain_rows_want();
-    };
+    auto chain_rows_request = [&]() __attribute__((always_inline)) { return pr_row >= 0 ? chain_word(64 + pr_row) : chain_rows_want(); };
+    auto chain_rows_ready = [&]() __attribute__((always_inline)) { return rows_v == chain_rows_want(); };
     // between tiles only (nothing of this workgroup in flight, so waiting here can block nobody this workgroup could unblock); bounded: a chain
     // in which NO tile of ANY workgroup has been published for a second (word 2 of the workspace counts published tiles: the clock restarts
     // whenever it has moved, so a workgroup that merely waits long for its turn -- pre-emption, a debugger, another stream's kernels on the
@@ -402,14 +400,10 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
         };
         if (a.dbg & 128) { give_up(); return false; }    // option conv_dbg bit 7: every workgroup gives up at its first tile -- the test of this path
         for (;;) {
-            chain_rows_issue();
-            if (chain_rows_take()) return true;
-            int ab, pg;
-            CHAIN_SADD("s101", 4, 0);                    // (s100 may hold a ticket in flight)
-            CHAIN_STAKE("s101", ab);
-            if (ab) return false;
-            CHAIN_SADD("s101", 8, 0);
-            CHAIN_STAKE("s101", pg);
+            rows_v = uni(chain_rows_request());
+            if (chain_rows_ready()) return true;
+            if (uni(chain_word(1))) return false;
+            const int pg = uni(chain_word(2));
             const unsigned now = (unsigned)__builtin_amdgcn_s_memrealtime();
             if (pg != prog) { prog = pg; t0 = now; }
             if (now - t0 > 100000000u) { give_up(); return false; }
@@ -981,18 +975,16 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
 
     // ---- prologue: step 0 staged in full, the row pieces of step 1 requested (nothing to hide them under) --------------------
     int t = bq;
-    // CHAIN: the scalar atomics are ISSUED only where a tile ends (behind init_acc, in front of the store wait and the barrier): an
-    // outstanding scalar request holds every `s_waitcnt lgkmcnt` of the LDS traffic -- the B fragments of a chunk body -- until it has
-    // returned (~700 cycles; issued inside a chunk they cost wave 0, and through the barrier the workgroup, 0.8 + 2.4 k cycles per tile).
-    // At the end of tile i: the ticket requested one tile earlier is taken (tile i + 2), its table entry written, its row word requested,
-    // the next ticket requested; under chunk 1 of tile i + 1 the row word is taken: the state of tile i + 2, used from chunk nch - 2 on.
+    // CHAIN, at the end of tile i: the ticket drawn one tile earlier becomes tile i + 2, its table entry is written, its row word and the next
+    // ticket are requested and have landed behind the wait for the tile's stores; under chunk 1 of tile i + 1 the row word decides the state
+    // of tile i + 2, used from chunk nch - 2 on.
     // A finished tile is published at its own end, once every wave has waited for its stores (s_waitcnt vmcnt(0): the acknowledgements take
     // 2-3 k cycles from the last store, partly under init_acc and the bookkeeping above).  CHAIN_DEFER = 1 is the alternative that was built and
     // measured: publish under chunk 1 of the NEXT tile without any explicit wait -- vmcnt retires loads and stores in one order on gfx950
     // (tools/ubench_chain.hip: [store sc1; load; s_waitcnt vmcnt(1)] takes the store's latency), and every wave parks, in chunk 1, row pieces
     // it requested in chunk 0, i.e. behind the last store of the tile before.  Exact too, and slower: the acknowledgements then hold up the
     // in-order queue of the next tile's first chunk.
-    bool tick_inflight = false, rows_inflight = false, pub_pending = false;
+    bool tick_drawn = false, rows_read = false, pub_pending = false;
     int pub_row = 0, pub_ty = 0;
     bool first_run = true;
     if constexpr (CHAIN) {
@@ -1033,9 +1025,8 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
         if (wave == 0) {                                 // a safe point: nothing of this workgroup in flight, blocking is allowed
             int st_cur = 1;
             if (first_run) {
-                chain_ticket_issue();
-                const int tk0 = chain_ticket_take();
-                if (tk0 < chain_total) { chain_entry(ti, tk0); chain_ticket_issue(); tick_inflight = true; } else st_cur = 0;
+                ticket_v = uni(chain_ticket_request());
+                if (ticket_v < chain_total) { chain_entry(ti, ticket_v); ticket_v = uni(chain_ticket_request()); tick_drawn = true; } else st_cur = 0;
             } else if (__builtin_amdgcn_readfirstlane(chs[1]) != 2) st_cur = 0;         // 2: the tile the last run polled too early (its entry is slot ti now)
             if (st_cur) {
                 const TileP tc = load_tile(ti);
@@ -1045,19 +1036,18 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
                 if (!chain_wait()) st_cur = 3;
             }
             int stp = 0;
-            if (st_cur == 1 && tick_inflight) {          // the tile after it: entry, one poll
-                const int tkp = chain_ticket_take();
-                tick_inflight = false;
-                if (tkp < chain_total) {
-                    chain_entry(ti + 1, tkp);
+            if (st_cur == 1 && tick_drawn) {             // the tile after it: entry, one poll
+                tick_drawn = false;
+                if (ticket_v < chain_total) {
+                    chain_entry(ti + 1, ticket_v);
                     pend_row = e_row; pend_ty = pr_ty;
-                    chain_rows_issue();
-                    stp = chain_rows_take() ? 1 : 2;
-                    chain_ticket_issue();
-                    tick_inflight = true;
+                    rows_v = uni(chain_rows_request());
+                    stp = chain_rows_ready() ? 1 : 2;
+                    ticket_v = uni(chain_ticket_request());
+                    tick_drawn = true;
                 }
             }
-            rows_inflight = false;
+            rows_read = false;
             if (lane_now() == 0) { chs[0] = st_cur; chs[1] = stp; }
         }
         __syncthreads();
@@ -1114,9 +1104,9 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
         if constexpr (!CHAIN) has_next = t_next < ntiles;
         for (int c = 0; c < nch; ++c) {
             if constexpr (CHAIN) {
-                if (wave == 0 && c == 1 && rows_inflight) {         // requested at the end of the tile before: the state of the tile after this one
-                    const int st = (chain_rows_take() || (CHAIN_ABL & 4)) ? 1 : 2;
-                    rows_inflight = false;
+                if (wave == 0 && c == 1 && rows_read) {             // read at the end of the tile before: the state of the tile after this one
+                    const int st = (chain_rows_ready() || (CHAIN_ABL & 4)) ? 1 : 2;
+                    rows_read = false;
                     if (lane_now() == 0) chs[1] = st;
                 }
                 if (c == nch - 2) has_next = __builtin_amdgcn_readfirstlane(chs[1]) == 1;
@@ -1153,23 +1143,23 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
                 rpre_on = false;
                 if constexpr (TR) bias_lane = bias_scaled(bias_v); else { if (lane < 32) bias_w[lane] = bias_scaled(bias_v); }    // the next tile's bias,
                 CHSTAMP(0);
-                const f32x16 bvec = init_bias();         // into its accumulators (below: CHAIN requests its scalar atomics in between, behind the last LDS read)
+                const f32x16 bvec = init_bias();         // into its accumulators
                 CHSTAMP(1);
+                int rows_l = 0, ticket_l = 0;            // requested here, read behind the wait for the stores
                 if constexpr (CHAIN) {
-                    if (wave == 0 && has_next) {         // (a run that ends here leaves the ticket in flight: the next run takes it)
+                    if (wave == 0 && has_next) {         // (a run that ends here keeps the ticket drawn: the next run takes it)
                         bool none = true;
-                        if (tick_inflight) {
-                            const int tkn = chain_ticket_take();
+                        if (tick_drawn) {
                             CHSTAMP(2);
-                            tick_inflight = false;
-                            if (tkn < chain_total) {
-                                chain_entry(ti + 2, tkn);
+                            tick_drawn = false;
+                            if (ticket_v < chain_total) {
+                                chain_entry(ti + 2, ticket_v);
                                 fut_row = e_row; fut_ty = pr_ty;
                                 CHSTAMP(3);
-                                chain_rows_issue();
-                                rows_inflight = true;
-                                chain_ticket_issue();
-                                tick_inflight = true;
+                                rows_l = chain_rows_request();
+                                rows_read = true;
+                                ticket_l = chain_ticket_request();
+                                tick_drawn = true;
                                 none = false;
                             }
                         }
@@ -1180,6 +1170,7 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
                 // CHAIN: the tile is published once every wave's stores have been acknowledged (a store is counted until it is written)
                 CHSTAMP(4);
                 if constexpr (CHAIN && !(CHAIN_ABL & 1)) { if (!has_next || !CHAIN_DEFER) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+                if constexpr (CHAIN) { if (wave == 0 && rows_read) { rows_v = uni(rows_l); ticket_v = uni(ticket_l); } }
                 CHSTAMP(5);
             }
             if (slot < 29) WNTRACE(slot + 1);
@@ -1188,7 +1179,7 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
                 if (last) CHSTAMP(6);
                 if (last) {
                     if (has_next && CHAIN_DEFER) { pub_pending = true; pub_row = cur_row; pub_ty = cur_ty; }
-                    else if (wave == 0) chain_publish(cur_row, cur_ty);   // (from scalar registers: an LDS read here would wait for the scalar atomics just requested)
+                    else if (wave == 0) chain_publish(cur_row, cur_ty);
                 }
                 if (c == 1 && pub_pending) {             // the tile before: see pub_pending
                     if (wave == 0) chain_publish(pub_row, pub_ty);
@@ -1211,9 +1202,6 @@ __device__ __forceinline__ void conv_wino_body(const ConvArgs& a, const int ntil
     }
     WNTRACE(31);
     WNTRACE_RT(29);
-#undef CHAIN_SADD
-#undef CHAIN_STAKE
-#undef CHAIN_SSET
 }
 
 template <int NP, bool MULTI, bool TR>

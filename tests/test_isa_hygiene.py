@@ -94,28 +94,19 @@ def test_wide_inline_assembly_stores_are_followed_by_two_wait_states(wino_isa):
             assert nxt.startswith("s_nop") and int(nxt.split()[1]) >= 1, "conv_wino_kernel %s: %s / %s" % (key, ins[i], nxt)
 
 
-def test_conv_wino_chain_kernel_signals_through_scalar_mailboxes_and_moves_activations_device_coherently(wino_isa):
-    """The chain kernel (motif_conv2d_chain_fwd): (i) its tickets and completion words are scalar atomics whose results land in s100 / s101
-    a chunk or a tile before they are used -- the compiler must never allocate those two registers (it stops at s99 on gfx950; were that to
-    change, a result could arrive in a register holding something else); (ii) activations, residuals and outputs move with sc1 (the XCDs' L2s
+def test_conv_wino_chain_kernel_signals_through_vector_memory_and_moves_activations_device_coherently(wino_isa):
+    """The chain kernel (motif_conv2d_chain_fwd): (i) its tickets are returning vector atomics and its completion words device-coherent vector
+    loads (scalar memory instructions only read, through the cache); the one pair inside the tile loop is requested where a tile ends, and
+    nothing waits between the ticket's request and the wait for the tile's stores; (ii) activations, residuals and outputs move with sc1 (the XCDs' L2s
     are not coherent inside a kernel), weights stay cached; (iii) the chunk body is the same single run of 72 matrix instructions."""
     kernels, _ = wino_isa
     lines = kernels["chain"]
-    in_asm, mailbox_outside, atomics = False, [], []
-    for ln in lines:
-        t = ln.strip()
-        if t.startswith(";;#ASMSTART"):
-            in_asm = True
-        elif t.startswith(";;#ASMEND"):
-            in_asm = False
-        elif re.search(r"\bs10[01]\b|s\[100:101\]|s\[9\d:10[01]\]", t) and not t.startswith(";"):
-            if not in_asm:
-                mailbox_outside.append(t)
-            if t.startswith("s_atomic_add"):
-                atomics.append(t)
-    assert not mailbox_outside, "compiler-generated code touches a mailbox register: %s" % mailbox_outside[:3]
-    assert len(atomics) >= 3 and all(t.endswith("glc") and re.match(r"s_atomic_add s10[01],", t) for t in atomics), atomics
     ins = list(_instr(lines))
+    assert not [t for t in ins if t.startswith("s_") and t.endswith("glc")]
+    tickets = [i for i, t in enumerate(ins) if t.startswith("global_atomic_inc")]
+    assert len(tickets) == 4 and all(ins[i].endswith("sc0") for i in tickets), [ins[i] for i in tickets]
+    assert len([t for t in ins if t.startswith("global_load_dword ") and t.endswith("sc1")]) == 5      # the row word x 3, the abort word, the progress count
+    assert not [t for t in ins[tickets[-1]:tickets[-1] + 12] if t.startswith("s_waitcnt")], ins[tickets[-1]:tickets[-1] + 12]
     stores = [t for t in ins if t.startswith("global_store_dwordx4")]
     assert stores and all(t.endswith("sc1") for t in stores), [t for t in stores if not t.endswith("sc1")][:3]
     loads = [t for t in ins if t.startswith("buffer_load_dwordx4")]
