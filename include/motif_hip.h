@@ -386,6 +386,26 @@ int motif_deconv4x4s2(const float* in, const float* weight /*[Cin,Cout,4,4]*/, c
 int motif_frames_u8_to_f32(const unsigned char* in, float* out, int N, int H, int W, int swap_rb, void* stream);
 int motif_frames_f32_to_u8(const float* in, unsigned char* out, int N, int H, int W, int round_mode, int swap_rb, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Sequence operators (no reference counterpart): tensors are token-major, [..., D] with the last axis dense, fp32, bf16 or fp16 by a
+ * type code; sums, statistics and states are fp32 whatever the type.  Row strides (_rs) are in elements.
+ * ---------------------------------------------------------------------------------------------- */
+#define MOTIF_F32 0
+#define MOTIF_BF16 1
+#define MOTIF_F16 2
+
+/* Layer normalisation over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias (weight / bias may be NULL: 1 / 0; of type
+ * param_dtype).  x [rows, D] with row stride x_rs, y [rows, D] dense.  stats [rows, 2] (may be NULL) receives mean and 1 / sqrt(var + eps)
+ * for the backward pass.  1 <= D <= 16384; rows = 0 is a call without work. */
+int motif_layer_norm_fwd(const void* x, long x_rs, const void* weight, const void* bias, void* y, float* stats,
+                         long rows, int D, float eps, int dtype, int param_dtype, void* stream);
+/* Its backward pass: dx [rows, D] dense (may be NULL), dweight / dbias [D] of param_dtype (either may be NULL).  workspace:
+ * motif_layer_norm_bwd_ws_floats(rows, D) floats, needed when dweight or dbias is wanted; its contents need no clearing.  Sums over rows are
+ * taken in fp32 in an order that depends on rows and D alone (no atomics). */
+long motif_layer_norm_bwd_ws_floats(long rows, int D);
+int motif_layer_norm_bwd(const void* x, long x_rs, const void* dy, long dy_rs, const void* weight, const float* stats, void* dx,
+                         void* dweight, void* dbias, float* workspace, long rows, int D, int dtype, int param_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,6 +74,9 @@ _SIGS = {
     "motif_axpby_bs": (c_int, [P, P, c_float, c_float, P, c_int, c_long, c_long, P]),
     "motif_flow_roundtrip": (c_int, [P, P, c_int, c_long, c_float, c_float, P]),
     "motif_deconv4x4s2": (c_int, [P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
+    "motif_layer_norm_fwd": (c_int, [P, c_long, P, P, P, P, c_long, c_int, c_float, c_int, c_int, P]),
+    "motif_layer_norm_bwd_ws_floats": (c_long, [c_long, c_int]),
+    "motif_layer_norm_bwd": (c_int, [P, c_long, P, c_long, P, P, P, P, P, P, c_long, c_int, c_int, c_int, P]),
 }
 ABI_VERSION = 9          # include/motif_hip.h / api.hip: motif_abi_version()
 EXPORTS = tuple(_SIGS)

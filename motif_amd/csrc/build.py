@@ -6,7 +6,11 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 OUT = os.path.join(os.path.dirname(HERE), "libmotif_hip.so")
-SOURCES = ["api.hip", "conv_igemm.hip", "conv_split.hip", "conv_split2.hip", "conv_wino.hip", "conv_pw.hip", "conv_ig16.hip", "conv_direct.hip", "siren.hip", "siren_split.hip", "splat.hip", "misc.hip", "corr.hip", "dcn.hip"]
+# The sequence operators: compiled without packed fp32 instructions (common.h: MOTIF_SCALAR_F32).  hipcc's host pass warns that it does not know
+# the feature: harmless.
+SEQ_SOURCES = ["layer_norm.hip"]
+SEQ_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SOURCES = ["api.hip", "conv_igemm.hip", "conv_split.hip", "conv_split2.hip", "conv_wino.hip", "conv_pw.hip", "conv_ig16.hip", "conv_direct.hip", "siren.hip", "siren_split.hip", "splat.hip", "misc.hip", "corr.hip", "dcn.hip"] + SEQ_SOURCES
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-value",
          "-Wno-pass-failed"]
 
@@ -34,14 +38,14 @@ def build(force=False, verbose=False):
 
 
 def _build_locked(objdir, force, verbose):
-    hdrs = [os.path.join(HERE, "common.h"), os.path.join(HERE, "conv_common.h"), os.path.join(HERE, "conv_split_common.h"), os.path.join(HERE, "conv_wave_epilogue.h"), os.path.join(HERE, "siren_common.h"), os.path.join(os.path.dirname(os.path.dirname(HERE)), "include", "motif_hip.h")]
+    hdrs = [os.path.join(HERE, "common.h"), os.path.join(HERE, "conv_common.h"), os.path.join(HERE, "conv_split_common.h"), os.path.join(HERE, "conv_wave_epilogue.h"), os.path.join(HERE, "siren_common.h"), os.path.join(HERE, "seq_common.h"), os.path.join(os.path.dirname(os.path.dirname(HERE)), "include", "motif_hip.h")]
     objs, jobs = [], []
     for s in SOURCES:
         src = os.path.join(HERE, s)
         obj = os.path.join(objdir, s.replace(".hip", ".o"))
         objs.append(obj)
         if force or _stale(obj, [src] + hdrs):
-            jobs.append((["hipcc"] + FLAGS + ["-c", src, "-o", obj + ".tmp.o"], obj + ".tmp.o", obj))
+            jobs.append((["hipcc"] + FLAGS + (SEQ_FLAGS if s in SEQ_SOURCES else []) + ["-c", src, "-o", obj + ".tmp.o"], obj + ".tmp.o", obj))
 
     def run(job):
         cmd, tmp, final = job

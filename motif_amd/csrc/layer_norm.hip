@@ -1,0 +1,289 @@
+// Layer normalisation over the last axis, forward and backward.
+//
+//   forward    m = mean(x), r = 1 / sqrt(mean((x - m)^2) + eps), y = (x - m) r w + b
+//   backward   n = (x - m) r, g = dy w:   dx = r (g - mean(g) - n mean(g n)),   dw = sum over rows of dy n,   db = sum over rows of dy
+//
+// Bound by memory: forward one read and one write of the data, backward two reads and one write.  A row therefore stays in registers
+// between its two reductions (E values in each of L lanes, the mean taken first and the squares of the differences second: no
+// cancellation), and the backward pass takes dx and the parameters' sums from the same read: a workgroup walks over rows with its lanes'
+// columns fixed, keeps the sums of its columns in registers (fp32) and writes them once; seq_colsum2 adds the workgroups' sums in a fixed
+// order.  No atomics: the same bits every time.
+#include "seq_common.h"
+
+namespace {
+
+constexpr int kMaxD = 16384;                             // 1024 lanes x 16 values
+
+// Sum over the L lanes that share a row, the same value in all of them.  L = 16, 64: lanes of one wave; else the workgroup, through LDS.
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float* sh) {
+    constexpr int W = L < 64 ? L : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    if constexpr (L > 64) {
+        __syncthreads();                                 // sh may still be read
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < L / 64; ++i) v += sh[i];
+    }
+    return v;
+}
+template <int L>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* sh) {
+    constexpr int W = L < 64 ? L : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+    if constexpr (L > 64) {
+        constexpr int N = L / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = a; sh[N + (threadIdx.x >> 6)] = b; }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) { a += sh[i]; b += sh[N + i]; }
+    }
+}
+
+// A lane's columns of a parameter; `none` where there is no parameter.  Columns behind D: 0.
+template <int L, int V, int NV>
+__device__ __forceinline__ void params(const void* p, int D, int pdt, int lane, float none, float (&out)[NV][V]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * L + lane) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[j][e] = c < D ? none : 0.f;
+        if (p && c < D) seq_param_vec<V>(p, c, pdt, out[j]);
+    }
+}
+
+template <typename T, int L, int V, int NV>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_fwd_kernel(const T* __restrict__ x, long xs, const void* __restrict__ w, const void* __restrict__ b, int pdt,
+                                                                          T* __restrict__ y, float* __restrict__ stats, long rows, int D, float eps) {
+    __shared__ float sh[32];
+    constexpr int TH = L < 256 ? 256 : L, R = TH / L;
+    const int lane = threadIdx.x % L;
+    const long row = (long)blockIdx.x * R + threadIdx.x / L;
+    const bool on = row < rows;
+    const T* xr = x + (on ? row : 0) * xs;
+    float v[NV][V], wv[NV][V], bv[NV][V];
+    params<L, V, NV>(w, D, pdt, lane, 1.f, wv);          // (requested first: on its way while the row is read and summed)
+    params<L, V, NV>(b, D, pdt, lane, 0.f, bv);
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * L + lane) * V;
+        if (on && c < D) seq_load<T, V>(xr + c, v[j]);
+        else
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[j][e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += v[j][e];
+    }
+    const float mean = row_sum<L>(s, sh) / (float)D;
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const bool in = (j * L + lane) * V < D;
+#pragma unroll
+        for (int e = 0; e < V; ++e) { v[j][e] -= mean; q += in ? v[j][e] * v[j][e] : 0.f; }
+    }
+    const float r = 1.f / sqrtf(row_sum<L>(q, sh) / (float)D + eps);
+    if (!on) return;
+    if (stats && lane == 0) { stats[2 * row] = mean; stats[2 * row + 1] = r; }
+    T* yr = y + row * (long)D;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * L + lane) * V;
+        if (c >= D) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[j][e] = v[j][e] * r * wv[j][e] + bv[j][e];
+        seq_store<T, V>(yr + c, v[j]);
+    }
+}
+
+template <typename T, int L, int V, int NV>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_bwd_kernel(const T* __restrict__ x, long xs, const T* __restrict__ dy, long dys, const void* __restrict__ w, int pdt,
+                                                                          const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, long rows, int D) {
+    constexpr int TH = L < 256 ? 256 : L, R = TH / L, E = NV * V;
+    __shared__ float sh[R > 1 ? 2 * L * E : 64];
+    const int lane = threadIdx.x % L, slot = threadIdx.x / L;
+    float wv[NV][V], aw[NV][V], ab[NV][V];
+    params<L, V, NV>(w, D, pdt, lane, 1.f, wv);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) aw[j][e] = ab[j][e] = 0.f;
+    const float inv = 1.f / (float)D;
+    for (long base = (long)blockIdx.x * R; base < rows; base += (long)gridDim.x * R) {
+        const long row = base + slot;
+        const bool on = row < rows;
+        const T* xr = x + (on ? row : 0) * xs;
+        const T* dr = dy + (on ? row : 0) * dys;
+        const float mean = on ? stats[2 * row] : 0.f, r = on ? stats[2 * row + 1] : 0.f;
+        float n[NV][V], g[NV][V];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * L + lane) * V;
+            const bool in = on && c < D;
+            if (in) { seq_load<T, V>(xr + c, n[j]); seq_load<T, V>(dr + c, g[j]); }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                n[j][e] = in ? (n[j][e] - mean) * r : 0.f;
+                g[j][e] = in ? g[j][e] : 0.f;
+                aw[j][e] += g[j][e] * n[j][e];
+                ab[j][e] += g[j][e];
+                g[j][e] *= wv[j][e];
+                s1 += g[j][e];
+                s2 += g[j][e] * n[j][e];
+            }
+        }
+        if (dx) {
+            row_sum2<L>(s1, s2, sh);
+            s1 *= inv; s2 *= inv;
+            if (on) {
+                T* xo = dx + row * (long)D;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int c = (j * L + lane) * V;
+                    if (c >= D) continue;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) g[j][e] = r * (g[j][e] - s1 - n[j][e] * s2);
+                    seq_store<T, V>(xo + c, g[j]);
+                }
+            }
+        }
+    }
+    if (!part) return;
+    float* p = part + (long)blockIdx.x * 2 * D;
+    if constexpr (R > 1) {                               // the workgroup's R row slots hold the same columns: added in order
+        for (int k = 0; k < R; ++k) {
+            __syncthreads();
+            if (slot == k) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const int at = (j * L + lane) * V + e;
+                        sh[at] = k ? sh[at] + aw[j][e] : aw[j][e];
+                        sh[L * E + at] = k ? sh[L * E + at] + ab[j][e] : ab[j][e];
+                    }
+            }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < D; c += TH) { p[c] = sh[c]; p[D + c] = sh[L * E + c]; }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const int c = (j * L + lane) * V + e;
+                if (c < D) { p[c] = aw[j][e]; p[D + c] = ab[j][e]; }
+            }
+    }
+}
+
+// 32 columns x 32 row slots per workgroup: a slot adds every 32nd row, the slots are added in order.
+__global__ __launch_bounds__(1024) void seq_colsum2_kernel(const float* __restrict__ part, int nb, long D, void* out0, void* out1, int dtype) {
+    __shared__ float sh[32][33];
+    const int cx = threadIdx.x & 31, slot = threadIdx.x >> 5;
+    const long c = (long)blockIdx.x * 32 + cx;
+    float s = 0.f;
+    if (c < 2 * D) {
+#pragma unroll 8
+        for (int i = slot; i < nb; i += 32) s += part[(long)i * 2 * D + c];
+    }
+    sh[slot][cx] = s;
+    __syncthreads();
+    if (slot == 0 && c < 2 * D) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) t += sh[i][cx];
+        void* out = c < D ? out0 : out1;
+        if (out) seq_param_store(out, c < D ? c : c - D, dtype, t);
+    }
+}
+
+// The layout of a row: the fewest lanes out of 16 (four rows to a wave), 64 (a wave), 256 and 1024 that hold it with 16 values each.
+template <typename T, int L, typename F>
+void with_values(bool vec, int D, F&& f) {
+    constexpr int V = 16 / sizeof(T);
+    if (vec) {
+        if (D <= L * V) f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::integral_constant<int, 1>());
+        else if (D <= L * V * 2 || V == 8) f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::integral_constant<int, 2>());
+        else f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::integral_constant<int, V == 8 ? 2 : 4>());
+    } else {
+        if (D <= L * 4) f(std::integral_constant<int, L>(), std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
+        else f(std::integral_constant<int, L>(), std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
+    }
+}
+template <typename T, typename F>
+void with_layout(bool vec, int D, F&& f) {
+    if (D <= 16 * 16) with_values<T, 16>(vec, D, f);
+    else if (D <= 64 * 16) with_values<T, 64>(vec, D, f);
+    else if (D <= 256 * 16) with_values<T, 256>(vec, D, f);
+    else with_values<T, 1024>(vec, D, f);
+}
+int rows_per_group(int D) { return D <= 256 ? 16 : D <= 1024 ? 4 : 1; }
+}  // namespace
+
+int seq_colsum2(const float* part, int nb, long D, void* out0, void* out1, int dtype, hipStream_t s) {
+    seq_colsum2_kernel<<<cdiv(2 * D, 32), 1024, 0, s>>>(part, nb, D, out0, out1, dtype);
+    MOTIF_LAUNCH_CHECK();
+    return MOTIF_OK;
+}
+
+extern "C" int motif_layer_norm_fwd(const void* x, long x_rs, const void* weight, const void* bias, void* y, float* stats,
+                                    long rows, int D, float eps, int dtype, int param_dtype, void* stream) {
+    if (rows < 0 || D < 1 || !seq_dtype_ok(dtype) || !seq_dtype_ok(param_dtype)) return MOTIF_EINVAL;
+    if (rows == 0) return MOTIF_OK;
+    if (!x || !y || x_rs < 0) return MOTIF_EINVAL;
+    if (D > kMaxD || rows > 0x7fffffffL) return MOTIF_ELIMIT;
+    seq_dispatch(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int V = 16 / sizeof(T);
+        const bool vec = D % V == 0 && x_rs % V == 0 && seq_aligned(x, 16) && seq_aligned(y, 16) && seq_aligned(weight, 16) && seq_aligned(bias, 16);
+        with_layout<T>(vec, D, [&](auto l, auto v, auto nv) {
+            constexpr int L = decltype(l)::value, TH = L < 256 ? 256 : L;
+            layer_norm_fwd_kernel<T, L, decltype(v)::value, decltype(nv)::value><<<cdiv(rows, TH / L), TH, 0, (hipStream_t)stream>>>(
+                (const T*)x, x_rs, weight, bias, param_dtype, (T*)y, stats, rows, D, eps);
+        });
+    });
+    MOTIF_LAUNCH_CHECK();
+    return MOTIF_OK;
+}
+
+static int bwd_groups(long rows, int D) {
+    const long want = cdiv(rows, rows_per_group(D));
+    const long most = 1024;
+    return (int)(want < most ? want : most);
+}
+
+extern "C" long motif_layer_norm_bwd_ws_floats(long rows, int D) {
+    if (rows < 0 || D < 1) return MOTIF_EINVAL;
+    if (D > kMaxD || rows > 0x7fffffffL) return MOTIF_ELIMIT;
+    return (long)bwd_groups(rows, D) * 2 * D;
+}
+
+extern "C" int motif_layer_norm_bwd(const void* x, long x_rs, const void* dy, long dy_rs, const void* weight, const float* stats, void* dx,
+                                    void* dweight, void* dbias, float* workspace, long rows, int D, int dtype, int param_dtype, void* stream) {
+    if (rows < 1 || D < 1 || !x || !dy || !stats || x_rs < 0 || dy_rs < 0 || !seq_dtype_ok(dtype) || !seq_dtype_ok(param_dtype)) return MOTIF_EINVAL;
+    const bool params = dweight || dbias;
+    if ((params && !workspace) || (!params && !dx)) return MOTIF_EINVAL;
+    if (D > kMaxD || rows > 0x7fffffffL) return MOTIF_ELIMIT;
+    const int nb = bwd_groups(rows, D);
+    seq_dispatch(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int V = 16 / sizeof(T);
+        const bool vec = D % V == 0 && x_rs % V == 0 && dy_rs % V == 0 && seq_aligned(x, 16) && seq_aligned(dy, 16) && seq_aligned(dx, 16) && seq_aligned(weight, 16);
+        with_layout<T>(vec, D, [&](auto l, auto v, auto nv) {
+            constexpr int L = decltype(l)::value, TH = L < 256 ? 256 : L;
+            layer_norm_bwd_kernel<T, L, decltype(v)::value, decltype(nv)::value><<<nb, TH, 0, (hipStream_t)stream>>>(
+                (const T*)x, x_rs, (const T*)dy, dy_rs, weight, param_dtype, stats, (T*)dx, params ? workspace : nullptr, rows, D);
+        });
+    });
+    MOTIF_LAUNCH_CHECK();
+    return params ? seq_colsum2(workspace, nb, D, dweight, dbias, param_dtype, (hipStream_t)stream) : MOTIF_OK;
+}

@@ -987,3 +987,127 @@ def frames_f32_to_u8(frames, round_half_even=True, swap_rb=True):
     out = torch.empty(n, h, w, 3, dtype=torch.uint8, device=x.device)
     check(lib.motif_frames_f32_to_u8(_p(x), _p8(out), n, h, w, int(round_half_even), int(swap_rb), _stream()), "motif_frames_f32_to_u8")
     return out
+
+
+# ----------------------------------------------------------------------------------------- sequence operators
+# Token-major tensors [..., D], the last axis dense, fp32, bf16 or fp16; statistics, sums and states fp32.  They work on the device and the
+# current stream of their tensors, allocate what they need per call (nothing is shared between calls, streams or captured graphs) and are
+# differentiable once.
+_SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _seq_type(t, what, name):
+    if t.dtype not in _SEQ_DTYPES:
+        raise RuntimeError("%s: %s must be fp32, bf16 or fp16, got %s" % (what, name, t.dtype))
+
+
+def _seq_same(t, like, shape, what, name, dtypes):
+    """Checks a further tensor of a call: shape, type and device."""
+    if t is None:
+        return
+    if tuple(t.shape) != tuple(shape):
+        raise RuntimeError("%s: %s must be %s, got %s" % (what, name, list(shape), list(t.shape)))
+    if t.dtype not in dtypes:
+        raise RuntimeError("%s: %s must be %s, got %s" % (what, name, " or ".join(str(d) for d in dtypes), t.dtype))
+    if t.device != like.device:
+        raise RuntimeError("%s: %s is on %s, the input on %s" % (what, name, t.device, like.device))
+
+
+def _seq_ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _seq_call(name, device, *args):
+    """One entry of the library on `device` and its current stream."""
+    fn = getattr(_lib.load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)          # torch.cuda.current_stream(device).cuda_stream, without 2 us of Python
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    check(rc, name)
+
+
+def _seq_rows(x):
+    """(tensor, row stride) of x as rows of its last axis; copied only where no single row stride describes it."""
+    d = x.shape[-1]
+    if x.is_contiguous():
+        return x, d
+    if x.stride(-1) == 1 or d == 1:
+        if x.dim() == 2:
+            return x, x.stride(0)
+        try:
+            return x, x.view(-1, d).stride(0)
+        except RuntimeError:
+            pass
+    return x.contiguous(), d
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _layer_norm_fwd(x, weight, bias, eps, want_stats):
+    d = x.shape[-1]
+    rows = x.numel() // d
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if want_stats else None
+    if rows:
+        xr, rs = _seq_rows(x)
+        p = weight if weight is not None else bias
+        _seq_call("motif_layer_norm_fwd", x.device, xr.data_ptr(), rs, _seq_ptr(weight), _seq_ptr(bias), y.data_ptr(), _seq_ptr(stats),
+                  rows, d, eps, _SEQ_DTYPES[x.dtype], _SEQ_DTYPES[p.dtype] if p is not None else 0)
+    return y, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = _layer_norm_fwd(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.param_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        d = x.shape[-1]
+        rows = x.numel() // d
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw, db = (torch.empty(d, dtype=ctx.param_dtype, device=x.device) if need else None for need in (need_w, need_b))
+        if rows:
+            xr, xs = _seq_rows(x)
+            dyr, ds = _seq_rows(dy)
+            ws = None
+            if need_w or need_b:
+                ws = torch.empty(_lib.load().motif_layer_norm_bwd_ws_floats(rows, d), dtype=torch.float32, device=x.device)
+            _seq_call("motif_layer_norm_bwd", x.device, xr.data_ptr(), xs, dyr.data_ptr(), ds, _seq_ptr(weight), stats.data_ptr(), _seq_ptr(dx),
+                      _seq_ptr(dw), _seq_ptr(db), _seq_ptr(ws), rows, d, _SEQ_DTYPES[x.dtype], _SEQ_DTYPES[ctx.param_dtype])
+        else:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        return dx, dw, db, None
+
+
+LAYER_NORM_MAX = 16384
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer normalisation over the last axis: (x - mean) / sqrt(var + eps) * weight + bias.  x [..., D] fp32 / bf16 / fp16 with D <= 16384, any
+    strides (a copy is made only where the rows have no common stride or the last axis is not dense); weight / bias [D] of x's type or fp32.
+    Differentiable in x, weight and bias.  (instance_norm is the planar counterpart: statistics over a channel's plane.)"""
+    what = "layer_norm"
+    _seq_type(x, what, "x")
+    d = x.shape[-1] if x.dim() else 0
+    if not 1 <= d <= LAYER_NORM_MAX:
+        raise RuntimeError("%s: the last axis must hold 1 to %d values, got shape %s" % (what, LAYER_NORM_MAX, list(x.shape)))
+    _seq_same(weight, x, (d,), what, "weight", (x.dtype, torch.float32))
+    _seq_same(bias, x, (d,), what, "bias", (x.dtype, torch.float32) if weight is None else (weight.dtype,))
+    require_device(x, "layer_norm needs CUDA(ROCm) tensors")
+    if _wants_grad(x, weight, bias):
+        return _LayerNorm.apply(x, weight if weight is None else _c(weight), bias if bias is None else _c(bias), float(eps))
+    return _layer_norm_fwd(x, None if weight is None else _c(weight), None if bias is None else _c(bias), float(eps), False)[0]
