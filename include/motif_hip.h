@@ -406,6 +406,21 @@ long motif_layer_norm_bwd_ws_floats(long rows, int D);
 int motif_layer_norm_bwd(const void* x, long x_rs, const void* dy, long dy_rs, const void* weight, const float* stats, void* dx,
                          void* dweight, void* dbias, float* workspace, long rows, int D, int dtype, int param_dtype, void* stream);
 
+/* The recurrence of motif_gru_update along sequences, for gates that do not read the state: h_t = (1 - z_t) h_{t-1} + z_t q_t, channel by
+ * channel.  Either B sequences of T rows -- z, q [B, T, D] with batch and row strides (_bs, _rs; the last axis dense), cu_seqlens NULL, h0 /
+ * h_last [B, D] --, or S sequences packed one behind the other -- z, q [T, D], B = 1, cu_seqlens [S + 1] on the device, sequence s = rows
+ * cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (empty ones keep their state), h0 / h_last [S, D]; rows that no sequence covers come out as zeros,
+ * whatever they hold.  h0 NULL: zeros.  h dense; h_last may be NULL.  States are fp32.  workspace: motif_gru_scan_ws_floats floats (of type
+ * dtype's call; NULL where that is 0), no clearing needed.  The result does not depend on timing: no atomics. */
+long motif_gru_scan_ws_floats(long B, long T, long D, int packed, int dtype);
+int motif_gru_scan_fwd(const void* z, long z_bs, long z_rs, const void* q, long q_bs, long q_rs, const float* h0, const int32_t* cu_seqlens, int S,
+                       void* h, float* h_last, float* workspace, long B, long T, long D, int dtype, void* stream);
+/* Its backward pass from the forward's h: dh like h with strides, dh_last [B or S, D] fp32 (NULL: zeros); dz, dq dense, dh0 fp32 (each may be
+ * NULL).  Rows that no sequence covers get zeros. */
+int motif_gru_scan_bwd(const void* z, long z_bs, long z_rs, const void* q, long q_bs, long q_rs, const float* h0, const int32_t* cu_seqlens, int S,
+                       const void* h, const void* dh, long dh_bs, long dh_rs, const float* dh_last, void* dz, void* dq, float* dh0, float* workspace,
+                       long B, long T, long D, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,410 @@
+// The recurrence of motif_gru_update over whole sequences, for gates that do not read the state:
+//
+//   forward    h_t = a_t h_{t-1} + z_t q_t,   a_t = 1 - z_t                         channel by channel
+//   backward   g_t = dh_t + c_t,  c_{t-1} = a_t g_t  (c of the last row: the gradient of the last state)
+//              dq_t = g_t z_t,    dz_t = g_t (q_t - h_{t-1}),    dh0 = a_0 g_0
+//
+// Both are first-order linear recurrences; the backward one runs from the end.  A run of rows acts on the state that enters it as
+// x -> A x + H, and two runs compose as (A2 A1, A2 H1 + H2): that is what lets time be split.  A packed sequence's first row has A = 0 and its
+// initial state inside H, so sequences packed one behind the other are one recurrence over all rows.
+//
+// Bound by memory (forward 2 reads and 1 write, backward 4 reads and 2 writes of the data).  A workgroup owns TX lanes x V channels and TY time
+// slots of R rows each: a tile of TY R rows lies in registers between the composition of its slots (lanes of a wave by shuffles, the waves
+// through LDS) and the second walk over its rows that writes them.  TY = 1 where channels alone fill the chip or the sequence is short.  Where
+// channels are few, a sequence is cut into segments: a first kernel reads what the composition needs and writes every segment's (A, H), and each
+// segment's workgroup then composes those before it, in a fixed order -- the cost is a second read of half the inputs.  The states, A and H are
+// fp32.  No atomics: the same bits every time.
+#include "seq_common.h"
+
+namespace {
+
+struct ScanArgs {
+    const void *z, *q, *h, *dh;                          // q, h: backward's second kernel and forward; dh: backward
+    const float *h0, *dlast;
+    void *out0, *out1;                                   // forward: h, -; backward: dz, dq (either may be null)
+    float* state;                                        // forward: the last states, backward: dh0 (may be null)
+    float* agg;                                          // [B][segs][2][D], null with one segment
+    const int* info;                                     // packed rows: owner << 2 | last << 1 | first, -1: no sequence's row.  null: B sequences of T rows
+    long zb, zr, qb, qr, db, dr;                         // batch and row strides of z, q, dh; h, out0 and out1 are dense
+    long T, seg_rows;
+    int B, D, groups, segs;
+};
+
+constexpr int kFirst = 1, kLast = 2;
+
+template <int V, int TX, int TY>
+struct Slots {                                           // 256 threads: TX lanes across channels, TY time slots
+    static constexpr int WX = TX < 64 ? TX : 64, WY = 64 / WX, WAVES = TY > 1 ? 4 : 1;
+    static_assert(TX * TY == 256 && (TY == 1 || TX <= 64), "");
+
+    // A, H of this slot -> of the slots in front of it in its wave (exclusive); the wave's own to tot[wave]
+    static __device__ __forceinline__ void wave_scan(float (&A)[V], float (&H)[V], float (*tot)[2][TX * V]) {
+        const int lane = threadIdx.x & 63, sy = lane / WX, tx = lane % WX, wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int d = 1; d < WY; d <<= 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float oa = __shfl_up(A[v], d * WX), oh = __shfl_up(H[v], d * WX);
+                if (sy >= d) { H[v] = fmaf(A[v], oh, H[v]); A[v] *= oa; }
+            }
+        }
+        if (sy == WY - 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) { tot[wave][0][tx * V + v] = A[v]; tot[wave][1][tx * V + v] = H[v]; }
+        }
+        if constexpr (WY > 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float oa = __shfl_up(A[v], WX), oh = __shfl_up(H[v], WX);
+                A[v] = sy ? oa : 1.f;
+                H[v] = sy ? oh : 0.f;
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) { A[v] = 1.f; H[v] = 0.f; }
+        }
+    }
+    // behind a barrier: the state that enters this wave's slots, and `carry` moved past all waves
+    static __device__ __forceinline__ void waves_apply(float (&carry)[V], float (&in)[V], const float (*tot)[2][TX * V], int tx) {
+        const int wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (w == wave) in[v] = carry[v];
+                carry[v] = fmaf(tot[w][0][tx * V + v], carry[v], tot[w][1][tx * V + v]);
+            }
+        }
+    }
+};
+
+template <int V>
+__device__ __forceinline__ void zero(float (&x)[V], float c = 0.f) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = c;
+}
+
+// The composition of one row: forward  x -> a x + z q (first: a h0 + z q),   backward  c -> a (c + dh) (last: a (dlast + dh)).
+template <bool BWD, int V>
+__device__ __forceinline__ void compose(float (&A)[V], float (&H)[V], const float (&z)[V], const float (&x)[V], int flag, const float* init, int c0, int D) {
+    float s[V];
+    zero(s);
+    const bool cut = flag >= 0 && (flag & (BWD ? kLast : kFirst));
+    if (cut && init) seq_load16<float, V>(init + (long)(flag >> 2) * D + c0, s);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const float a = 1.f - z[v];
+        if (cut) { A[v] = 0.f; H[v] = s[v]; }
+        if (flag < 0) { A[v] = 0.f; H[v] = 0.f; continue; }
+        H[v] = BWD ? a * (H[v] + x[v]) : fmaf(a, H[v], z[v] * x[v]);
+        A[v] *= a;
+    }
+}
+
+// What row t of sequence b is.
+__device__ __forceinline__ int row_flag(const ScanArgs& p, long b, long t) {
+    if (p.info) return p.info[t];
+    return (int)(b << 2) | (t == 0 ? kFirst : 0) | (t == p.T - 1 ? kLast : 0);
+}
+
+struct Where { int group, seg; long b; };
+__device__ __forceinline__ Where where(const ScanArgs& p) {
+    const long bs = blockIdx.x / p.groups;
+    return {(int)(blockIdx.x % p.groups), (int)(bs % p.segs), bs / p.segs};
+}
+
+// (A, H) of every segment but the last: each slot walks its own run of the segment's rows, four rows requested at a time.
+template <typename T, int V, int TX, int TY, bool BWD>
+__global__ __launch_bounds__(256) void gru_scan_segments_kernel(ScanArgs p) {
+    using S = Slots<V, TX, TY>;
+    __shared__ float tot[4][2][TX * V];
+    const Where at = where(p);
+    if (at.seg == p.segs - 1) return;
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, c0 = (at.group * TX + tx) * V;
+    const bool on = c0 < p.D;
+    const T* z = (const T*)p.z + at.b * p.zb + c0;
+    const T* x = BWD ? (const T*)p.dh + at.b * p.db + c0 : (const T*)p.q + at.b * p.qb + c0;
+    const long xr = BWD ? p.dr : p.qr;
+    const long run = p.seg_rows / TY, k0 = at.seg * p.seg_rows + ty * run;     // rows in the order of the recurrence; a segment that is not the last is full
+    float A[V], H[V];
+    zero(A, 1.f);
+    zero(H);
+    if (on) {
+        for (long k = k0; k < k0 + run; k += 4) {
+            float zv[4][V], xv[4][V];
+            int f[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const long t = BWD ? p.T - 1 - (k + r) : k + r;
+                seq_load<T, V>(z + t * p.zr, zv[r]);
+                seq_load<T, V>(x + t * xr, xv[r]);
+                f[r] = row_flag(p, at.b, t);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) compose<BWD, V>(A, H, zv[r], xv[r], f[r], BWD ? p.dlast : p.h0, c0, p.D);
+        }
+    }
+    S::wave_scan(A, H, tot);
+    __syncthreads();
+    if (ty == 0 && on) {
+        float* o = p.agg + ((at.b * p.segs + at.seg) * 2) * p.D + c0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            A[v] = 1.f;
+            H[v] = 0.f;
+#pragma unroll
+            for (int w = 0; w < S::WAVES; ++w) { H[v] = fmaf(tot[w][0][tx * V + v], H[v], tot[w][1][tx * V + v]); A[v] *= tot[w][0][tx * V + v]; }
+        }
+        seq_store16<float, V>(o, A);
+        seq_store16<float, V>(o + p.D, H);
+    }
+}
+
+template <typename T, int V, int TX, int TY, int R, bool BWD>
+__global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
+    using S = Slots<V, TX, TY>;
+    __shared__ float tot[2][4][2][TX * V];
+    const Where at = where(p);
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, c0 = (at.group * TX + tx) * V;
+    const bool on = c0 < p.D;
+    const T* z = (const T*)p.z + at.b * p.zb + c0;
+    const T* q = (const T*)p.q + at.b * p.qb + c0;
+    const T* dh = BWD ? (const T*)p.dh + at.b * p.db + c0 : nullptr;
+    const T* hs = BWD ? (const T*)p.h + at.b * p.T * p.D + c0 : nullptr;
+    T* out0 = p.out0 ? (T*)p.out0 + at.b * p.T * p.D + c0 : nullptr;
+    T* out1 = p.out1 ? (T*)p.out1 + at.b * p.T * p.D + c0 : nullptr;
+    const long k_end = min(p.T, (at.seg + 1) * p.seg_rows);
+    float carry[V];
+    zero(carry);                                         // (a sequence's own initial value enters at its first row)
+    int buf = 0;
+    if (TY > 1 && at.seg > 0) {                          // the segments in front: slot ty composes a run of them, then the slots compose
+        float A[V], H[V], in[V];
+        zero(A, 1.f);
+        zero(H);
+        const int per = (at.seg + TY - 1) / TY;
+        if (on) {
+            for (int s = ty * per; s < min(at.seg, (ty + 1) * per); ++s) {
+                float a[V], h[V];
+                const float* g = p.agg + ((at.b * p.segs + s) * 2) * p.D + c0;
+                seq_load16<float, V>(g, a);
+                seq_load16<float, V>(g + p.D, h);
+#pragma unroll
+                for (int v = 0; v < V; ++v) { H[v] = fmaf(a[v], H[v], h[v]); A[v] *= a[v]; }
+            }
+        }
+        S::wave_scan(A, H, tot[0]);
+        __syncthreads();
+        S::waves_apply(carry, in, tot[0], tx);
+        buf = 1;
+    }
+    for (long k0 = at.seg * p.seg_rows; k0 < k_end; k0 += TY * R) {
+        float zv[R][V], qv[R][V], dv[BWD ? R : 1][V], hv[BWD ? R : 1][V];
+        int f[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const long k = k0 + ty * R + r, t = BWD ? p.T - 1 - k : k;
+            const bool in = on && k < k_end;
+            f[r] = in ? row_flag(p, at.b, t) : 0;
+            if (in) {
+                seq_load<T, V>(z + t * p.zr, zv[r]);
+                if (!BWD || out0) seq_load<T, V>(q + t * p.qr, qv[r]); else zero(qv[r]);
+                if constexpr (BWD) {
+                    seq_load<T, V>(dh + t * p.dr, dv[r]);
+                    if (out0 && t > 0) seq_load<T, V>(hs + (t - 1) * p.D, hv[r]); else zero(hv[r]);
+                }
+            } else {                                     // no row: x -> x
+                zero(zv[r]);
+                zero(qv[r]);
+                if constexpr (BWD) { zero(dv[r]); zero(hv[r]); }
+            }
+        }
+        float h[V];
+        if constexpr (TY > 1) {
+            float A[V], H[V], in[V];
+            zero(A, 1.f);
+            zero(H);
+#pragma unroll
+            for (int r = 0; r < R; ++r) compose<BWD, V>(A, H, zv[r], BWD ? dv[BWD ? r : 0] : qv[r], f[r], BWD ? p.dlast : p.h0, c0, p.D);
+            S::wave_scan(A, H, tot[buf]);
+            __syncthreads();                             // one barrier a tile: the next tile's sums go to the other buffer
+            S::waves_apply(carry, in, tot[buf], tx);
+            buf ^= 1;
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[v] = fmaf(A[v], in[v], H[v]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[v] = carry[v];
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const long k = k0 + ty * R + r, t = BWD ? p.T - 1 - k : k;
+            if (!on || k >= k_end) continue;
+            const long own = (long)(f[r] >> 2) * p.D + c0;
+            if constexpr (!BWD) {
+                if (f[r] >= 0 && (f[r] & kFirst)) { if (p.h0) seq_load16<float, V>(p.h0 + own, h); else zero(h); }
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[v] = f[r] < 0 ? 0.f : fmaf(1.f - zv[r][v], h[v], zv[r][v] * qv[r][v]);
+                seq_store<T, V>(out0 + t * p.D, h);
+                if (p.state && f[r] >= 0 && (f[r] & kLast)) seq_store16<float, V>(p.state + own, h);
+            } else {
+                if (f[r] >= 0 && (f[r] & kLast)) { if (p.dlast) seq_load16<float, V>(p.dlast + own, h); else zero(h); }
+                if (f[r] >= 0 && (f[r] & kFirst)) { if (p.h0) seq_load16<float, V>(p.h0 + own, hv[r]); else zero(hv[r]); }
+                float dz[V], dq[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float g = f[r] < 0 ? 0.f : dv[r][v] + h[v];
+                    dz[v] = f[r] < 0 ? 0.f : g * (qv[r][v] - hv[r][v]);
+                    dq[v] = f[r] < 0 ? 0.f : g * zv[r][v];
+                    h[v] = f[r] < 0 ? 0.f : (1.f - zv[r][v]) * g;
+                }
+                if (out0) seq_store<T, V>(out0 + t * p.D, dz);
+                if (out1) seq_store<T, V>(out1 + t * p.D, dq);
+                if (p.state && f[r] >= 0 && (f[r] & kFirst)) seq_store16<float, V>(p.state + own, h);
+            }
+        }
+        if constexpr (TY == 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) carry[v] = h[v];
+        }
+    }
+}
+
+// Packed rows: what each row is.  cu [S + 1] need not be sound for memory's sake: an owner is always one of the S sequences.
+__global__ __launch_bounds__(256) void gru_scan_rows_kernel(const int* __restrict__ cu, int S, int rows, int* __restrict__ info) {
+    const long t = (long)blockIdx.x * 256 + threadIdx.x;
+    if (t >= rows) return;
+    int lo = 0, hi = S + 1;                              // the first bound behind t
+    while (lo < hi) {
+        const int m = (lo + hi) >> 1;
+        if (cu[m] <= t) lo = m + 1; else hi = m;
+    }
+    const int s = lo - 1;
+    if (s < 0 || s >= S) { info[t] = -1; return; }
+    info[t] = (s << 2) | (cu[s] == t ? kFirst : 0) | (cu[s + 1] == t + 1 ? kLast : 0);
+}
+// ... and an empty sequence's state, which no row carries: out = in (or 0).
+__global__ __launch_bounds__(256) void gru_scan_empty_kernel(const int* __restrict__ cu, int D, const float* __restrict__ in, float* __restrict__ out) {
+    const int s = blockIdx.x;
+    if (cu[s + 1] > cu[s]) return;
+    for (long c = threadIdx.x; c < D; c += 256) out[(long)s * D + c] = in ? in[(long)s * D + c] : 0.f;
+}
+
+struct Plan { int V, TX, TY, R, groups, segs; long seg_rows; };
+
+// Vectors of 16 bytes where every row of every tensor allows them, single values else.  TY = 1 (a lane walks the whole sequence) where the
+// sequence is no longer than 16 rows or the channels alone give every CU two workgroups; else 32 time slots (8 with single values, whose
+// rows need more lanes to fill a cache line).  Segments: as many as give every CU four workgroups, none below two tiles.
+Plan plan_of(int V, long B, long T, long D) {
+    Plan p;
+    p.V = V;
+    const long lanes = (D + V - 1) / V;
+    const bool serial = T <= 16 || B * ((lanes + 255) / 256) >= 512;
+    p.TY = serial ? 1 : V > 1 ? 32 : 8;
+    p.TX = 256 / p.TY;
+    p.R = 4;
+    p.groups = (int)((lanes + p.TX - 1) / p.TX);
+    p.segs = 1;
+    p.seg_rows = T;
+    if (!serial) {
+        const long tile = (long)p.TY * p.R, tiles = (T + tile - 1) / tile;
+        long segs = 1024 / (B * p.groups);
+        segs = segs < 1 ? 1 : segs > 128 ? 128 : segs;
+        const long per = segs < 2 ? tiles : (tiles + segs - 1) / segs < 2 ? 2 : (tiles + segs - 1) / segs;
+        p.segs = (int)((tiles + per - 1) / per);
+        p.seg_rows = per * tile;
+    }
+    return p;
+}
+
+template <typename T, int V, bool BWD>
+void launch(const Plan& pl, const ScanArgs& a, hipStream_t s) {
+    const unsigned grid = (unsigned)((long)a.B * pl.segs * pl.groups);
+    constexpr int TY = V > 1 ? 32 : 8;
+    if (pl.TY == 1) { gru_scan_kernel<T, V, 256, 1, 4, BWD><<<grid, 256, 0, s>>>(a); return; }
+    if (pl.segs > 1) gru_scan_segments_kernel<T, V, 256 / TY, TY, BWD><<<grid, 256, 0, s>>>(a);
+    gru_scan_kernel<T, V, 256 / TY, TY, 4, BWD><<<grid, 256, 0, s>>>(a);
+}
+
+// Vector width of a call: every tensor's base and strides are multiples of 16 bytes (fp32 rows of states: of 16 bytes too).
+int vec_of(int dtype, long D, const long* strides, int ns, const void* const* ptrs, int np) {
+    const int V = 16 / seq_size(dtype);
+    if (D % V) return 1;
+    for (int i = 0; i < ns; ++i) if (strides[i] % V) return 1;
+    for (int i = 0; i < np; ++i) if (!seq_aligned(ptrs[i], 16)) return 1;
+    return V;
+}
+
+int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const float* empty_in, hipStream_t s) {
+    const long strides[6] = {a.zb, a.zr, a.qb, a.qr, a.db, a.dr};
+    const void* ptrs[10] = {a.z, a.q, a.h, a.dh, a.h0, a.dlast, a.out0, a.out1, a.state, ws};
+    const int V = vec_of(dtype, a.D, strides, 6, ptrs, 10);
+    const Plan pl = plan_of(V, a.B, a.T, a.D);
+    if ((long)a.B * pl.segs * pl.groups > 0x7fffffffL) return MOTIF_ELIMIT;
+    a.groups = pl.groups;
+    a.segs = pl.segs;
+    a.seg_rows = pl.seg_rows;
+    if (pl.segs > 1) a.agg = ws;
+    if (cu) {
+        int* info = (int*)(ws + (pl.segs > 1 ? (((long)pl.segs * 2 * a.D + 3) & ~3L) : 0));
+        if (a.T > 0) gru_scan_rows_kernel<<<cdiv(a.T, 256), 256, 0, s>>>(cu, S, (int)a.T, info);
+        if (a.state) gru_scan_empty_kernel<<<S, 256, 0, s>>>(cu, a.D, empty_in, a.state);
+        a.info = info;
+    }
+    if (a.T > 0)
+        seq_dispatch(dtype, [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            constexpr int W = 16 / sizeof(T);
+            if (bwd) { if (V == 1) launch<T, 1, true>(pl, a, s); else launch<T, W, true>(pl, a, s); }
+            else { if (V == 1) launch<T, 1, false>(pl, a, s); else launch<T, W, false>(pl, a, s); }
+        });
+    MOTIF_LAUNCH_CHECK();
+    return MOTIF_OK;
+}
+
+int check_sizes(long B, long T, long D, int S, const void* cu, int dtype) {
+    if (B < 1 || T < 0 || D < 1 || !seq_dtype_ok(dtype)) return MOTIF_EINVAL;
+    if (cu ? (B != 1 || S < 1) : T < 1) return MOTIF_EINVAL;
+    if (D > 0x3fffffffL || T > 0x7ffffff0L || B >= (1L << 29) || S >= (1 << 29)) return MOTIF_ELIMIT;
+    return MOTIF_OK;
+}
+}  // namespace
+
+extern "C" long motif_gru_scan_ws_floats(long B, long T, long D, int packed, int dtype) {
+    const int rc = check_sizes(B, T, D, packed ? 1 : 0, packed ? (const void*)&B : nullptr, dtype);
+    if (rc) return rc;
+    long need = 0;                                       // of either vector width: the pointers decide at the call
+    for (int V : {1, 16 / seq_size(dtype)}) {
+        const Plan p = plan_of(V, B, T, D);
+        const long n = p.segs > 1 ? ((B * p.segs * 2 * D + 3) & ~3L) : 0;
+        need = n > need ? n : need;
+    }
+    return need + (packed ? T : 0);
+}
+
+extern "C" int motif_gru_scan_fwd(const void* z, long z_bs, long z_rs, const void* q, long q_bs, long q_rs, const float* h0, const int32_t* cu_seqlens, int S,
+                                  void* h, float* h_last, float* workspace, long B, long T, long D, int dtype, void* stream) {
+    const int rc = check_sizes(B, T, D, S, cu_seqlens, dtype);
+    if (rc) return rc;
+    if ((T > 0 && (!z || !q || !h)) || z_bs < 0 || z_rs < 0 || q_bs < 0 || q_rs < 0) return MOTIF_EINVAL;
+    if (!workspace && motif_gru_scan_ws_floats(B, T, D, cu_seqlens != nullptr, dtype) > 0) return MOTIF_EINVAL;
+    ScanArgs a = {};
+    a.z = z; a.q = q; a.h0 = h0; a.out0 = h; a.state = h_last;
+    a.zb = z_bs; a.zr = z_rs; a.qb = q_bs; a.qr = q_rs;
+    a.T = T; a.B = (int)B; a.D = (int)D;
+    return run(false, dtype, a, cu_seqlens, S, workspace, h0, (hipStream_t)stream);
+}
+
+extern "C" int motif_gru_scan_bwd(const void* z, long z_bs, long z_rs, const void* q, long q_bs, long q_rs, const float* h0, const int32_t* cu_seqlens, int S,
+                                  const void* h, const void* dh, long dh_bs, long dh_rs, const float* dh_last, void* dz, void* dq, float* dh0, float* workspace,
+                                  long B, long T, long D, int dtype, void* stream) {
+    const int rc = check_sizes(B, T, D, S, cu_seqlens, dtype);
+    if (rc) return rc;
+    if ((T > 0 && (!z || !q || !h || !dh)) || z_bs < 0 || z_rs < 0 || q_bs < 0 || q_rs < 0 || dh_bs < 0 || dh_rs < 0) return MOTIF_EINVAL;
+    if (T > 0 && !dz && !dq && !dh0) return MOTIF_EINVAL;
+    if (!workspace && motif_gru_scan_ws_floats(B, T, D, cu_seqlens != nullptr, dtype) > 0) return MOTIF_EINVAL;
+    ScanArgs a = {};
+    a.z = z; a.q = q; a.h = h; a.dh = dh; a.h0 = h0; a.dlast = dh_last; a.out0 = dz; a.out1 = dq; a.state = dh0;
+    a.zb = z_bs; a.zr = z_rs; a.qb = q_bs; a.qr = q_rs; a.db = dh_bs; a.dr = dh_rs;
+    a.T = T; a.B = (int)B; a.D = (int)D;
+    return run(true, dtype, a, cu_seqlens, S, workspace, dh_last, (hipStream_t)stream);
+}

@@ -49,6 +49,17 @@ __device__ __forceinline__ void seq_load16(const T* p, float (&out)[N]) {
         for (int i = 0; i < P; ++i) out[j + i] = (float)x.v[i];
     }
 }
+template <typename T, int N>
+__device__ __forceinline__ void seq_store16(T* p, const float (&in)[N]) {
+    constexpr int P = 16 / (int)sizeof(T) < N ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+    for (int j = 0; j < N; j += P) {
+        SeqVec<T, P> x;
+#pragma unroll
+        for (int i = 0; i < P; ++i) x.v[i] = (T)in[j + i];
+        *(SeqVec<T, P>*)(p + j) = x;
+    }
+}
 template <int N>
 __device__ __forceinline__ void seq_param_vec(const void* p, long i, int dtype, float (&out)[N]) {
     if (dtype == MOTIF_F32) seq_load16<float, N>((const float*)p + i, out);

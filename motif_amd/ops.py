@@ -1111,3 +1111,85 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if _wants_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight if weight is None else _c(weight), bias if bias is None else _c(bias), float(eps))
     return _layer_norm_fwd(x, None if weight is None else _c(weight), None if bias is None else _c(bias), float(eps), False)[0]
+
+
+def _scan_strides(t):
+    """(tensor, batch stride, row stride) of [B, T, D] or [T, D]; copied only where the last axis is not dense."""
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        t = t.contiguous()
+    return (t, t.stride(0), t.stride(1)) if t.dim() == 3 else (t, 0, t.stride(0))
+
+
+def _scan_sizes(z, cu):
+    return (1, z.shape[0], z.shape[1], cu.numel() - 1) if cu is not None else tuple(z.shape) + (0,)
+
+
+def _scan_workspace(b, t, d, cu, z):
+    n = _lib.load().motif_gru_scan_ws_floats(b, t, d, int(cu is not None), _SEQ_DTYPES[z.dtype])
+    if n < 0:
+        raise RuntimeError("gru_scan: sizes %s outside what the kernels support (%d)" % (list(z.shape), n))
+    return torch.empty(n, dtype=torch.float32, device=z.device) if n else None
+
+
+def _gru_scan_fwd(z, q, h0, cu):
+    b, t, d, s = _scan_sizes(z, cu)
+    h = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    last = torch.empty(s if cu is not None else b, d, dtype=torch.float32, device=q.device)
+    if b * d == 0 or (t == 0 and cu is None):            # nothing to walk: the states stay what they were
+        return h, last.copy_(h0) if h0 is not None else last.zero_()
+    zt, zb, zr = _scan_strides(z)
+    qt, qb, qr = _scan_strides(q)
+    ws = _scan_workspace(b, t, d, cu, z)
+    _seq_call("motif_gru_scan_fwd", z.device, zt.data_ptr(), zb, zr, qt.data_ptr(), qb, qr, _seq_ptr(h0), _seq_ptr(cu), s, h.data_ptr(), last.data_ptr(),
+              _seq_ptr(ws), b, t, d, _SEQ_DTYPES[z.dtype])
+    return h, last
+
+
+class _GruScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, q, h0, cu):
+        h, last = _gru_scan_fwd(z, q, h0, cu)
+        ctx.save_for_backward(z, q, h0, cu, h)
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dlast):
+        z, q, h0, cu, h = ctx.saved_tensors
+        b, t, d, s = _scan_sizes(z, cu)
+        need_z, need_q, need_h, _ = ctx.needs_input_grad
+        dz, dq = (torch.empty(q.shape, dtype=q.dtype, device=q.device) if need else None for need in (need_z, need_q))
+        dh0 = torch.empty(dlast.shape, dtype=torch.float32, device=q.device) if need_h else None
+        if b * d == 0 or (t == 0 and cu is None):
+            return dz, dq, dlast.clone() if need_h else None, None
+        zt, zb, zr = _scan_strides(z)
+        qt, qb, qr = _scan_strides(q)
+        dt, db, dr = _scan_strides(dh)
+        dlast = _c(dlast)
+        ws = _scan_workspace(b, t, d, cu, z)
+        _seq_call("motif_gru_scan_bwd", z.device, zt.data_ptr(), zb, zr, qt.data_ptr(), qb, qr, _seq_ptr(h0), _seq_ptr(cu), s, h.data_ptr(), dt.data_ptr(),
+                  db, dr, dlast.data_ptr(), _seq_ptr(dz), _seq_ptr(dq), _seq_ptr(dh0), _seq_ptr(ws), b, t, d, _SEQ_DTYPES[z.dtype])
+        return dz, dq, dh0, None
+
+
+def gru_scan(z, q, h0=None, cu_seqlens=None):
+    """gru_update along whole sequences, for gates that do not read the state: h_t = (1 - z_t) h_{t-1} + z_t q_t, channel by channel.
+
+    z, q: [B, T, D], fp32 / bf16 / fp16, any batch and row strides; h0: fp32 [B, D] (None: zeros).  Returns (h like q, the last states fp32 [B, D]);
+    the states can be handed to the next call: a sequence may come in pieces, down to single rows.  With cu_seqlens -- int32 [S + 1] on the device,
+    not decreasing, within 0 .. T -- z and q are [T, D] with S sequences packed one behind the other, h0 and the last states [S, D]; an empty
+    sequence keeps its state, and rows that no sequence covers come out as zeros, whatever they hold.  Differentiable in z, q and h0."""
+    what = "gru_scan"
+    _seq_type(q, what, "q")
+    if q.dim() != (3 if cu_seqlens is None else 2):
+        raise RuntimeError("%s: q must be %s, got %s" % (what, "[B, T, D]" if cu_seqlens is None else "[T, D] with cu_seqlens", list(q.shape)))
+    _seq_same(z, q, q.shape, what, "z", (q.dtype,))
+    if cu_seqlens is not None and (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.device != q.device):
+        raise RuntimeError("%s: cu_seqlens must be int32 [S + 1], S >= 1, on %s, got %s %s on %s" % (what, q.device, cu_seqlens.dtype, list(cu_seqlens.shape), cu_seqlens.device))
+    _seq_same(h0, q, (q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1, q.shape[-1]), what, "h0", (torch.float32,))
+    require_device(q, "gru_scan needs CUDA(ROCm) tensors")
+    h0 = None if h0 is None else _c(h0)
+    cu = None if cu_seqlens is None else _c(cu_seqlens)
+    if _wants_grad(z, q, h0):
+        return _GruScan.apply(z, q, h0, cu)
+    return _gru_scan_fwd(z, q, h0, cu)

@@ -196,3 +196,222 @@ def test_layer_norm_gives_the_same_bits_every_time_on_any_stream_and_in_a_graph(
         x.copy_(x * 2)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(held, step()))
+
+
+# ------------------------------------------------------------------------------------------------------------------ gru_scan
+def scan_reference(z, q, h0, dh, dlast):
+    """One batch of whole sequences [B, T, D], row by row in 64 bits: h, last, dz, dq, dh0, and bounds of the errors that fp32 sums carry.
+    mh_t is the same recurrence on absolute values: every product and sum on the way is at most that."""
+    z, q, dh, dlast = z.double(), q.double(), dh.double(), dlast.double()
+    B, T, D = z.shape
+    s = torch.zeros(B, D, dtype=torch.float64, device=z.device) if h0 is None else h0.double()
+    h, mh, m, first = [], [], s.abs(), s
+    a = 1 - z
+    for t in range(T):
+        s = a[:, t] * s + z[:, t] * q[:, t]
+        m = a[:, t].abs() * m + (z[:, t] * q[:, t]).abs()
+        h.append(s)
+        mh.append(m)
+    dz, dq, c, mc = torch.zeros_like(z), torch.zeros_like(z), dlast, dlast.abs()
+    mg, mb = torch.zeros_like(z), torch.zeros_like(z)
+    for t in range(T - 1, -1, -1):
+        g, mg[:, t] = c + dh[:, t], mc + dh[:, t].abs()
+        before = h[t - 1] if t else first
+        dz[:, t], dq[:, t] = g * (q[:, t] - before), g * z[:, t]
+        mb[:, t] = mh[t - 1] if t else first.abs()
+        c, mc = a[:, t] * g, a[:, t].abs() * mg[:, t]
+    last = s
+    return (torch.stack(h, 1) if T else q.clone(), last, dz, dq, c), (torch.stack(mh, 1) if T else q.clone(), m, mg, mb, mc)
+
+
+# Roundings that one value collects relative to the magnitudes above: a row adds three (1 - z, the product, the sum), and what is older than
+# the last n rows has shrunk by prod(1 - z); in the worst case, z = 0, every row adds 3.  A composition of runs replaces additions of rows by
+# as many of runs.  chain(T) = 3 T + 64 is safe whatever z is.
+def chain(T):
+    return (3 * T + 64) * F32
+
+
+def scan_check(ops, z, q, h0, cu=None, seed=0, grads=True):
+    g = gen(seed + 7)
+    S = (cu.numel() - 1) if cu is not None else z.shape[0]
+    D = z.shape[-1]
+    dh = torch.randn(z.shape, generator=g, device="cuda").to(z.dtype)
+    dlast = torch.randn(S, D, generator=g, device="cuda")
+    leaves = [t.detach().requires_grad_() for t in (z, q, h0) if t is not None]
+    hl = leaves[2] if h0 is not None else None
+    h, last = ops.gru_scan(leaves[0], leaves[1], hl, cu_seqlens=cu)
+    assert h.dtype == q.dtype and h.shape == q.shape and last.dtype == torch.float32 and last.shape == (S, D)
+    with torch.no_grad():
+        h2, last2 = ops.gru_scan(z, q, h0, cu_seqlens=cu)
+    assert torch.equal(h, h2) and torch.equal(last, last2)
+    got = torch.autograd.grad([h, last], leaves, [dh, dlast])
+    spans = [(slice(i, i + 1), lo, hi) for i, (lo, hi) in enumerate(zip(cu.tolist(), cu.tolist()[1:]))] if cu is not None else [(slice(None), 0, z.shape[1])]
+    cut = (lambda x, lo, hi: x[lo:hi].unsqueeze(0)) if cu is not None else (lambda x, lo, hi: x)
+    for own, lo, hi in spans:
+        (h0r, lr, dzr, dqr, dh0r), (mh, ml, mg, mb, mc) = scan_reference(cut(z, lo, hi), cut(q, lo, hi), None if h0 is None else h0[own], cut(dh, lo, hi), dlast[own])
+        e = chain(hi - lo)
+        if hi > lo:
+            within(cut(h, lo, hi), h0r, half_step(q.dtype, h0r) + e * mh)
+        within(last[own], lr, e * ml)
+        if hi > lo:
+            # dz = g (q - h_{t-1}): g's error, and h_{t-1} as it was written, half a step of its type off
+            qb = cut(q, lo, hi).double().abs() + mb
+            within(cut(got[0], lo, hi), dzr, half_step(q.dtype, dzr) * (1 + 2 ** -6) + 2 * e * mg * qb + mg * half_step(q.dtype, mb) * (1 + 2 ** -6))
+            within(cut(got[1], lo, hi), dqr, half_step(q.dtype, dqr) + e * mg * cut(z, lo, hi).double().abs())
+        if h0 is not None:
+            within(got[2][own], dh0r, e * mc)
+    if cu is not None:
+        covered = torch.zeros(z.shape[0], dtype=torch.bool)
+        for _, lo, hi in spans:
+            covered[lo:hi] = True
+        behind = (~covered).cuda()
+        for t in (h, got[0], got[1]):
+            assert torch.equal(t[behind], torch.zeros_like(t[behind])), "rows that no sequence covers"
+    return h, last, got
+
+
+def scan_inputs(shape, S, dtype, seed, shift=-2.0):
+    g = gen(seed)
+    z = torch.sigmoid(torch.randn(*shape, generator=g, device="cuda") * 1.5 + shift).to(dtype)
+    q = torch.tanh(torch.randn(*shape, generator=g, device="cuda")).to(dtype)
+    return z, q, torch.randn(S, shape[-1], generator=g, device="cuda") * 0.5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B, T, D", [(1, 1, 1), (3, 1, 64), (2, 2, 7), (1, 16, 128), (1, 17, 128), (2, 127, 33), (1, 128, 64), (3, 129, 72), (1, 1000, 8), (1, 4099, 24),
+                                     (1, 3000, 5), (5, 300, 520), (1, 40, 140000), (2, 7, 4096), (600, 20, 40)])
+def test_gru_scan_and_its_gradients(ops, dtype, B, T, D):
+    z, q, h0 = scan_inputs((B, T, D), B, dtype, B * 7 + T + D)
+    scan_check(ops, z, q, h0)
+    if T <= 200:
+        scan_check(ops, z, q, None)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [1, 24, 33, 64, 136, 1100])
+@pytest.mark.parametrize("bounds, T", [([0, 5], 5), ([0, 0, 1, 1, 1, 40, 41, 300, 300], 310), ([3, 3, 10, 700], 700), ([0, 0, 0], 4), ([0, 0], 0),
+                                       ([0, 1, 2, 3, 131, 259, 388, 1500, 1501, 3999], 4001)])
+def test_gru_scan_of_packed_sequences(ops, dtype, D, bounds, T):
+    cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    z, q, h0 = scan_inputs((T, D), len(bounds) - 1, dtype, T + D)
+    covered = torch.zeros(T, dtype=torch.bool, device="cuda")
+    for lo, hi in zip(bounds, bounds[1:]):
+        covered[lo:hi] = True
+    z[~covered], q[~covered] = math.nan, math.inf
+    scan_check(ops, z, q, h0, cu)
+    if D == 24:
+        scan_check(ops, z, q, None, cu)
+
+
+def test_gru_scan_packed_equals_the_sequences_alone(ops):
+    bounds = [0, 300, 300, 301, 700, 1211]
+    cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    z, q, h0 = scan_inputs((1211, 40), 5, torch.float32, 3)
+    h, last = ops.gru_scan(z, q, h0, cu_seqlens=cu)
+    for i, (lo, hi) in enumerate(zip(bounds, bounds[1:])):
+        if hi == lo:
+            assert torch.equal(last[i], h0[i])
+            continue
+        alone, end = ops.gru_scan(z[None, lo:hi], q[None, lo:hi], h0[i:i + 1])
+        m = 2 * chain(hi - lo)                            # both are within chain() of the exact state, |h| <= 1 + |h0|
+        within(h[None, lo:hi], alone, m * (1 + h0[i].abs().double()))
+        within(last[i:i + 1], end, m * (1 + h0[i].abs().double()))
+
+
+def test_gru_scan_in_pieces_down_to_single_rows_continues_the_state(ops):
+    z, q, h0 = scan_inputs((2, 50, 96), 2, torch.float32, 4)
+    whole, last = ops.gru_scan(z, q, h0)
+    state, rows = h0, []
+    for lo, hi in [(0, 20), (20, 21), (21, 22), (22, 22), (22, 50)]:
+        h, state = ops.gru_scan(z[:, lo:hi], q[:, lo:hi], state)
+        rows.append(h)
+    m = 2 * chain(50) * 3
+    within(torch.cat(rows, 1), whole, m)
+    within(state, last, m)
+    one = ops.gru_update(z[:, 0].contiguous(), q[:, 0].contiguous(), h0)
+    within(ops.gru_scan(z[:, :1], q[:, :1], h0)[1], one, 8 * F32 * 4)
+
+
+@pytest.mark.parametrize("kind", ["columns", "odd columns", "time first", "every second row", "broadcast gate", "transposed"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gru_scan_takes_strided_inputs(ops, dtype, kind):
+    z0, q0, _ = scan_inputs((4, 320, 160), 4, dtype, 9)
+    pick = {"columns": lambda x: x[:, :, 32:96], "odd columns": lambda x: x[:, :, 3:67], "time first": lambda x: x.transpose(0, 1)[:150],
+            "every second row": lambda x: x[:, ::2], "broadcast gate": lambda x: x[:1].expand(4, 320, 160), "transposed": lambda x: x.transpose(1, 2)}[kind]
+    z, q = pick(z0), (q0 if kind == "broadcast gate" else pick(q0))
+    h0 = torch.randn(z.shape[0], z.shape[2], generator=gen(1), device="cuda")
+    scan_check(ops, z, q, h0)
+
+
+def test_gru_scan_gates_at_their_ends_and_bad_values_stay_in_their_channel(ops):
+    z, q, h0 = scan_inputs((1, 700, 64), 1, torch.float32, 5)
+    z[:, ::3], z[:, 1::3] = 0.0, 1.0                      # keep all / take all
+    scan_check(ops, z, q, h0)
+    want, wl = ops.gru_scan(z * 0.5, q, h0)
+    bad = q.clone()
+    bad[0, 300, 5], bad[0, 10, 40] = math.inf, math.nan
+    got, gl = ops.gru_scan(z * 0.5, bad, h0)
+    keep = [c for c in range(64) if c not in (5, 40)]
+    assert torch.equal(got[..., keep], want[..., keep]) and torch.equal(gl[:, keep], wl[:, keep])
+    assert torch.equal(got[:, :300, 5], want[:, :300, 5]) and torch.equal(got[:, :10, 40], want[:, :10, 40])
+
+
+def test_gru_scan_of_no_rows_and_no_sequences(ops):
+    h0 = torch.randn(3, 8, device="cuda", requires_grad=True)
+    z = torch.empty(3, 0, 8, device="cuda", requires_grad=True)
+    h, last = ops.gru_scan(z, z.detach(), h0)
+    assert h.shape == (3, 0, 8) and torch.equal(last, h0)
+    dz, dh0 = torch.autograd.grad(last, (z, h0), torch.ones_like(last))
+    assert dz.shape == z.shape and torch.equal(dh0, torch.ones_like(dh0))
+    z = torch.empty(0, 5, 8, device="cuda")
+    h, last = ops.gru_scan(z, z)
+    assert h.shape == (0, 5, 8) and last.shape == (0, 8)
+
+
+def test_gru_scan_gradient_against_differences(ops):
+    g = gen(11)
+    z, q, h0 = scan_inputs((2, 150, 16), 2, torch.float32, 6)
+    leaves = [t.requires_grad_() for t in (z, q, h0)]
+    dh, dl = torch.randn(2, 150, 16, generator=g, device="cuda"), torch.randn(2, 16, generator=g, device="cuda")
+    grads = torch.autograd.grad(ops.gru_scan(*leaves), leaves, (dh, dl))
+    with torch.no_grad():
+        for i, t in enumerate(leaves):
+            way = torch.randn(t.shape, generator=g, device="cuda")
+            h = 2.0 ** -10
+            f = []
+            for s in (1, -1):
+                a, b = ops.gru_scan(*[v + s * h * way if j == i else v for j, v in enumerate(leaves)])
+                f.append(float((a.double() * dh.double()).sum() + (b.double() * dl.double()).sum()))
+            got, want = (f[0] - f[1]) / (2 * h), float((grads[i].double() * way.double()).sum())
+            # linear in q and h0; in z the cubic share is h^2 / 6 x (third differences of products of up to 150 gates, each |way| / 0.1)
+            size = float(dh.double().abs().sum() + dl.double().abs().sum())
+            assert abs(got - want) <= size * (chain(150) / h + h * h / 6 * 1000), (i, got, want)
+
+
+def test_gru_scan_gives_the_same_bits_every_time_on_any_stream_and_in_a_graph(ops):
+    cu = torch.tensor([0, 100, 100, 2500, 2990], dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    for args, c in ((scan_inputs((3000, 72), 4, torch.float32, 8), cu), (scan_inputs((2, 1500, 96), 2, torch.bfloat16, 8), None)):
+        z, q, h0 = leaves = [t.requires_grad_() for t in args]
+        dh, dl = torch.ones_like(q.detach()), torch.ones_like(h0.detach())
+
+        def step():
+            h, last = ops.gru_scan(z, q, h0, cu_seqlens=c)
+            return (h.detach(), last.detach()) + torch.autograd.grad((h, last), leaves, (dh, dl))
+        want = [t.clone() for t in step()]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, b) for a, b in zip(other, want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = step()
+        for k in range(3):
+            for t in held:
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(held, want)), k
+            assert all(torch.equal(a, b) for a, b in zip(step(), want)), k
+            torch.cuda.synchronize()
