@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 OUT = os.path.join(os.path.dirname(HERE), "libmotif_hip.so")
 # The sequence operators: compiled without packed fp32 instructions (common.h: MOTIF_SCALAR_F32).  hipcc's host pass warns that it does not know
 # the feature: harmless.
-SEQ_SOURCES = ["layer_norm.hip", "gru_scan.hip"]
+SEQ_SOURCES = ["layer_norm.hip", "gru_scan.hip", "gated_mlp.hip"]
 SEQ_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SOURCES = ["api.hip", "conv_igemm.hip", "conv_split.hip", "conv_split2.hip", "conv_wino.hip", "conv_pw.hip", "conv_ig16.hip", "conv_direct.hip", "siren.hip", "siren_split.hip", "splat.hip", "misc.hip", "corr.hip", "dcn.hip"] + SEQ_SOURCES
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-value",

@@ -1,0 +1,644 @@
+// Gated feed-forward block: both projections, the activation and the product in one kernel, and its backward pass.
+//
+//   forward    G = x Wg^T + bg,  U = x Wu^T + bu,  h = act(G) * U
+//   backward   dG = dh * U * act'(G),  dU = dh * act(G)
+//              dx = dG Wg + dU Wu,   dWg = dG^T x,  dWu = dU^T x,   dbg, dbu = sums of dG, dU over the rows
+//
+// Three matrix products with two right-hand sides each, all bound by the matrix cores from a few hundred rows on.  One kernel serves them
+// (gemm_kernel): C = sum over segments of A_s B_s^T with both operands' reduction axis dense, and a tile's columns in two halves that come
+// from two matrices -- the gate's and the up projection's (forward: the same columns of both, so that a wave holds G and U of the same
+// outputs in its accumulators; weights' gradients: dG^T and dU^T), or the two neighbouring runs of one (dx).  fp32 runs on the same
+// kernel: every operand is split exactly into three bf16 parts and the six products that reach fp32's last place are six segments of the
+// reduction.  Operands whose reduction axis is not dense, or not a multiple of 32, are laid out first (layout_kernel).
+// G and U are kept in fp32 for the backward pass: rounded to the data's type they would add an error of their own to every gradient; dG and
+// dU are rounded once, to be operands of the matrix cores.
+// Up to 64 rows the forward pass is bound by reading the weights (rows_kernel).
+// Sums over rows and over the pieces of a split reduction are taken in a fixed order: no atomics, the same bits every time.
+#include "seq_common.h"
+
+namespace {
+
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kSegs = 12;                                // dx in fp32: two pairs of operands, six products each
+
+// ---- activations.  FAST: v_exp_f32 and v_rcp_f32 as they are (relative error about 2^-21 at |g| = 8, behind a rounding to 8 or 11 bits) -------
+template <bool FAST>
+__device__ __forceinline__ float sigm(float g) { return FAST ? __builtin_amdgcn_rcpf(1.f + __expf(-g)) : 1.f / (1.f + expf(-g)); }
+template <bool FAST>
+__device__ __forceinline__ float gate(float g, int act) {
+    if (act == MOTIF_GATE_SIGMOID) return sigm<FAST>(g);
+    if (act == MOTIF_GATE_SILU) return g * sigm<FAST>(g);
+    return 0.5f * g * (1.f + erff(g * 0.70710678f));
+}
+// act(g) and its derivative
+__device__ __forceinline__ void gate_grad(float g, int act, float& v, float& d) {
+    if (act == MOTIF_GATE_GELU) {
+        const float phi = 0.5f * (1.f + erff(g * 0.70710678f));
+        v = g * phi;
+        d = fmaf(g * 0.39894228f, expf(-0.5f * g * g), phi);
+        return;
+    }
+    const float s = sigm<false>(g);
+    if (act == MOTIF_GATE_SIGMOID) { v = s; d = s * (1.f - s); }
+    else { v = g * s; d = s * fmaf(g, 1.f - s, 1.f); }
+}
+
+// ---- the matrix product ------------------------------------------------------------------------------------------------------------------
+struct GemmArgs {
+    const void* a[kSegs];                                // rows of A: [M][lda], reduction axis dense
+    const void* b0[kSegs];                               // the two halves' rows: [N][ldb]
+    const void* b1[kSegs];
+    long lda, ldb;                                       // in elements
+    int nseg, steps;                                     // segments; reduction steps of 32 in each
+    int M, N;                                            // rows of A, of the B matrices
+    int tiles_m, tiles_n, splits, steps_per_split;
+    void *c0, *c1;                                       // outputs of type dtype: GATED h [M][N], ONE C [M][N], TWO C0, C1 [N][M]
+    float *g, *u;                                        // GATED: G and U to keep (may be null)
+    const void *bias0, *bias1;
+    float* part;                                         // split reduction, fp32 instead of the outputs: ONE [split][M][N], TWO [split][2][N][M]
+    int act, dtype, vec;                                 // vec: rows of the outputs allow runs of four values
+};
+// GATED: the halves are the same columns of two matrices, combined.  ONE: neighbouring columns of one matrix.  TWO: the same columns of two
+// matrices, written transposed (a lane then holds four consecutive rows of A: the matrix instruction takes its operands the other way round).
+enum GemmMode { GATED, ONE, TWO };
+
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, bf16_t*) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, f16_t*) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// 64 lanes x 16 bytes from global memory to `lds` .. + 1024: base + off of each lane.  Written as assembly so that the compiler does not make
+// every LDS read wait for all of them (it takes any for the one that fills what is read); the waits are counted by hand in the kernel.
+__device__ __forceinline__ void to_lds(unsigned lds, const void* base, unsigned off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+
+template <typename T, typename O, int N>
+__device__ __forceinline__ void store_run(void* p, long at, const float (&v)[N], int n, bool vec) {      // n of N values; whole aligned runs as one store
+    O* o = (O*)p + at;
+    if (vec && n == N) seq_store16<O, N>(o, v);
+    else
+#pragma unroll
+        for (int i = 0; i < N; ++i) if (i < n) o[i] = (O)v[i];
+}
+template <int N>
+__device__ __forceinline__ void store_as(void* p, long at, const float (&v)[N], int n, bool vec, int dtype) {
+    if (dtype == MOTIF_F32) store_run<float, float, N>(p, at, v, n, vec);
+    else if (dtype == MOTIF_BF16) store_run<bf16_t, bf16_t, N>(p, at, v, n, vec);
+    else store_run<f16_t, f16_t, N>(p, at, v, n, vec);
+}
+
+// Tile BM rows of A x BN / 2 rows of either half, WM x WN waves.  The reduction advances in steps of 32: a stage holds 64 bytes of every row, its
+// four 16-byte pieces exchanged by a pattern of the row's number so that the 16 rows of a fragment lie in different banks; four stages lie in
+// LDS, three of them requested ahead of the one that is multiplied, one barrier a step: behind it every wave has finished the stage that the
+// next request overwrites.
+template <typename T, int BM, int BN, int WM, int WN, GemmMode MODE>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(GemmArgs p) {
+    constexpr int NW = WM * WN, MF = BM / WM / 16, HF = BN / 2 / WN / 16;        // fragments of a wave: rows, columns of either half
+    constexpr int STAGE = (BM + BN) * 64, STAGES = 4;
+    static_assert(BM / 16 == 2 * NW && BN / 16 == 2 * NW, "each wave requests two pieces of 16 rows of either operand per stage");
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+
+    // Workgroups are dealt to the eight XCDs in turn: each XCD takes a contiguous run of tiles, column by column within bands of 8 tile rows,
+    // so that the tiles in flight on one XCD share their rows of both operands in its L2.
+    const int tiles = p.tiles_m * p.tiles_n;
+    int id = blockIdx.x;
+    const int split = id / tiles;
+    id -= split * tiles;
+    {
+        const int xcd = id & 7, q = tiles >> 3, r = tiles & 7;
+        id = xcd * q + (xcd < r ? xcd : r) + (id >> 3);
+    }
+    const int band = id / (8 * p.tiles_n), in = id - band * 8 * p.tiles_n, bh = min(8, p.tiles_m - band * 8);
+    const int m0 = (band * 8 + in % bh) * BM, tn = in / bh;
+    const int n0[2] = {tn * (MODE == ONE ? BN : BN / 2), MODE == ONE ? tn * BN + BN / 2 : tn * (BN / 2)};
+    const int nb[2] = {n0[0], min(n0[1], p.N - 1)};      // where the halves' pointers stand: a row that exists
+
+    // this lane's share of a request: LDS row (lane >> 2) of the piece, position lane & 3
+    const int lr = lane >> 2, lp = lane & 3;
+    const int sw = ((lr >> 1) & 1) ^ ((lr >> 3) & 1) | (((lr >> 2) & 1) << 1);
+    unsigned offa[2], offb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = (i * NW + wave) * 16 + lr;
+        offa[i] = (unsigned)(min(row, p.M - 1 - m0) * (unsigned)p.lda * 2u) + (unsigned)((lp ^ sw) * 16);
+        offb[i] = (unsigned)((min(n0[i] + wave * 16 + lr, p.N - 1) - nb[i]) * (unsigned)p.ldb * 2u) + (unsigned)((lp ^ sw) * 16);      // half i
+    }
+    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
+
+    const int s_begin = split * p.steps_per_split, s_end = min(p.nseg * p.steps, s_begin + p.steps_per_split), count = s_end - s_begin;
+    int seg = s_begin / p.steps, left = p.steps - (s_begin - seg * p.steps);      // steps left in the segment that is requested
+    const char *pa, *pb0, *pb1;
+    auto segment = [&](int step) __attribute__((always_inline)) {
+        pa = (const char*)p.a[seg] + ((long)m0 * p.lda + (long)step * 32) * 2;
+        pb0 = (const char*)p.b0[seg] + ((long)nb[0] * p.ldb + (long)step * 32) * 2;
+        pb1 = (const char*)p.b1[seg] + ((long)nb[1] * p.ldb + (long)step * 32) * 2;
+    };
+    segment(s_begin - seg * p.steps);
+    auto request = [&](int stage) __attribute__((always_inline)) {
+        const unsigned at = lds0 + stage * STAGE + wave * 1024;
+        to_lds(at, pa, offa[0]);
+        to_lds(at + NW * 1024, pa, offa[1]);
+        to_lds(at + BM * 64, pb0, offb[0]);
+        to_lds(at + BM * 64 + NW * 1024, pb1, offb[1]);
+        pa += 64; pb0 += 64; pb1 += 64;
+        if (--left == 0 && seg + 1 < p.nseg) { ++seg; left = p.steps; segment(0); }
+    };
+
+    f32x4 acc[MF][2][HF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < HF; ++j) acc[i][h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // a fragment: row lane & 15, the 8 values of piece lane >> 4
+    const int fr = lane & 15, fs = ((fr >> 1) & 1) ^ ((fr >> 3) & 1) | (((fr >> 2) & 1) << 1);
+    const int frag = fr * 64 + (((lane >> 4) ^ fs) * 16);
+    const int fa = wm * MF * 1024 + frag, fb = BM * 64 + wn * HF * 1024 + frag;
+
+    for (int s = 0; s < 3 && s < count; ++s) request(s);
+    for (int s = 0; s < count; ++s) {
+        // the stages requested behind this one may still be on their way (four requests each); then everybody's part of it is there
+        if (s + 2 < count) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else if (s + 1 < count) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + 3 < count) request((s + 3) & 3);
+        const char* st = lds + (s & 3) * STAGE;
+        s16x8 av[MF], bv[2][HF];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < HF; ++j) bv[h][j] = *(const s16x8*)(st + fb + (h * (BN / 2) + j * 16) * 64);
+#pragma unroll
+        for (int i = 0; i < MF; ++i) av[i] = *(const s16x8*)(st + fa + i * 1024);
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < HF; ++j) acc[i][h][j] = MODE != TWO ? mfma(bv[h][j], av[i], acc[i][h][j], (T*)nullptr) : mfma(av[i], bv[h][j], acc[i][h][j], (T*)nullptr);
+    }
+
+    const int lo = lane & 15, hi = (lane >> 4) * 4;
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+#pragma unroll
+        for (int j = 0; j < HF; ++j) {
+            const int mt = m0 + (wm * MF + i) * 16, off = (wn * HF + j) * 16;
+            if constexpr (MODE == GATED) {
+                const int m = mt + lo, n = n0[0] + off + hi, cnt = min(4, p.N - n);
+                if (m >= p.M || cnt <= 0) continue;
+                float g[4], u[4], v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int c = min(n + e, p.N - 1);
+                    g[e] = acc[i][0][j][e] + (p.bias0 ? seq_param(p.bias0, c, p.dtype) : 0.f);
+                    u[e] = acc[i][1][j][e] + (p.bias1 ? seq_param(p.bias1, c, p.dtype) : 0.f);
+                    v[e] = p.dtype == MOTIF_F32 ? gate<false>(g[e], p.act) * u[e] : gate<true>(g[e], p.act) * u[e];
+                }
+                const long at = (long)m * p.N + n;
+                store_as<4>(p.c0, at, v, cnt, p.vec, p.dtype);
+                if (p.g) { store_run<float, float, 4>(p.g, at, g, cnt, p.vec); store_run<float, float, 4>(p.u, at, u, cnt, p.vec); }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = MODE == ONE ? mt + lo : n0[h] + off + lo, col = MODE == ONE ? n0[h] + off + hi : mt + hi;
+                    const int rows = MODE == ONE ? p.M : p.N, cols = MODE == ONE ? p.N : p.M, cnt = min(4, cols - col);
+                    if (row >= rows || cnt <= 0) continue;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[i][h][j][e];
+                    const long at = (long)row * cols + col;
+                    if (p.part) store_run<float, float, 4>(p.part + (MODE == ONE ? (long)split : (long)split * 2 + h) * rows * cols, at, v, cnt, p.vec);
+                    else store_as<4>(MODE == ONE || h == 0 ? p.c0 : p.c1, at, v, cnt, p.vec, p.dtype);
+                }
+            }
+        }
+    }
+}
+
+// The pieces of a split reduction, added in order.  part [splits][n], n = n0 + n1 values to out0 and out1.
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, long n0, long n1, void* out0, void* out1, int dtype) {
+    const long n = n0 + n1;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+        float s = 0.f;
+        for (int k = 0; k < splits; ++k) s += part[k * n + i];
+        if (i < n0) { if (out0) seq_param_store(out0, i, dtype, s); }
+        else if (out1) seq_param_store(out1, i - n0, dtype, s);
+    }
+}
+
+// ---- laying operands out -----------------------------------------------------------------------------------------------------------------
+// fp32 as three bf16 parts of 8 bits each, by truncation: x = p0 + p1 + p2 exactly (but for what is below bf16's smallest number).  An infinity or
+// NaN has no further parts: their differences would make other NaNs of it.
+__device__ __forceinline__ void split3(float x, bf16_t (&out)[3]) {
+    float r = x;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const unsigned top = __builtin_bit_cast(unsigned, r) & 0xffff0000u;
+        out[i] = __builtin_bit_cast(bf16_t, (unsigned short)(top >> 16));
+        r = (top & 0x7f800000u) == 0x7f800000u ? 0.f : r - __builtin_bit_cast(float, top);
+    }
+    // a NaN whose payload lies in the lower half only must not become an infinity
+    if (x != x) out[0] = __builtin_bit_cast(bf16_t, (unsigned short)0x7fc0);
+}
+// value v of a [rows][ld] image at (r, c): one plane of T, or three of bf16, `plane` elements apart
+__device__ __forceinline__ void put(float* /*type*/, void* dst, long plane, long at, float v) {
+    bf16_t s[3];
+    split3(v, s);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) ((bf16_t*)dst)[i * plane + at] = s[i];
+}
+__device__ __forceinline__ void put(bf16_t*, void* dst, long, long at, float v) { ((bf16_t*)dst)[at] = (bf16_t)v; }
+__device__ __forceinline__ void put(f16_t*, void* dst, long, long at, float v) { ((f16_t*)dst)[at] = (f16_t)v; }
+
+// src [rows][cols] with row stride rs -> as it lies (dst: rows of ld, may be null) and transposed (tdst: cols of tld, may be null), zeros behind the
+// last value of every row.  64 x 64 values per workgroup; the grid covers ld and tld.
+template <typename T>
+__global__ __launch_bounds__(256) void layout_kernel(const T* __restrict__ src, long rs, int rows, int cols, void* dst, long plane, int ld, void* tdst, long tplane, int tld) {
+    __shared__ float sh[64][65];
+    const int c0 = blockIdx.y * 64, r0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    for (int i = y; i < 64; i += 4) {
+        const int r = r0 + i, c = c0 + x;
+        const float v = r < rows && c < cols ? (float)src[(long)r * rs + c] : 0.f;
+        if (dst && r < rows && c < ld) put((T*)nullptr, dst, plane, (long)r * ld + c, v);
+        sh[i][x] = v;
+    }
+    if (!tdst) return;
+    __syncthreads();
+    for (int i = y; i < 64; i += 4) {
+        const int c = c0 + i, r = r0 + x;
+        if (c < cols && r < tld) put((T*)nullptr, tdst, tplane, (long)c * tld + r, sh[x][i]);
+    }
+}
+
+// dG and dU of 64 rows x 64 columns: as they lie (dst: [rows][ld], dU `pair` elements behind dG), transposed (tdst: [F][tld], `tpair`), and summed over
+// the 64 rows (part [row blocks][2 F], may be null).  fp32: three planes, `plane` / `tplane` apart.
+template <typename T>
+__global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh, long dhs, const float* __restrict__ G, const float* __restrict__ U, int M, int F, int act,
+                                                       void* dst, long plane, long pair, int ld, void* tdst, long tplane, long tpair, int tld, float* part) {
+    using O = std::conditional_t<sizeof(T) == 4, bf16_t, T>;
+    __shared__ float sg[64][65], su[64][65];
+    const int c0 = blockIdx.y * 64, r0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    const int c = c0 + x;
+    for (int i = y; i < 64; i += 4) {
+        const int r = r0 + i;
+        float dg = 0.f, du = 0.f;
+        if (r < M && c < F) {
+            const long at = (long)r * F + c;
+            const float d = (float)dh[r * dhs + c];
+            float v, dv;
+            gate_grad(G[at], act, v, dv);
+            dg = d * U[at] * dv;
+            du = d * v;
+        }
+        sg[i][x] = dg;
+        su[i][x] = du;
+        if (dst && r < M && c < ld) {
+            put((T*)nullptr, dst, plane, (long)r * ld + c, dg);
+            put((T*)nullptr, (O*)dst + pair, plane, (long)r * ld + c, du);
+        }
+    }
+    __syncthreads();
+    if (tdst)
+        for (int i = y; i < 64; i += 4) {
+            const int cc = c0 + i, r = r0 + x;
+            if (cc < F && r < tld) {
+                put((T*)nullptr, tdst, tplane, (long)cc * tld + r, sg[x][i]);
+                put((T*)nullptr, (O*)tdst + tpair, tplane, (long)cc * tld + r, su[x][i]);
+            }
+        }
+    if (part && y < 2 && c < F) {
+        float s = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < 64; ++i) s += y ? su[i][x] : sg[i][x];
+        part[((long)blockIdx.x * 2 + y) * F + c] = s;
+    }
+}
+
+// ---- few rows ----------------------------------------------------------------------------------------------------------------------------
+// Up to 16 MT rows: a workgroup takes 16 columns of both projections, its 8 waves share the reduction, each lane reads 16 bytes of a weight row
+// (16 rows x 4 pieces per instruction) straight into the matrix instruction's operand; the waves' sums meet in LDS in a fixed order.  Bound by
+// the weights' bytes.  fp32 runs on the fp32 matrix instruction.  VEC: every row allows 16-byte reads.
+template <typename T, int MT, bool VEC>
+__global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long xs, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ bg, const T* __restrict__ bu,
+                                                   T* __restrict__ h, float* __restrict__ G, float* __restrict__ U, int M, int K, int F, int act) {
+    constexpr int V = 16 / sizeof(T), STEP = 4 * V, NW = 8;
+    __shared__ float sh[NW][2][16 * MT][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, kq = (lane >> 4) * V;
+    const int f0 = blockIdx.x * 16, fr = min(f0 + lo, F - 1);
+    const T* pg = wg + (long)fr * K;
+    const T* pu = wu + (long)fr * K;
+    f32x4 ag[MT], au[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) ag[i] = au[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto read = [&](const T* row, int k) __attribute__((always_inline)) {
+        SeqVec<T, V> v;
+        if (VEC) {
+            if (k < K) v = *(const SeqVec<T, V>*)(row + k);
+            else
+#pragma unroll
+                for (int e = 0; e < V; ++e) v.v[e] = (T)0.f;
+        } else
+#pragma unroll
+            for (int e = 0; e < V; ++e) v.v[e] = k + e < K ? row[k + e] : (T)0.f;
+        return v;
+    };
+    const int steps = (K + STEP - 1) / STEP;
+    constexpr int AHEAD = MT == 1 ? 4 : 2;
+    for (int s = wave; s < steps; s += NW * AHEAD) {
+        SeqVec<T, V> a[AHEAD], b[AHEAD], c[AHEAD][MT];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int k = (s + j * NW) * STEP + kq;      // behind the last step: zeros
+            a[j] = read(pg, k);
+            b[j] = read(pu, k);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) c[j][i] = read(x + (long)min(i * 16 + lo, M - 1) * xs, k);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                if constexpr (sizeof(T) == 2) {
+                    const s16x8 cv = __builtin_bit_cast(s16x8, c[j][i]);
+                    ag[i] = mfma(__builtin_bit_cast(s16x8, a[j]), cv, ag[i], (T*)nullptr);
+                    au[i] = mfma(__builtin_bit_cast(s16x8, b[j]), cv, au[i], (T*)nullptr);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        ag[i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)a[j].v[e], (float)c[j][i].v[e], ag[i], 0, 0, 0);
+                        au[i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)b[j].v[e], (float)c[j][i].v[e], au[i], 0, 0, 0);
+                    }
+                }
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {                    // lane: row lo, columns 4 (lane / 16) + e
+            sh[wave][0][i * 16 + lo][(lane >> 4) * 4 + e] = ag[i][e];
+            sh[wave][1][i * 16 + lo][(lane >> 4) * 4 + e] = au[i][e];
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256 * MT; i += 512) {
+        const int m = i >> 4, f = f0 + (i & 15);
+        if (m >= M || f >= F) continue;
+        float g = 0.f, u = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { g += sh[w][0][m][i & 15]; u += sh[w][1][m][i & 15]; }
+        if (bg) g += (float)bg[f];
+        if (bu) u += (float)bu[f];
+        const long at = (long)m * F + f;
+        h[at] = (T)(gate<sizeof(T) == 2>(g, act) * u);
+        if (G) { G[at] = g; U[at] = u; }
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------------------
+constexpr int kFewRows = 64;
+constexpr long kMostRows = 1L << 22;                    // offsets within a tile are 32 bits: 256 rows x this x 2 bytes
+int up32(long n) { return (int)((n + 31) & ~31L); }
+long up16b(long bytes) { return (bytes + 255) & ~255L; }
+int planes(int dtype) { return dtype == MOTIF_F32 ? 3 : 1; }
+
+// A workspace that is measured (base null) or handed out.
+struct Arena {
+    char* base;
+    long used;
+    void* take(long bytes) { char* p = base ? base + used : nullptr; used += up16b(bytes); return p; }
+};
+// An operand: `n` planes, `plane` elements apart, rows of ld.
+struct Image { const void* p; long plane; int ld, n; };
+const void* plane_of(const Image& m, int i) { return (const char*)m.p + (long)i * m.plane * 2; }
+
+template <typename T>
+void layout(const void* src, long rs, int rows, int cols, const Image* as, const Image* tr, hipStream_t s) {
+    const int w = as ? (as->ld > cols ? as->ld : cols) : cols, hgt = tr ? (tr->ld > rows ? tr->ld : rows) : rows;
+    layout_kernel<T><<<dim3(cdiv(hgt, 64), cdiv(w, 64)), 256, 0, s>>>((const T*)src, rs, rows, cols, as ? (void*)as->p : nullptr, as ? as->plane : 0, as ? as->ld : 0,
+                                                                   tr ? (void*)tr->p : nullptr, tr ? tr->plane : 0, tr ? tr->ld : 0);
+}
+
+// The products of two operands' parts that reach fp32's last place, smallest first: 2^-16 each of (0,2) (1,1) (2,0), 2^-8 of (0,1) (1,0), (0,0).
+void segments(GemmArgs& g, const Image& a, const Image& b0, const Image& b1) {
+    if (a.n == 1) {
+        g.a[g.nseg] = a.p; g.b0[g.nseg] = b0.p; g.b1[g.nseg] = b1.p;
+        ++g.nseg;
+        return;
+    }
+    static const int pairs[6][2] = {{0, 2}, {1, 1}, {2, 0}, {0, 1}, {1, 0}, {0, 0}};
+    for (auto& q : pairs) {
+        g.a[g.nseg] = plane_of(a, q[0]); g.b0[g.nseg] = plane_of(b0, q[1]); g.b1[g.nseg] = plane_of(b1, q[1]);
+        ++g.nseg;
+    }
+}
+
+// Tiles of 256 x 256 where they give every CU at least one, else of 128 x 128.  The reduction is split where even those leave CUs without work and
+// the pieces stay long (16 steps at least); the pieces' sums are fp32 and joined in order.
+struct GemmPlan { bool big; int tiles_m, tiles_n, splits, steps_per_split; };
+GemmPlan gemm_plan(long M, long N, int halves, long total_steps, bool may_split) {
+    GemmPlan p;
+    auto tiles = [&](int t) { return (long)cdiv(M, t) * cdiv(N, halves == 2 ? t / 2 : t); };
+    p.big = tiles(256) >= 256;
+    const int t = p.big ? 256 : 128;
+    p.tiles_m = cdiv(M, t);
+    p.tiles_n = cdiv(N, halves == 2 ? t / 2 : t);
+    long splits = may_split && !p.big ? 512 / tiles(t) : 1;
+    if (splits > total_steps / 16) splits = total_steps / 16;
+    if (splits < 1) splits = 1;
+    p.steps_per_split = (int)((total_steps + splits - 1) / splits);
+    p.splits = (int)((total_steps + p.steps_per_split - 1) / p.steps_per_split);
+    return p;
+}
+
+template <typename T, GemmMode MODE>
+void gemm(const GemmPlan& pl, GemmArgs& g, hipStream_t s) {
+    g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n; g.splits = pl.splits; g.steps_per_split = pl.steps_per_split;
+    const unsigned grid = (unsigned)((long)pl.tiles_m * pl.tiles_n * pl.splits);
+    if (pl.big) gemm_kernel<T, 256, 256, 2, 4, MODE><<<grid, 512, 0, s>>>(g);
+    else gemm_kernel<T, 128, 128, 2, 2, MODE><<<grid, 256, 0, s>>>(g);
+}
+template <GemmMode MODE>
+void gemm_dtype(int dtype, const GemmPlan& pl, GemmArgs& g, hipStream_t s) {
+    if (dtype == MOTIF_F16) gemm<f16_t, MODE>(pl, g, s);
+    else gemm<bf16_t, MODE>(pl, g, s);
+}
+
+// Whether an operand can be read as it lies: 16-bit values, rows of whole steps at 16-byte addresses.
+bool direct(const void* p, long rs, long cols, int dtype) { return dtype != MOTIF_F32 && cols % 32 == 0 && rs % 8 == 0 && rs <= kMostRows && seq_aligned(p, 16); }
+
+int check_mlp(long M, long K, long F, int act, int dtype) {
+    if (M < 0 || K < 1 || F < 1 || !seq_dtype_ok(dtype) || act < MOTIF_GATE_SIGMOID || act > MOTIF_GATE_GELU) return MOTIF_EINVAL;
+    if (K > 65536 || F > 65536 || M > kMostRows) return MOTIF_ELIMIT;
+    return MOTIF_OK;
+}
+
+template <typename T, int MT>
+void few_rows(bool vec, const void* x, long xs, const void* wg, const void* wu, const void* bg, const void* bu, void* h, float* G, float* U, int M, int K, int F, int act, hipStream_t s) {
+    if (vec) rows_kernel<T, MT, true><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, M, K, F, act);
+    else rows_kernel<T, MT, false><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, M, K, F, act);
+}
+
+struct FwdImages { Image x, wg, wu; bool lay_x, lay_w; };
+FwdImages fwd_images(Arena& ws, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype) {
+    FwdImages f;
+    const int n = planes(dtype), ld = up32(K);
+    f.lay_x = !direct(x, xs, K, dtype);
+    f.lay_w = !direct(wg, K, K, dtype) || !direct(wu, K, K, dtype);
+    f.x = f.lay_x ? Image{ws.take(2 * n * M * ld), M * ld, ld, n} : Image{x, 0, (int)xs, 1};
+    f.wg = f.lay_w ? Image{ws.take(2 * n * F * ld), F * ld, ld, n} : Image{wg, 0, (int)K, 1};
+    f.wu = f.lay_w ? Image{ws.take(2 * n * F * ld), F * ld, ld, n} : Image{wu, 0, (int)K, 1};
+    return f;
+}
+
+struct BwdImages { Image dg, du, dgt, dut, xt, wgt, wut; float *bias_part, *split_part; GemmPlan dx, dw; };
+BwdImages bwd_images(Arena& ws, long M, long K, long F, int dtype, bool need_x, bool need_w, bool need_b) {
+    BwdImages b = {};
+    const int n = planes(dtype), ldf = up32(F), ldm = up32(M);
+    if (need_x) {
+        char* p = (char*)ws.take(2L * 2 * n * M * ldf);
+        b.dg = {p, M * ldf, ldf, n};
+        b.du = {p ? p + 2L * n * M * ldf : nullptr, M * ldf, ldf, n};
+        b.wgt = {ws.take(2L * n * K * ldf), K * ldf, ldf, n};
+        b.wut = {ws.take(2L * n * K * ldf), K * ldf, ldf, n};
+        b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * ldf / 32, true);
+    }
+    if (need_w) {
+        char* p = (char*)ws.take(2L * 2 * n * F * ldm);
+        b.dgt = {p, F * ldm, ldm, n};
+        b.dut = {p ? p + 2L * n * F * ldm : nullptr, F * ldm, ldm, n};
+        b.xt = {ws.take(2L * n * K * ldm), K * ldm, ldm, n};
+        b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * ldm / 32, true);
+    }
+    if (need_b) b.bias_part = (float*)ws.take(4L * cdiv(M, 64) * 2 * F);
+    long part = 0;                                       // the two products run one behind the other: one piece of memory serves both
+    if (need_x && b.dx.splits > 1) part = 4L * b.dx.splits * M * K;
+    if (need_w && b.dw.splits > 1) { const long w = 4L * b.dw.splits * 2 * F * K; part = w > part ? w : part; }
+    if (part) b.split_part = (float*)ws.take(part);
+    return b;
+}
+void join(const float* part, int splits, long n0, long n1, void* o0, void* o1, int dtype, hipStream_t s) {
+    const long blocks = (n0 + n1 + 255) / 256;
+    join_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(part, splits, n0, n1, o0, o1, dtype);
+}
+}  // namespace
+
+extern "C" long motif_gated_mlp_ws_bytes(const void* x, long x_rs, const void* w_gate, const void* w_up, long M, long K, long F, int dtype) {
+    const int rc = check_mlp(M, K, F, MOTIF_GATE_SILU, dtype);
+    if (rc) return rc;
+    if (M <= kFewRows) return 0;
+    Arena ws = {nullptr, 0};
+    fwd_images(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+    return ws.used;
+}
+
+extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* h, float* G, float* U,
+                                   void* workspace, long M, long K, long F, int act, int dtype, void* stream) {
+    const int rc = check_mlp(M, K, F, act, dtype);
+    if (rc) return rc;
+    if (M == 0) return MOTIF_OK;
+    if (!x || !w_gate || !w_up || !h || x_rs < 0 || !G != !U) return MOTIF_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    if (M <= kFewRows) {
+        const int V = 16 / seq_size(dtype);
+        const bool vec = K % V == 0 && x_rs % V == 0 && seq_aligned(x, 16) && seq_aligned(w_gate, 16) && seq_aligned(w_up, 16);
+        seq_dispatch(dtype, [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            if (M <= 16) few_rows<T, 1>(vec, x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
+            else if (M <= 32) few_rows<T, 2>(vec, x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
+            else few_rows<T, 4>(vec, x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
+        });
+        MOTIF_LAUNCH_CHECK();
+        return MOTIF_OK;
+    }
+    Arena ws = {(char*)workspace, 0};
+    const FwdImages f = fwd_images(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+    if (ws.used && !workspace) return MOTIF_EINVAL;
+    seq_dispatch(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (f.lay_x) layout<T>(x, x_rs, (int)M, (int)K, &f.x, nullptr, s);
+        if (f.lay_w) { layout<T>(w_gate, K, (int)F, (int)K, &f.wg, nullptr, s); layout<T>(w_up, K, (int)F, (int)K, &f.wu, nullptr, s); }
+    });
+    GemmArgs g = {};
+    segments(g, f.x, f.wg, f.wu);
+    g.lda = f.x.ld; g.ldb = f.wg.ld;
+    g.steps = up32(K) / 32;
+    g.M = (int)M; g.N = (int)F;
+    g.c0 = h; g.g = G; g.u = U; g.bias0 = b_gate; g.bias1 = b_up;
+    g.act = act; g.dtype = dtype;
+    g.vec = F % 4 == 0 && seq_aligned(h, 16) && seq_aligned(G, 16) && seq_aligned(U, 16);
+    gemm_dtype<GATED>(dtype, gemm_plan(M, F, 2, (long)g.nseg * g.steps, false), g, s);
+    MOTIF_LAUNCH_CHECK();
+    return MOTIF_OK;
+}
+
+extern "C" long motif_gated_mlp_bwd_ws_bytes(long M, long K, long F, int dtype, int need_x, int need_w, int need_b) {
+    const int rc = check_mlp(M, K, F, MOTIF_GATE_SILU, dtype);
+    if (rc) return rc;
+    Arena ws = {nullptr, 0};
+    bwd_images(ws, M, K, F, dtype, need_x, need_w, need_b);
+    return ws.used;
+}
+
+extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate, const void* w_up, const float* G, const float* U, const void* dh, long dh_rs,
+                                   void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* workspace, long M, long K, long F, int act, int dtype, void* stream) {
+    const int rc = check_mlp(M, K, F, act, dtype);
+    if (rc) return rc;
+    const bool need_x = dx, need_w = dw_gate || dw_up, need_b = db_gate || db_up;
+    if (need_w && (!dw_gate || !dw_up)) return MOTIF_EINVAL;
+    if (M < 1 || !x || !w_gate || !w_up || !G || !U || !dh || !workspace || x_rs < 0 || dh_rs < 0 || !(need_x || need_w || need_b)) return MOTIF_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    Arena ws = {(char*)workspace, 0};
+    const BwdImages b = bwd_images(ws, M, K, F, dtype, need_x, need_w, need_b);
+    seq_dispatch(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        const int w = need_x ? b.dg.ld : (int)F, hgt = need_w ? b.dgt.ld : (int)M;
+        gate_grad_kernel<T><<<dim3(cdiv(hgt, 64), cdiv(w, 64)), 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, act,
+            need_x ? (void*)b.dg.p : nullptr, b.dg.plane, b.dg.plane * b.dg.n, b.dg.ld, need_w ? (void*)b.dgt.p : nullptr, b.dgt.plane, b.dgt.plane * b.dgt.n, b.dgt.ld, b.bias_part);
+        if (need_x) { layout<T>(w_gate, K, (int)F, (int)K, nullptr, &b.wgt, s); layout<T>(w_up, K, (int)F, (int)K, nullptr, &b.wut, s); }
+        if (need_w) layout<T>(x, x_rs, (int)M, (int)K, nullptr, &b.xt, s);
+    });
+    if (need_b) {
+        const int r = seq_colsum2(b.bias_part, cdiv(M, 64), F, db_gate, db_up, dtype, s);
+        if (r) return r;
+    }
+    if (need_x) {                                        // dx = [dG dU] [Wg^T Wu^T]^T: the second pair continues the reduction
+        GemmArgs g = {};
+        segments(g, b.dg, b.wgt, b.wgt);
+        segments(g, b.du, b.wut, b.wut);
+        g.lda = b.dg.ld; g.ldb = b.wgt.ld;
+        g.steps = b.dg.ld / 32;
+        g.M = (int)M; g.N = (int)K;
+        g.c0 = dx; g.dtype = dtype;
+        g.part = b.dx.splits > 1 ? b.split_part : nullptr;
+        g.vec = K % 4 == 0 && seq_aligned(dx, 16);
+        gemm_dtype<ONE>(dtype, b.dx, g, s);
+        if (g.part) join(g.part, b.dx.splits, M * K, 0, dx, nullptr, dtype, s);
+    }
+    if (need_w) {
+        GemmArgs g = {};
+        segments(g, b.xt, b.dgt, b.dut);
+        g.lda = b.xt.ld; g.ldb = b.dgt.ld;
+        g.steps = b.xt.ld / 32;
+        g.M = (int)K; g.N = (int)F;
+        g.c0 = dw_gate; g.c1 = dw_up; g.dtype = dtype;
+        g.part = b.dw.splits > 1 ? b.split_part : nullptr;
+        g.vec = K % 4 == 0 && seq_aligned(dw_gate, 16) && seq_aligned(dw_up, 16);
+        gemm_dtype<TWO>(dtype, b.dw, g, s);
+        if (g.part) join(g.part, b.dw.splits, F * K, F * K, dw_gate, dw_up, dtype, s);
+    }
+    MOTIF_LAUNCH_CHECK();
+    return MOTIF_OK;
+}

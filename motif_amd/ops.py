@@ -1193,3 +1193,83 @@ def gru_scan(z, q, h0=None, cu_seqlens=None):
     if _wants_grad(z, q, h0):
         return _GruScan.apply(z, q, h0, cu)
     return _gru_scan_fwd(z, q, h0, cu)
+
+
+_GATES = {"sigmoid": 0, "silu": 1, "gelu": 2}
+
+
+def _mlp_workspace(n, x, k, f):
+    if n < 0:
+        raise RuntimeError("gated_mlp: x %s with %d outputs is outside what the kernels support (%d)" % (list(x.shape), f, n))
+    return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+
+
+def _gated_mlp_fwd(x, wg, wu, bg, bu, act, keep):
+    f, k = wg.shape
+    m, code = x.numel() // k, _SEQ_DTYPES[x.dtype]
+    h = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
+    g, u = (torch.empty(m, f, dtype=torch.float32, device=x.device) for _ in range(2)) if keep else (None, None)
+    if m:
+        xr, rs = _seq_rows(x)
+        args = (xr.data_ptr(), rs, wg.data_ptr(), wu.data_ptr())
+        ws = _mlp_workspace(_lib.load().motif_gated_mlp_ws_bytes(*args, m, k, f, code), x, k, f)
+        _seq_call("motif_gated_mlp_fwd", x.device, *args, _seq_ptr(bg), _seq_ptr(bu), h.data_ptr(), _seq_ptr(g), _seq_ptr(u), _seq_ptr(ws), m, k, f, act, code)
+    return h, g, u
+
+
+class _GatedMlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, bg, bu, act):
+        h, g, u = _gated_mlp_fwd(x, wg, wu, bg, bu, act, True)
+        ctx.save_for_backward(x, wg, wu, g, u)
+        ctx.act = act
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, wg, wu, g, u = ctx.saved_tensors
+        f, k = wg.shape
+        m, code = x.numel() // k, _SEQ_DTYPES[x.dtype]
+        need_x, need_wg, need_wu, need_bg, need_bu, _ = ctx.needs_input_grad
+        new = lambda shape, need: torch.empty(shape, dtype=x.dtype, device=x.device) if need else None  # noqa: E731
+        dx = new(x.shape, need_x)
+        dwg, dwu = (new((f, k), need_wg or need_wu) for _ in range(2))
+        dbg, dbu = new((f,), need_bg), new((f,), need_bu)
+        if m:
+            xr, xs = _seq_rows(x)
+            dr, ds = _seq_rows(dh)
+            ws = _mlp_workspace(_lib.load().motif_gated_mlp_bwd_ws_bytes(m, k, f, code, need_x, dwg is not None, need_bg or need_bu), x, k, f)
+            _seq_call("motif_gated_mlp_bwd", x.device, xr.data_ptr(), xs, wg.data_ptr(), wu.data_ptr(), g.data_ptr(), u.data_ptr(), dr.data_ptr(), ds,
+                      _seq_ptr(dx), _seq_ptr(dwg), _seq_ptr(dwu), _seq_ptr(dbg), _seq_ptr(dbu), _seq_ptr(ws), m, k, f, ctx.act, code)
+        else:
+            for t in (dwg, dwu, dbg, dbu):
+                if t is not None:
+                    t.zero_()
+        return dx, dwg if need_wg else None, dwu if need_wu else None, dbg, dbu, None
+
+
+def gated_mlp(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
+    """Gated feed-forward block act(x w_gate^T + b_gate) * (x w_up^T + b_up) in one kernel; act: "silu", "gelu" (exact) or "sigmoid".
+
+    x [..., K], w_gate / w_up [F, K] (nn.Linear's layout), b_gate / b_up [F], all fp32, bf16 or fp16; K, F <= 65536, at most 2^22 rows.  Sums are
+    fp32; fp32 data keep fp32's accuracy on the matrix cores (three exact bf16 parts of every operand; an infinite operand makes its outputs NaN).
+    With gradients the two projections are kept in fp32 (8 bytes per output value).  Differentiable in all tensors."""
+    what = "gated_mlp"
+    _seq_type(x, what, "x")
+    if act not in _GATES:
+        raise RuntimeError("%s: act must be one of %s, got %r" % (what, sorted(_GATES), act))
+    if x.dim() < 1 or w_gate.dim() != 2 or not 1 <= w_gate.shape[0] <= 65536 or not 1 <= w_gate.shape[1] <= 65536 or x.shape[-1] != w_gate.shape[1]:
+        raise RuntimeError("%s: x [..., K] and w_gate [F, K] with 1 <= K, F <= 65536, got %s and %s" % (what, list(x.shape), list(w_gate.shape)))
+    if x.numel() // x.shape[-1] > 1 << 22:
+        raise RuntimeError("%s: at most %d rows, got %s" % (what, 1 << 22, list(x.shape)))
+    f = w_gate.shape[0]
+    _seq_same(w_gate, x, w_gate.shape, what, "w_gate", (x.dtype,))
+    _seq_same(w_up, x, w_gate.shape, what, "w_up", (x.dtype,))
+    _seq_same(b_gate, x, (f,), what, "b_gate", (x.dtype,))
+    _seq_same(b_up, x, (f,), what, "b_up", (x.dtype,))
+    require_device(x, "gated_mlp needs CUDA(ROCm) tensors")
+    params = [None if p is None else _c(p) for p in (w_gate, w_up, b_gate, b_up)]
+    if _wants_grad(x, *params):
+        return _GatedMlp.apply(x, *params, _GATES[act])
+    return _gated_mlp_fwd(x, *params, _GATES[act], False)[0]

@@ -415,3 +415,194 @@ def test_gru_scan_gives_the_same_bits_every_time_on_any_stream_and_in_a_graph(op
             assert all(torch.equal(a, b) for a, b in zip(held, want)), k
             assert all(torch.equal(a, b) for a, b in zip(step(), want)), k
             torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------------------------ gated_mlp
+def gate_reference(g, act):
+    s = torch.sigmoid(g)
+    if act == "sigmoid":
+        return s, s * (1 - s)
+    if act == "silu":
+        return g * s, s * (1 + g * (1 - s))
+    phi = 0.5 * (1 + torch.erf(g / math.sqrt(2)))
+    return g * phi, phi + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+
+
+def mlp_check(ops, x, wg, wu, bg, bu, act, seed=0):
+    """Against 64 bits.  A product of n terms in fp32 is off by at most c(n) x the sum of the terms' absolute values: n / 32 accumulations of the
+    matrix instruction with up to 32 roundings inside (n + 64 in all, counted fully: c(n) = (n + 64) x 2^-24).  fp32 data: three parts lose three
+    products of at most 2^-23 each, and add six times the accumulations.  Every |.| below is of the exact values."""
+    dt = x.dtype
+    M, K, F = x.numel() // x.shape[-1], x.shape[-1], wg.shape[0]
+    dh = torch.randn(x.shape[:-1] + (F,), generator=gen(seed + 5), device="cuda").to(dt)
+    many = 6 if dt == torch.float32 else 1
+    c = lambda n: (many * n + 64) * F32 + (3 * 2.0 ** -23 if many > 1 else 0)  # noqa: E731
+    params = [x, wg, wu, bg, bu]
+    leaves = [None if t is None else t.detach().requires_grad_() for t in params]
+    h = ops.gated_mlp(*leaves, act=act)
+    assert h.dtype == dt and h.shape == x.shape[:-1] + (F,)
+    with torch.no_grad():
+        assert torch.equal(ops.gated_mlp(*params, act=act), h)
+    live = [t for t in leaves if t is not None]
+    got = dict(zip([n for n, t in zip(("x", "wg", "wu", "bg", "bu"), leaves) if t is not None], torch.autograd.grad(h, live, dh)))
+    X, WG, WU, DH = x.double().reshape(M, K), wg.double(), wu.double(), dh.double().reshape(M, F)
+    G, U = X @ WG.t(), X @ WU.t()
+    eG, eU = c(K) * (X.abs() @ WG.abs().t()), c(K) * (X.abs() @ WU.abs().t())
+    if bg is not None:
+        G, eG = G + bg.double(), eG + F32 * (G.abs() + bg.double().abs())
+    if bu is not None:
+        U, eU = U + bu.double(), eU + F32 * (U.abs() + bu.double().abs())
+    v, dv = gate_reference(G, act)
+    # the activations: |act'| <= 1.13, |act''| <= 1; v_exp_f32 and v_rcp_f32 on g to 2^-24 (|g| + 4) relative of the sigmoid; erff, expf a few places
+    rel = (16 + 2 * G.abs()) * F32
+    ev = 1.13 * eG + rel * v.abs() + (16 * F32 * G.abs() if act == "gelu" else 0)
+    edv = eG + rel * (dv.abs() + 1)
+    within(h.reshape(M, F), v * U, half_step(dt, v * U) + 1.001 * (ev * U.abs() + eU * v.abs() + ev * eU) + 2 * F32 * (v * U).abs())
+    dG, dU = DH * U * dv, DH * v
+    # rounded once to operands (fp32: kept to 2^-23 by their parts)
+    step = (lambda t: half_step(dt, t)) if many == 1 else (lambda t: 2.0 ** -23 * t.abs())
+    edG = DH.abs() * (eU * dv.abs() + edv * U.abs() + eU * edv) + 4 * F32 * dG.abs()
+    edU = DH.abs() * ev + 4 * F32 * dU.abs()
+    rG, rU = edG + 1.01 * step(dG.abs() + edG), edU + 1.01 * step(dU.abs() + edU)
+    dx = dG @ WG + dU @ WU
+    tx = rG @ WG.abs() + rU @ WU.abs() + c(2 * F) * (dG.abs() @ WG.abs() + dU.abs() @ WU.abs())
+    within(got["x"].reshape(M, K), dx, half_step(dt, dx) + 1.01 * tx)
+    for n, d, r in (("wg", dG, rG), ("wu", dU, rU)):
+        w = d.t() @ X
+        within(got[n], w, half_step(dt, w) + 1.01 * (r.t() @ X.abs() + c(M) * (d.abs().t() @ X.abs())))
+    for n, d, e in (("bg", dG, edG), ("bu", dU, edU)):
+        if n in got:
+            within(got[n], d.sum(0), half_step(dt, d.sum(0)) + 1.01 * (e.sum(0) + (64 + M / 64) * F32 * d.abs().sum(0)))
+    return h, got
+
+
+def mlp_inputs(M, K, F, dtype, seed, bias):
+    g = gen(seed)
+    n = lambda *s, scale=1.0: (torch.randn(*s, generator=g, device="cuda") * scale).to(dtype)  # noqa: E731
+    x, wg, wu = n(M, K), n(F, K, scale=K ** -0.5), n(F, K, scale=K ** -0.5)
+    return x, wg, wu, n(F, scale=0.2) if bias else None, n(F, scale=0.2) if bias else None
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M, K, F, act, bias", [(1, 1, 1, "silu", True), (1, 64, 64, "gelu", False), (3, 40, 17, "sigmoid", True), (16, 33, 100, "silu", False),
+                                                (17, 128, 48, "gelu", True), (33, 100, 130, "silu", True), (64, 72, 31, "sigmoid", False), (65, 32, 64, "silu", True),
+                                                (65, 31, 65, "gelu", True), (127, 64, 63, "silu", False), (128, 96, 128, "gelu", False), (129, 160, 129, "sigmoid", True),
+                                                (300, 1000, 70, "silu", True), (1030, 48, 258, "gelu", True), (4100, 64, 40, "silu", False), (70, 520, 2050, "gelu", False)])
+def test_gated_mlp_and_its_gradients(ops, dtype, M, K, F, act, bias):
+    mlp_check(ops, *mlp_inputs(M, K, F, dtype, M + K + F, bias), act)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_mlp_in_large_tiles(ops, dtype):
+    """Enough rows and columns for the 256 x 256 tiles in all three products, with edges in both axes."""
+    mlp_check(ops, *mlp_inputs(4229, 4130, 2060, dtype, 1, True), "silu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [5, 200])
+@pytest.mark.parametrize("kind", ["columns", "odd columns", "every second row", "three axes", "transposed", "weights transposed", "one bias"])
+def test_gated_mlp_takes_strided_inputs(ops, dtype, rows, kind):
+    x, wg, wu, bg, bu = mlp_inputs(rows, 96, 72, dtype, 3, True)
+    g = gen(4)
+    base = torch.randn(2 * rows, 160, generator=g, device="cuda").to(dtype)
+    if kind == "columns":
+        x = base[:rows, 32:128]
+    elif kind == "odd columns":
+        x = base[:rows, 3:99]
+    elif kind == "every second row":
+        x = base[::2, :96]
+    elif kind == "three axes":
+        x = base[:rows].reshape(rows, 1, 160)[:, :, :96].expand(rows, 2, 96)
+    elif kind == "transposed":
+        x = torch.randn(96, rows, generator=g, device="cuda").to(dtype).t()
+    elif kind == "weights transposed":
+        wg = torch.randn(96, 72, generator=g, device="cuda").to(dtype).t()
+    else:
+        bg = None
+    mlp_check(ops, x, wg, wu, bg, bu, "silu")
+
+
+def test_gated_mlp_keeps_bad_rows_to_themselves_and_takes_none(ops):
+    for rows in (40, 300):
+        x, wg, wu, bg, bu = mlp_inputs(rows, 128, 96, torch.float32, 6, True)
+        want = ops.gated_mlp(x, wg, wu, bg, bu)
+        bad = x.clone()
+        bad[3, 7], bad[20, 127] = math.inf, math.nan
+        got = ops.gated_mlp(bad, wg, wu, bg, bu)
+        rest = [i for i in range(rows) if i not in (3, 20)]
+        assert torch.equal(got[rest], want[rest])
+        assert not torch.isfinite(got[3]).all() and torch.isnan(got[20]).all()
+    x = torch.empty(2, 0, 128, device="cuda", requires_grad=True)
+    w = wg.detach().requires_grad_()
+    h = ops.gated_mlp(x, w, wu)
+    dx, dw = torch.autograd.grad(h, (x, w), torch.empty_like(h))
+    assert h.shape == (2, 0, 96) and dx.shape == x.shape and torch.equal(dw, torch.zeros_like(dw))
+
+
+def test_gated_mlp_of_fp32_spans_its_magnitudes(ops):
+    """The three parts carry 24 bits at any exponent: rows of 1e-20 and of 1e+15 beside one another."""
+    x, wg, wu, _, _ = mlp_inputs(200, 64, 64, torch.float32, 9, False)
+    scale = torch.logspace(-20, 15, 200, device="cuda")[:, None]
+    h = ops.gated_mlp(x * scale, wg, wu, act="sigmoid")
+    X = (x * scale).double()
+    G, U = X @ wg.double().t(), X @ wu.double().t()
+    s = torch.sigmoid(G)
+    size = X.abs() @ wu.double().abs().t()
+    eG = (7 * 64 + 64) * F32 * (X.abs() @ wg.double().abs().t())
+    # the sigmoid moves by its own derivative over G's error, and by its relative error where it is small (underflows: below 1e-38)
+    lo, hi = torch.sigmoid(G - eG), torch.sigmoid(G + eG)
+    within(h, s * U, 1.01 * ((hi - lo) * U.abs() + (16 + 2 * G.abs().clamp_max(100)) * F32 * (s * U).abs() + (7 * 64 + 64) * F32 * size * hi) + 1e-37 * U.abs() + 1e-38)
+
+
+def test_gated_mlp_gradient_against_differences(ops):
+    g = gen(13)
+    params = [t.requires_grad_() for t in mlp_inputs(100, 48, 40, torch.float32, 12, True)]
+    dh = torch.randn(100, 40, generator=g, device="cuda")
+    grads = torch.autograd.grad(ops.gated_mlp(*params, act="gelu"), params, dh)
+    with torch.no_grad():
+        for i, t in enumerate(params):
+            way = torch.randn(t.shape, generator=g, device="cuda") * (48 ** -0.5 if t.dim() == 2 and i else 1)
+            h = 2.0 ** -6
+            f = [float((ops.gated_mlp(*[v + s * h * way if j == i else v for j, v in enumerate(params)], act="gelu").double() * dh.double()).sum()) for s in (1, -1)]
+            got, want = (f[0] - f[1]) / (2 * h), float((grads[i].double() * way.double()).sum())
+            # third differences of act(g) u along a way of order 1 in g and u are of order 10; values of order 10 rounded at c(48)
+            size = float(dh.abs().sum()) * 10
+            assert abs(got - want) <= size * (h * h / 6 + (6 * 48 + 64) * F32 / h), (i, got, want)
+
+
+def test_gated_mlp_gives_the_same_bits_every_time_on_any_stream_and_in_a_graph(ops):
+    side = torch.cuda.Stream()
+    for shape, dtype in (((500, 200, 136), torch.bfloat16), ((3000, 64, 96), torch.float32), ((9, 64, 96), torch.float16)):
+        leaves = [t.requires_grad_() for t in mlp_inputs(*shape, dtype, 2, True)]
+        dh = torch.ones(shape[0], shape[2], device="cuda", dtype=dtype)
+
+        def step():
+            h = ops.gated_mlp(*leaves)
+            return (h.detach(),) + torch.autograd.grad(h, leaves, dh)
+        want = [t.clone() for t in step()]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, b) for a, b in zip(other, want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = step()
+        for k in range(3):
+            for t in held:
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(held, want)), k
+            assert all(torch.equal(a, b) for a, b in zip(step(), want)), k
+            torch.cuda.synchronize()
+
+
+def test_gated_mlp_gradients_of_some_tensors_only(ops):
+    for which in ("x", "wg", "wu", "bg", "bu"):
+        tensors = dict(zip(("x", "wg", "wu", "bg", "bu"), mlp_inputs(130, 64, 72, torch.bfloat16, 8, True)))
+        full = mlp_check(ops, *tensors.values(), "silu")[1]
+        tensors[which].requires_grad_()
+        h = ops.gated_mlp(*tensors.values())
+        dh = torch.randn(130, 72, generator=gen(5), device="cuda").to(torch.bfloat16)
+        assert torch.equal(torch.autograd.grad(h, tensors[which], dh)[0], full[which]), which
