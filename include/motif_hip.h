@@ -423,8 +423,8 @@ int motif_gru_scan_bwd(const void* z, long z_bs, long z_rs, const void* q, long 
 
 /* Gated feed-forward block: h = act(x Wg^T + bg) * (x Wu^T + bu), both projections, the activation and the product in one kernel.
  * x [M, K] with row stride x_rs, w_gate / w_up [F, K] dense, b_gate / b_up [F] (may be NULL), h [M, F] dense, all of one type; sums are fp32
- * (fp32 data: the products of three exact bf16 parts, six per multiplication).  G, U [M, F] fp32 (both or neither): the two projections with
- * their biases, kept for the backward pass.  K, F <= 65536, M <= 4194304.  workspace: motif_gated_mlp_ws_bytes bytes for the same arguments at 256-byte
+ * (fp32 data: the products of three exact bf16 parts, six per multiplication).  G, U fp32, M rows of F rounded up to 8, at 16-byte
+ * addresses (both or neither): the two projections with their biases, kept for the backward pass (what lies behind F is not read).  K, F <= 65536, M <= 4194304.  workspace: motif_gated_mlp_ws_bytes bytes for the same arguments at 256-byte
  * addresses (NULL where that is 0); no clearing needed. */
 #define MOTIF_GATE_SIGMOID 0
 #define MOTIF_GATE_SILU 1
@@ -433,8 +433,8 @@ long motif_gated_mlp_ws_bytes(const void* x, long x_rs, const void* w_gate, cons
 int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* h, float* G, float* U,
                         void* workspace, long M, long K, long F, int act, int dtype, void* stream);
 /* Its backward pass from G and U: dx [M, K] dense (may be NULL), dw_gate and dw_up [F, K] (both or neither), db_gate / db_up [F] (either may be
- * NULL).  workspace: motif_gated_mlp_bwd_ws_bytes bytes for the gradients that are wanted. */
-long motif_gated_mlp_bwd_ws_bytes(long M, long K, long F, int dtype, int need_x, int need_w, int need_b);
+ * NULL).  workspace: motif_gated_mlp_bwd_ws_bytes bytes for the same inputs and the gradients that are wanted. */
+long motif_gated_mlp_bwd_ws_bytes(const void* x, long x_rs, const void* w_gate, const void* w_up, long M, long K, long F, int dtype, int need_x, int need_w, int need_b);
 int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate, const void* w_up, const float* G, const float* U, const void* dh, long dh_rs,
                         void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* workspace, long M, long K, long F, int act, int dtype, void* stream);
 

@@ -5,11 +5,12 @@
 //              dx = dG Wg + dU Wu,   dWg = dG^T x,  dWu = dU^T x,   dbg, dbu = sums of dG, dU over the rows
 //
 // Three matrix products with two right-hand sides each, all bound by the matrix cores from a few hundred rows on.  One kernel serves them
-// (gemm_kernel): C = sum over segments of A_s B_s^T with both operands' reduction axis dense, and a tile's columns in two halves that come
-// from two matrices -- the gate's and the up projection's (forward: the same columns of both, so that a wave holds G and U of the same
-// outputs in its accumulators; weights' gradients: dG^T and dU^T), or the two neighbouring runs of one (dx).  fp32 runs on the same
-// kernel: every operand is split exactly into three bf16 parts and the six products that reach fp32's last place are six segments of the
-// reduction.  Operands whose reduction axis is not dense, or not a multiple of 32, are laid out first (layout_kernel).
+// (gemm_kernel): C = sum over segments of A_s B_s with a tile's columns in two halves that come from two matrices -- the gate's and the up
+// projection's (forward: the same columns of both, so that a wave holds G and U of the same outputs in its accumulators; weights'
+// gradients: dG and dU) -- or are the two neighbouring runs of one (dx).  Either operand may lie with its reduction axis dense or across
+// (transposed on the way from LDS to the registers), so every tensor is read as it lies.  fp32 runs on the same kernel: every operand is
+// split exactly into three bf16 parts, and the six products that reach fp32's last place are six segments of the reduction.  Operands
+// whose rows are not whole 16-byte pieces are laid out first (layout_kernel).
 // G and U are kept in fp32 for the backward pass: rounded to the data's type they would add an error of their own to every gradient; dG and
 // dU are rounded once, to be operands of the matrix cores.
 // Up to 64 rows the forward pass is bound by reading the weights (rows_kernel).
@@ -48,23 +49,27 @@ __device__ __forceinline__ void gate_grad(float g, int act, float& v, float& d) 
 }
 
 // ---- the matrix product ------------------------------------------------------------------------------------------------------------------
+// GATED  h = act(A B0^T + bias0) * (A B1^T + bias1), G and U to keep         A [M][K], B0, B1 [N][K]
+// ONE    C = sum of A_s B_s                                                  A [M][K], B [K][N]: the halves are neighbouring columns of it
+// TWO    C0^T = A^T B0, C1^T = A^T B1                                        A [K][M], B0, B1 [K][N], C0, C1 [N][M]: a lane then holds four
+//                                                                           consecutive rows of A, the matrix instruction takes its operands the other way round
+enum GemmMode { GATED, ONE, TWO };
 struct GemmArgs {
-    const void* a[kSegs];                                // rows of A: [M][lda], reduction axis dense
-    const void* b0[kSegs];                               // the two halves' rows: [N][ldb]
+    const void* a[kSegs];
+    const void* b0[kSegs];
     const void* b1[kSegs];
-    long lda, ldb;                                       // in elements
+    long lda, ldb;                                       // in elements, multiples of 8
     int nseg, steps;                                     // segments; reduction steps of 32 in each
-    int M, N;                                            // rows of A, of the B matrices
+    int ka, kb;                                          // reduction length of either operand's tensors: what lies behind it counts as zeros
+    int M, N, wa, wb;                                    // output rows / columns of either half; ONE, TWO: columns of B, of A that may be read (multiples of 8)
     int tiles_m, tiles_n, splits, steps_per_split;
-    void *c0, *c1;                                       // outputs of type dtype: GATED h [M][N], ONE C [M][N], TWO C0, C1 [N][M]
-    float *g, *u;                                        // GATED: G and U to keep (may be null)
+    void *c0, *c1;                                       // outputs of type dtype, dense
+    float *g, *u;                                        // GATED: [M][ldg], may be null
+    long ldg;
     const void *bias0, *bias1;
     float* part;                                         // split reduction, fp32 instead of the outputs: ONE [split][M][N], TWO [split][2][N][M]
     int act, dtype, vec;                                 // vec: rows of the outputs allow runs of four values
 };
-// GATED: the halves are the same columns of two matrices, combined.  ONE: neighbouring columns of one matrix.  TWO: the same columns of two
-// matrices, written transposed (a lane then holds four consecutive rows of A: the matrix instruction takes its operands the other way round).
-enum GemmMode { GATED, ONE, TWO };
 
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, bf16_t*) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -73,11 +78,16 @@ __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, f16_t*) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// 64 lanes x 16 bytes from global memory to `lds` .. + 1024: base + off of each lane.  Written as assembly so that the compiler does not make
-// every LDS read wait for all of them (it takes any for the one that fills what is read); the waits are counted by hand in the kernel.
+// 64 lanes x 16 bytes from global memory to `lds` .. + 1024: base + off of each lane, or an address of its own.  Written as assembly so that the
+// compiler does not make every LDS read wait for all of them (it takes any for the one that fills what is read); the waits are counted by
+// hand in the kernel.
 __device__ __forceinline__ void to_lds(unsigned lds, const void* base, unsigned off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
+__device__ __forceinline__ void to_lds(unsigned lds, const void* own) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(own) : "memory", "m0");
+}
+__device__ u32x4 g_zeros;                                // what lies behind the end of a reduction
 
 template <typename T, typename O, int N>
 __device__ __forceinline__ void store_run(void* p, long at, const float (&v)[N], int n, bool vec) {      // n of N values; whole aligned runs as one store
@@ -94,16 +104,56 @@ __device__ __forceinline__ void store_as(void* p, long at, const float (&v)[N], 
     else store_run<f16_t, f16_t, N>(p, at, v, n, vec);
 }
 
-// Tile BM rows of A x BN / 2 rows of either half, WM x WN waves.  The reduction advances in steps of 32: a stage holds 64 bytes of every row, its
-// four 16-byte pieces exchanged by a pattern of the row's number so that the 16 rows of a fragment lie in different banks; four stages lie in
-// LDS, three of them requested ahead of the one that is multiplied, one barrier a step: behind it every wave has finished the stage that the
-// next request overwrites.
-template <typename T, int BM, int BN, int WM, int WN, GemmMode MODE>
-__global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(GemmArgs p) {
-    constexpr int NW = WM * WN, MF = BM / WM / 16, HF = BN / 2 / WN / 16;        // fragments of a wave: rows, columns of either half
-    constexpr int STAGE = (BM + BN) * 64, STAGES = 4;
-    static_assert(BM / 16 == 2 * NW && BN / 16 == 2 * NW, "each wave requests two pieces of 16 rows of either operand per stage");
-    __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
+// One operand of a tile: two blocks of C rows (of the output), 32 steps of the reduction deep, 64 C bytes each.  A wave requests one piece of 1 KB
+// of either block per stage.
+//   dense     [C][32]: a piece is 16 rows of 64 bytes, a lane's 16 bytes the steps 8 j .. 8 j + 7 of its row.  The four pieces of a row are
+//             exchanged by a pattern of the row's number, so that the 16 rows x 16 bytes of a fragment's read lie in different banks.
+//   across    [32][C]: a piece is 2 C bytes of 4 (C = 128) or 8 steps.  A fragment's read takes 32 bytes (16 rows) of 16 steps and turns them
+//             in 4 x 4 steps (ds_read_b64_tr_b16: lane i of 16 gets row i of four steps); 32-byte units are exchanged by a pattern of the step.
+template <bool ACROSS, int C>
+struct Operand {
+    static constexpr int kUnits = C / 16, kPieces = C / 8;                       // of an across row
+    static __device__ __forceinline__ int dense_swap(int row) { return (((row >> 1) ^ (row >> 3)) & 1) | (((row >> 2) & 1) << 1); }
+    static __device__ __forceinline__ int across_swap(int k) { return C == 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2); }
+    // this lane's first step of a stage and its byte offset from (row `at` of the matrix, step 0), rows up to `most`
+    static __device__ __forceinline__ void lane_of(int wave, int lane, int first, int at, int most, long ld, int& step, unsigned& off) {
+        if (!ACROSS) {
+            const int r = lane >> 2;
+            step = ((lane & 3) ^ dense_swap(r)) * 8;
+            off = (unsigned)(min(first + wave * 16 + r, most - 1) - at) * (unsigned)ld * 2u + (unsigned)step * 2u;
+        } else {
+            const int k = wave * (64 / kPieces) + lane / kPieces, c = lane % kPieces;
+            step = k;
+            off = (unsigned)k * (unsigned)ld * 2u + (unsigned)(min(first + (((c >> 1) ^ across_swap(k)) * 2 + (c & 1)) * 8, most - 8) - at) * 2u;
+        }
+    }
+    // this lane's byte of the fragment of rows `row` .. + 15 in a block (dense: + 1024 per 16 rows; across: the unit is part of the pattern)
+    static __device__ __forceinline__ int frag_of(int lane) {
+        if (!ACROSS) return (lane & 15) * 64 + (((lane >> 4) ^ dense_swap(lane & 15)) * 16);
+        return ((lane >> 4) * 8 + ((lane & 15) >> 2)) * (2 * C) + (lane & 3) * 8;
+    }
+    static __device__ __forceinline__ s16x8 read(const char* block, int frag, int row, int lane) {
+        if constexpr (!ACROSS) return *(const s16x8*)(block + frag + row * 64);
+        else {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* P;
+            // the second four steps have the same pattern (it does not depend on bit 2 of the step)
+            const int unit = ((row >> 4) ^ across_swap((lane >> 4) * 8 + ((lane & 15) >> 2))) * 32;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(block + frag + unit)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(block + frag + unit + 8 * C));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+// Tile 2 C rows of A x C columns of either half of B; C / 16 waves (two along A), each C x 32 x 2 outputs.  The reduction advances in steps of 32:
+// four stages lie in LDS, three of them on their way, and a step's fragments are read from LDS while the step before is multiplied: one barrier
+// a step, behind which the next step's stage is whole and the current one's place free (every wave has its fragments in registers).
+template <typename T, int C, GemmMode MODE>
+__global__ __launch_bounds__(C * 4) void gemm_kernel(GemmArgs p) {
+    constexpr int NW = C / 16, WN = NW / 2, MF = C / 16, HF = 2, BLOCK = C * 64, STAGE = 4 * BLOCK;
+    using A = Operand<MODE == TWO, C>;
+    using B = Operand<MODE != GATED, C>;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
@@ -118,38 +168,47 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(GemmArgs p) {
         id = xcd * q + (xcd < r ? xcd : r) + (id >> 3);
     }
     const int band = id / (8 * p.tiles_n), in = id - band * 8 * p.tiles_n, bh = min(8, p.tiles_m - band * 8);
-    const int m0 = (band * 8 + in % bh) * BM, tn = in / bh;
-    const int n0[2] = {tn * (MODE == ONE ? BN : BN / 2), MODE == ONE ? tn * BN + BN / 2 : tn * (BN / 2)};
-    const int nb[2] = {n0[0], min(n0[1], p.N - 1)};      // where the halves' pointers stand: a row that exists
+    const int m0 = (band * 8 + in % bh) * 2 * C, tn = in / bh;
+    const int n0[2] = {tn * (MODE == ONE ? 2 * C : C), MODE == ONE ? tn * 2 * C + C : tn * C};
+    const int am = MODE == TWO ? p.wa : p.M, bm = MODE != GATED ? p.wb : p.N;      // rows (columns) that may be read
+    const int bat[2] = {n0[0], min(n0[1], bm - 8 < 0 ? 0 : bm - 8)};              // where the halves' pointers stand
 
-    // this lane's share of a request: LDS row (lane >> 2) of the piece, position lane & 3
-    const int lr = lane >> 2, lp = lane & 3;
-    const int sw = ((lr >> 1) & 1) ^ ((lr >> 3) & 1) | (((lr >> 2) & 1) << 1);
     unsigned offa[2], offb[2];
+    int ka[2], kb[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = (i * NW + wave) * 16 + lr;
-        offa[i] = (unsigned)(min(row, p.M - 1 - m0) * (unsigned)p.lda * 2u) + (unsigned)((lp ^ sw) * 16);
-        offb[i] = (unsigned)((min(n0[i] + wave * 16 + lr, p.N - 1) - nb[i]) * (unsigned)p.ldb * 2u) + (unsigned)((lp ^ sw) * 16);      // half i
+    for (int h = 0; h < 2; ++h) {
+        A::lane_of(wave, lane, m0 + h * C, m0, am, p.lda, ka[h], offa[h]);
+        B::lane_of(wave, lane, n0[h], bat[h], bm, p.ldb, kb[h], offb[h]);
     }
-    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds;
+    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds + wave * 1024;
+    const long stepa = MODE == TWO ? 64 * p.lda : 64, stepb = MODE != GATED ? 64 * p.ldb : 64;      // bytes per step
+    const int enda = p.ka - (p.steps - 1) * 32, endb = p.kb - (p.steps - 1) * 32;  // what the last step of a segment holds
+    const bool ragged = enda < 32 || endb < 32;
 
     const int s_begin = split * p.steps_per_split, s_end = min(p.nseg * p.steps, s_begin + p.steps_per_split), count = s_end - s_begin;
     int seg = s_begin / p.steps, left = p.steps - (s_begin - seg * p.steps);      // steps left in the segment that is requested
     const char *pa, *pb0, *pb1;
     auto segment = [&](int step) __attribute__((always_inline)) {
-        pa = (const char*)p.a[seg] + ((long)m0 * p.lda + (long)step * 32) * 2;
-        pb0 = (const char*)p.b0[seg] + ((long)nb[0] * p.ldb + (long)step * 32) * 2;
-        pb1 = (const char*)p.b1[seg] + ((long)nb[1] * p.ldb + (long)step * 32) * 2;
+        pa = (const char*)p.a[seg] + (MODE == TWO ? m0 : (long)m0 * p.lda) * 2 + step * stepa;
+        pb0 = (const char*)p.b0[seg] + (MODE != GATED ? bat[0] : (long)bat[0] * p.ldb) * 2 + step * stepb;
+        pb1 = (const char*)p.b1[seg] + (MODE != GATED ? bat[1] : (long)bat[1] * p.ldb) * 2 + step * stepb;
     };
     segment(s_begin - seg * p.steps);
     auto request = [&](int stage) __attribute__((always_inline)) {
-        const unsigned at = lds0 + stage * STAGE + wave * 1024;
-        to_lds(at, pa, offa[0]);
-        to_lds(at + NW * 1024, pa, offa[1]);
-        to_lds(at + BM * 64, pb0, offb[0]);
-        to_lds(at + BM * 64 + NW * 1024, pb1, offb[1]);
-        pa += 64; pb0 += 64; pb1 += 64;
+        const unsigned at = lds0 + stage * STAGE;
+        if (ragged && left == 1) {
+            const char* zeros = (const char*)&g_zeros;
+            to_lds(at, ka[0] < enda ? pa + offa[0] : zeros);
+            to_lds(at + BLOCK, ka[1] < enda ? pa + offa[1] : zeros);
+            to_lds(at + 2 * BLOCK, kb[0] < endb ? pb0 + offb[0] : zeros);
+            to_lds(at + 3 * BLOCK, kb[1] < endb ? pb1 + offb[1] : zeros);
+        } else {
+            to_lds(at, pa, offa[0]);
+            to_lds(at + BLOCK, pa, offa[1]);
+            to_lds(at + 2 * BLOCK, pb0, offb[0]);
+            to_lds(at + 3 * BLOCK, pb1, offb[1]);
+        }
+        pa += stepa; pb0 += stepb; pb1 += stepb;
         if (--left == 0 && seg + 1 < p.nseg) { ++seg; left = p.steps; segment(0); }
     };
 
@@ -161,34 +220,48 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(GemmArgs p) {
 #pragma unroll
             for (int j = 0; j < HF; ++j) acc[i][h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // a fragment: row lane & 15, the 8 values of piece lane >> 4
-    const int fr = lane & 15, fs = ((fr >> 1) & 1) ^ ((fr >> 3) & 1) | (((fr >> 2) & 1) << 1);
-    const int frag = fr * 64 + (((lane >> 4) ^ fs) * 16);
-    const int fa = wm * MF * 1024 + frag, fb = BM * 64 + wn * HF * 1024 + frag;
-
-    for (int s = 0; s < 3 && s < count; ++s) request(s);
-    for (int s = 0; s < count; ++s) {
-        // the stages requested behind this one may still be on their way (four requests each); then everybody's part of it is there
-        if (s + 2 < count) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-        else if (s + 1 < count) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (s + 3 < count) request((s + 3) & 3);
-        const char* st = lds + (s & 3) * STAGE;
-        s16x8 av[MF], bv[2][HF];
+    struct Frags { s16x8 a[MF], b[2][HF]; };
+    const int fa = A::frag_of(lane), fb = B::frag_of(lane);
+    auto fetch = [&](Frags& f, int stage) __attribute__((always_inline)) {
+        const char* st = lds + stage * STAGE;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < HF; ++j) bv[h][j] = *(const s16x8*)(st + fb + (h * (BN / 2) + j * 16) * 64);
+            for (int j = 0; j < HF; ++j) f.b[h][j] = B::read(st + (2 + h) * BLOCK, fb, wn * 32 + j * 16, lane);
 #pragma unroll
-        for (int i = 0; i < MF; ++i) av[i] = *(const s16x8*)(st + fa + i * 1024);
+        for (int i = 0; i < MF; ++i) f.a[i] = A::read(st + wm * BLOCK, fa, i * 16, lane);
+    };
+    // the requests behind stage s + 1 may still be on their way, four each; then everybody's part of it is there
+    auto arrive = [&](int behind) __attribute__((always_inline)) {
+        if (behind >= 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else if (behind == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto step = [&](int s, const Frags& now, Frags& next) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        arrive(count - 2 - s);
+        if (s + 4 < count) request(s & 3);
+        if (s + 1 < count) fetch(next, (s + 1) & 3);
 #pragma unroll
         for (int i = 0; i < MF; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < HF; ++j) acc[i][h][j] = MODE != TWO ? mfma(bv[h][j], av[i], acc[i][h][j], (T*)nullptr) : mfma(av[i], bv[h][j], acc[i][h][j], (T*)nullptr);
+                for (int j = 0; j < HF; ++j) acc[i][h][j] = MODE != TWO ? mfma(now.b[h][j], now.a[i], acc[i][h][j], (T*)nullptr) : mfma(now.a[i], now.b[h][j], acc[i][h][j], (T*)nullptr);
+    };
+
+    for (int s = 0; s < 4 && s < count; ++s) request(s);
+    if (count >= 4) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    Frags f0, f1;
+    fetch(f0, 0);
+    for (int s = 0; s < count; s += 2) {
+        step(s, f0, f1);
+        if (s + 1 < count) step(s + 1, f1, f0);
     }
 
     const int lo = lane & 15, hi = (lane >> 4) * 4;
@@ -196,7 +269,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(GemmArgs p) {
     for (int i = 0; i < MF; ++i) {
 #pragma unroll
         for (int j = 0; j < HF; ++j) {
-            const int mt = m0 + (wm * MF + i) * 16, off = (wn * HF + j) * 16;
+            const int mt = m0 + wm * C + i * 16, off = wn * 32 + j * 16;
             if constexpr (MODE == GATED) {
                 const int m = mt + lo, n = n0[0] + off + hi, cnt = min(4, p.N - n);
                 if (m >= p.M || cnt <= 0) continue;
@@ -210,7 +283,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(GemmArgs p) {
                 }
                 const long at = (long)m * p.N + n;
                 store_as<4>(p.c0, at, v, cnt, p.vec, p.dtype);
-                if (p.g) { store_run<float, float, 4>(p.g, at, g, cnt, p.vec); store_run<float, float, 4>(p.u, at, u, cnt, p.vec); }
+                if (p.g) {                               // (their rows are padded to whole runs)
+                    seq_store16<float, 4>(p.g + m * p.ldg + n, g);
+                    seq_store16<float, 4>(p.u + m * p.ldg + n, u);
+                }
             } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -254,77 +330,85 @@ __device__ __forceinline__ void split3(float x, bf16_t (&out)[3]) {
     // a NaN whose payload lies in the lower half only must not become an infinity
     if (x != x) out[0] = __builtin_bit_cast(bf16_t, (unsigned short)0x7fc0);
 }
-// value v of a [rows][ld] image at (r, c): one plane of T, or three of bf16, `plane` elements apart
-__device__ __forceinline__ void put(float* /*type*/, void* dst, long plane, long at, float v) {
-    bf16_t s[3];
-    split3(v, s);
+// eight values: one plane of T, or three of bf16, `plane` elements apart
+__device__ __forceinline__ void put8(float* /*type*/, void* dst, long plane, long at, const float (&v)[8]) {
+    SeqVec<bf16_t, 8> o[3];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) ((bf16_t*)dst)[i * plane + at] = s[i];
-}
-__device__ __forceinline__ void put(bf16_t*, void* dst, long, long at, float v) { ((bf16_t*)dst)[at] = (bf16_t)v; }
-__device__ __forceinline__ void put(f16_t*, void* dst, long, long at, float v) { ((f16_t*)dst)[at] = (f16_t)v; }
-
-// src [rows][cols] with row stride rs -> as it lies (dst: rows of ld, may be null) and transposed (tdst: cols of tld, may be null), zeros behind the
-// last value of every row.  64 x 64 values per workgroup; the grid covers ld and tld.
-template <typename T>
-__global__ __launch_bounds__(256) void layout_kernel(const T* __restrict__ src, long rs, int rows, int cols, void* dst, long plane, int ld, void* tdst, long tplane, int tld) {
-    __shared__ float sh[64][65];
-    const int c0 = blockIdx.y * 64, r0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    for (int i = y; i < 64; i += 4) {
-        const int r = r0 + i, c = c0 + x;
-        const float v = r < rows && c < cols ? (float)src[(long)r * rs + c] : 0.f;
-        if (dst && r < rows && c < ld) put((T*)nullptr, dst, plane, (long)r * ld + c, v);
-        sh[i][x] = v;
+    for (int e = 0; e < 8; ++e) {
+        bf16_t s[3];
+        split3(v[e], s);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) o[i].v[e] = s[i];
     }
-    if (!tdst) return;
-    __syncthreads();
-    for (int i = y; i < 64; i += 4) {
-        const int c = c0 + i, r = r0 + x;
-        if (c < cols && r < tld) put((T*)nullptr, tdst, tplane, (long)c * tld + r, sh[x][i]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *(SeqVec<bf16_t, 8>*)((bf16_t*)dst + i * plane + at) = o[i];
+}
+__device__ __forceinline__ void put8(bf16_t*, void* dst, long, long at, const float (&v)[8]) { seq_store16<bf16_t, 8>((bf16_t*)dst + at, v); }
+__device__ __forceinline__ void put8(f16_t*, void* dst, long, long at, const float (&v)[8]) { seq_store16<f16_t, 8>((f16_t*)dst + at, v); }
+
+// src [rows][cols] with row stride rs -> dst rows of ld = cols rounded up to 8, zeros behind the last value of a row.  Eight values per thread.
+template <typename T>
+__global__ __launch_bounds__(256) void layout_kernel(const T* __restrict__ src, long rs, int rows, int cols, void* dst, long plane, int ld) {
+    const int per = ld / 8;
+    const long n = (long)rows * per;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+        const long r = i / per;
+        const int c = (int)(i - r * per) * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? (float)src[r * rs + c + e] : 0.f;
+        put8((T*)nullptr, dst, plane, r * ld + c, v);
     }
 }
 
-// dG and dU of 64 rows x 64 columns: as they lie (dst: [rows][ld], dU `pair` elements behind dG), transposed (tdst: [F][tld], `tpair`), and summed over
-// the 64 rows (part [row blocks][2 F], may be null).  fp32: three planes, `plane` / `tplane` apart.
-template <typename T>
-__global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh, long dhs, const float* __restrict__ G, const float* __restrict__ U, int M, int F, int act,
-                                                       void* dst, long plane, long pair, int ld, void* tdst, long tplane, long tpair, int tld, float* part) {
+// dG and dU: [rows][ld], ld = F rounded up to 8 (G and U have it too), zeros behind F; fp32: three planes.  dU lies `pair` elements behind dG.
+// A workgroup takes 256 columns x 64 rows, eight columns per thread, and sums its columns over its rows (part [row blocks][2][F], may be null).
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh, long dhs, const float* __restrict__ G, const float* __restrict__ U, int M, int F, int ld, int act,
+                                                       void* dst, long plane, long pair, float* part) {
     using O = std::conditional_t<sizeof(T) == 4, bf16_t, T>;
-    __shared__ float sg[64][65], su[64][65];
-    const int c0 = blockIdx.y * 64, r0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    const int c = c0 + x;
-    for (int i = y; i < 64; i += 4) {
-        const int r = r0 + i;
-        float dg = 0.f, du = 0.f;
-        if (r < M && c < F) {
-            const long at = (long)r * F + c;
-            const float d = (float)dh[r * dhs + c];
-            float v, dv;
-            gate_grad(G[at], act, v, dv);
-            dg = d * U[at] * dv;
-            du = d * v;
-        }
-        sg[i][x] = dg;
-        su[i][x] = du;
-        if (dst && r < M && c < ld) {
-            put((T*)nullptr, dst, plane, (long)r * ld + c, dg);
-            put((T*)nullptr, (O*)dst + pair, plane, (long)r * ld + c, du);
+    __shared__ float sh[8][2][32][9];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.y * 256 + x * 8;
+    const long r0 = (long)blockIdx.x * 64;
+    float sg[8], su[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sg[e] = su[e] = 0.f;
+    if (c < ld) {
+#pragma unroll 2
+        for (int i = y; i < 64; i += 8) {
+            const long r = r0 + i;
+            if (r >= M) break;
+            float d[8], g[8], u[8];
+            if (VEC) seq_load16<T, 8>(dh + r * dhs + c, d);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[e] = c + e < F ? (float)dh[r * dhs + c + e] : 0.f;
+            seq_load16<float, 8>(G + r * ld + c, g);
+            seq_load16<float, 8>(U + r * ld + c, u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float v, dv;
+                gate_grad(g[e], act, v, dv);
+                g[e] = c + e < F ? d[e] * u[e] * dv : 0.f;
+                u[e] = c + e < F ? d[e] * v : 0.f;
+                sg[e] += g[e];
+                su[e] += u[e];
+            }
+            put8((T*)nullptr, dst, plane, r * ld + c, g);
+            put8((T*)nullptr, (O*)dst + pair, plane, r * ld + c, u);
         }
     }
+    if (!part) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { sh[y][0][x][e] = sg[e]; sh[y][1][x][e] = su[e]; }
     __syncthreads();
-    if (tdst)
-        for (int i = y; i < 64; i += 4) {
-            const int cc = c0 + i, r = r0 + x;
-            if (cc < F && r < tld) {
-                put((T*)nullptr, tdst, tplane, (long)cc * tld + r, sg[x][i]);
-                put((T*)nullptr, (O*)tdst + tpair, tplane, (long)cc * tld + r, su[x][i]);
-            }
-        }
-    if (part && y < 2 && c < F) {
+    for (int i = threadIdx.x; i < 512; i += 256) {
+        const int k = i >> 8, cx = i & 255, cc = blockIdx.y * 256 + cx;
+        if (cc >= F) continue;
         float s = 0.f;
-#pragma unroll 8
-        for (int i = 0; i < 64; ++i) s += y ? su[i][x] : sg[i][x];
-        part[((long)blockIdx.x * 2 + y) * F + c] = s;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s += sh[q][k][cx >> 3][cx & 7];
+        part[((long)blockIdx.x * 2 + k) * F + cc] = s;
     }
 }
 
@@ -334,7 +418,7 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
 // the weights' bytes.  fp32 runs on the fp32 matrix instruction.  VEC: every row allows 16-byte reads.
 template <typename T, int MT, bool VEC>
 __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long xs, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ bg, const T* __restrict__ bu,
-                                                   T* __restrict__ h, float* __restrict__ G, float* __restrict__ U, int M, int K, int F, int act) {
+                                                   T* __restrict__ h, float* __restrict__ G, float* __restrict__ U, long ldg, int M, int K, int F, int act) {
     constexpr int V = 16 / sizeof(T), STEP = 4 * V, NW = 8;
     __shared__ float sh[NW][2][16 * MT][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, kq = (lane >> 4) * V;
@@ -401,16 +485,16 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
         for (int w = 0; w < NW; ++w) { g += sh[w][0][m][i & 15]; u += sh[w][1][m][i & 15]; }
         if (bg) g += (float)bg[f];
         if (bu) u += (float)bu[f];
-        const long at = (long)m * F + f;
-        h[at] = (T)(gate<sizeof(T) == 2>(g, act) * u);
-        if (G) { G[at] = g; U[at] = u; }
+        h[(long)m * F + f] = (T)(gate<sizeof(T) == 2>(g, act) * u);
+        if (G) { G[m * ldg + f] = g; U[m * ldg + f] = u; }
     }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 64;
 constexpr long kMostRows = 1L << 22;                    // offsets within a tile are 32 bits: 256 rows x this x 2 bytes
-int up32(long n) { return (int)((n + 31) & ~31L); }
+int up8(long n) { return (int)((n + 7) & ~7L); }
+int steps_of(long n) { return (int)((n + 31) / 32); }
 long up16b(long bytes) { return (bytes + 255) & ~255L; }
 int planes(int dtype) { return dtype == MOTIF_F32 ? 3 : 1; }
 
@@ -425,10 +509,9 @@ struct Image { const void* p; long plane; int ld, n; };
 const void* plane_of(const Image& m, int i) { return (const char*)m.p + (long)i * m.plane * 2; }
 
 template <typename T>
-void layout(const void* src, long rs, int rows, int cols, const Image* as, const Image* tr, hipStream_t s) {
-    const int w = as ? (as->ld > cols ? as->ld : cols) : cols, hgt = tr ? (tr->ld > rows ? tr->ld : rows) : rows;
-    layout_kernel<T><<<dim3(cdiv(hgt, 64), cdiv(w, 64)), 256, 0, s>>>((const T*)src, rs, rows, cols, as ? (void*)as->p : nullptr, as ? as->plane : 0, as ? as->ld : 0,
-                                                                   tr ? (void*)tr->p : nullptr, tr ? tr->plane : 0, tr ? tr->ld : 0);
+void layout(const void* src, long rs, long rows, int cols, const Image& to, hipStream_t s) {
+    const long blocks = (rows * (to.ld / 8) + 255) / 256;
+    layout_kernel<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>((const T*)src, rs, (int)rows, cols, (void*)to.p, to.plane, to.ld);
 }
 
 // The products of two operands' parts that reach fp32's last place, smallest first: 2^-16 each of (0,2) (1,1) (2,0), 2^-8 of (0,1) (1,0), (0,0).
@@ -445,7 +528,7 @@ void segments(GemmArgs& g, const Image& a, const Image& b0, const Image& b1) {
     }
 }
 
-// Tiles of 256 x 256 where they give every CU at least one, else of 128 x 128.  The reduction is split where even those leave CUs without work and
+// Tiles of 256 x 256 (C = 128) where they give every CU at least one, else of 128 x 128.  The reduction is split where even those leave CUs without work and
 // the pieces stay long (16 steps at least); the pieces' sums are fp32 and joined in order.
 struct GemmPlan { bool big; int tiles_m, tiles_n, splits, steps_per_split; };
 GemmPlan gemm_plan(long M, long N, int halves, long total_steps, bool may_split) {
@@ -467,8 +550,8 @@ template <typename T, GemmMode MODE>
 void gemm(const GemmPlan& pl, GemmArgs& g, hipStream_t s) {
     g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n; g.splits = pl.splits; g.steps_per_split = pl.steps_per_split;
     const unsigned grid = (unsigned)((long)pl.tiles_m * pl.tiles_n * pl.splits);
-    if (pl.big) gemm_kernel<T, 256, 256, 2, 4, MODE><<<grid, 512, 0, s>>>(g);
-    else gemm_kernel<T, 128, 128, 2, 2, MODE><<<grid, 256, 0, s>>>(g);
+    if (pl.big) gemm_kernel<T, 128, MODE><<<grid, 512, 0, s>>>(g);
+    else gemm_kernel<T, 64, MODE><<<grid, 256, 0, s>>>(g);
 }
 template <GemmMode MODE>
 void gemm_dtype(int dtype, const GemmPlan& pl, GemmArgs& g, hipStream_t s) {
@@ -476,8 +559,8 @@ void gemm_dtype(int dtype, const GemmPlan& pl, GemmArgs& g, hipStream_t s) {
     else gemm<bf16_t, MODE>(pl, g, s);
 }
 
-// Whether an operand can be read as it lies: 16-bit values, rows of whole steps at 16-byte addresses.
-bool direct(const void* p, long rs, long cols, int dtype) { return dtype != MOTIF_F32 && cols % 32 == 0 && rs % 8 == 0 && rs <= kMostRows && seq_aligned(p, 16); }
+// Whether an operand can be read as it lies: 16-bit values, rows of whole 16-byte pieces at 16-byte addresses.
+bool direct(const void* p, long rs, long cols, int dtype) { return dtype != MOTIF_F32 && cols % 8 == 0 && rs % 8 == 0 && rs <= kMostRows && seq_aligned(p, 16); }
 
 int check_mlp(long M, long K, long F, int act, int dtype) {
     if (M < 0 || K < 1 || F < 1 || !seq_dtype_ok(dtype) || act < MOTIF_GATE_SIGMOID || act > MOTIF_GATE_GELU) return MOTIF_EINVAL;
@@ -487,14 +570,15 @@ int check_mlp(long M, long K, long F, int act, int dtype) {
 
 template <typename T, int MT>
 void few_rows(bool vec, const void* x, long xs, const void* wg, const void* wu, const void* bg, const void* bu, void* h, float* G, float* U, int M, int K, int F, int act, hipStream_t s) {
-    if (vec) rows_kernel<T, MT, true><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, M, K, F, act);
-    else rows_kernel<T, MT, false><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, M, K, F, act);
+    if (vec) rows_kernel<T, MT, true><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
+    else rows_kernel<T, MT, false><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
 }
 
-struct FwdImages { Image x, wg, wu; bool lay_x, lay_w; };
-FwdImages fwd_images(Arena& ws, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype) {
-    FwdImages f;
-    const int n = planes(dtype), ld = up32(K);
+// x, Wg and Wu as the products read them: as they lie, or laid out in the workspace.
+struct Inputs { Image x, wg, wu; bool lay_x, lay_w; };
+Inputs inputs_of(Arena& ws, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype) {
+    Inputs f;
+    const int n = planes(dtype), ld = up8(K);
     f.lay_x = !direct(x, xs, K, dtype);
     f.lay_w = !direct(wg, K, K, dtype) || !direct(wu, K, K, dtype);
     f.x = f.lay_x ? Image{ws.take(2 * n * M * ld), M * ld, ld, n} : Image{x, 0, (int)xs, 1};
@@ -502,26 +586,24 @@ FwdImages fwd_images(Arena& ws, const void* x, long xs, const void* wg, const vo
     f.wu = f.lay_w ? Image{ws.take(2 * n * F * ld), F * ld, ld, n} : Image{wu, 0, (int)K, 1};
     return f;
 }
+void lay_out(const Inputs& f, bool need_x, bool need_w, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype, hipStream_t s) {
+    seq_dispatch(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (f.lay_x && need_x) layout<T>(x, xs, M, (int)K, f.x, s);
+        if (f.lay_w && need_w) { layout<T>(wg, K, F, (int)K, f.wg, s); layout<T>(wu, K, F, (int)K, f.wu, s); }
+    });
+}
 
-struct BwdImages { Image dg, du, dgt, dut, xt, wgt, wut; float *bias_part, *split_part; GemmPlan dx, dw; };
-BwdImages bwd_images(Arena& ws, long M, long K, long F, int dtype, bool need_x, bool need_w, bool need_b) {
-    BwdImages b = {};
-    const int n = planes(dtype), ldf = up32(F), ldm = up32(M);
-    if (need_x) {
-        char* p = (char*)ws.take(2L * 2 * n * M * ldf);
-        b.dg = {p, M * ldf, ldf, n};
-        b.du = {p ? p + 2L * n * M * ldf : nullptr, M * ldf, ldf, n};
-        b.wgt = {ws.take(2L * n * K * ldf), K * ldf, ldf, n};
-        b.wut = {ws.take(2L * n * K * ldf), K * ldf, ldf, n};
-        b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * ldf / 32, true);
-    }
-    if (need_w) {
-        char* p = (char*)ws.take(2L * 2 * n * F * ldm);
-        b.dgt = {p, F * ldm, ldm, n};
-        b.dut = {p ? p + 2L * n * F * ldm : nullptr, F * ldm, ldm, n};
-        b.xt = {ws.take(2L * n * K * ldm), K * ldm, ldm, n};
-        b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * ldm / 32, true);
-    }
+struct Backward { Inputs in; Image dg, du; float *bias_part, *split_part; GemmPlan dx, dw; };
+Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype, bool need_x, bool need_w, bool need_b) {
+    Backward b = {};
+    const int n = planes(dtype), ld = up8(F);
+    b.in = inputs_of(ws, x, xs, wg, wu, M, K, F, dtype);
+    char* p = (char*)ws.take(2L * 2 * n * M * ld);
+    b.dg = {p, M * ld, ld, n};
+    b.du = {p ? p + 2L * n * M * ld : nullptr, M * ld, ld, n};
+    if (need_x) b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * steps_of(ld), true);
+    if (need_w) b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * steps_of(M), true);
     if (need_b) b.bias_part = (float*)ws.take(4L * cdiv(M, 64) * 2 * F);
     long part = 0;                                       // the two products run one behind the other: one piece of memory serves both
     if (need_x && b.dx.splits > 1) part = 4L * b.dx.splits * M * K;
@@ -540,7 +622,7 @@ extern "C" long motif_gated_mlp_ws_bytes(const void* x, long x_rs, const void* w
     if (rc) return rc;
     if (M <= kFewRows) return 0;
     Arena ws = {nullptr, 0};
-    fwd_images(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+    inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
     return ws.used;
 }
 
@@ -564,31 +646,28 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
         return MOTIF_OK;
     }
     Arena ws = {(char*)workspace, 0};
-    const FwdImages f = fwd_images(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+    const Inputs f = inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
     if (ws.used && !workspace) return MOTIF_EINVAL;
-    seq_dispatch(dtype, [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        if (f.lay_x) layout<T>(x, x_rs, (int)M, (int)K, &f.x, nullptr, s);
-        if (f.lay_w) { layout<T>(w_gate, K, (int)F, (int)K, &f.wg, nullptr, s); layout<T>(w_up, K, (int)F, (int)K, &f.wu, nullptr, s); }
-    });
+    lay_out(f, true, true, x, x_rs, w_gate, w_up, M, K, F, dtype, s);
     GemmArgs g = {};
     segments(g, f.x, f.wg, f.wu);
     g.lda = f.x.ld; g.ldb = f.wg.ld;
-    g.steps = up32(K) / 32;
+    g.ka = g.kb = up8(K);
+    g.steps = steps_of(K);
     g.M = (int)M; g.N = (int)F;
-    g.c0 = h; g.g = G; g.u = U; g.bias0 = b_gate; g.bias1 = b_up;
+    g.c0 = h; g.g = G; g.u = U; g.ldg = up8(F); g.bias0 = b_gate; g.bias1 = b_up;
     g.act = act; g.dtype = dtype;
-    g.vec = F % 4 == 0 && seq_aligned(h, 16) && seq_aligned(G, 16) && seq_aligned(U, 16);
+    g.vec = F % 4 == 0 && seq_aligned(h, 16);
     gemm_dtype<GATED>(dtype, gemm_plan(M, F, 2, (long)g.nseg * g.steps, false), g, s);
     MOTIF_LAUNCH_CHECK();
     return MOTIF_OK;
 }
 
-extern "C" long motif_gated_mlp_bwd_ws_bytes(long M, long K, long F, int dtype, int need_x, int need_w, int need_b) {
+extern "C" long motif_gated_mlp_bwd_ws_bytes(const void* x, long x_rs, const void* w_gate, const void* w_up, long M, long K, long F, int dtype, int need_x, int need_w, int need_b) {
     const int rc = check_mlp(M, K, F, MOTIF_GATE_SILU, dtype);
     if (rc) return rc;
     Arena ws = {nullptr, 0};
-    bwd_images(ws, M, K, F, dtype, need_x, need_w, need_b);
+    backward_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype, need_x, need_w, need_b);
     return ws.used;
 }
 
@@ -599,28 +678,31 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
     const bool need_x = dx, need_w = dw_gate || dw_up, need_b = db_gate || db_up;
     if (need_w && (!dw_gate || !dw_up)) return MOTIF_EINVAL;
     if (M < 1 || !x || !w_gate || !w_up || !G || !U || !dh || !workspace || x_rs < 0 || dh_rs < 0 || !(need_x || need_w || need_b)) return MOTIF_EINVAL;
+    if (!seq_aligned(G, 16) || !seq_aligned(U, 16)) return MOTIF_EINVAL;
     hipStream_t s = (hipStream_t)stream;
     Arena ws = {(char*)workspace, 0};
-    const BwdImages b = bwd_images(ws, M, K, F, dtype, need_x, need_w, need_b);
+    const Backward b = backward_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype, need_x, need_w, need_b);
+    lay_out(b.in, need_w, need_x, x, x_rs, w_gate, w_up, M, K, F, dtype, s);
     seq_dispatch(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const int w = need_x ? b.dg.ld : (int)F, hgt = need_w ? b.dgt.ld : (int)M;
-        gate_grad_kernel<T><<<dim3(cdiv(hgt, 64), cdiv(w, 64)), 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, act,
-            need_x ? (void*)b.dg.p : nullptr, b.dg.plane, b.dg.plane * b.dg.n, b.dg.ld, need_w ? (void*)b.dgt.p : nullptr, b.dgt.plane, b.dgt.plane * b.dgt.n, b.dgt.ld, b.bias_part);
-        if (need_x) { layout<T>(w_gate, K, (int)F, (int)K, nullptr, &b.wgt, s); layout<T>(w_up, K, (int)F, (int)K, nullptr, &b.wut, s); }
-        if (need_w) layout<T>(x, x_rs, (int)M, (int)K, nullptr, &b.xt, s);
+        const dim3 grid(cdiv(M, 64), cdiv(b.dg.ld, 256));
+        if (F % 8 == 0 && dh_rs % 8 == 0 && seq_aligned(dh, 16))
+            gate_grad_kernel<T, true><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part);
+        else
+            gate_grad_kernel<T, false><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part);
     });
     if (need_b) {
         const int r = seq_colsum2(b.bias_part, cdiv(M, 64), F, db_gate, db_up, dtype, s);
         if (r) return r;
     }
-    if (need_x) {                                        // dx = [dG dU] [Wg^T Wu^T]^T: the second pair continues the reduction
+    if (need_x) {                                        // the second pair continues the reduction of the first
         GemmArgs g = {};
-        segments(g, b.dg, b.wgt, b.wgt);
-        segments(g, b.du, b.wut, b.wut);
-        g.lda = b.dg.ld; g.ldb = b.wgt.ld;
-        g.steps = b.dg.ld / 32;
-        g.M = (int)M; g.N = (int)K;
+        segments(g, b.dg, b.in.wg, b.in.wg);
+        segments(g, b.du, b.in.wu, b.in.wu);
+        g.lda = b.dg.ld; g.ldb = b.in.wg.ld;
+        g.ka = b.dg.ld; g.kb = (int)F;
+        g.steps = steps_of(b.dg.ld);
+        g.M = (int)M; g.N = (int)K; g.wb = up8(K);
         g.c0 = dx; g.dtype = dtype;
         g.part = b.dx.splits > 1 ? b.split_part : nullptr;
         g.vec = K % 4 == 0 && seq_aligned(dx, 16);
@@ -629,10 +711,11 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
     }
     if (need_w) {
         GemmArgs g = {};
-        segments(g, b.xt, b.dgt, b.dut);
-        g.lda = b.xt.ld; g.ldb = b.dgt.ld;
-        g.steps = b.xt.ld / 32;
-        g.M = (int)K; g.N = (int)F;
+        segments(g, b.in.x, b.dg, b.du);
+        g.lda = b.in.x.ld; g.ldb = b.dg.ld;
+        g.ka = g.kb = (int)M;
+        g.steps = steps_of(M);
+        g.M = (int)K; g.N = (int)F; g.wa = up8(K); g.wb = b.dg.ld;
         g.c0 = dw_gate; g.c1 = dw_up; g.dtype = dtype;
         g.part = b.dw.splits > 1 ? b.split_part : nullptr;
         g.vec = K % 4 == 0 && seq_aligned(dw_gate, 16) && seq_aligned(dw_up, 16);

@@ -1208,7 +1208,7 @@ def _gated_mlp_fwd(x, wg, wu, bg, bu, act, keep):
     f, k = wg.shape
     m, code = x.numel() // k, _SEQ_DTYPES[x.dtype]
     h = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
-    g, u = (torch.empty(m, f, dtype=torch.float32, device=x.device) for _ in range(2)) if keep else (None, None)
+    g, u = (torch.empty(m, (f + 7) & ~7, dtype=torch.float32, device=x.device) for _ in range(2)) if keep else (None, None)
     if m:
         xr, rs = _seq_rows(x)
         args = (xr.data_ptr(), rs, wg.data_ptr(), wu.data_ptr())
@@ -1239,8 +1239,9 @@ class _GatedMlp(torch.autograd.Function):
         if m:
             xr, xs = _seq_rows(x)
             dr, ds = _seq_rows(dh)
-            ws = _mlp_workspace(_lib.load().motif_gated_mlp_bwd_ws_bytes(m, k, f, code, need_x, dwg is not None, need_bg or need_bu), x, k, f)
-            _seq_call("motif_gated_mlp_bwd", x.device, xr.data_ptr(), xs, wg.data_ptr(), wu.data_ptr(), g.data_ptr(), u.data_ptr(), dr.data_ptr(), ds,
+            args = (xr.data_ptr(), xs, wg.data_ptr(), wu.data_ptr())
+            ws = _mlp_workspace(_lib.load().motif_gated_mlp_bwd_ws_bytes(*args, m, k, f, code, need_x, dwg is not None, need_bg or need_bu), x, k, f)
+            _seq_call("motif_gated_mlp_bwd", x.device, *args, g.data_ptr(), u.data_ptr(), dr.data_ptr(), ds,
                       _seq_ptr(dx), _seq_ptr(dwg), _seq_ptr(dwu), _seq_ptr(dbg), _seq_ptr(dbu), _seq_ptr(ws), m, k, f, ctx.act, code)
         else:
             for t in (dwg, dwu, dbg, dbu):
