@@ -59,10 +59,10 @@ struct GemmArgs {
     const void* b0[kSegs];
     const void* b1[kSegs];
     long lda, ldb;                                       // in elements, multiples of 8
-    int nseg, steps;                                     // segments; reduction steps of 32 in each
+    int nseg, units;                                     // segments; units of 64 of the reduction in each
     int ka, kb;                                          // reduction length of either operand's tensors: what lies behind it counts as zeros
     int M, N, wa, wb;                                    // output rows / columns of either half; ONE, TWO: columns of B, of A that may be read (multiples of 8)
-    int tiles_m, tiles_n, splits, steps_per_split;
+    int tiles_m, tiles_n, splits, units_per_split;
     void *c0, *c1;                                       // outputs of type dtype, dense
     float *g, *u;                                        // GATED: [M][ldg], may be null
     long ldg;
@@ -104,56 +104,68 @@ __device__ __forceinline__ void store_as(void* p, long at, const float (&v)[N], 
     else store_run<f16_t, f16_t, N>(p, at, v, n, vec);
 }
 
-// One operand of a tile: two blocks of C rows (of the output), 32 steps of the reduction deep, 64 C bytes each.  A wave requests one piece of 1 KB
-// of either block per stage.
-//   dense     [C][32]: a piece is 16 rows of 64 bytes, a lane's 16 bytes the steps 8 j .. 8 j + 7 of its row.  The four pieces of a row are
-//             exchanged by a pattern of the row's number, so that the 16 rows x 16 bytes of a fragment's read lie in different banks.
-//   across    [32][C]: a piece is 2 C bytes of 4 (C = 128) or 8 steps.  A fragment's read takes 32 bytes (16 rows) of 16 steps and turns them
-//             in 4 x 4 steps (ds_read_b64_tr_b16: lane i of 16 gets row i of four steps); 32-byte units are exchanged by a pattern of the step.
+// One operand of a tile: two blocks of C rows (of the output), 64 of the reduction deep, 128 C bytes each.  A wave requests two pieces of 1 KB of
+// either block per unit.
+//   dense     [C][64]: a piece is 8 rows of 128 bytes -- whole cache lines: rows of 64 bytes (units of 32) make twice the requests to L2, which then
+//             bound the kernel.  The eight 16-byte pieces of a row are exchanged by a pattern of the row's number, so that the 16 rows x 16
+//             bytes of a fragment's read lie in different banks.
+//   across    [64][C]: a piece is 2 C bytes of 4 (C = 128) or 8 steps.  A fragment's read takes 32 bytes (16 rows) of 16 steps and turns them
+//             in 4 x 4 steps (ds_read_b64_tr_b16: lane i of 16 gets row i of four steps); 32-byte pieces are exchanged by a pattern of the step.
 template <bool ACROSS, int C>
 struct Operand {
-    static constexpr int kUnits = C / 16, kPieces = C / 8;                       // of an across row
-    static __device__ __forceinline__ int dense_swap(int row) { return ((row >> 3) & 1) | ((((row >> 2) ^ (row >> 3)) & 1) << 1); }
+    static constexpr int kWaves = C / 16, kPieces = C / 8;                        // 16-byte pieces of an across row
     static __device__ __forceinline__ int across_swap(int k) { return C == 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2); }
-    // this lane's first step of a stage and its byte offset from (row `at` of the matrix, step 0), rows up to `most`
-    static __device__ __forceinline__ void lane_of(int wave, int lane, int first, int at, int most, long ld, int& step, unsigned& off) {
+    // piece i of this lane: its first step of a unit, its byte offset from (row `at` of the matrix, step 0); rows up to `most` exist
+    static __device__ __forceinline__ void lane_of(int wave, int lane, int i, int first, int at, int most, long ld, int& step, unsigned& off) {
         if (!ACROSS) {
-            const int r = lane >> 2;
-            step = ((lane & 3) ^ dense_swap(r)) * 8;
-            off = (unsigned)(min(first + wave * 16 + r, most - 1) - at) * (unsigned)ld * 2u + (unsigned)step * 2u;
+            const int r = (i * kWaves + wave) * 8 + (lane >> 3);
+            step = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+            off = (unsigned)(min(first + r, most - 1) - at) * (unsigned)ld * 2u + (unsigned)step * 2u;
         } else {
-            const int k = wave * (64 / kPieces) + lane / kPieces, c = lane % kPieces;
-            step = k;
-            off = (unsigned)k * (unsigned)ld * 2u + (unsigned)(min(first + (((c >> 1) ^ across_swap(k)) * 2 + (c & 1)) * 8, most - 8) - at) * 2u;
+            const int c = lane % kPieces;
+            step = (i * kWaves + wave) * (64 / kPieces) + lane / kPieces;
+            off = (unsigned)step * (unsigned)ld * 2u + (unsigned)(min(first + (((c >> 1) ^ across_swap(step)) * 2 + (c & 1)) * 8, most - 8) - at) * 2u;
         }
     }
-    // this lane's byte of the fragment of rows `row` .. + 15 in a block (dense: + 1024 per 16 rows; across: the unit is part of the pattern)
-    static __device__ __forceinline__ int frag_of(int lane) {
-        if (!ACROSS) return (lane & 15) * 64 + (((lane >> 4) ^ dense_swap(lane & 15)) * 16);
-        return ((lane >> 4) * 8 + ((lane & 15) >> 2)) * (2 * C) + (lane & 3) * 8;
+    // this lane's byte of a fragment of half `kk` of a unit, but for its row
+    static __device__ __forceinline__ int frag_of(int lane, int kk) {
+        if (!ACROSS) return (lane & 15) * 128 + ((kk * 4 + (lane >> 4)) ^ ((lane >> 1) & 7)) * 16;
+        return (kk * 32 + (lane >> 4) * 8 + ((lane & 15) >> 2)) * (2 * C) + (lane & 3) * 8;
     }
     static __device__ __forceinline__ s16x8 read(const char* block, int frag, int row, int lane) {
-        if constexpr (!ACROSS) return *(const s16x8*)(block + frag + row * 64);
+        if constexpr (!ACROSS) return *(const s16x8*)(block + frag + row * 128);
         else {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s16x4* P;
-            // the second four steps have the same pattern (it does not depend on bit 2 of the step)
-            const int unit = ((row >> 4) ^ across_swap((lane >> 4) * 8 + ((lane & 15) >> 2))) * 32;
-            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(block + frag + unit)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(block + frag + unit + 8 * C));
+            // the pattern is that of the step, whatever its bits 2 and 5 are: the same for the second four steps and for either half
+            const int piece = ((row >> 4) ^ across_swap((lane >> 4) * 8 + ((lane & 15) >> 2))) * 32;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(block + frag + piece)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(block + frag + piece + 8 * C));
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
 };
 
-// Tile 2 C rows of A x C columns of either half of B; C / 16 waves (two along A), each C x 32 x 2 outputs.  The reduction advances in steps of 32:
-// four stages lie in LDS, three of them on their way, and a step's fragments are read from LDS while the step before is multiplied: one barrier
-// a step, behind which the next step's stage is whole and the current one's place free (every wave has its fragments in registers).
+template <bool FAST, int ACT>
+__device__ __forceinline__ void gate4_as(const float (&g)[4], const float (&u)[4], float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = gate<FAST>(g[e], ACT) * u[e];
+}
+template <bool FAST>
+__device__ __forceinline__ void gate4(const float (&g)[4], const float (&u)[4], float (&v)[4], int act) {
+    if (act == MOTIF_GATE_SILU) gate4_as<FAST, MOTIF_GATE_SILU>(g, u, v);
+    else if (act == MOTIF_GATE_GELU) gate4_as<FAST, MOTIF_GATE_GELU>(g, u, v);
+    else gate4_as<FAST, MOTIF_GATE_SIGMOID>(g, u, v);
+}
+
+// Tile 2 C rows of A x C columns of either half of B; C / 16 waves (two along A), each C x 32 x 2 outputs.  The reduction advances in units of 64, two
+// of which lie in LDS; the fragments of half a unit are read from LDS while those before them are multiplied.  One barrier a unit, in its middle:
+// behind it every wave has the unit's second half in registers, so the unit after next may be requested into its place, and the next one is whole.
 template <typename T, int C, GemmMode MODE>
 __global__ __launch_bounds__(C * 4) void gemm_kernel(GemmArgs p) {
-    constexpr int NW = C / 16, WN = NW / 2, MF = C / 16, HF = 2, BLOCK = C * 64, STAGE = 4 * BLOCK;
+    constexpr int NW = C / 16, WN = NW / 2, MF = C / 16, HF = 2, BLOCK = C * 128, STAGE = 4 * BLOCK;
     using A = Operand<MODE == TWO, C>;
     using B = Operand<MODE != GATED, C>;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * STAGE];
+    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
@@ -173,45 +185,47 @@ __global__ __launch_bounds__(C * 4) void gemm_kernel(GemmArgs p) {
     const int am = MODE == TWO ? p.wa : p.M, bm = MODE != GATED ? p.wb : p.N;      // rows (columns) that may be read
     const int bat[2] = {n0[0], min(n0[1], bm - 8 < 0 ? 0 : bm - 8)};              // where the halves' pointers stand
 
-    unsigned offa[2], offb[2];
-    int ka[2], kb[2];
+    unsigned offa[2][2], offb[2][2];                     // [block][piece]
+    int ka[2][2], kb[2][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        A::lane_of(wave, lane, m0 + h * C, m0, am, p.lda, ka[h], offa[h]);
-        B::lane_of(wave, lane, n0[h], bat[h], bm, p.ldb, kb[h], offb[h]);
-    }
-    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds + wave * 1024;
-    const long stepa = MODE == TWO ? 64 * p.lda : 64, stepb = MODE != GATED ? 64 * p.ldb : 64;      // bytes per step
-    const int enda = p.ka - (p.steps - 1) * 32, endb = p.kb - (p.steps - 1) * 32;  // what the last step of a segment holds
-    const bool ragged = enda < 32 || endb < 32;
-
-    const int s_begin = split * p.steps_per_split, s_end = min(p.nseg * p.steps, s_begin + p.steps_per_split), count = s_end - s_begin;
-    int seg = s_begin / p.steps, left = p.steps - (s_begin - seg * p.steps);      // steps left in the segment that is requested
-    const char *pa, *pb0, *pb1;
-    auto segment = [&](int step) __attribute__((always_inline)) {
-        pa = (const char*)p.a[seg] + (MODE == TWO ? m0 : (long)m0 * p.lda) * 2 + step * stepa;
-        pb0 = (const char*)p.b0[seg] + (MODE != GATED ? bat[0] : (long)bat[0] * p.ldb) * 2 + step * stepb;
-        pb1 = (const char*)p.b1[seg] + (MODE != GATED ? bat[1] : (long)bat[1] * p.ldb) * 2 + step * stepb;
-    };
-    segment(s_begin - seg * p.steps);
-    auto advance = [&]() __attribute__((always_inline)) {
-        pa += stepa; pb0 += stepb; pb1 += stepb;
-        if (--left == 0 && seg + 1 < p.nseg) { ++seg; left = p.steps; segment(0); }
-    };
-    auto request = [&](int stage) __attribute__((always_inline)) {
-        const unsigned at = lds0 + stage * STAGE;
-        if (ragged && left == 1) {
-            const char* zeros = (const char*)&g_zeros;
-            to_lds(at, ka[0] < enda ? pa + offa[0] : zeros);
-            to_lds(at + BLOCK, ka[1] < enda ? pa + offa[1] : zeros);
-            to_lds(at + 2 * BLOCK, kb[0] < endb ? pb0 + offb[0] : zeros);
-            to_lds(at + 3 * BLOCK, kb[1] < endb ? pb1 + offb[1] : zeros);
-        } else {
-            to_lds(at, pa, offa[0]);
-            to_lds(at + BLOCK, pa, offa[1]);
-            to_lds(at + 2 * BLOCK, pb0, offb[0]);
-            to_lds(at + 3 * BLOCK, pb1, offb[1]);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            A::lane_of(wave, lane, i, m0 + h * C, m0, am, p.lda, ka[h][i], offa[h][i]);
+            B::lane_of(wave, lane, i, n0[h], bat[h], bm, p.ldb, kb[h][i], offb[h][i]);
         }
+    const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds + wave * 1024;
+    const long unita = MODE == TWO ? 128 * p.lda : 128, unitb = MODE != GATED ? 128 * p.ldb : 128;      // bytes per unit
+    const int enda = p.ka - (p.units - 1) * 64, endb = p.kb - (p.units - 1) * 64;  // what the last unit of a segment holds
+    const bool ragged = enda < 64 || endb < 64;
+
+    const int u_begin = split * p.units_per_split, u_end = min(p.nseg * p.units, u_begin + p.units_per_split), count = u_end - u_begin;
+    int seg = u_begin / p.units, left = p.units - (u_begin - seg * p.units);      // units left in the segment that is requested
+    const char *pa, *pb0, *pb1;
+    auto segment = [&](int unit) __attribute__((always_inline)) {
+        pa = (const char*)p.a[seg] + (MODE == TWO ? m0 : (long)m0 * p.lda) * 2 + unit * unita;
+        pb0 = (const char*)p.b0[seg] + (MODE != GATED ? bat[0] : (long)bat[0] * p.ldb) * 2 + unit * unitb;
+        pb1 = (const char*)p.b1[seg] + (MODE != GATED ? bat[1] : (long)bat[1] * p.ldb) * 2 + unit * unitb;
+    };
+    segment(u_begin - seg * p.units);
+    auto advance = [&]() __attribute__((always_inline)) {
+        pa += unita; pb0 += unitb; pb1 += unitb;
+        if (--left == 0 && seg + 1 < p.nseg) { ++seg; left = p.units; segment(0); }
+    };
+    auto piece = [&](int slot, int b, int i) __attribute__((always_inline)) {      // piece i of block b: A's two, B's two
+        to_lds(lds0 + slot * STAGE + b * BLOCK + i * NW * 1024, b < 2 ? pa : b == 2 ? pb0 : pb1, b < 2 ? offa[b & 1][i] : offb[b & 1][i]);
+    };
+    auto request = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (ragged && left == 1) {
+                    const bool in = b < 2 ? ka[b & 1][i] < enda : kb[b & 1][i] < endb;
+                    const char* own = b < 2 ? pa + offa[b & 1][i] : (b == 2 ? pb0 : pb1) + offb[b & 1][i];
+                    to_lds(lds0 + slot * STAGE + b * BLOCK + i * NW * 1024, in ? own : (const char*)&g_zeros);
+                } else piece(slot, b, i);
+            }
         advance();
     };
 
@@ -224,12 +238,13 @@ __global__ __launch_bounds__(C * 4) void gemm_kernel(GemmArgs p) {
             for (int j = 0; j < HF; ++j) acc[i][h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     struct Frags { s16x8 a[MF], b[2][HF]; };
-    const int fa = A::frag_of(lane), fb = B::frag_of(lane);
-    // a quarter of the fragments of a stage / of a step's products
-    auto fetch = [&](Frags& f, const char* st, int q) __attribute__((always_inline)) {
-        f.b[q >> 1][q & 1] = B::read(st + (2 + (q >> 1)) * BLOCK, fb, wn * 32 + (q & 1) * 16, lane);
+    const int fa[2] = {A::frag_of(lane, 0), A::frag_of(lane, 1)}, fb[2] = {B::frag_of(lane, 0), B::frag_of(lane, 1)};
+    // a quarter of the fragments of half a unit / of its products
+    auto fetch = [&](Frags& f, int slot, int kk, int q) __attribute__((always_inline)) {
+        const char* st = lds + slot * STAGE;
+        f.b[q >> 1][q & 1] = B::read(st + (2 + (q >> 1)) * BLOCK, fb[kk], wn * 32 + (q & 1) * 16, lane);
 #pragma unroll
-        for (int i = q * MF / 4; i < (q + 1) * MF / 4; ++i) f.a[i] = A::read(st + wm * BLOCK, fa, i * 16, lane);
+        for (int i = q * MF / 4; i < (q + 1) * MF / 4; ++i) f.a[i] = A::read(st + wm * BLOCK, fa[kk], i * 16, lane);
     };
     auto multiply = [&](const Frags& f, int q) __attribute__((always_inline)) {
 #pragma unroll
@@ -239,89 +254,103 @@ __global__ __launch_bounds__(C * 4) void gemm_kernel(GemmArgs p) {
 #pragma unroll
                 for (int j = 0; j < HF; ++j) acc[i][h][j] = MODE != TWO ? mfma(f.b[h][j], f.a[i], acc[i][h][j], (T*)nullptr) : mfma(f.a[i], f.b[h][j], acc[i][h][j], (T*)nullptr);
     };
-    // the requests behind stage s + 1 may still be on their way, four each; then everybody's part of it is there
-    auto arrive = [&](int behind) __attribute__((always_inline)) {
-        if (behind >= 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-        else if (behind == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // Requests and reads are spread between the multiplications: issued in one go behind the barrier, by all waves at once, they hold up every wave's
+    // first multiplication until the memory path and the LDS have taken all of them (measured: 500 of 1650 cycles per 32 of the reduction).
+    auto spread = [&]() __attribute__((always_inline)) {
+        constexpr int RA = MODE == TWO ? 2 : 1, RB = MODE != GATED ? 2 : 1, READS = RB + RA * MF / 4, MMAS = MF / 4 * 2 * HF, EACH = MMAS / READS;
+#pragma unroll
+        for (int i = 0; i < READS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                      // an LDS read
+            __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);                   // matrix instructions
+        }
+        if constexpr (EACH * READS < MMAS) __builtin_amdgcn_sched_group_barrier(0x008, MMAS - EACH * READS, 0);
+    };
+    auto arrived = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    for (int s = 0; s < 4 && s < count; ++s) request(s);
-    if (count >= 4) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+    request(0);
+    if (count > 1) {
+        request(1);
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    // One step: multiply `now` (stage s), read `next` (stage s + 1), request stage s + 4.  In the middle of a segment the requests and reads are spread
-    // between the multiplications: issued in one go behind the barrier, by all waves at once, they hold up every wave's first multiplication
-    // until the memory path and the LDS have taken all of them (measured: 500 of a step's 1650 cycles).
-    auto middle = [&](int s, const Frags& now, Frags& next) __attribute__((always_inline)) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        arrive(2);
-        const char* st = lds + ((s + 1) & 3) * STAGE;
-        const unsigned at = lds0 + (s & 3) * STAGE;
-        constexpr int RA = MODE == TWO ? 2 : 1, RB = MODE != GATED ? 2 : 1, READS = RB + RA * MF / 4, MMAS = MF / 4 * 2 * HF, EACH = MMAS / READS;
+    Frags f0, f1;                                        // of a unit's first and second half
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            to_lds(at + q * BLOCK, q < 2 ? pa : q == 2 ? pb0 : pb1, q < 2 ? offa[q & 1] : offb[q & 1]);
-            fetch(next, st, q);
-            multiply(now, q);
+    for (int q = 0; q < 4; ++q) fetch(f0, 0, 0, q);
+    for (int u = 0; u < count; ++u) {
+        for (int plain = min(count - 2 - u, left - (int)ragged); plain > 0; --plain, ++u) {
 #pragma unroll
-            for (int i = 0; i < READS; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                  // an LDS read
-                __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);               // matrix instructions
+            for (int q = 0; q < 4; ++q) {
+                fetch(f1, u & 1, 1, q);
+                multiply(f0, q);
+                spread();
             }
-            if constexpr (EACH * READS < MMAS) __builtin_amdgcn_sched_group_barrier(0x008, MMAS - EACH * READS, 0);
-        }
-        advance();
-    };
-    auto any = [&](int s, const Frags& now, Frags& next) __attribute__((always_inline)) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        arrive(count - 2 - s);
-        if (s + 4 < count) request(s & 3);
-        if (s + 1 < count) {
+            arrived();
 #pragma unroll
-            for (int q = 0; q < 4; ++q) fetch(next, lds + ((s + 1) & 3) * STAGE, q);
+            for (int q = 0; q < 4; ++q) {
+                piece(u & 1, q, 0);
+                piece(u & 1, q, 1);
+                fetch(f0, (u + 1) & 1, 0, q);
+                multiply(f1, q);
+                spread();
+            }
+            advance();
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) multiply(now, q);
-    };
-    Frags f0, f1;
+        for (int q = 0; q < 4; ++q) { fetch(f1, u & 1, 1, q); multiply(f0, q); }
+        arrived();
+        if (u + 2 < count) request(u & 1);
+        if (u + 1 < count) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) fetch(f0, lds, q);
-    for (int s = 0; s < count; s += 2) {
-        for (int plain = min(count - 4 - s, left - (int)ragged); plain >= 2; plain -= 2, s += 2) {
-            middle(s, f0, f1);
-            middle(s + 1, f1, f0);
+            for (int q = 0; q < 4; ++q) fetch(f0, (u + 1) & 1, 0, q);
         }
-        any(s, f0, f1);
-        if (s + 1 < count) any(s + 1, f1, f0);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) multiply(f1, q);
     }
 
+    if constexpr (MODE == GATED) {
+        const int n = n0[0] + wn * 32 + (lane >> 4) * 4;
+        float bg[HF][4], bu[HF][4];
+#pragma unroll
+        for (int j = 0; j < HF; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = min(n + j * 16 + e, p.N - 1);
+                bg[j][e] = p.bias0 ? seq_param(p.bias0, c, p.dtype) : 0.f;
+                bu[j][e] = p.bias1 ? seq_param(p.bias1, c, p.dtype) : 0.f;
+            }
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+            const int m = m0 + wm * C + i * 16 + (lane & 15);
+            if (m >= p.M) continue;
+#pragma unroll
+            for (int j = 0; j < HF; ++j) {
+                const int cnt = min(4, p.N - n - j * 16);
+                if (cnt <= 0) continue;
+                float g[4], u[4], v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { g[e] = acc[i][0][j][e] + bg[j][e]; u[e] = acc[i][1][j][e] + bu[j][e]; }
+                if (p.dtype == MOTIF_F32) gate4<false>(g, u, v, p.act); else gate4<true>(g, u, v, p.act);
+                store_as<4>(p.c0, (long)m * p.N + n + j * 16, v, cnt, p.vec, p.dtype);
+                if (p.g) {                               // (their rows are padded to whole runs)
+                    seq_store16<float, 4>(p.g + m * p.ldg + n + j * 16, g);
+                    seq_store16<float, 4>(p.u + m * p.ldg + n + j * 16, u);
+                }
+            }
+        }
+        return;
+    }
     const int lo = lane & 15, hi = (lane >> 4) * 4;
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
 #pragma unroll
         for (int j = 0; j < HF; ++j) {
             const int mt = m0 + wm * C + i * 16, off = wn * 32 + j * 16;
-            if constexpr (MODE == GATED) {
-                const int m = mt + lo, n = n0[0] + off + hi, cnt = min(4, p.N - n);
-                if (m >= p.M || cnt <= 0) continue;
-                float g[4], u[4], v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int c = min(n + e, p.N - 1);
-                    g[e] = acc[i][0][j][e] + (p.bias0 ? seq_param(p.bias0, c, p.dtype) : 0.f);
-                    u[e] = acc[i][1][j][e] + (p.bias1 ? seq_param(p.bias1, c, p.dtype) : 0.f);
-                    v[e] = p.dtype == MOTIF_F32 ? gate<false>(g[e], p.act) * u[e] : gate<true>(g[e], p.act) * u[e];
-                }
-                const long at = (long)m * p.N + n;
-                store_as<4>(p.c0, at, v, cnt, p.vec, p.dtype);
-                if (p.g) {                               // (their rows are padded to whole runs)
-                    seq_store16<float, 4>(p.g + m * p.ldg + n, g);
-                    seq_store16<float, 4>(p.u + m * p.ldg + n, u);
-                }
-            } else {
+            {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int row = MODE == ONE ? mt + lo : n0[h] + off + lo, col = MODE == ONE ? n0[h] + off + hi : mt + hi;
@@ -528,7 +557,7 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
 constexpr int kFewRows = 64;
 constexpr long kMostRows = 1L << 22;                    // offsets within a tile are 32 bits: 256 rows x this x 2 bytes
 int up8(long n) { return (int)((n + 7) & ~7L); }
-int steps_of(long n) { return (int)((n + 31) / 32); }
+int units_of(long n) { return (int)((n + 63) / 64); }
 long up16b(long bytes) { return (bytes + 255) & ~255L; }
 int planes(int dtype) { return dtype == MOTIF_F32 ? 3 : 1; }
 
@@ -563,9 +592,9 @@ void segments(GemmArgs& g, const Image& a, const Image& b0, const Image& b1) {
 }
 
 // Tiles of 256 x 256 (C = 128) where they give every CU at least one, else of 128 x 128.  The reduction is split where even those leave CUs without work and
-// the pieces stay long (16 steps at least); the pieces' sums are fp32 and joined in order.
-struct GemmPlan { bool big; int tiles_m, tiles_n, splits, steps_per_split; };
-GemmPlan gemm_plan(long M, long N, int halves, long total_steps, bool may_split) {
+// the pieces stay long (8 units of 64 at least); the pieces' sums are fp32 and joined in order.
+struct GemmPlan { bool big; int tiles_m, tiles_n, splits, units_per_split; };
+GemmPlan gemm_plan(long M, long N, int halves, long total_units, bool may_split) {
     GemmPlan p;
     auto tiles = [&](int t) { return (long)cdiv(M, t) * cdiv(N, halves == 2 ? t / 2 : t); };
     p.big = tiles(256) >= 256;
@@ -573,16 +602,16 @@ GemmPlan gemm_plan(long M, long N, int halves, long total_steps, bool may_split)
     p.tiles_m = cdiv(M, t);
     p.tiles_n = cdiv(N, halves == 2 ? t / 2 : t);
     long splits = may_split && !p.big ? 512 / tiles(t) : 1;
-    if (splits > total_steps / 16) splits = total_steps / 16;
+    if (splits > total_units / 8) splits = total_units / 8;
     if (splits < 1) splits = 1;
-    p.steps_per_split = (int)((total_steps + splits - 1) / splits);
-    p.splits = (int)((total_steps + p.steps_per_split - 1) / p.steps_per_split);
+    p.units_per_split = (int)((total_units + splits - 1) / splits);
+    p.splits = (int)((total_units + p.units_per_split - 1) / p.units_per_split);
     return p;
 }
 
 template <typename T, GemmMode MODE>
 void gemm(const GemmPlan& pl, GemmArgs& g, hipStream_t s) {
-    g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n; g.splits = pl.splits; g.steps_per_split = pl.steps_per_split;
+    g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n; g.splits = pl.splits; g.units_per_split = pl.units_per_split;
     const unsigned grid = (unsigned)((long)pl.tiles_m * pl.tiles_n * pl.splits);
     if (pl.big) gemm_kernel<T, 128, MODE><<<grid, 512, 0, s>>>(g);
     else gemm_kernel<T, 64, MODE><<<grid, 256, 0, s>>>(g);
@@ -636,8 +665,8 @@ Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const vo
     char* p = (char*)ws.take(2L * 2 * n * M * ld);
     b.dg = {p, M * ld, ld, n};
     b.du = {p ? p + 2L * n * M * ld : nullptr, M * ld, ld, n};
-    if (need_x) b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * steps_of(ld), true);
-    if (need_w) b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * steps_of(M), true);
+    if (need_x) b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * units_of(ld), true);
+    if (need_w) b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * units_of(M), true);
     if (need_b) b.bias_part = (float*)ws.take(4L * cdiv(M, 64) * 2 * F);
     long part = 0;                                       // the two products run one behind the other: one piece of memory serves both
     if (need_x && b.dx.splits > 1) part = 4L * b.dx.splits * M * K;
@@ -687,12 +716,12 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
     segments(g, f.x, f.wg, f.wu);
     g.lda = f.x.ld; g.ldb = f.wg.ld;
     g.ka = g.kb = up8(K);
-    g.steps = steps_of(K);
+    g.units = units_of(K);
     g.M = (int)M; g.N = (int)F;
     g.c0 = h; g.g = G; g.u = U; g.ldg = up8(F); g.bias0 = b_gate; g.bias1 = b_up;
     g.act = act; g.dtype = dtype;
     g.vec = F % 4 == 0 && seq_aligned(h, 16);
-    gemm_dtype<GATED>(dtype, gemm_plan(M, F, 2, (long)g.nseg * g.steps, false), g, s);
+    gemm_dtype<GATED>(dtype, gemm_plan(M, F, 2, (long)g.nseg * g.units, false), g, s);
     MOTIF_LAUNCH_CHECK();
     return MOTIF_OK;
 }
@@ -735,7 +764,7 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         segments(g, b.du, b.in.wu, b.in.wu);
         g.lda = b.dg.ld; g.ldb = b.in.wg.ld;
         g.ka = b.dg.ld; g.kb = (int)F;
-        g.steps = steps_of(b.dg.ld);
+        g.units = units_of(b.dg.ld);
         g.M = (int)M; g.N = (int)K; g.wb = up8(K);
         g.c0 = dx; g.dtype = dtype;
         g.part = b.dx.splits > 1 ? b.split_part : nullptr;
@@ -748,7 +777,7 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         segments(g, b.in.x, b.dg, b.du);
         g.lda = b.in.x.ld; g.ldb = b.dg.ld;
         g.ka = g.kb = (int)M;
-        g.steps = steps_of(M);
+        g.units = units_of(M);
         g.M = (int)K; g.N = (int)F; g.wa = up8(K); g.wb = b.dg.ld;
         g.c0 = dw_gate; g.c1 = dw_up; g.dtype = dtype;
         g.part = b.dw.splits > 1 ? b.split_part : nullptr;
