@@ -36,14 +36,15 @@ __device__ __forceinline__ float gate(float g, int act) {
     return 0.5f * g * (1.f + erff(g * 0.70710678f));
 }
 // act(g) and its derivative
+template <bool FAST>
 __device__ __forceinline__ void gate_grad(float g, int act, float& v, float& d) {
     if (act == MOTIF_GATE_GELU) {
         const float phi = 0.5f * (1.f + erff(g * 0.70710678f));
         v = g * phi;
-        d = fmaf(g * 0.39894228f, expf(-0.5f * g * g), phi);
+        d = fmaf(g * 0.39894228f, FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g), phi);
         return;
     }
-    const float s = sigm<false>(g);
+    const float s = sigm<FAST>(g);
     if (act == MOTIF_GATE_SIGMOID) { v = s; d = s * (1.f - s); }
     else { v = g * s; d = s * fmaf(g, 1.f - s, 1.f); }
 }
@@ -62,12 +63,12 @@ struct GemmArgs {
     int nseg, units;                                     // segments; units of 64 of the reduction in each
     int ka, kb;                                          // reduction length of either operand's tensors: what lies behind it counts as zeros
     int M, N, wa, wb;                                    // output rows / columns of either half; ONE, TWO: columns of B, of A that may be read (multiples of 8)
-    int tiles_m, tiles_n, splits, units_per_split;
+    int tiles_m, tiles_n, whole, pieces, units_per_piece;   // tiles 0 .. whole - 1 are one workgroup's; the others' reductions are cut into pieces
     void *c0, *c1;                                       // outputs of type dtype, dense
     float *g, *u;                                        // GATED: [M][ldg], may be null
     long ldg;
     const void *bias0, *bias1;
-    float* part;                                         // split reduction, fp32 instead of the outputs: ONE [split][M][N], TWO [split][2][N][M]
+    f32x4* part;                                         // pieces' accumulators: [tile - whole][piece][accumulator][thread]
     int act, dtype, vec;                                 // vec: rows of the outputs allow runs of four values
 };
 
@@ -157,6 +158,73 @@ __device__ __forceinline__ void gate4(const float (&g)[4], const float (&u)[4], 
     else gate4_as<FAST, MOTIF_GATE_SIGMOID>(g, u, v);
 }
 
+// Where a tile lies.  Workgroups are dealt to the eight XCDs in turn: each XCD takes a contiguous run of tiles, column by column within bands of 8 tile
+// rows, so that the tiles in flight on one XCD share their rows of both operands in its L2.
+template <int C, GemmMode MODE>
+struct Tile {
+    int m0, n0[2];
+    __device__ __forceinline__ Tile(const GemmArgs& p, int id) {
+        const int tiles = p.tiles_m * p.tiles_n, xcd = id & 7, q = tiles >> 3, r = tiles & 7;
+        id = xcd * q + (xcd < r ? xcd : r) + (id >> 3);
+        const int band = id / (8 * p.tiles_n), in = id - band * 8 * p.tiles_n, bh = min(8, p.tiles_m - band * 8), tn = in / bh;
+        m0 = (band * 8 + in % bh) * 2 * C;
+        n0[0] = tn * (MODE == ONE ? 2 * C : C);
+        n0[1] = MODE == ONE ? n0[0] + C : n0[0];
+    }
+};
+
+// One fragment pair (i, j) of a wave's outputs: o0, o1 of the two halves.
+template <int C, GemmMode MODE>
+struct Store {
+    const GemmArgs& p;
+    const Tile<C, MODE>& t;
+    int m, c, lo, hi;                                    // this wave's first row of A and column of a half; of a fragment: the lane's place
+    float bias[2][2][4];                                 // GATED: [half][j]
+    __device__ __forceinline__ Store(const GemmArgs& p_, const Tile<C, MODE>& t_, int wave, int lane) : p(p_), t(t_) {
+        constexpr int WN = C / 32;
+        m = t.m0 + wave / WN * C;
+        c = wave % WN * 32;
+        lo = lane & 15;
+        hi = (lane >> 4) * 4;
+        if constexpr (MODE == GATED) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int n = min(t.n0[0] + c + j * 16 + hi + e, p.N - 1);
+                    bias[0][j][e] = p.bias0 ? seq_param(p.bias0, n, p.dtype) : 0.f;
+                    bias[1][j][e] = p.bias1 ? seq_param(p.bias1, n, p.dtype) : 0.f;
+                }
+        }
+    }
+    __device__ __forceinline__ void operator()(int i, int j, const f32x4& o0, const f32x4& o1) const {
+        if constexpr (MODE == GATED) {
+            const int row = m + i * 16 + lo, n = t.n0[0] + c + j * 16 + hi, cnt = min(4, p.N - n);
+            if (row >= p.M || cnt <= 0) return;
+            float g[4], u[4], v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { g[e] = o0[e] + bias[0][j][e]; u[e] = o1[e] + bias[1][j][e]; }
+            if (p.dtype == MOTIF_F32) gate4<false>(g, u, v, p.act); else gate4<true>(g, u, v, p.act);
+            store_as<4>(p.c0, (long)row * p.N + n, v, cnt, p.vec, p.dtype);
+            if (p.g) {                                   // (their rows are padded to whole runs)
+                seq_store16<float, 4>(p.g + row * p.ldg + n, g);
+                seq_store16<float, 4>(p.u + row * p.ldg + n, u);
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int a = m + i * 16, n = t.n0[h] + c + j * 16;
+                const int row = MODE == ONE ? a + lo : n + lo, col = MODE == ONE ? n + hi : a + hi;
+                const int rows = MODE == ONE ? p.M : p.N, cols = MODE == ONE ? p.N : p.M, cnt = min(4, cols - col);
+                if (row >= rows || cnt <= 0) continue;
+                const f32x4& o = h ? o1 : o0;
+                const float v[4] = {o[0], o[1], o[2], o[3]};
+                store_as<4>(MODE == ONE || h == 0 ? p.c0 : p.c1, (long)row * cols + col, v, cnt, p.vec, p.dtype);
+            }
+        }
+    }
+};
+
 // Tile 2 C rows of A x C columns of either half of B; C / 16 waves (two along A), each C x 32 x 2 outputs.  The reduction advances in units of 64, two
 // of which lie in LDS; the fragments of half a unit are read from LDS while those before them are multiplied.  One barrier a unit, in its middle:
 // behind it every wave has the unit's second half in registers, so the unit after next may be requested into its place, and the next one is whole.
@@ -169,19 +237,10 @@ __global__ __launch_bounds__(C * 4) void gemm_kernel(GemmArgs p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
-    // Workgroups are dealt to the eight XCDs in turn: each XCD takes a contiguous run of tiles, column by column within bands of 8 tile rows,
-    // so that the tiles in flight on one XCD share their rows of both operands in its L2.
-    const int tiles = p.tiles_m * p.tiles_n;
-    int id = blockIdx.x;
-    const int split = id / tiles;
-    id -= split * tiles;
-    {
-        const int xcd = id & 7, q = tiles >> 3, r = tiles & 7;
-        id = xcd * q + (xcd < r ? xcd : r) + (id >> 3);
-    }
-    const int band = id / (8 * p.tiles_n), in = id - band * 8 * p.tiles_n, bh = min(8, p.tiles_m - band * 8);
-    const int m0 = (band * 8 + in % bh) * 2 * C, tn = in / bh;
-    const int n0[2] = {tn * (MODE == ONE ? 2 * C : C), MODE == ONE ? tn * 2 * C + C : tn * C};
+    int id = blockIdx.x, part = -1;
+    if (id >= p.whole && p.pieces > 1) { part = id - p.whole; id = p.whole + part / p.pieces; }
+    const Tile<C, MODE> tile(p, id);
+    const int m0 = tile.m0, n0[2] = {tile.n0[0], tile.n0[1]};
     const int am = MODE == TWO ? p.wa : p.M, bm = MODE != GATED ? p.wb : p.N;      // rows (columns) that may be read
     const int bat[2] = {n0[0], min(n0[1], bm - 8 < 0 ? 0 : bm - 8)};              // where the halves' pointers stand
 
@@ -199,7 +258,8 @@ __global__ __launch_bounds__(C * 4) void gemm_kernel(GemmArgs p) {
     const int enda = p.ka - (p.units - 1) * 64, endb = p.kb - (p.units - 1) * 64;  // what the last unit of a segment holds
     const bool ragged = enda < 64 || endb < 64;
 
-    const int u_begin = split * p.units_per_split, u_end = min(p.nseg * p.units, u_begin + p.units_per_split), count = u_end - u_begin;
+    const int u_begin = part < 0 ? 0 : part % p.pieces * p.units_per_piece;
+    const int count = part < 0 ? p.nseg * p.units : min(p.nseg * p.units - u_begin, p.units_per_piece);
     int seg = u_begin / p.units, left = p.units - (u_begin - seg * p.units);      // units left in the segment that is requested
     const char *pa, *pb0, *pb1;
     auto segment = [&](int unit) __attribute__((always_inline)) {
@@ -312,71 +372,46 @@ __global__ __launch_bounds__(C * 4) void gemm_kernel(GemmArgs p) {
         for (int q = 0; q < 4; ++q) multiply(f1, q);
     }
 
-    if constexpr (MODE == GATED) {
-        const int n = n0[0] + wn * 32 + (lane >> 4) * 4;
-        float bg[HF][4], bu[HF][4];
+    if (part < 0) {
+        const Store<C, MODE> store(p, tile, wave, lane);
 #pragma unroll
-        for (int j = 0; j < HF; ++j)
+        for (int i = 0; i < MF; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int c = min(n + j * 16 + e, p.N - 1);
-                bg[j][e] = p.bias0 ? seq_param(p.bias0, c, p.dtype) : 0.f;
-                bu[j][e] = p.bias1 ? seq_param(p.bias1, c, p.dtype) : 0.f;
-            }
+            for (int j = 0; j < HF; ++j) store(i, j, acc[i][0][j], acc[i][1][j]);
+    } else {
+        f32x4* o = p.part + ((long)part * (MF * 2 * HF)) * (C * 4) + threadIdx.x;
 #pragma unroll
-        for (int i = 0; i < MF; ++i) {
-            const int m = m0 + wm * C + i * 16 + (lane & 15);
-            if (m >= p.M) continue;
+        for (int i = 0; i < MF; ++i)
 #pragma unroll
-            for (int j = 0; j < HF; ++j) {
-                const int cnt = min(4, p.N - n - j * 16);
-                if (cnt <= 0) continue;
-                float g[4], u[4], v[4];
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { g[e] = acc[i][0][j][e] + bg[j][e]; u[e] = acc[i][1][j][e] + bu[j][e]; }
-                if (p.dtype == MOTIF_F32) gate4<false>(g, u, v, p.act); else gate4<true>(g, u, v, p.act);
-                store_as<4>(p.c0, (long)m * p.N + n + j * 16, v, cnt, p.vec, p.dtype);
-                if (p.g) {                               // (their rows are padded to whole runs)
-                    seq_store16<float, 4>(p.g + m * p.ldg + n + j * 16, g);
-                    seq_store16<float, 4>(p.u + m * p.ldg + n + j * 16, u);
-                }
-            }
-        }
-        return;
-    }
-    const int lo = lane & 15, hi = (lane >> 4) * 4;
-#pragma unroll
-    for (int i = 0; i < MF; ++i) {
-#pragma unroll
-        for (int j = 0; j < HF; ++j) {
-            const int mt = m0 + wm * C + i * 16, off = wn * 32 + j * 16;
-            {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = MODE == ONE ? mt + lo : n0[h] + off + lo, col = MODE == ONE ? n0[h] + off + hi : mt + hi;
-                    const int rows = MODE == ONE ? p.M : p.N, cols = MODE == ONE ? p.N : p.M, cnt = min(4, cols - col);
-                    if (row >= rows || cnt <= 0) continue;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = acc[i][h][j][e];
-                    const long at = (long)row * cols + col;
-                    if (p.part) store_run<float, float, 4>(p.part + (MODE == ONE ? (long)split : (long)split * 2 + h) * rows * cols, at, v, cnt, p.vec);
-                    else store_as<4>(MODE == ONE || h == 0 ? p.c0 : p.c1, at, v, cnt, p.vec, p.dtype);
-                }
-            }
-        }
+                for (int j = 0; j < HF; ++j) o[((i * 2 + h) * HF + j) * (C * 4)] = acc[i][h][j];
     }
 }
 
-// The pieces of a split reduction, added in order.  part [splits][n], n = n0 + n1 values to out0 and out1.
-__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, long n0, long n1, void* out0, void* out1, int dtype) {
-    const long n = n0 + n1;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
-        float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += part[k * n + i];
-        if (i < n0) { if (out0) seq_param_store(out0, i, dtype, s); }
-        else if (out1) seq_param_store(out1, i - n0, dtype, s);
+// The pieces of a tile's reduction, added in a fixed order, and the tile's outputs: a workgroup takes one fragment pair of all waves, its 1024 threads
+// as groups of a tile's threads, each of which adds a run of the pieces.
+template <int C, GemmMode MODE>
+__global__ __launch_bounds__(1024) void join_kernel(GemmArgs p) {
+    constexpr int MF = C / 16, TH = C * 4, GROUPS = 1024 / TH;
+    __shared__ f32x4 sh[GROUPS - 1][2][TH];
+    const int id = blockIdx.x / (MF * 2), i = blockIdx.x / 2 % MF, j = blockIdx.x % 2, tid = threadIdx.x % TH, group = threadIdx.x / TH;
+    const int run = (p.pieces + GROUPS - 1) / GROUPS, k1 = min(p.pieces, (group + 1) * run);
+    const f32x4* o = p.part + ((long)id * p.pieces * (MF * 4) + i * 4 + j) * TH + tid;
+    f32x4 v0 = {0.f, 0.f, 0.f, 0.f}, v1 = v0;
+#pragma unroll 4
+    for (int k = group * run; k < k1; ++k) {
+        v0 += o[(long)k * (MF * 4) * TH];
+        v1 += o[((long)k * (MF * 4) + 2) * TH];
     }
+    if (group) { sh[group - 1][0][tid] = v0; sh[group - 1][1][tid] = v1; }
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 0; g < GROUPS - 1; ++g) { v0 += sh[g][0][tid]; v1 += sh[g][1][tid]; }
+    const Tile<C, MODE> tile(p, p.whole + id);
+    const Store<C, MODE> store(p, tile, __builtin_amdgcn_readfirstlane(tid >> 6), tid & 63);
+    if (j == 0) store(i, 0, v0, v1); else store(i, 1, v0, v1);
 }
 
 // ---- laying operands out -----------------------------------------------------------------------------------------------------------------
@@ -425,20 +460,20 @@ __global__ __launch_bounds__(256) void layout_kernel(const T* __restrict__ src, 
 }
 
 // dG and dU: [rows][ld], ld = F rounded up to 8 (G and U have it too), zeros behind F; fp32: three planes.  dU lies `pair` elements behind dG.
-// A workgroup takes 256 columns x 64 rows, eight columns per thread, and sums its columns over its rows (part [row blocks][2][F], may be null).
+// A workgroup takes 256 columns x `rows` rows, eight columns per thread, and sums its columns over its rows (part [row blocks][2][F], may be null).
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh, long dhs, const float* __restrict__ G, const float* __restrict__ U, int M, int F, int ld, int act,
-                                                       void* dst, long plane, long pair, float* part) {
+                                                       void* dst, long plane, long pair, float* part, int rows) {
     using O = std::conditional_t<sizeof(T) == 4, bf16_t, T>;
     __shared__ float sh[8][2][32][9];
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.y * 256 + x * 8;
-    const long r0 = (long)blockIdx.x * 64;
+    const long r0 = (long)blockIdx.x * rows;
     float sg[8], su[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sg[e] = su[e] = 0.f;
     if (c < ld) {
 #pragma unroll 2
-        for (int i = y; i < 64; i += 8) {
+        for (int i = y; i < rows; i += 8) {
             const long r = r0 + i;
             if (r >= M) break;
             float d[8], g[8], u[8];
@@ -451,7 +486,7 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 float v, dv;
-                gate_grad(g[e], act, v, dv);
+                gate_grad<sizeof(T) == 2>(g[e], act, v, dv);
                 g[e] = c + e < F ? d[e] * u[e] * dv : 0.f;
                 u[e] = c + e < F ? d[e] * v : 0.f;
                 sg[e] += g[e];
@@ -591,30 +626,42 @@ void segments(GemmArgs& g, const Image& a, const Image& b0, const Image& b1) {
     }
 }
 
-// Tiles of 256 x 256 (C = 128) where they give every CU at least one, else of 128 x 128.  The reduction is split where even those leave CUs without work and
-// the pieces stay long (8 units of 64 at least); the pieces' sums are fp32 and joined in order.
-struct GemmPlan { bool big; int tiles_m, tiles_n, splits, units_per_split; };
-GemmPlan gemm_plan(long M, long N, int halves, long total_units, bool may_split) {
+// Tiles of 256 x 256 (C = 128) where they give every CU at least one, else of 128 x 128, of which a CU holds two.  The tiles behind the last whole round
+// of the chip are cut along the reduction so that their pieces fill it: the accumulators of a round are 64 MB, written and read again in about as long
+// as 24 units of a tile take (8192 x 2048 x 5632 bf16, weights' gradients: 352 tiles, 380 us in two rounds, 326 us with the second one cut in two).
+struct GemmPlan { bool big; int tiles_m, tiles_n, whole, pieces, units_per_piece; };
+GemmPlan gemm_plan(long M, long N, int halves, long units) {
     GemmPlan p;
-    auto tiles = [&](int t) { return (long)cdiv(M, t) * cdiv(N, halves == 2 ? t / 2 : t); };
-    p.big = tiles(256) >= 256;
+    auto tiles_of = [&](int t) { return (long)cdiv(M, t) * cdiv(N, halves == 2 ? t / 2 : t); };
+    p.big = tiles_of(256) >= 256;
     const int t = p.big ? 256 : 128;
+    const long tiles = tiles_of(t), slots = p.big ? 256 : 512, rest = tiles % slots;
     p.tiles_m = cdiv(M, t);
     p.tiles_n = cdiv(N, halves == 2 ? t / 2 : t);
-    long splits = may_split && !p.big ? 512 / tiles(t) : 1;
-    if (splits > total_units / 8) splits = total_units / 8;
-    if (splits < 1) splits = 1;
-    p.units_per_split = (int)((total_units + splits - 1) / splits);
-    p.splits = (int)((total_units + p.units_per_split - 1) / p.units_per_split);
+    long pieces = rest ? slots / rest : 1;
+    if (pieces > units / 8) pieces = units / 8;
+    if (pieces < 2 || units * (pieces - 1) < 24 * pieces) pieces = 1;
+    p.units_per_piece = (int)((units + pieces - 1) / pieces);
+    p.pieces = (int)((units + p.units_per_piece - 1) / p.units_per_piece);
+    p.whole = (int)(p.pieces > 1 ? tiles - rest : tiles);
     return p;
 }
+long part_bytes(const GemmPlan& p) {
+    const long cut = (long)p.tiles_m * p.tiles_n - p.whole;
+    return cut * p.pieces * (p.big ? 4L * 256 * 256 : 4L * 128 * 128);
+}
 
+template <typename T, int C, GemmMode MODE>
+void gemm_tiles(const GemmPlan& pl, const GemmArgs& g, hipStream_t s) {
+    const int cut = pl.tiles_m * pl.tiles_n - pl.whole;
+    gemm_kernel<T, C, MODE><<<(unsigned)(pl.whole + (long)cut * pl.pieces), C * 4, 0, s>>>(g);
+    if (cut) join_kernel<C, MODE><<<cut * (C / 16) * 2, 1024, 0, s>>>(g);
+}
 template <typename T, GemmMode MODE>
 void gemm(const GemmPlan& pl, GemmArgs& g, hipStream_t s) {
-    g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n; g.splits = pl.splits; g.units_per_split = pl.units_per_split;
-    const unsigned grid = (unsigned)((long)pl.tiles_m * pl.tiles_n * pl.splits);
-    if (pl.big) gemm_kernel<T, 128, MODE><<<grid, 512, 0, s>>>(g);
-    else gemm_kernel<T, 64, MODE><<<grid, 256, 0, s>>>(g);
+    g.tiles_m = pl.tiles_m; g.tiles_n = pl.tiles_n; g.whole = pl.whole; g.pieces = pl.pieces; g.units_per_piece = pl.units_per_piece;
+    if (pl.big) gemm_tiles<T, 128, MODE>(pl, g, s);
+    else gemm_tiles<T, 64, MODE>(pl, g, s);
 }
 template <GemmMode MODE>
 void gemm_dtype(int dtype, const GemmPlan& pl, GemmArgs& g, hipStream_t s) {
@@ -657,7 +704,15 @@ void lay_out(const Inputs& f, bool need_x, bool need_w, const void* x, long xs, 
     });
 }
 
-struct Backward { Inputs in; Image dg, du; float *bias_part, *split_part; GemmPlan dx, dw; };
+// Rows of a workgroup of gate_grad_kernel: 64, fewer where that would leave less than four workgroups per CU.
+int grad_rows(long M, long F) {
+    int rows = 64;
+    while (rows > 8 && (long)cdiv(M, rows) * cdiv(F, 256) < 1024) rows /= 2;
+    return rows;
+}
+GemmPlan fwd_plan(long M, long K, long F, int dtype) { return gemm_plan(M, F, 2, (long)(planes(dtype) == 3 ? 6 : 1) * units_of(K)); }
+
+struct Backward { Inputs in; Image dg, du; float* bias_part; f32x4* part; GemmPlan dx, dw; };
 Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype, bool need_x, bool need_w, bool need_b) {
     Backward b = {};
     const int n = planes(dtype), ld = up8(F);
@@ -665,18 +720,13 @@ Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const vo
     char* p = (char*)ws.take(2L * 2 * n * M * ld);
     b.dg = {p, M * ld, ld, n};
     b.du = {p ? p + 2L * n * M * ld : nullptr, M * ld, ld, n};
-    if (need_x) b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * units_of(ld), true);
-    if (need_w) b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * units_of(M), true);
-    if (need_b) b.bias_part = (float*)ws.take(4L * cdiv(M, 64) * 2 * F);
-    long part = 0;                                       // the two products run one behind the other: one piece of memory serves both
-    if (need_x && b.dx.splits > 1) part = 4L * b.dx.splits * M * K;
-    if (need_w && b.dw.splits > 1) { const long w = 4L * b.dw.splits * 2 * F * K; part = w > part ? w : part; }
-    if (part) b.split_part = (float*)ws.take(part);
+    if (need_x) b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * units_of(ld));
+    if (need_w) b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * units_of(M));
+    if (need_b) b.bias_part = (float*)ws.take(4L * cdiv(M, grad_rows(M, F)) * 2 * F);
+    long part = need_x ? part_bytes(b.dx) : 0;           // the two products run one behind the other: one piece of memory serves both
+    if (need_w && part_bytes(b.dw) > part) part = part_bytes(b.dw);
+    if (part) b.part = (f32x4*)ws.take(part);
     return b;
-}
-void join(const float* part, int splits, long n0, long n1, void* o0, void* o1, int dtype, hipStream_t s) {
-    const long blocks = (n0 + n1 + 255) / 256;
-    join_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(part, splits, n0, n1, o0, o1, dtype);
 }
 }  // namespace
 
@@ -686,6 +736,7 @@ extern "C" long motif_gated_mlp_ws_bytes(const void* x, long x_rs, const void* w
     if (M <= kFewRows) return 0;
     Arena ws = {nullptr, 0};
     inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+    ws.take(part_bytes(fwd_plan(M, K, F, dtype)));
     return ws.used;
 }
 
@@ -710,6 +761,8 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
     }
     Arena ws = {(char*)workspace, 0};
     const Inputs f = inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+    const GemmPlan plan = fwd_plan(M, K, F, dtype);
+    f32x4* part = (f32x4*)ws.take(part_bytes(plan));
     if (ws.used && !workspace) return MOTIF_EINVAL;
     lay_out(f, true, true, x, x_rs, w_gate, w_up, M, K, F, dtype, s);
     GemmArgs g = {};
@@ -721,7 +774,8 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
     g.c0 = h; g.g = G; g.u = U; g.ldg = up8(F); g.bias0 = b_gate; g.bias1 = b_up;
     g.act = act; g.dtype = dtype;
     g.vec = F % 4 == 0 && seq_aligned(h, 16);
-    gemm_dtype<GATED>(dtype, gemm_plan(M, F, 2, (long)g.nseg * g.units, false), g, s);
+    g.part = part;
+    gemm_dtype<GATED>(dtype, plan, g, s);
     MOTIF_LAUNCH_CHECK();
     return MOTIF_OK;
 }
@@ -748,14 +802,15 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
     lay_out(b.in, need_w, need_x, x, x_rs, w_gate, w_up, M, K, F, dtype, s);
     seq_dispatch(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const dim3 grid(cdiv(M, 64), cdiv(b.dg.ld, 256));
+        const int rows = grad_rows(M, F);
+        const dim3 grid(cdiv(M, rows), cdiv(b.dg.ld, 256));
         if (F % 8 == 0 && dh_rs % 8 == 0 && seq_aligned(dh, 16))
-            gate_grad_kernel<T, true><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part);
+            gate_grad_kernel<T, true><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows);
         else
-            gate_grad_kernel<T, false><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part);
+            gate_grad_kernel<T, false><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows);
     });
     if (need_b) {
-        const int r = seq_colsum2(b.bias_part, cdiv(M, 64), F, db_gate, db_up, dtype, s);
+        const int r = seq_colsum2(b.bias_part, cdiv(M, grad_rows(M, F)), F, db_gate, db_up, dtype, s);
         if (r) return r;
     }
     if (need_x) {                                        // the second pair continues the reduction of the first
@@ -767,10 +822,9 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         g.units = units_of(b.dg.ld);
         g.M = (int)M; g.N = (int)K; g.wb = up8(K);
         g.c0 = dx; g.dtype = dtype;
-        g.part = b.dx.splits > 1 ? b.split_part : nullptr;
+        g.part = b.part;
         g.vec = K % 4 == 0 && seq_aligned(dx, 16);
         gemm_dtype<ONE>(dtype, b.dx, g, s);
-        if (g.part) join(g.part, b.dx.splits, M * K, 0, dx, nullptr, dtype, s);
     }
     if (need_w) {
         GemmArgs g = {};
@@ -780,10 +834,9 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         g.units = units_of(M);
         g.M = (int)K; g.N = (int)F; g.wa = up8(K); g.wb = b.dg.ld;
         g.c0 = dw_gate; g.c1 = dw_up; g.dtype = dtype;
-        g.part = b.dw.splits > 1 ? b.split_part : nullptr;
+        g.part = b.part;
         g.vec = K % 4 == 0 && seq_aligned(dw_gate, 16) && seq_aligned(dw_up, 16);
         gemm_dtype<TWO>(dtype, b.dw, g, s);
-        if (g.part) join(g.part, b.dw.splits, F * K, F * K, dw_gate, dw_up, dtype, s);
     }
     MOTIF_LAUNCH_CHECK();
     return MOTIF_OK;
