@@ -93,7 +93,7 @@ __device__ u32x4 g_zeros;                                // what lies behind the
 template <typename T, typename O, int N>
 __device__ __forceinline__ void store_run(void* p, long at, const float (&v)[N], int n, bool vec) {      // n of N values; whole aligned runs as one store
     O* o = (O*)p + at;
-    if (vec && n == N) seq_store16<O, N>(o, v);
+    if (vec && n == N) seq_store<O, N>(o, v);
     else
 #pragma unroll
         for (int i = 0; i < N; ++i) if (i < n) o[i] = (O)v[i];
@@ -207,8 +207,8 @@ struct Store {
             if (p.dtype == MOTIF_F32) gate4<false>(g, u, v, p.act); else gate4<true>(g, u, v, p.act);
             store_as<4>(p.c0, (long)row * p.N + n, v, cnt, p.vec, p.dtype);
             if (p.g) {                                   // (their rows are padded to whole runs)
-                seq_store16<float, 4>(p.g + row * p.ldg + n, g);
-                seq_store16<float, 4>(p.u + row * p.ldg + n, u);
+                seq_store<float, 4>(p.g + row * p.ldg + n, g);
+                seq_store<float, 4>(p.u + row * p.ldg + n, u);
             }
         } else {
 #pragma unroll
@@ -430,19 +430,19 @@ __device__ __forceinline__ void split3(float x, bf16_t (&out)[3]) {
 }
 // eight values: one plane of T, or three of bf16, `plane` elements apart
 __device__ __forceinline__ void put8(float* /*type*/, void* dst, long plane, long at, const float (&v)[8]) {
-    SeqVec<bf16_t, 8> o[3];
+    float o[3][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         bf16_t s[3];
         split3(v[e], s);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) o[i].v[e] = s[i];
+        for (int i = 0; i < 3; ++i) o[i][e] = (float)s[i];
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) *(SeqVec<bf16_t, 8>*)((bf16_t*)dst + i * plane + at) = o[i];
+    for (int i = 0; i < 3; ++i) seq_store<bf16_t, 8>((bf16_t*)dst + i * plane + at, o[i]);
 }
-__device__ __forceinline__ void put8(bf16_t*, void* dst, long, long at, const float (&v)[8]) { seq_store16<bf16_t, 8>((bf16_t*)dst + at, v); }
-__device__ __forceinline__ void put8(f16_t*, void* dst, long, long at, const float (&v)[8]) { seq_store16<f16_t, 8>((f16_t*)dst + at, v); }
+__device__ __forceinline__ void put8(bf16_t*, void* dst, long, long at, const float (&v)[8]) { seq_store<bf16_t, 8>((bf16_t*)dst + at, v); }
+__device__ __forceinline__ void put8(f16_t*, void* dst, long, long at, const float (&v)[8]) { seq_store<f16_t, 8>((f16_t*)dst + at, v); }
 
 // src [rows][cols] with row stride rs -> dst rows of ld = cols rounded up to 8, zeros behind the last value of a row.  Eight values per thread.
 template <typename T>
@@ -453,15 +453,17 @@ __global__ __launch_bounds__(256) void layout_kernel(const T* __restrict__ src, 
         const long r = i / per;
         const int c = (int)(i - r * per) * 8;
         float v[8];
+        if (c + 8 <= cols) seq_load<T, 8>(src + r * rs + c, v);
+        else
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? (float)src[r * rs + c + e] : 0.f;
+            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? (float)src[r * rs + c + e] : 0.f;
         put8((T*)nullptr, dst, plane, r * ld + c, v);
     }
 }
 
 // dG and dU: [rows][ld], ld = F rounded up to 8 (G and U have it too), zeros behind F; fp32: three planes.  dU lies `pair` elements behind dG.
 // A workgroup takes 256 columns x `rows` rows, eight columns per thread, and sums its columns over its rows (part [row blocks][2][F], may be null).
-template <typename T, bool VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh, long dhs, const float* __restrict__ G, const float* __restrict__ U, int M, int F, int ld, int act,
                                                        void* dst, long plane, long pair, float* part, int rows) {
     using O = std::conditional_t<sizeof(T) == 4, bf16_t, T>;
@@ -477,12 +479,12 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
             const long r = r0 + i;
             if (r >= M) break;
             float d[8], g[8], u[8];
-            if (VEC) seq_load16<T, 8>(dh + r * dhs + c, d);
+            if (c + 8 <= F) seq_load<T, 8>(dh + r * dhs + c, d);
             else
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[e] = c + e < F ? (float)dh[r * dhs + c + e] : 0.f;
-            seq_load16<float, 8>(G + r * ld + c, g);
-            seq_load16<float, 8>(U + r * ld + c, u);
+            seq_load<float, 8>(G + r * ld + c, g);
+            seq_load<float, 8>(U + r * ld + c, u);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 float v, dv;
@@ -513,8 +515,8 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
 // ---- few rows ----------------------------------------------------------------------------------------------------------------------------
 // Up to 16 MT rows: a workgroup takes 16 columns of both projections, its 8 waves share the reduction, each lane reads 16 bytes of a weight row
 // (16 rows x 4 pieces per instruction) straight into the matrix instruction's operand; the waves' sums meet in LDS in a fixed order.  Bound by
-// the weights' bytes.  fp32 runs on the fp32 matrix instruction.  VEC: every row allows 16-byte reads.
-template <typename T, int MT, bool VEC>
+// the weights' bytes.  fp32 runs on the fp32 matrix instruction.
+template <typename T, int MT>
 __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long xs, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ bg, const T* __restrict__ bu,
                                                    T* __restrict__ h, float* __restrict__ G, float* __restrict__ U, long ldg, int M, int K, int F, int act) {
     constexpr int V = 16 / sizeof(T), STEP = 4 * V, NW = 8;
@@ -527,21 +529,16 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
 #pragma unroll
     for (int i = 0; i < MT; ++i) ag[i] = au[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto read = [&](const T* row, int k) __attribute__((always_inline)) {
-        SeqVec<T, V> v;
-        if (VEC) {
-            if (k < K) v = *(const SeqVec<T, V>*)(row + k);
-            else
+        if (k + V <= K) return seq_raw<T, V>(row + k);
+        SeqRaw<T, V> v;
 #pragma unroll
-                for (int e = 0; e < V; ++e) v.v[e] = (T)0.f;
-        } else
-#pragma unroll
-            for (int e = 0; e < V; ++e) v.v[e] = k + e < K ? row[k + e] : (T)0.f;
+        for (int e = 0; e < V; ++e) v.v[e] = k + e < K ? row[k + e] : (T)0.f;
         return v;
     };
     const int steps = (K + STEP - 1) / STEP;
     constexpr int AHEAD = MT == 1 ? 4 : 2;
     for (int s = wave; s < steps; s += NW * AHEAD) {
-        SeqVec<T, V> a[AHEAD], b[AHEAD], c[AHEAD][MT];
+        SeqRaw<T, V> a[AHEAD], b[AHEAD], c[AHEAD][MT];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             const int k = (s + j * NW) * STEP + kq;      // behind the last step: zeros
@@ -561,8 +558,8 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
                 } else {
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        ag[i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)a[j].v[e], (float)c[j][i].v[e], ag[i], 0, 0, 0);
-                        au[i] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)b[j].v[e], (float)c[j][i].v[e], au[i], 0, 0, 0);
+                        ag[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j][e], c[j][i][e], ag[i], 0, 0, 0);
+                        au[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j][e], c[j][i][e], au[i], 0, 0, 0);
                     }
                 }
             }
@@ -679,9 +676,8 @@ int check_mlp(long M, long K, long F, int act, int dtype) {
 }
 
 template <typename T, int MT>
-void few_rows(bool vec, const void* x, long xs, const void* wg, const void* wu, const void* bg, const void* bu, void* h, float* G, float* U, int M, int K, int F, int act, hipStream_t s) {
-    if (vec) rows_kernel<T, MT, true><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
-    else rows_kernel<T, MT, false><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
+void few_rows(const void* x, long xs, const void* wg, const void* wu, const void* bg, const void* bu, void* h, float* G, float* U, int M, int K, int F, int act, hipStream_t s) {
+    rows_kernel<T, MT><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
 }
 
 // x, Wg and Wu as the products read them: as they lie, or laid out in the workspace.
@@ -748,13 +744,11 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
     if (!x || !w_gate || !w_up || !h || x_rs < 0 || !G != !U) return MOTIF_EINVAL;
     hipStream_t s = (hipStream_t)stream;
     if (M <= kFewRows) {
-        const int V = 16 / seq_size(dtype);
-        const bool vec = K % V == 0 && x_rs % V == 0 && seq_aligned(x, 16) && seq_aligned(w_gate, 16) && seq_aligned(w_up, 16);
         seq_dispatch(dtype, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            if (M <= 16) few_rows<T, 1>(vec, x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
-            else if (M <= 32) few_rows<T, 2>(vec, x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
-            else few_rows<T, 4>(vec, x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
+            if (M <= 16) few_rows<T, 1>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
+            else if (M <= 32) few_rows<T, 2>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
+            else few_rows<T, 4>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
         });
         MOTIF_LAUNCH_CHECK();
         return MOTIF_OK;
@@ -804,10 +798,7 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         using T = std::remove_pointer_t<decltype(t)>;
         const int rows = grad_rows(M, F);
         const dim3 grid(cdiv(M, rows), cdiv(b.dg.ld, 256));
-        if (F % 8 == 0 && dh_rs % 8 == 0 && seq_aligned(dh, 16))
-            gate_grad_kernel<T, true><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows);
-        else
-            gate_grad_kernel<T, false><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows);
+        gate_grad_kernel<T><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows);
     });
     if (need_b) {
         const int r = seq_colsum2(b.bias_part, cdiv(M, grad_rows(M, F)), F, db_gate, db_up, dtype, s);

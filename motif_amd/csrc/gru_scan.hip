@@ -9,7 +9,7 @@
 // initial state inside H, so sequences packed one behind the other are one recurrence over all rows.
 //
 // Bound by memory (forward 2 reads and 1 write, backward 4 reads and 2 writes of the data).  A workgroup owns TX lanes x V channels and TY time
-// slots of R rows each: a tile of TY R rows lies in registers between the composition of its slots (lanes of a wave by shuffles, the waves
+// slots of R rows each: a tile of TY R rows lies in registers, as it was read, between the composition of its slots (lanes of a wave by shuffles, the waves
 // through LDS) and the second walk over its rows that writes them.  TY = 1 where channels alone fill the chip or the sequence is short.  Where
 // channels are few, a sequence is cut into segments: a first kernel reads what the composition needs and writes every segment's (A, H), and each
 // segment's workgroup then composes those before it, in a fixed order -- the cost is a second read of half the inputs.  The states, A and H are
@@ -85,12 +85,12 @@ __device__ __forceinline__ void zero(float (&x)[V], float c = 0.f) {
 }
 
 // The composition of one row: forward  x -> a x + z q (first: a h0 + z q),   backward  c -> a (c + dh) (last: a (dlast + dh)).
-template <bool BWD, int V>
-__device__ __forceinline__ void compose(float (&A)[V], float (&H)[V], const float (&z)[V], const float (&x)[V], int flag, const float* init, int c0, int D) {
+template <bool BWD, int V, typename X>
+__device__ __forceinline__ void compose(float (&A)[V], float (&H)[V], const X& z, const X& x, int flag, const float* init, int c0, int D) {
     float s[V];
     zero(s);
     const bool cut = flag >= 0 && (flag & (BWD ? kLast : kFirst));
-    if (cut && init) seq_load16<float, V>(init + (long)(flag >> 2) * D + c0, s);
+    if (cut && init) seq_load<float, V>(init + (long)(flag >> 2) * D + c0, s);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const float a = 1.f - z[v];
@@ -120,8 +120,8 @@ __global__ __launch_bounds__(256) void gru_scan_segments_kernel(ScanArgs p) {
     __shared__ float tot[4][2][TX * V];
     const Where at = where(p);
     if (at.seg == p.segs - 1) return;
-    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, c0 = (at.group * TX + tx) * V;
-    const bool on = c0 < p.D;
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, first = (at.group * TX + tx) * V, c0 = min(first, p.D - V);
+    const bool on = first < p.D;                         // (the last lane of a row takes its last V channels: those it shares are written twice, alike)
     const T* z = (const T*)p.z + at.b * p.zb + c0;
     const T* x = BWD ? (const T*)p.dh + at.b * p.db + c0 : (const T*)p.q + at.b * p.qb + c0;
     const long xr = BWD ? p.dr : p.qr;
@@ -131,13 +131,13 @@ __global__ __launch_bounds__(256) void gru_scan_segments_kernel(ScanArgs p) {
     zero(H);
     if (on) {
         for (long k = k0; k < k0 + run; k += 4) {
-            float zv[4][V], xv[4][V];
+            SeqRaw<T, V> zv[4], xv[4];
             int f[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const long t = BWD ? p.T - 1 - (k + r) : k + r;
-                seq_load<T, V>(z + t * p.zr, zv[r]);
-                seq_load<T, V>(x + t * xr, xv[r]);
+                zv[r] = seq_raw<T, V>(z + t * p.zr);
+                xv[r] = seq_raw<T, V>(x + t * xr);
                 f[r] = row_flag(p, at.b, t);
             }
 #pragma unroll
@@ -155,8 +155,8 @@ __global__ __launch_bounds__(256) void gru_scan_segments_kernel(ScanArgs p) {
 #pragma unroll
             for (int w = 0; w < S::WAVES; ++w) { H[v] = fmaf(tot[w][0][tx * V + v], H[v], tot[w][1][tx * V + v]); A[v] *= tot[w][0][tx * V + v]; }
         }
-        seq_store16<float, V>(o, A);
-        seq_store16<float, V>(o + p.D, H);
+        seq_store<float, V>(o, A);
+        seq_store<float, V>(o + p.D, H);
     }
 }
 
@@ -165,14 +165,19 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
     using S = Slots<V, TX, TY>;
     __shared__ float tot[2][4][2][TX * V];
     const Where at = where(p);
-    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, c0 = (at.group * TX + tx) * V;
-    const bool on = c0 < p.D;
-    const T* z = (const T*)p.z + at.b * p.zb + c0;
-    const T* q = (const T*)p.q + at.b * p.qb + c0;
-    const T* dh = BWD ? (const T*)p.dh + at.b * p.db + c0 : nullptr;
-    const T* hs = BWD ? (const T*)p.h + at.b * p.T * p.D + c0 : nullptr;
-    T* out0 = p.out0 ? (T*)p.out0 + at.b * p.T * p.D + c0 : nullptr;
-    T* out1 = p.out1 ? (T*)p.out1 + at.b * p.T * p.D + c0 : nullptr;
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, first = (at.group * TX + tx) * V, c0 = min(first, p.D - V);
+    const bool on = first < p.D;                         // (the last lane of a row takes its last V channels: those it shares are written twice, alike)
+    // Addresses: a uniform row of the tile, and a lane's offset from it in bytes (32 bits: the host bounds the strides where TY > 1).  Backward, time
+    // runs down: slot TY - 1 has the tile's first rows.
+    const int slot = (BWD ? TY - 1 - ty : ty) * R;
+    const unsigned oz = (unsigned)(slot * (unsigned)p.zr + c0) * sizeof(T), oq = (unsigned)(slot * (unsigned)p.qr + c0) * sizeof(T);
+    const unsigned od = BWD ? (unsigned)(slot * (unsigned)p.dr + c0) * sizeof(T) : 0u, oo = (unsigned)(slot * (unsigned)p.D + c0) * sizeof(T);
+    const char* z = (const char*)((const T*)p.z + at.b * p.zb);
+    const char* q = (const char*)((const T*)p.q + at.b * p.qb);
+    const char* dh = BWD ? (const char*)((const T*)p.dh + at.b * p.db) : nullptr;
+    const char* hs = BWD ? (const char*)((const T*)p.h + at.b * p.T * p.D) : nullptr;
+    char* out0 = p.out0 ? (char*)((T*)p.out0 + at.b * p.T * p.D) : nullptr;
+    char* out1 = p.out1 ? (char*)((T*)p.out1 + at.b * p.T * p.D) : nullptr;
     const long k_end = min(p.T, (at.seg + 1) * p.seg_rows);
     float carry[V];
     zero(carry);                                         // (a sequence's own initial value enters at its first row)
@@ -186,8 +191,8 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
             for (int s = ty * per; s < min(at.seg, (ty + 1) * per); ++s) {
                 float a[V], h[V];
                 const float* g = p.agg + ((at.b * p.segs + s) * 2) * p.D + c0;
-                seq_load16<float, V>(g, a);
-                seq_load16<float, V>(g + p.D, h);
+                seq_load<float, V>(g, a);
+                seq_load<float, V>(g + p.D, h);
 #pragma unroll
                 for (int v = 0; v < V; ++v) { H[v] = fmaf(a[v], H[v], h[v]); A[v] *= a[v]; }
             }
@@ -198,24 +203,24 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
         buf = 1;
     }
     for (long k0 = at.seg * p.seg_rows; k0 < k_end; k0 += TY * R) {
-        float zv[R][V], qv[R][V], dv[BWD ? R : 1][V], hv[BWD ? R : 1][V];
+        typedef SeqRaw<T, V> Raw;
+        Raw zv[R], qv[R], dv[BWD ? R : 1], hv[BWD ? R : 1];
         int f[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const long k = k0 + ty * R + r, t = BWD ? p.T - 1 - k : k;
             const bool in = on && k < k_end;
             f[r] = in ? row_flag(p, at.b, t) : 0;
+            zv[r] = qv[r] = Raw{};                       // no row: x -> x
+            if constexpr (BWD) dv[r] = hv[r] = Raw{};
+            const long t0 = BWD ? p.T - 1 - k0 - (TY * R - 1) + (R - 1 - r) : k0 + r;      // the uniform row (it need not exist: no lane reads it then)
             if (in) {
-                seq_load<T, V>(z + t * p.zr, zv[r]);
-                if (!BWD || out0) seq_load<T, V>(q + t * p.qr, qv[r]); else zero(qv[r]);
+                zv[r] = seq_raw<T, V>((const T*)(z + t0 * p.zr * (long)sizeof(T) + oz));
+                if (!BWD || out0) qv[r] = seq_raw<T, V>((const T*)(q + t0 * p.qr * (long)sizeof(T) + oq));
                 if constexpr (BWD) {
-                    seq_load<T, V>(dh + t * p.dr, dv[r]);
-                    if (out0 && t > 0) seq_load<T, V>(hs + (t - 1) * p.D, hv[r]); else zero(hv[r]);
+                    dv[r] = seq_raw<T, V>((const T*)(dh + t0 * p.dr * (long)sizeof(T) + od));
+                    if (out0 && t > 0) hv[r] = seq_raw<T, V>((const T*)(hs + (t0 - 1) * p.D * (long)sizeof(T) + oo));
                 }
-            } else {                                     // no row: x -> x
-                zero(zv[r]);
-                zero(qv[r]);
-                if constexpr (BWD) { zero(dv[r]); zero(hv[r]); }
             }
         }
         float h[V];
@@ -225,6 +230,8 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
             zero(H);
 #pragma unroll
             for (int r = 0; r < R; ++r) compose<BWD, V>(A, H, zv[r], BWD ? dv[BWD ? r : 0] : qv[r], f[r], BWD ? p.dlast : p.h0, c0, p.D);
+#pragma unroll
+            for (int r = 0; r < R; ++r) { seq_hold(zv[r]); if constexpr (BWD) seq_hold(dv[r]); else seq_hold(qv[r]); }
             S::wave_scan(A, H, tot[buf]);
             __syncthreads();                             // one barrier a tile: the next tile's sums go to the other buffer
             S::waves_apply(carry, in, tot[buf], tx);
@@ -237,29 +244,30 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const long k = k0 + ty * R + r, t = BWD ? p.T - 1 - k : k;
-            if (!on || k >= k_end) continue;
-            const long own = (long)(f[r] >> 2) * p.D + c0;
+            if (!on || k0 + ty * R + r >= k_end) continue;
+            const long own = (long)(f[r] >> 2) * p.D + c0, t0 = BWD ? p.T - 1 - k0 - (TY * R - 1) + (R - 1 - r) : k0 + r, out = t0 * p.D * (long)sizeof(T);
             if constexpr (!BWD) {
-                if (f[r] >= 0 && (f[r] & kFirst)) { if (p.h0) seq_load16<float, V>(p.h0 + own, h); else zero(h); }
+                if (f[r] >= 0 && (f[r] & kFirst)) { if (p.h0) seq_load<float, V>(p.h0 + own, h); else zero(h); }
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[v] = f[r] < 0 ? 0.f : fmaf(1.f - zv[r][v], h[v], zv[r][v] * qv[r][v]);
-                seq_store<T, V>(out0 + t * p.D, h);
-                if (p.state && f[r] >= 0 && (f[r] & kLast)) seq_store16<float, V>(p.state + own, h);
+                seq_store<T, V>((T*)(out0 + out + oo), h);
+                if (p.state && f[r] >= 0 && (f[r] & kLast)) seq_store<float, V>(p.state + own, h);
             } else {
-                if (f[r] >= 0 && (f[r] & kLast)) { if (p.dlast) seq_load16<float, V>(p.dlast + own, h); else zero(h); }
-                if (f[r] >= 0 && (f[r] & kFirst)) { if (p.h0) seq_load16<float, V>(p.h0 + own, hv[r]); else zero(hv[r]); }
-                float dz[V], dq[V];
+                if (f[r] >= 0 && (f[r] & kLast)) { if (p.dlast) seq_load<float, V>(p.dlast + own, h); else zero(h); }
+                float dz[V], dq[V], before[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) before[v] = hv[r][v];
+                if (f[r] >= 0 && (f[r] & kFirst)) { if (p.h0) seq_load<float, V>(p.h0 + own, before); else zero(before); }
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     const float g = f[r] < 0 ? 0.f : dv[r][v] + h[v];
-                    dz[v] = f[r] < 0 ? 0.f : g * (qv[r][v] - hv[r][v]);
+                    dz[v] = f[r] < 0 ? 0.f : g * (qv[r][v] - before[v]);
                     dq[v] = f[r] < 0 ? 0.f : g * zv[r][v];
                     h[v] = f[r] < 0 ? 0.f : (1.f - zv[r][v]) * g;
                 }
-                if (out0) seq_store<T, V>(out0 + t * p.D, dz);
-                if (out1) seq_store<T, V>(out1 + t * p.D, dq);
-                if (p.state && f[r] >= 0 && (f[r] & kFirst)) seq_store16<float, V>(p.state + own, h);
+                if (out0) seq_store<T, V>((T*)(out0 + out + oo), dz);
+                if (out1) seq_store<T, V>((T*)(out1 + out + oo), dq);
+                if (p.state && f[r] >= 0 && (f[r] & kFirst)) seq_store<float, V>(p.state + own, h);
             }
         }
         if constexpr (TY == 1) {
@@ -291,9 +299,10 @@ __global__ __launch_bounds__(256) void gru_scan_empty_kernel(const int* __restri
 
 struct Plan { int V, TX, TY, R, groups, segs; long seg_rows; };
 
-// Vectors of 16 bytes where every row of every tensor allows them, single values else.  TY = 1 (a lane walks the whole sequence) where the
+// Vectors of 16 bytes, single values for rows shorter than that.  TY = 1 (a lane walks the whole sequence) where the
 // sequence is no longer than 16 rows or the channels alone give every CU two workgroups; else 32 time slots (8 with single values, whose
 // rows need more lanes to fill a cache line).  Segments: as many as give every CU four workgroups, none below two tiles.
+int vec_of(int dtype, long D) { const int V = 16 / seq_size(dtype); return D < V ? 1 : V; }
 Plan plan_of(int V, long B, long T, long D) {
     Plan p;
     p.V = V;
@@ -320,26 +329,17 @@ template <typename T, int V, bool BWD>
 void launch(const Plan& pl, const ScanArgs& a, hipStream_t s) {
     const unsigned grid = (unsigned)((long)a.B * pl.segs * pl.groups);
     constexpr int TY = V > 1 ? 32 : 8;
-    if (pl.TY == 1) { gru_scan_kernel<T, V, 256, 1, 4, BWD><<<grid, 256, 0, s>>>(a); return; }
+    constexpr int R = BWD ? 2 : 4;                       // backward holds four tensors' rows
+    if (pl.TY == 1) { gru_scan_kernel<T, V, 256, 1, R, BWD><<<grid, 256, 0, s>>>(a); return; }
     if (pl.segs > 1) gru_scan_segments_kernel<T, V, 256 / TY, TY, BWD><<<grid, 256, 0, s>>>(a);
-    gru_scan_kernel<T, V, 256 / TY, TY, 4, BWD><<<grid, 256, 0, s>>>(a);
-}
-
-// Vector width of a call: every tensor's base and strides are multiples of 16 bytes (fp32 rows of states: of 16 bytes too).
-int vec_of(int dtype, long D, const long* strides, int ns, const void* const* ptrs, int np) {
-    const int V = 16 / seq_size(dtype);
-    if (D % V) return 1;
-    for (int i = 0; i < ns; ++i) if (strides[i] % V) return 1;
-    for (int i = 0; i < np; ++i) if (!seq_aligned(ptrs[i], 16)) return 1;
-    return V;
+    gru_scan_kernel<T, V, 256 / TY, TY, R, BWD><<<grid, 256, 0, s>>>(a);
 }
 
 int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const float* empty_in, hipStream_t s) {
-    const long strides[6] = {a.zb, a.zr, a.qb, a.qr, a.db, a.dr};
-    const void* ptrs[10] = {a.z, a.q, a.h, a.dh, a.h0, a.dlast, a.out0, a.out1, a.state, ws};
-    const int V = vec_of(dtype, a.D, strides, 6, ptrs, 10);
+    const int V = vec_of(dtype, a.D);
     const Plan pl = plan_of(V, a.B, a.T, a.D);
     if ((long)a.B * pl.segs * pl.groups > 0x7fffffffL) return MOTIF_ELIMIT;
+    if (pl.TY > 1) for (long stride : {a.zr, a.qr, a.dr, (long)a.D}) if (stride > 1L << 22) return MOTIF_ELIMIT;      // 128 rows x 4 bytes in 32 bits
     a.groups = pl.groups;
     a.segs = pl.segs;
     a.seg_rows = pl.seg_rows;
@@ -372,13 +372,8 @@ int check_sizes(long B, long T, long D, int S, const void* cu, int dtype) {
 extern "C" long motif_gru_scan_ws_floats(long B, long T, long D, int packed, int dtype) {
     const int rc = check_sizes(B, T, D, packed ? 1 : 0, packed ? (const void*)&B : nullptr, dtype);
     if (rc) return rc;
-    long need = 0;                                       // of either vector width: the pointers decide at the call
-    for (int V : {1, 16 / seq_size(dtype)}) {
-        const Plan p = plan_of(V, B, T, D);
-        const long n = p.segs > 1 ? ((B * p.segs * 2 * D + 3) & ~3L) : 0;
-        need = n > need ? n : need;
-    }
-    return need + (packed ? T : 0);
+    const Plan p = plan_of(vec_of(dtype, D), B, T, D);
+    return (p.segs > 1 ? ((B * p.segs * 2 * D + 3) & ~3L) : 0) + (packed ? T : 0);
 }
 
 extern "C" int motif_gru_scan_fwd(const void* z, long z_bs, long z_rs, const void* q, long q_bs, long q_rs, const float* h0, const int32_t* cu_seqlens, int S,

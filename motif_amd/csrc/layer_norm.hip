@@ -46,15 +46,30 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* sh) {
     }
 }
 
-// A lane's columns of a parameter; `none` where there is no parameter.  Columns behind D: 0.
+// Run j of a lane: V columns from `c`.  Rows need not be whole runs: the run that would pass the row's end moves back onto the row's last V values,
+// of which `skip` belong to the run before -- they count for nothing in the sums and are written twice, alike.
+template <int L, int V>
+struct Run {
+    int c, skip;
+    bool on;
+    __device__ __forceinline__ Run(int j, int lane, int D) {
+        const int first = (j * L + lane) * V;
+        on = first < D;
+        c = min(first, D - V);
+        skip = first - c;
+    }
+    __device__ __forceinline__ bool counts(int e) const { return on && e >= skip; }
+};
+
+// A lane's columns of a parameter; `none` where there is no parameter.
 template <int L, int V, int NV>
 __device__ __forceinline__ void params(const void* p, int D, int pdt, int lane, float none, float (&out)[NV][V]) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (j * L + lane) * V;
+        const Run<L, V> run(j, lane, D);
 #pragma unroll
-        for (int e = 0; e < V; ++e) out[j][e] = c < D ? none : 0.f;
-        if (p && c < D) seq_param_vec<V>(p, c, pdt, out[j]);
+        for (int e = 0; e < V; ++e) out[j][e] = none;
+        if (p && run.on) seq_param_vec<V>(p, run.c, pdt, out[j]);
     }
 }
 
@@ -68,26 +83,29 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_fwd_kernel(const
     const bool on = row < rows;
     const T* xr = x + (on ? row : 0) * xs;
     float v[NV][V], wv[NV][V], bv[NV][V];
-    params<L, V, NV>(w, D, pdt, lane, 1.f, wv);          // (requested first: on its way while the row is read and summed)
-    params<L, V, NV>(b, D, pdt, lane, 0.f, bv);
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (j * L + lane) * V;
-        if (on && c < D) seq_load<T, V>(xr + c, v[j]);
-        else
+        const Run<L, V> run(j, lane, D);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[j][e] = 0.f;
+        for (int e = 0; e < V; ++e) v[j][e] = 0.f;
+        if (on && run.on) seq_load<T, V>(xr + run.c, v[j]);
+    }
+    params<L, V, NV>(w, D, pdt, lane, 1.f, wv);          // (on its way while the row is summed)
+    params<L, V, NV>(b, D, pdt, lane, 0.f, bv);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += v[j][e];
+    for (int j = 0; j < NV; ++j) {
+        const Run<L, V> run(j, lane, D);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += run.counts(e) ? v[j][e] : 0.f;
     }
     const float mean = row_sum<L>(s, sh) / (float)D;
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const bool in = (j * L + lane) * V < D;
+        const Run<L, V> run(j, lane, D);
 #pragma unroll
-        for (int e = 0; e < V; ++e) { v[j][e] -= mean; q += in ? v[j][e] * v[j][e] : 0.f; }
+        for (int e = 0; e < V; ++e) { v[j][e] -= mean; q += run.counts(e) ? v[j][e] * v[j][e] : 0.f; }
     }
     const float r = 1.f / sqrtf(row_sum<L>(q, sh) / (float)D + eps);
     if (!on) return;
@@ -95,11 +113,11 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_fwd_kernel(const
     T* yr = y + row * (long)D;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (j * L + lane) * V;
-        if (c >= D) continue;
+        const Run<L, V> run(j, lane, D);
+        if (!run.on) continue;
 #pragma unroll
         for (int e = 0; e < V; ++e) v[j][e] = v[j][e] * r * wv[j][e] + bv[j][e];
-        seq_store<T, V>(yr + c, v[j]);
+        seq_store<T, V>(yr + run.c, v[j]);
     }
 }
 
@@ -116,30 +134,47 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_bwd_kernel(const
 #pragma unroll
         for (int e = 0; e < V; ++e) aw[j][e] = ab[j][e] = 0.f;
     const float inv = 1.f / (float)D;
-    for (long base = (long)blockIdx.x * R; base < rows; base += (long)gridDim.x * R) {
+    typedef SeqRaw<T, V> Raw;
+    const long step = (long)gridDim.x * R;
+    constexpr bool AHEAD = L < 1024;                     // 16 waves have 128 registers each: none to spare
+    Raw xn[NV], dn[NV];                                  // the next row, requested while this one is summed
+    float mean_n = 0.f, r_n = 0.f;
+    auto request = [&](long row) __attribute__((always_inline)) {
+        if (row >= rows) return;
+        mean_n = stats[2 * row];
+        r_n = stats[2 * row + 1];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const Run<L, V> run(j, lane, D);
+            if (run.on) { xn[j] = seq_raw<T, V>(x + row * xs + run.c); dn[j] = seq_raw<T, V>(dy + row * dys + run.c); }
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < NV; ++j) xn[j] = dn[j] = Raw{};
+    if (AHEAD) request((long)blockIdx.x * R + slot);
+    for (long base = (long)blockIdx.x * R; base < rows; base += step) {
         const long row = base + slot;
         const bool on = row < rows;
-        const T* xr = x + (on ? row : 0) * xs;
-        const T* dr = dy + (on ? row : 0) * dys;
-        const float mean = on ? stats[2 * row] : 0.f, r = on ? stats[2 * row + 1] : 0.f;
+        if (!AHEAD) request(row);
+        const float mean = mean_n, r = r_n;
         float n[NV][V], g[NV][V];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * L + lane) * V;
-            const bool in = on && c < D;
-            if (in) { seq_load<T, V>(xr + c, n[j]); seq_load<T, V>(dr + c, g[j]); }
+            const Run<L, V> run(j, lane, D);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                n[j][e] = in ? (n[j][e] - mean) * r : 0.f;
-                g[j][e] = in ? g[j][e] : 0.f;
-                aw[j][e] += g[j][e] * n[j][e];
-                ab[j][e] += g[j][e];
-                g[j][e] *= wv[j][e];
-                s1 += g[j][e];
-                s2 += g[j][e] * n[j][e];
+                n[j][e] = (xn[j][e] - mean) * r;
+                const float d = dn[j][e], gw = d * wv[j][e];
+                const bool counts = on && run.counts(e);
+                aw[j][e] += counts ? d * n[j][e] : 0.f;
+                ab[j][e] += counts ? d : 0.f;
+                s1 += counts ? gw : 0.f;
+                s2 += counts ? gw * n[j][e] : 0.f;
+                g[j][e] = gw;
             }
         }
+        if (AHEAD) request(row + step);
         if (dx) {
             row_sum2<L>(s1, s2, sh);
             s1 *= inv; s2 *= inv;
@@ -147,11 +182,17 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_bwd_kernel(const
                 T* xo = dx + row * (long)D;
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
-                    const int c = (j * L + lane) * V;
-                    if (c >= D) continue;
+                    const Run<L, V> run(j, lane, D);
+                    if (!run.on) continue;
+                    if constexpr (!AHEAD) {              // (from what was read: n and g of the first walk would not fit)
+                        seq_hold(xn[j]);
+                        seq_hold(dn[j]);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) { n[j][e] = (xn[j][e] - mean) * r; g[j][e] = dn[j][e] * wv[j][e]; }
+                    }
 #pragma unroll
                     for (int e = 0; e < V; ++e) g[j][e] = r * (g[j][e] - s1 - n[j][e] * s2);
-                    seq_store<T, V>(xo + c, g[j]);
+                    seq_store<T, V>(xo + run.c, g[j]);
                 }
             }
         }
@@ -163,25 +204,28 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_bwd_kernel(const
             __syncthreads();
             if (slot == k) {
 #pragma unroll
-                for (int j = 0; j < NV; ++j)
+                for (int j = 0; j < NV; ++j) {
+                    const Run<L, V> run(j, lane, D);
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        const int at = (j * L + lane) * V + e;
+                        const int at = run.c + e;
+                        if (!run.counts(e)) continue;
                         sh[at] = k ? sh[at] + aw[j][e] : aw[j][e];
                         sh[L * E + at] = k ? sh[L * E + at] + ab[j][e] : ab[j][e];
                     }
+                }
             }
         }
         __syncthreads();
         for (int c = threadIdx.x; c < D; c += TH) { p[c] = sh[c]; p[D + c] = sh[L * E + c]; }
     } else {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            const Run<L, V> run(j, lane, D);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int c = (j * L + lane) * V + e;
-                if (c < D) { p[c] = aw[j][e]; p[D + c] = ab[j][e]; }
-            }
+            for (int e = 0; e < V; ++e)
+                if (run.counts(e)) { p[run.c + e] = aw[j][e]; p[D + run.c + e] = ab[j][e]; }
+        }
     }
 }
 
@@ -206,25 +250,22 @@ __global__ __launch_bounds__(1024) void seq_colsum2_kernel(const float* __restri
     }
 }
 
-// The layout of a row: the fewest lanes out of 16 (four rows to a wave), 64 (a wave), 256 and 1024 that hold it with 16 values each.
+// The layout of a row: the fewest lanes out of 16 (four rows to a wave), 64 (a wave), 256 and 1024 that hold it with 16 values each, in runs of 16
+// bytes; single values for rows shorter than a run.
 template <typename T, int L, typename F>
-void with_values(bool vec, int D, F&& f) {
+void with_values(int D, F&& f) {
     constexpr int V = 16 / sizeof(T);
-    if (vec) {
-        if (D <= L * V) f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::integral_constant<int, 1>());
-        else if (D <= L * V * 2 || V == 8) f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::integral_constant<int, 2>());
-        else f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::integral_constant<int, V == 8 ? 2 : 4>());
-    } else {
-        if (D <= L * 4) f(std::integral_constant<int, L>(), std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
-        else f(std::integral_constant<int, L>(), std::integral_constant<int, 1>(), std::integral_constant<int, 16>());
-    }
+    if (D < V) f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
+    else if (D <= L * V) f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::integral_constant<int, 1>());
+    else if (D <= L * V * 2) f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::integral_constant<int, 2>());
+    else f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::integral_constant<int, 16 / V>());
 }
 template <typename T, typename F>
-void with_layout(bool vec, int D, F&& f) {
-    if (D <= 16 * 16) with_values<T, 16>(vec, D, f);
-    else if (D <= 64 * 16) with_values<T, 64>(vec, D, f);
-    else if (D <= 256 * 16) with_values<T, 256>(vec, D, f);
-    else with_values<T, 1024>(vec, D, f);
+void with_layout(int D, F&& f) {
+    if (D <= 16 * 16) with_values<T, 16>(D, f);
+    else if (D <= 64 * 16) with_values<T, 64>(D, f);
+    else if (D <= 256 * 16) with_values<T, 256>(D, f);
+    else with_values<T, 1024>(D, f);
 }
 int rows_per_group(int D) { return D <= 256 ? 16 : D <= 1024 ? 4 : 1; }
 }  // namespace
@@ -243,9 +284,7 @@ extern "C" int motif_layer_norm_fwd(const void* x, long x_rs, const void* weight
     if (D > kMaxD || rows > 0x7fffffffL) return MOTIF_ELIMIT;
     seq_dispatch(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        constexpr int V = 16 / sizeof(T);
-        const bool vec = D % V == 0 && x_rs % V == 0 && seq_aligned(x, 16) && seq_aligned(y, 16) && seq_aligned(weight, 16) && seq_aligned(bias, 16);
-        with_layout<T>(vec, D, [&](auto l, auto v, auto nv) {
+        with_layout<T>(D, [&](auto l, auto v, auto nv) {
             constexpr int L = decltype(l)::value, TH = L < 256 ? 256 : L;
             layer_norm_fwd_kernel<T, L, decltype(v)::value, decltype(nv)::value><<<cdiv(rows, TH / L), TH, 0, (hipStream_t)stream>>>(
                 (const T*)x, x_rs, weight, bias, param_dtype, (T*)y, stats, rows, D, eps);
@@ -276,9 +315,7 @@ extern "C" int motif_layer_norm_bwd(const void* x, long x_rs, const void* dy, lo
     const int nb = bwd_groups(rows, D);
     seq_dispatch(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        constexpr int V = 16 / sizeof(T);
-        const bool vec = D % V == 0 && x_rs % V == 0 && dy_rs % V == 0 && seq_aligned(x, 16) && seq_aligned(dy, 16) && seq_aligned(dx, 16) && seq_aligned(weight, 16);
-        with_layout<T>(vec, D, [&](auto l, auto v, auto nv) {
+        with_layout<T>(D, [&](auto l, auto v, auto nv) {
             constexpr int L = decltype(l)::value, TH = L < 256 ? 256 : L;
             layer_norm_bwd_kernel<T, L, decltype(v)::value, decltype(nv)::value><<<nb, TH, 0, (hipStream_t)stream>>>(
                 (const T*)x, x_rs, (const T*)dy, dy_rs, weight, param_dtype, stats, (T*)dx, params ? workspace : nullptr, rows, D);

@@ -22,49 +22,58 @@ static inline bool seq_dtype_ok(int dtype) { return dtype == MOTIF_F32 || dtype 
 // A null pointer counts as aligned.
 static inline bool seq_aligned(const void* p, int bytes) { return ((unsigned long long)p & (unsigned long long)(bytes - 1)) == 0; }
 
+// N values of T as they lie in memory, at any address that is a multiple of T's size: global memory takes 16-byte accesses at such addresses, so rows of
+// any length and offset are read in 16-byte pieces (a lane whose piece would pass the row's end takes the last N values instead).
 template <typename T, int N>
-struct alignas(sizeof(T) * N) SeqVec { T v[N]; };
+struct SeqRaw {
+    T v[N];
+    __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
+};
+template <int BYTES> struct SeqWords { typedef unsigned type __attribute__((ext_vector_type(BYTES / 4))); };
+template <> struct SeqWords<4> { typedef unsigned type; };
+template <> struct SeqWords<2> { typedef unsigned short type; };
 
 template <typename T, int N>
-__device__ __forceinline__ void seq_load(const T* p, float (&out)[N]) {
-    const SeqVec<T, N> x = *(const SeqVec<T, N>*)p;
+__device__ __forceinline__ SeqRaw<T, N> seq_raw(const T* p) {
+    constexpr int B = sizeof(T) * N, P = B < 16 ? B : 16;
+    typedef typename SeqWords<P>::type W;
+    struct { W w[B / P]; } x;
 #pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = (float)x.v[i];
+    for (int i = 0; i < B / P; ++i) __builtin_memcpy(&x.w[i], (const char*)p + i * P, P);
+    return __builtin_bit_cast(SeqRaw<T, N>, x);
+}
+// Keeps what was read as it was read: without this the compiler holds the fp32 values of the first walk for the second one, twice the registers.
+template <typename T, int V>
+__device__ __forceinline__ void seq_hold(SeqRaw<T, V>& x) {
+    constexpr int B = sizeof(T) * V, P = B < 16 ? B : 16;
+    static_assert(B == P, "");
+    auto w = __builtin_bit_cast(typename SeqWords<P>::type, x);
+    asm volatile("" : "+v"(w));
+    x = __builtin_bit_cast(SeqRaw<T, V>, w);
+}
+template <typename T, int N>
+__device__ __forceinline__ void seq_load(const T* p, float (&out)[N]) {
+    const SeqRaw<T, N> x = seq_raw<T, N>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = x[i];
 }
 template <typename T, int N>
 __device__ __forceinline__ void seq_store(T* p, const float (&in)[N]) {
-    SeqVec<T, N> x;
+    constexpr int B = sizeof(T) * N, P = B < 16 ? B : 16;
+    typedef typename SeqWords<P>::type W;
+    SeqRaw<T, N> x;
 #pragma unroll
     for (int i = 0; i < N; ++i) x.v[i] = (T)in[i];
-    *(SeqVec<T, N>*)p = x;
-}
-// N values from an address that is a multiple of 16 bytes, or of their whole size where that is less.
-template <typename T, int N>
-__device__ __forceinline__ void seq_load16(const T* p, float (&out)[N]) {
-    constexpr int P = 16 / (int)sizeof(T) < N ? 16 / (int)sizeof(T) : N;
+    struct Words { W w[B / P]; };
+    const Words y = __builtin_bit_cast(Words, x);
 #pragma unroll
-    for (int j = 0; j < N; j += P) {
-        const SeqVec<T, P> x = *(const SeqVec<T, P>*)(p + j);
-#pragma unroll
-        for (int i = 0; i < P; ++i) out[j + i] = (float)x.v[i];
-    }
-}
-template <typename T, int N>
-__device__ __forceinline__ void seq_store16(T* p, const float (&in)[N]) {
-    constexpr int P = 16 / (int)sizeof(T) < N ? 16 / (int)sizeof(T) : N;
-#pragma unroll
-    for (int j = 0; j < N; j += P) {
-        SeqVec<T, P> x;
-#pragma unroll
-        for (int i = 0; i < P; ++i) x.v[i] = (T)in[j + i];
-        *(SeqVec<T, P>*)(p + j) = x;
-    }
+    for (int i = 0; i < B / P; ++i) __builtin_memcpy((char*)p + i * P, &y.w[i], P);
 }
 template <int N>
 __device__ __forceinline__ void seq_param_vec(const void* p, long i, int dtype, float (&out)[N]) {
-    if (dtype == MOTIF_F32) seq_load16<float, N>((const float*)p + i, out);
-    else if (dtype == MOTIF_BF16) seq_load16<bf16_t, N>((const bf16_t*)p + i, out);
-    else seq_load16<f16_t, N>((const f16_t*)p + i, out);
+    if (dtype == MOTIF_F32) seq_load<float, N>((const float*)p + i, out);
+    else if (dtype == MOTIF_BF16) seq_load<bf16_t, N>((const bf16_t*)p + i, out);
+    else seq_load<f16_t, N>((const f16_t*)p + i, out);
 }
 // One value of a parameter whose type is not the data's (uniform branch).
 __device__ __forceinline__ float seq_param(const void* p, long i, int dtype) {

@@ -1114,8 +1114,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 
 def _scan_strides(t):
-    """(tensor, batch stride, row stride) of [B, T, D] or [T, D]; copied only where the last axis is not dense."""
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
+    """(tensor, batch stride, row stride) of [B, T, D] or [T, D]; copied only where the last axis is not dense or the rows lie very far apart."""
+    if (t.stride(-1) != 1 and t.shape[-1] != 1) or t.stride(-2) > max(1 << 22, t.shape[-1]):
         t = t.contiguous()
     return (t, t.stride(0), t.stride(1)) if t.dim() == 3 else (t, 0, t.stride(0))
 
