@@ -5,8 +5,9 @@
 //              dq_t = g_t z_t,    dz_t = g_t (q_t - h_{t-1}),    dh0 = a_0 g_0
 //
 // Both are first-order linear recurrences; the backward one runs from the end.  A run of rows acts on the state that enters it as
-// x -> A x + H, and two runs compose as (A2 A1, A2 H1 + H2): that is what lets time be split.  A packed sequence's first row has A = 0 and its
-// initial state inside H, so sequences packed one behind the other are one recurrence over all rows.
+// x -> A x + H, and two runs compose as (A2 A1, A2 H1 + H2): that is what lets time be split.  Sequences packed one behind the other are one recurrence
+// over all rows: a run that holds a sequence's first row (or a row of none) is marked as cut and composes as (0, H2) with what lies before it,
+// whatever that is -- an infinite state of one sequence must not meet the next one's 0.
 //
 // Bound by memory (forward 2 reads and 1 write, backward 4 reads and 2 writes of the data).  A workgroup owns TX lanes x V channels and TY time
 // slots of R rows each: a tile of TY R rows lies in registers, as it was read, between the composition of its slots (lanes of a wave by shuffles, the waves
@@ -24,6 +25,7 @@ struct ScanArgs {
     void *out0, *out1;                                   // forward: h, -; backward: dz, dq (either may be null)
     float* state;                                        // forward: the last states, backward: dh0 (may be null)
     float* agg;                                          // [B][segs][2][D], null with one segment
+    int* cuts;                                           // packed: whether a segment is cut, [segs]
     const int* info;                                     // packed rows: owner << 2 | last << 1 | first, -1: no sequence's row.  null: B sequences of T rows
     long zb, zr, qb, qr, db, dr;                         // batch and row strides of z, q, dh; h, out0 and out1 are dense
     long T, seg_rows;
@@ -37,42 +39,47 @@ struct Slots {                                           // 256 threads: TX lane
     static constexpr int WX = TX < 64 ? TX : 64, WY = 64 / WX, WAVES = TY > 1 ? 4 : 1;
     static_assert(TX * TY == 256 && (TY == 1 || TX <= 64), "");
 
-    // A, H of this slot -> of the slots in front of it in its wave (exclusive); the wave's own to tot[wave]
-    static __device__ __forceinline__ void wave_scan(float (&A)[V], float (&H)[V], float (*tot)[2][TX * V]) {
+    struct Sums { float v[4][2][TX * V]; int cut[4]; };  // of the waves
+
+    // A, H (and the cut) of this slot -> of the slots in front of it in its wave; the wave's own to sums
+    template <bool PACKED>
+    static __device__ __forceinline__ void wave_scan(float (&A)[V], float (&H)[V], int& cut, Sums& sums) {
         const int lane = threadIdx.x & 63, sy = lane / WX, tx = lane % WX, wave = threadIdx.x >> 6;
 #pragma unroll
         for (int d = 1; d < WY; d <<= 1) {
+            const int oc = PACKED ? __shfl_up(cut, d * WX) : 0;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float oa = __shfl_up(A[v], d * WX), oh = __shfl_up(H[v], d * WX);
-                if (sy >= d) { H[v] = fmaf(A[v], oh, H[v]); A[v] *= oa; }
+                if (sy >= d && !(PACKED && cut)) { H[v] = fmaf(A[v], oh, H[v]); A[v] *= oa; }
             }
+            if (PACKED && sy >= d) cut |= oc;
         }
         if (sy == WY - 1) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) { tot[wave][0][tx * V + v] = A[v]; tot[wave][1][tx * V + v] = H[v]; }
+            for (int v = 0; v < V; ++v) { sums.v[wave][0][tx * V + v] = A[v]; sums.v[wave][1][tx * V + v] = H[v]; }
+            if (PACKED && tx == 0) sums.cut[wave] = cut; // (the same in every lane of a slot that has channels; the first always has)
         }
-        if constexpr (WY > 1) {
+        const int oc = PACKED && WY > 1 ? __shfl_up(cut, WX) : 0;
+        if (PACKED) cut = sy ? oc : 0;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float oa = __shfl_up(A[v], WX), oh = __shfl_up(H[v], WX);
-                A[v] = sy ? oa : 1.f;
-                H[v] = sy ? oh : 0.f;
-            }
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) { A[v] = 1.f; H[v] = 0.f; }
+        for (int v = 0; v < V; ++v) {
+            const float oa = WY > 1 ? __shfl_up(A[v], WX) : 1.f, oh = WY > 1 ? __shfl_up(H[v], WX) : 0.f;
+            A[v] = sy ? oa : 1.f;
+            H[v] = sy ? oh : 0.f;
         }
     }
     // behind a barrier: the state that enters this wave's slots, and `carry` moved past all waves
-    static __device__ __forceinline__ void waves_apply(float (&carry)[V], float (&in)[V], const float (*tot)[2][TX * V], int tx) {
+    template <bool PACKED>
+    static __device__ __forceinline__ void waves_apply(float (&carry)[V], float (&in)[V], const Sums& sums, int tx) {
         const int wave = threadIdx.x >> 6;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
+            const bool cut = PACKED && sums.cut[w];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 if (w == wave) in[v] = carry[v];
-                carry[v] = fmaf(tot[w][0][tx * V + v], carry[v], tot[w][1][tx * V + v]);
+                carry[v] = cut ? sums.v[w][1][tx * V + v] : fmaf(sums.v[w][0][tx * V + v], carry[v], sums.v[w][1][tx * V + v]);
             }
         }
     }
@@ -84,27 +91,22 @@ __device__ __forceinline__ void zero(float (&x)[V], float c = 0.f) {
     for (int v = 0; v < V; ++v) x[v] = c;
 }
 
-// The composition of one row: forward  x -> a x + z q (first: a h0 + z q),   backward  c -> a (c + dh) (last: a (dlast + dh)).
-template <bool BWD, int V, typename X>
-__device__ __forceinline__ void compose(float (&A)[V], float (&H)[V], const X& z, const X& x, int flag, const float* init, int c0, int D) {
-    float s[V];
-    zero(s);
-    const bool cut = flag >= 0 && (flag & (BWD ? kLast : kFirst));
-    if (cut && init) seq_load<float, V>(init + (long)(flag >> 2) * D + c0, s);
+// One row more behind a run: forward  x -> a x + z q,   backward  c -> a (c + dh).  Packed: a sequence's first row in the recurrence's order starts
+// from the sequence's own state, a row of none from nothing; both cut.
+template <bool BWD, bool PACKED, int V, typename X>
+__device__ __forceinline__ void compose(float (&A)[V], float (&H)[V], int& cut, const X& z, const X& x, int flag, const float* init, int c0, int D) {
+    if (PACKED && (flag < 0 || (flag & (BWD ? kLast : kFirst)))) {
+        cut = 1;
+        zero(A);
+        zero(H);
+        if (flag >= 0 && init) seq_load<float, V>(init + (long)(flag >> 2) * D + c0, H);
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const float a = 1.f - z[v];
-        if (cut) { A[v] = 0.f; H[v] = s[v]; }
-        if (flag < 0) { A[v] = 0.f; H[v] = 0.f; continue; }
-        H[v] = BWD ? a * (H[v] + x[v]) : fmaf(a, H[v], z[v] * x[v]);
-        A[v] *= a;
+        const float a = 1.f - z[v], n = BWD ? a * (H[v] + x[v]) : fmaf(a, H[v], z[v] * x[v]);
+        H[v] = PACKED && flag < 0 ? 0.f : n;
+        A[v] = PACKED && flag < 0 ? 0.f : A[v] * a;
     }
-}
-
-// What row t of sequence b is.
-__device__ __forceinline__ int row_flag(const ScanArgs& p, long b, long t) {
-    if (p.info) return p.info[t];
-    return (int)(b << 2) | (t == 0 ? kFirst : 0) | (t == p.T - 1 ? kLast : 0);
 }
 
 struct Where { int group, seg; long b; };
@@ -113,11 +115,11 @@ __device__ __forceinline__ Where where(const ScanArgs& p) {
     return {(int)(blockIdx.x % p.groups), (int)(bs % p.segs), bs / p.segs};
 }
 
-// (A, H) of every segment but the last: each slot walks its own run of the segment's rows, four rows requested at a time.
-template <typename T, int V, int TX, int TY, bool BWD>
+// (A, H) of every segment but the last: each slot walks its own run of the segment's rows, four rows at a time, the next four requested ahead.
+template <typename T, int V, int TX, int TY, bool BWD, bool PACKED>
 __global__ __launch_bounds__(256) void gru_scan_segments_kernel(ScanArgs p) {
     using S = Slots<V, TX, TY>;
-    __shared__ float tot[4][2][TX * V];
+    __shared__ typename S::Sums sums;
     const Where at = where(p);
     if (at.seg == p.segs - 1) return;
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, first = (at.group * TX + tx) * V, c0 = min(first, p.D - V);
@@ -126,44 +128,57 @@ __global__ __launch_bounds__(256) void gru_scan_segments_kernel(ScanArgs p) {
     const T* x = BWD ? (const T*)p.dh + at.b * p.db + c0 : (const T*)p.q + at.b * p.qb + c0;
     const long xr = BWD ? p.dr : p.qr;
     const long run = p.seg_rows / TY, k0 = at.seg * p.seg_rows + ty * run;     // rows in the order of the recurrence; a segment that is not the last is full
+    struct Rows { SeqRaw<T, V> z[4], x[4]; int f[4]; };
+    auto read = [&](Rows& w, long k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const long t = BWD ? p.T - 1 - (k + r) : k + r;
+            w.z[r] = seq_raw<T, V>(z + t * p.zr);
+            w.x[r] = seq_raw<T, V>(x + t * xr);
+            if (PACKED) w.f[r] = p.info[t];
+        }
+    };
     float A[V], H[V];
+    int cut = 0;
     zero(A, 1.f);
     zero(H);
     if (on) {
+        Rows now, next;
+        read(now, k0);
         for (long k = k0; k < k0 + run; k += 4) {
-            SeqRaw<T, V> zv[4], xv[4];
-            int f[4];
+            if (k + 4 < k0 + run) read(next, k + 4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const long t = BWD ? p.T - 1 - (k + r) : k + r;
-                zv[r] = seq_raw<T, V>(z + t * p.zr);
-                xv[r] = seq_raw<T, V>(x + t * xr);
-                f[r] = row_flag(p, at.b, t);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) compose<BWD, V>(A, H, zv[r], xv[r], f[r], BWD ? p.dlast : p.h0, c0, p.D);
+            for (int r = 0; r < 4; ++r) compose<BWD, PACKED, V>(A, H, cut, now.z[r], now.x[r], now.f[r], BWD ? p.dlast : p.h0, c0, p.D);
+            now = next;
         }
     }
-    S::wave_scan(A, H, tot);
+    S::template wave_scan<PACKED>(A, H, cut, sums);
     __syncthreads();
     if (ty == 0 && on) {
         float* o = p.agg + ((at.b * p.segs + at.seg) * 2) * p.D + c0;
+        zero(A, 1.f);
+        zero(H);
+        cut = 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            A[v] = 1.f;
-            H[v] = 0.f;
+        for (int w = 0; w < S::WAVES; ++w) {
+            const bool c = PACKED && sums.cut[w];
+            cut |= c;
 #pragma unroll
-            for (int w = 0; w < S::WAVES; ++w) { H[v] = fmaf(tot[w][0][tx * V + v], H[v], tot[w][1][tx * V + v]); A[v] *= tot[w][0][tx * V + v]; }
+            for (int v = 0; v < V; ++v) {
+                H[v] = c ? sums.v[w][1][tx * V + v] : fmaf(sums.v[w][0][tx * V + v], H[v], sums.v[w][1][tx * V + v]);
+                A[v] = c ? 0.f : sums.v[w][0][tx * V + v] * A[v];
+            }
         }
         seq_store<float, V>(o, A);
         seq_store<float, V>(o + p.D, H);
+        if (PACKED && first == 0) p.cuts[at.seg] = cut;
     }
 }
 
-template <typename T, int V, int TX, int TY, int R, bool BWD>
+template <typename T, int V, int TX, int TY, int R, bool BWD, bool PACKED>
 __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
     using S = Slots<V, TX, TY>;
-    __shared__ float tot[2][4][2][TX * V];
+    __shared__ typename S::Sums sums[2];
     const Where at = where(p);
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, first = (at.group * TX + tx) * V, c0 = min(first, p.D - V);
     const bool on = first < p.D;                         // (the last lane of a row takes its last V channels: those it shares are written twice, alike)
@@ -179,101 +194,118 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
     char* out0 = p.out0 ? (char*)((T*)p.out0 + at.b * p.T * p.D) : nullptr;
     char* out1 = p.out1 ? (char*)((T*)p.out1 + at.b * p.T * p.D) : nullptr;
     const long k_end = min(p.T, (at.seg + 1) * p.seg_rows);
+    const float* init = BWD ? p.dlast : p.h0;
+
+    // R rows of every tensor; `t0`: the uniform row of row r of a tile (where the tile passes the end it need not exist: no lane reads it then)
+    typedef SeqRaw<T, V> Raw;
+    struct Rows { Raw z[R], q[R], d[BWD ? R : 1], h[BWD ? R : 1]; int f[R]; };
+    auto row = [&](long k0, int r) __attribute__((always_inline)) { return BWD ? p.T - 1 - k0 - (TY * R - 1) + (R - 1 - r) : k0 + r; };
+    auto read = [&](Rows& w, long k0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const long k = k0 + ty * R + r, t = BWD ? p.T - 1 - k : k, t0 = row(k0, r);
+            w.z[r] = w.q[r] = Raw{};                     // no row: x -> x
+            if constexpr (BWD) w.d[r] = w.h[r] = Raw{};
+            if (PACKED) w.f[r] = 0;
+            if (on && k < k_end) {
+                w.z[r] = seq_raw<T, V>((const T*)(z + t0 * p.zr * (long)sizeof(T) + oz));
+                if (!BWD || out0) w.q[r] = seq_raw<T, V>((const T*)(q + t0 * p.qr * (long)sizeof(T) + oq));
+                if constexpr (BWD) {
+                    w.d[r] = seq_raw<T, V>((const T*)(dh + t0 * p.dr * (long)sizeof(T) + od));
+                    if (out0 && t > 0) w.h[r] = seq_raw<T, V>((const T*)(hs + (t0 - 1) * p.D * (long)sizeof(T) + oo));
+                }
+                if (PACKED) w.f[r] = p.info[t];
+            }
+        }
+    };
+    Rows now, next;
+    read(now, at.seg * p.seg_rows);
+
     float carry[V];
-    zero(carry);                                         // (a sequence's own initial value enters at its first row)
+    zero(carry);                                         // (packed: a sequence's own state enters at its first row)
+    if (!PACKED && init && on) seq_load<float, V>(init + at.b * p.D + c0, carry);
     int buf = 0;
     if (TY > 1 && at.seg > 0) {                          // the segments in front: slot ty composes a run of them, then the slots compose
         float A[V], H[V], in[V];
+        int cut = 0;
         zero(A, 1.f);
         zero(H);
         const int per = (at.seg + TY - 1) / TY;
         if (on) {
+#pragma unroll 2
             for (int s = ty * per; s < min(at.seg, (ty + 1) * per); ++s) {
                 float a[V], h[V];
                 const float* g = p.agg + ((at.b * p.segs + s) * 2) * p.D + c0;
                 seq_load<float, V>(g, a);
                 seq_load<float, V>(g + p.D, h);
+                const bool c = PACKED && p.cuts[s];
+                cut |= c;
 #pragma unroll
-                for (int v = 0; v < V; ++v) { H[v] = fmaf(a[v], H[v], h[v]); A[v] *= a[v]; }
+                for (int v = 0; v < V; ++v) { H[v] = c ? h[v] : fmaf(a[v], H[v], h[v]); A[v] = c ? 0.f : A[v] * a[v]; }
             }
         }
-        S::wave_scan(A, H, tot[0]);
+        S::template wave_scan<PACKED>(A, H, cut, sums[0]);
         __syncthreads();
-        S::waves_apply(carry, in, tot[0], tx);
+        S::template waves_apply<PACKED>(carry, in, sums[0], tx);
         buf = 1;
     }
     for (long k0 = at.seg * p.seg_rows; k0 < k_end; k0 += TY * R) {
-        typedef SeqRaw<T, V> Raw;
-        Raw zv[R], qv[R], dv[BWD ? R : 1], hv[BWD ? R : 1];
-        int f[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const long k = k0 + ty * R + r, t = BWD ? p.T - 1 - k : k;
-            const bool in = on && k < k_end;
-            f[r] = in ? row_flag(p, at.b, t) : 0;
-            zv[r] = qv[r] = Raw{};                       // no row: x -> x
-            if constexpr (BWD) dv[r] = hv[r] = Raw{};
-            const long t0 = BWD ? p.T - 1 - k0 - (TY * R - 1) + (R - 1 - r) : k0 + r;      // the uniform row (it need not exist: no lane reads it then)
-            if (in) {
-                zv[r] = seq_raw<T, V>((const T*)(z + t0 * p.zr * (long)sizeof(T) + oz));
-                if (!BWD || out0) qv[r] = seq_raw<T, V>((const T*)(q + t0 * p.qr * (long)sizeof(T) + oq));
-                if constexpr (BWD) {
-                    dv[r] = seq_raw<T, V>((const T*)(dh + t0 * p.dr * (long)sizeof(T) + od));
-                    if (out0 && t > 0) hv[r] = seq_raw<T, V>((const T*)(hs + (t0 - 1) * p.D * (long)sizeof(T) + oo));
-                }
-            }
-        }
+        if (k0 + TY * R < k_end) read(next, k0 + TY * R);
         float h[V];
         if constexpr (TY > 1) {
             float A[V], H[V], in[V];
+            int cut = 0;
             zero(A, 1.f);
             zero(H);
 #pragma unroll
-            for (int r = 0; r < R; ++r) compose<BWD, V>(A, H, zv[r], BWD ? dv[BWD ? r : 0] : qv[r], f[r], BWD ? p.dlast : p.h0, c0, p.D);
+            for (int r = 0; r < R; ++r) compose<BWD, PACKED, V>(A, H, cut, now.z[r], BWD ? now.d[BWD ? r : 0] : now.q[r], now.f[r], init, c0, p.D);
 #pragma unroll
-            for (int r = 0; r < R; ++r) { seq_hold(zv[r]); if constexpr (BWD) seq_hold(dv[r]); else seq_hold(qv[r]); }
-            S::wave_scan(A, H, tot[buf]);
+            for (int r = 0; r < R; ++r) { seq_hold(now.z[r]); if constexpr (BWD) seq_hold(now.d[r]); else seq_hold(now.q[r]); }
+            S::template wave_scan<PACKED>(A, H, cut, sums[buf]);
             __syncthreads();                             // one barrier a tile: the next tile's sums go to the other buffer
-            S::waves_apply(carry, in, tot[buf], tx);
+            S::template waves_apply<PACKED>(carry, in, sums[buf], tx);
             buf ^= 1;
 #pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = fmaf(A[v], in[v], H[v]);
+            for (int v = 0; v < V; ++v) h[v] = PACKED && cut ? H[v] : fmaf(A[v], in[v], H[v]);
         } else {
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = carry[v];
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (!on || k0 + ty * R + r >= k_end) continue;
-            const long own = (long)(f[r] >> 2) * p.D + c0, t0 = BWD ? p.T - 1 - k0 - (TY * R - 1) + (R - 1 - r) : k0 + r, out = t0 * p.D * (long)sizeof(T);
+            const long k = k0 + ty * R + r, t = BWD ? p.T - 1 - k : k, out = row(k0, r) * p.D * (long)sizeof(T);
+            if (!on || k >= k_end) continue;
+            const int f = PACKED ? now.f[r] : 0;
+            const bool none = PACKED && f < 0, head = PACKED ? f >= 0 && (f & kFirst) : t == 0, tail = PACKED ? f >= 0 && (f & kLast) : t == p.T - 1;
+            const long own = (PACKED ? (long)(f >> 2) : at.b) * p.D + c0;
+            if (PACKED && (BWD ? tail : head)) { if (init) seq_load<float, V>(init + own, h); else zero(h); }
             if constexpr (!BWD) {
-                if (f[r] >= 0 && (f[r] & kFirst)) { if (p.h0) seq_load<float, V>(p.h0 + own, h); else zero(h); }
 #pragma unroll
-                for (int v = 0; v < V; ++v) h[v] = f[r] < 0 ? 0.f : fmaf(1.f - zv[r][v], h[v], zv[r][v] * qv[r][v]);
+                for (int v = 0; v < V; ++v) h[v] = none ? 0.f : fmaf(1.f - now.z[r][v], h[v], now.z[r][v] * now.q[r][v]);
                 seq_store<T, V>((T*)(out0 + out + oo), h);
-                if (p.state && f[r] >= 0 && (f[r] & kLast)) seq_store<float, V>(p.state + own, h);
+                if (tail && p.state) seq_store<float, V>(p.state + own, h);
             } else {
-                if (f[r] >= 0 && (f[r] & kLast)) { if (p.dlast) seq_load<float, V>(p.dlast + own, h); else zero(h); }
                 float dz[V], dq[V], before[V];
 #pragma unroll
-                for (int v = 0; v < V; ++v) before[v] = hv[r][v];
-                if (f[r] >= 0 && (f[r] & kFirst)) { if (p.h0) seq_load<float, V>(p.h0 + own, before); else zero(before); }
+                for (int v = 0; v < V; ++v) before[v] = now.h[r][v];
+                if (head) { if (p.h0) seq_load<float, V>(p.h0 + own, before); else zero(before); }
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float g = f[r] < 0 ? 0.f : dv[r][v] + h[v];
-                    dz[v] = f[r] < 0 ? 0.f : g * (qv[r][v] - before[v]);
-                    dq[v] = f[r] < 0 ? 0.f : g * zv[r][v];
-                    h[v] = f[r] < 0 ? 0.f : (1.f - zv[r][v]) * g;
+                    const float g = none ? 0.f : now.d[r][v] + h[v];
+                    dz[v] = none ? 0.f : g * (now.q[r][v] - before[v]);
+                    dq[v] = none ? 0.f : g * now.z[r][v];
+                    h[v] = none ? 0.f : (1.f - now.z[r][v]) * g;
                 }
                 if (out0) seq_store<T, V>((T*)(out0 + out + oo), dz);
                 if (out1) seq_store<T, V>((T*)(out1 + out + oo), dq);
-                if (p.state && f[r] >= 0 && (f[r] & kFirst)) seq_store<float, V>(p.state + own, h);
+                if (head && p.state) seq_store<float, V>(p.state + own, h);
             }
         }
         if constexpr (TY == 1) {
 #pragma unroll
             for (int v = 0; v < V; ++v) carry[v] = h[v];
         }
+        now = next;
     }
 }
 
@@ -325,15 +357,24 @@ Plan plan_of(int V, long B, long T, long D) {
     return p;
 }
 
-template <typename T, int V, bool BWD>
+template <typename T, int V, bool BWD, bool PACKED>
 void launch(const Plan& pl, const ScanArgs& a, hipStream_t s) {
     const unsigned grid = (unsigned)((long)a.B * pl.segs * pl.groups);
-    constexpr int TY = V > 1 ? 32 : 8;
-    constexpr int R = BWD ? 2 : 4;                       // backward holds four tensors' rows
-    if (pl.TY == 1) { gru_scan_kernel<T, V, 256, 1, R, BWD><<<grid, 256, 0, s>>>(a); return; }
-    if (pl.segs > 1) gru_scan_segments_kernel<T, V, 256 / TY, TY, BWD><<<grid, 256, 0, s>>>(a);
-    gru_scan_kernel<T, V, 256 / TY, TY, R, BWD><<<grid, 256, 0, s>>>(a);
+    constexpr int TY = V > 1 ? 32 : 8, R = BWD ? 2 : 4;  // backward holds four tensors' rows
+    if (pl.TY == 1) { gru_scan_kernel<T, V, 256, 1, R, BWD, PACKED><<<grid, 256, 0, s>>>(a); return; }
+    if (pl.segs > 1) gru_scan_segments_kernel<T, V, 256 / TY, TY, BWD, PACKED><<<grid, 256, 0, s>>>(a);
+    gru_scan_kernel<T, V, 256 / TY, TY, R, BWD, PACKED><<<grid, 256, 0, s>>>(a);
 }
+template <typename T, bool BWD>
+void launch_any(const Plan& pl, const ScanArgs& a, hipStream_t s) {
+    constexpr int W = 16 / sizeof(T);
+    if (a.info) { if (pl.V == 1) launch<T, 1, BWD, true>(pl, a, s); else launch<T, W, BWD, true>(pl, a, s); }
+    else { if (pl.V == 1) launch<T, 1, BWD, false>(pl, a, s); else launch<T, W, BWD, false>(pl, a, s); }
+}
+
+// The workspace: the segments' (A, H), their cuts, the packed rows' meaning.
+long agg_floats(const Plan& p, long B, long D) { return p.segs > 1 ? (B * p.segs * 2 * D + 3) & ~3L : 0; }
+long cut_floats(const Plan& p, bool packed) { return packed && p.segs > 1 ? (p.segs + 3) & ~3 : 0; }
 
 int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const float* empty_in, hipStream_t s) {
     const int V = vec_of(dtype, a.D);
@@ -343,9 +384,10 @@ int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const 
     a.groups = pl.groups;
     a.segs = pl.segs;
     a.seg_rows = pl.seg_rows;
-    if (pl.segs > 1) a.agg = ws;
+    a.agg = ws;
     if (cu) {
-        int* info = (int*)(ws + (pl.segs > 1 ? (((long)pl.segs * 2 * a.D + 3) & ~3L) : 0));
+        a.cuts = (int*)(ws + agg_floats(pl, a.B, a.D));
+        int* info = (int*)(ws + agg_floats(pl, a.B, a.D) + cut_floats(pl, true));
         if (a.T > 0) gru_scan_rows_kernel<<<cdiv(a.T, 256), 256, 0, s>>>(cu, S, (int)a.T, info);
         if (a.state) gru_scan_empty_kernel<<<S, 256, 0, s>>>(cu, a.D, empty_in, a.state);
         a.info = info;
@@ -353,9 +395,7 @@ int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const 
     if (a.T > 0)
         seq_dispatch(dtype, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            constexpr int W = 16 / sizeof(T);
-            if (bwd) { if (V == 1) launch<T, 1, true>(pl, a, s); else launch<T, W, true>(pl, a, s); }
-            else { if (V == 1) launch<T, 1, false>(pl, a, s); else launch<T, W, false>(pl, a, s); }
+            if (bwd) launch_any<T, true>(pl, a, s); else launch_any<T, false>(pl, a, s);
         });
     MOTIF_LAUNCH_CHECK();
     return MOTIF_OK;
@@ -373,7 +413,7 @@ extern "C" long motif_gru_scan_ws_floats(long B, long T, long D, int packed, int
     const int rc = check_sizes(B, T, D, packed ? 1 : 0, packed ? (const void*)&B : nullptr, dtype);
     if (rc) return rc;
     const Plan p = plan_of(vec_of(dtype, D), B, T, D);
-    return (p.segs > 1 ? ((B * p.segs * 2 * D + 3) & ~3L) : 0) + (packed ? T : 0);
+    return agg_floats(p, B, D) + cut_floats(p, packed) + (packed ? T : 0);
 }
 
 extern "C" int motif_gru_scan_fwd(const void* z, long z_bs, long z_rs, const void* q, long q_bs, long q_rs, const float* h0, const int32_t* cu_seqlens, int S,

@@ -606,3 +606,30 @@ def test_gated_mlp_gradients_of_some_tensors_only(ops):
         h = ops.gated_mlp(*tensors.values())
         dh = torch.randn(130, 72, generator=gen(5), device="cuda").to(torch.bfloat16)
         assert torch.equal(torch.autograd.grad(h, tensors[which], dh)[0], full[which]), which
+
+
+@pytest.mark.parametrize("D", [3, 64, 200])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gru_scan_bad_values_stay_in_their_packed_sequence(ops, dtype, D):
+    bounds = [0, 400, 400, 410, 1500, 1501, 3000]
+    cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    z, q, h0 = scan_inputs((3000, D), 6, dtype, 21)
+    dh, dl = torch.randn(3000, D, generator=gen(2), device="cuda").to(dtype), torch.randn(6, D, generator=gen(3), device="cuda")
+
+    def step(q, h0, dh, dl):
+        leaves = [t.detach().requires_grad_() for t in (z, q, h0)]
+        h, last = ops.gru_scan(*leaves, cu_seqlens=cu)
+        return (h.detach(), last.detach()) + torch.autograd.grad((h, last), leaves, (dh, dl))
+    want = step(q, h0, dh, dl)
+    bad_q, bad_h0, bad_dh, bad_dl = q.clone(), h0.clone(), dh.clone(), dl.clone()
+    bad_q[100], bad_q[2000] = math.inf, math.nan          # sequences 0 and 5
+    bad_h0[3] = -math.inf
+    bad_dh[1500], bad_dl[0] = math.inf, math.nan          # the single row between 3 and 5
+    got = step(bad_q, bad_h0, bad_dh, bad_dl)
+    for a, b in zip(got, want):
+        if a.shape[0] == 3000:
+            assert torch.equal(a[400:410], b[400:410])
+        else:
+            assert torch.equal(a[1:3], b[1:3])
+    assert torch.equal(got[0][:100], want[0][:100]) and torch.equal(got[0][1500:2000], want[0][1500:2000])      # forward: what lies before them
+    assert torch.equal(got[3][1501:], want[3][1501:])     # dq of the sequence behind the bad gradient: it reads neither q nor h
