@@ -429,7 +429,7 @@ __device__ __forceinline__ void split3(float x, bf16_t (&out)[3]) {
     if (x != x) out[0] = __builtin_bit_cast(bf16_t, (unsigned short)0x7fc0);
 }
 // eight values: one plane of T, or three of bf16, `plane` elements apart
-__device__ __forceinline__ void put8(float* /*type*/, void* dst, long plane, long at, const float (&v)[8]) {
+__device__ __forceinline__ void put8(float* /*type*/, void* dst, long plane, long at, const float (&v)[8], bool stream = false) {
     float o[3][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -439,10 +439,10 @@ __device__ __forceinline__ void put8(float* /*type*/, void* dst, long plane, lon
         for (int i = 0; i < 3; ++i) o[i][e] = (float)s[i];
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) seq_store<bf16_t, 8>((bf16_t*)dst + i * plane + at, o[i]);
+    for (int i = 0; i < 3; ++i) seq_store<bf16_t, 8>((bf16_t*)dst + i * plane + at, o[i], stream);
 }
-__device__ __forceinline__ void put8(bf16_t*, void* dst, long, long at, const float (&v)[8]) { seq_store<bf16_t, 8>((bf16_t*)dst + at, v); }
-__device__ __forceinline__ void put8(f16_t*, void* dst, long, long at, const float (&v)[8]) { seq_store<f16_t, 8>((f16_t*)dst + at, v); }
+__device__ __forceinline__ void put8(bf16_t*, void* dst, long, long at, const float (&v)[8], bool stream = false) { seq_store<bf16_t, 8>((bf16_t*)dst + at, v, stream); }
+__device__ __forceinline__ void put8(f16_t*, void* dst, long, long at, const float (&v)[8], bool stream = false) { seq_store<f16_t, 8>((f16_t*)dst + at, v, stream); }
 
 // src [rows][cols] with row stride rs -> dst rows of ld = cols rounded up to 8, zeros behind the last value of a row.  Eight values per thread.
 template <typename T>
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(256) void layout_kernel(const T* __restrict__ src, 
 // A workgroup takes 256 columns x `rows` rows, eight columns per thread, and sums its columns over its rows (part [row blocks][2][F], may be null).
 template <typename T>
 __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh, long dhs, const float* __restrict__ G, const float* __restrict__ U, int M, int F, int ld, int act,
-                                                       void* dst, long plane, long pair, float* part, int rows) {
+                                                       void* dst, long plane, long pair, float* part, int rows, bool stream) {
     using O = std::conditional_t<sizeof(T) == 4, bf16_t, T>;
     __shared__ float sh[8][2][32][9];
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.y * 256 + x * 8;
@@ -494,8 +494,8 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
                 sg[e] += g[e];
                 su[e] += u[e];
             }
-            put8((T*)nullptr, dst, plane, r * ld + c, g);
-            put8((T*)nullptr, (O*)dst + pair, plane, r * ld + c, u);
+            put8((T*)nullptr, dst, plane, r * ld + c, g, stream);
+            put8((T*)nullptr, (O*)dst + pair, plane, r * ld + c, u, stream);
         }
     }
     if (!part) return;
@@ -798,7 +798,7 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         using T = std::remove_pointer_t<decltype(t)>;
         const int rows = grad_rows(M, F);
         const dim3 grid(cdiv(M, rows), cdiv(b.dg.ld, 256));
-        gate_grad_kernel<T><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows);
+        gate_grad_kernel<T><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows, 4 * b.dg.plane * b.dg.n >= kSeqStream);
     });
     if (need_b) {
         const int r = seq_colsum2(b.bias_part, cdiv(M, grad_rows(M, F)), F, db_gate, db_up, dtype, s);

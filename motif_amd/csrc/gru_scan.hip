@@ -30,6 +30,7 @@ struct ScanArgs {
     long zb, zr, qb, qr, db, dr;                         // batch and row strides of z, q, dh; h, out0 and out1 are dense
     long T, seg_rows;
     int B, D, groups, segs;
+    bool stream;
 };
 
 constexpr int kFirst = 1, kLast = 2;
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
             if constexpr (!BWD) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[v] = none ? 0.f : fmaf(1.f - now.z[r][v], h[v], now.z[r][v] * now.q[r][v]);
-                seq_store<T, V>((T*)(out0 + out + oo), h);
+                seq_store<T, V>((T*)(out0 + out + oo), h, p.stream);
                 if (tail && p.state) seq_store<float, V>(p.state + own, h);
             } else {
                 float dz[V], dq[V], before[V];
@@ -296,8 +297,8 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
                     dq[v] = none ? 0.f : g * now.z[r][v];
                     h[v] = none ? 0.f : (1.f - now.z[r][v]) * g;
                 }
-                if (out0) seq_store<T, V>((T*)(out0 + out + oo), dz);
-                if (out1) seq_store<T, V>((T*)(out1 + out + oo), dq);
+                if (out0) seq_store<T, V>((T*)(out0 + out + oo), dz, p.stream);
+                if (out1) seq_store<T, V>((T*)(out1 + out + oo), dq, p.stream);
                 if (head && p.state) seq_store<float, V>(p.state + own, h);
             }
         }
@@ -384,6 +385,7 @@ int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const 
     a.groups = pl.groups;
     a.segs = pl.segs;
     a.seg_rows = pl.seg_rows;
+    a.stream = a.B * a.T * a.D * seq_size(dtype) >= kSeqStream;
     a.agg = ws;
     if (cu) {
         a.cuts = (int*)(ws + agg_floats(pl, a.B, a.D));

@@ -73,57 +73,67 @@ __device__ __forceinline__ void params(const void* p, int D, int pdt, int lane, 
     }
 }
 
+// A workgroup walks over rows with its columns' weights and biases in registers, the next row requested while this one is summed.
 template <typename T, int L, int V, int NV>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_fwd_kernel(const T* __restrict__ x, long xs, const void* __restrict__ w, const void* __restrict__ b, int pdt,
-                                                                          T* __restrict__ y, float* __restrict__ stats, long rows, int D, float eps) {
+                                                                          T* __restrict__ y, float* __restrict__ stats, long rows, int D, float eps, bool stream) {
     __shared__ float sh[32];
     constexpr int TH = L < 256 ? 256 : L, R = TH / L;
     const int lane = threadIdx.x % L;
-    const long row = (long)blockIdx.x * R + threadIdx.x / L;
-    const bool on = row < rows;
-    const T* xr = x + (on ? row : 0) * xs;
-    float v[NV][V], wv[NV][V], bv[NV][V];
-    float s = 0.f;
+    const long step = (long)gridDim.x * R;
+    SeqRaw<T, V> next[NV];
+    auto request = [&](long row) __attribute__((always_inline)) {
+        if (row >= rows) return;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const Run<L, V> run(j, lane, D);
+        for (int j = 0; j < NV; ++j) {
+            const Run<L, V> run(j, lane, D);
+            if (run.on) next[j] = seq_raw<T, V>(x + row * xs + run.c);
+        }
+    };
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[j][e] = 0.f;
-        if (on && run.on) seq_load<T, V>(xr + run.c, v[j]);
-    }
-    params<L, V, NV>(w, D, pdt, lane, 1.f, wv);          // (on its way while the row is summed)
+    for (int j = 0; j < NV; ++j) next[j] = SeqRaw<T, V>{};
+    long row = (long)blockIdx.x * R + threadIdx.x / L;
+    request(row);
+    float wv[NV][V], bv[NV][V];
+    params<L, V, NV>(w, D, pdt, lane, 1.f, wv);
     params<L, V, NV>(b, D, pdt, lane, 0.f, bv);
+    for (long base = (long)blockIdx.x * R; base < rows; base += step, row += step) {
+        const bool on = row < rows;
+        float v[NV][V];
+        float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const Run<L, V> run(j, lane, D);
+        for (int j = 0; j < NV; ++j) {
+            const Run<L, V> run(j, lane, D);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += run.counts(e) ? v[j][e] : 0.f;
-    }
-    const float mean = row_sum<L>(s, sh) / (float)D;
-    float q = 0.f;
+            for (int e = 0; e < V; ++e) { v[j][e] = next[j][e]; s += run.counts(e) ? v[j][e] : 0.f; }
+        }
+        request(row + step);
+        const float mean = row_sum<L>(s, sh) / (float)D;
+        float q = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const Run<L, V> run(j, lane, D);
+        for (int j = 0; j < NV; ++j) {
+            const Run<L, V> run(j, lane, D);
 #pragma unroll
-        for (int e = 0; e < V; ++e) { v[j][e] -= mean; q += run.counts(e) ? v[j][e] * v[j][e] : 0.f; }
-    }
-    const float r = 1.f / sqrtf(row_sum<L>(q, sh) / (float)D + eps);
-    if (!on) return;
-    if (stats && lane == 0) { stats[2 * row] = mean; stats[2 * row + 1] = r; }
-    T* yr = y + row * (long)D;
+            for (int e = 0; e < V; ++e) { v[j][e] -= mean; q += run.counts(e) ? v[j][e] * v[j][e] : 0.f; }
+        }
+        const float r = 1.f / sqrtf(row_sum<L>(q, sh) / (float)D + eps);
+        if (!on) continue;                               // (rows of a workgroup end together where its lanes meet at barriers: R = 1)
+        if (stats && lane == 0) { stats[2 * row] = mean; stats[2 * row + 1] = r; }
+        T* yr = y + row * (long)D;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const Run<L, V> run(j, lane, D);
-        if (!run.on) continue;
+        for (int j = 0; j < NV; ++j) {
+            const Run<L, V> run(j, lane, D);
+            if (!run.on) continue;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[j][e] = v[j][e] * r * wv[j][e] + bv[j][e];
-        seq_store<T, V>(yr + run.c, v[j]);
+            for (int e = 0; e < V; ++e) v[j][e] = v[j][e] * r * wv[j][e] + bv[j][e];
+            seq_store<T, V>(yr + run.c, v[j], stream);
+        }
     }
 }
 
 template <typename T, int L, int V, int NV>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_bwd_kernel(const T* __restrict__ x, long xs, const T* __restrict__ dy, long dys, const void* __restrict__ w, int pdt,
-                                                                          const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, long rows, int D) {
+                                                                          const float* __restrict__ stats, T* __restrict__ dx, float* __restrict__ part, long rows, int D, bool stream) {
     constexpr int TH = L < 256 ? 256 : L, R = TH / L, E = NV * V;
     __shared__ float sh[R > 1 ? 2 * L * E : 64];
     const int lane = threadIdx.x % L, slot = threadIdx.x / L;
@@ -192,7 +202,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_bwd_kernel(const
                     }
 #pragma unroll
                     for (int e = 0; e < V; ++e) g[j][e] = r * (g[j][e] - s1 - n[j][e] * s2);
-                    seq_store<T, V>(xo + run.c, g[j]);
+                    seq_store<T, V>(xo + run.c, g[j], stream);
                 }
             }
         }
@@ -267,7 +277,13 @@ void with_layout(int D, F&& f) {
     else if (D <= 256 * 16) with_values<T, 256>(D, f);
     else with_values<T, 1024>(D, f);
 }
-int rows_per_group(int D) { return D <= 256 ? 16 : D <= 1024 ? 4 : 1; }
+// Workgroups: as many as their registers let the chip hold at once, each with a share of the rows (backward: 150 registers at 16 values a lane, three
+// workgroups of 256 to a CU; a fourth share would be a round of its own).
+int groups_of(long rows, int D, long most) {
+    const long want = cdiv(rows, D <= 256 ? 16 : D <= 1024 ? 4 : 1);
+    return (int)(want < most ? want : most);
+}
+int bwd_groups(long rows, int D) { return groups_of(rows, D, D > 4096 ? 512 : D > 512 ? 768 : 1024); }
 }  // namespace
 
 int seq_colsum2(const float* part, int nb, long D, void* out0, void* out1, int dtype, hipStream_t s) {
@@ -286,18 +302,12 @@ extern "C" int motif_layer_norm_fwd(const void* x, long x_rs, const void* weight
         using T = std::remove_pointer_t<decltype(t)>;
         with_layout<T>(D, [&](auto l, auto v, auto nv) {
             constexpr int L = decltype(l)::value, TH = L < 256 ? 256 : L;
-            layer_norm_fwd_kernel<T, L, decltype(v)::value, decltype(nv)::value><<<cdiv(rows, TH / L), TH, 0, (hipStream_t)stream>>>(
-                (const T*)x, x_rs, weight, bias, param_dtype, (T*)y, stats, rows, D, eps);
+            layer_norm_fwd_kernel<T, L, decltype(v)::value, decltype(nv)::value><<<groups_of(rows, D, 2048), TH, 0, (hipStream_t)stream>>>(
+                (const T*)x, x_rs, weight, bias, param_dtype, (T*)y, stats, rows, D, eps, rows * D * (long)sizeof(T) >= kSeqStream);
         });
     });
     MOTIF_LAUNCH_CHECK();
     return MOTIF_OK;
-}
-
-static int bwd_groups(long rows, int D) {
-    const long want = cdiv(rows, rows_per_group(D));
-    const long most = 1024;
-    return (int)(want < most ? want : most);
 }
 
 extern "C" long motif_layer_norm_bwd_ws_floats(long rows, int D) {
@@ -318,7 +328,7 @@ extern "C" int motif_layer_norm_bwd(const void* x, long x_rs, const void* dy, lo
         with_layout<T>(D, [&](auto l, auto v, auto nv) {
             constexpr int L = decltype(l)::value, TH = L < 256 ? 256 : L;
             layer_norm_bwd_kernel<T, L, decltype(v)::value, decltype(nv)::value><<<nb, TH, 0, (hipStream_t)stream>>>(
-                (const T*)x, x_rs, (const T*)dy, dy_rs, weight, param_dtype, stats, (T*)dx, params ? workspace : nullptr, rows, D);
+                (const T*)x, x_rs, (const T*)dy, dy_rs, weight, param_dtype, stats, (T*)dx, params ? workspace : nullptr, rows, D, rows * D * (long)sizeof(T) >= kSeqStream);
         });
     });
     MOTIF_LAUNCH_CHECK();

@@ -57,17 +57,23 @@ __device__ __forceinline__ void seq_load(const T* p, float (&out)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) out[i] = x[i];
 }
+// `stream`: past the caches, for outputs that they would not hold until they are read (kSeqStream bytes and more).
+constexpr long kSeqStream = 96L << 20;
 template <typename T, int N>
-__device__ __forceinline__ void seq_store(T* p, const float (&in)[N]) {
+__device__ __forceinline__ void seq_store(T* p, const float (&in)[N], bool stream = false) {
     constexpr int B = sizeof(T) * N, P = B < 16 ? B : 16;
     typedef typename SeqWords<P>::type W;
+    typedef W __attribute__((aligned(sizeof(T)))) AnyW;
     SeqRaw<T, N> x;
 #pragma unroll
     for (int i = 0; i < N; ++i) x.v[i] = (T)in[i];
     struct Words { W w[B / P]; };
     const Words y = __builtin_bit_cast(Words, x);
 #pragma unroll
-    for (int i = 0; i < B / P; ++i) __builtin_memcpy((char*)p + i * P, &y.w[i], P);
+    for (int i = 0; i < B / P; ++i) {
+        if (stream) __builtin_nontemporal_store(y.w[i], (AnyW*)((char*)p + i * P));
+        else __builtin_memcpy((char*)p + i * P, &y.w[i], P);
+    }
 }
 template <int N>
 __device__ __forceinline__ void seq_param_vec(const void* p, long i, int dtype, float (&out)[N]) {

@@ -1044,6 +1044,12 @@ def _seq_rows(x):
     return x.contiguous(), d
 
 
+def _once():
+    """A backward pass that is itself recorded (create_graph=True) would record nothing of what the library computes."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("motif_amd's sequence operators are differentiable once: their gradients cannot be differentiated (create_graph=True)")
+
+
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -1070,8 +1076,8 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once()
         x, weight, stats = ctx.saved_tensors
         d = x.shape[-1]
         rows = x.numel() // d
@@ -1153,8 +1159,8 @@ class _GruScan(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast):
+        _once()
         z, q, h0, cu, h = ctx.saved_tensors
         b, t, d, s = _scan_sizes(z, cu)
         need_z, need_q, need_h, _ = ctx.needs_input_grad
@@ -1226,8 +1232,8 @@ class _GatedMlp(torch.autograd.Function):
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
+        _once()
         x, wg, wu, g, u = ctx.saved_tensors
         f, k = wg.shape
         m, code = x.numel() // k, _SEQ_DTYPES[x.dtype]

@@ -633,3 +633,12 @@ def test_gru_scan_bad_values_stay_in_their_packed_sequence(ops, dtype, D):
             assert torch.equal(a[1:3], b[1:3])
     assert torch.equal(got[0][:100], want[0][:100]) and torch.equal(got[0][1500:2000], want[0][1500:2000])      # forward: what lies before them
     assert torch.equal(got[3][1501:], want[3][1501:])     # dq of the sequence behind the bad gradient: it reads neither q nor h
+
+
+def test_gradients_of_gradients_are_refused(ops):
+    x = torch.randn(5, 40, device="cuda", requires_grad=True)
+    z = torch.rand(1, 5, 40, device="cuda", requires_grad=True)
+    w = torch.randn(16, 40, device="cuda", requires_grad=True)
+    for y, leaf in ((ops.layer_norm(x), x), (ops.gru_scan(z, z.detach())[0], z), (ops.gated_mlp(x, w, w), x)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y.sum(), leaf, create_graph=True)
