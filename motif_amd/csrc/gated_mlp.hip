@@ -513,57 +513,77 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------------------
-// Up to 16 MT rows: a workgroup takes 16 columns of both projections, its 8 waves share the reduction, each lane reads 16 bytes of a weight row
-// (16 rows x 4 pieces per instruction) straight into the matrix instruction's operand; the waves' sums meet in LDS in a fixed order.  Bound by
-// the weights' bytes.  fp32 runs on the fp32 matrix instruction.
+// Up to 16 MT rows: a workgroup takes 16 columns of both projections, its 8 waves share the reduction, each lane reads 32 bytes of a weight row at a time
+// (16 rows x 128 bytes: whole cache lines) straight into the matrix instruction's operands -- which of the reduction's values a lane holds is free as
+// long as both operands agree --; the waves' sums meet in LDS in a fixed order.  Bound by the weights' bytes.  fp32 runs on the fp32 matrix instruction.
 template <typename T, int MT>
 __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long xs, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ bg, const T* __restrict__ bu,
                                                    T* __restrict__ h, float* __restrict__ G, float* __restrict__ U, long ldg, int M, int K, int F, int act) {
-    constexpr int V = 16 / sizeof(T), STEP = 4 * V, NW = 8;
+    constexpr int V = 16 / sizeof(T), STEP = 8 * V, NW = 8;
     __shared__ float sh[NW][2][16 * MT][17];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, kq = (lane >> 4) * V;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, kq = (lane >> 4) * 2 * V;
     const int f0 = blockIdx.x * 16, fr = min(f0 + lo, F - 1);
-    const T* pg = wg + (long)fr * K;
-    const T* pu = wu + (long)fr * K;
+    const T* pg = wg + (long)fr * K + kq;
+    const T* pu = wu + (long)fr * K + kq;
+    const T* px[MT];
     f32x4 ag[MT], au[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) ag[i] = au[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto read = [&](const T* row, int k) __attribute__((always_inline)) {
-        if (k + V <= K) return seq_raw<T, V>(row + k);
-        SeqRaw<T, V> v;
+    for (int i = 0; i < MT; ++i) {
+        px[i] = x + (long)min(i * 16 + lo, M - 1) * xs + kq;
+        ag[i] = au[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    typedef SeqRaw<T, V> Raw;
+    auto multiply = [&](const Raw& a, const Raw& b, const Raw& c, int i) __attribute__((always_inline)) {
+        if constexpr (sizeof(T) == 2) {
+            const s16x8 cv = __builtin_bit_cast(s16x8, c);
+            ag[i] = mfma(__builtin_bit_cast(s16x8, a), cv, ag[i], (T*)nullptr);
+            au[i] = mfma(__builtin_bit_cast(s16x8, b), cv, au[i], (T*)nullptr);
+        } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v.v[e] = k + e < K ? row[k + e] : (T)0.f;
-        return v;
-    };
-    const int steps = (K + STEP - 1) / STEP;
-    constexpr int AHEAD = MT == 1 ? 4 : 2;
-    for (int s = wave; s < steps; s += NW * AHEAD) {
-        SeqRaw<T, V> a[AHEAD], b[AHEAD], c[AHEAD][MT];
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            const int k = (s + j * NW) * STEP + kq;      // behind the last step: zeros
-            a[j] = read(pg, k);
-            b[j] = read(pu, k);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) c[j][i] = read(x + (long)min(i * 16 + lo, M - 1) * xs, k);
+            for (int e = 0; e < V; ++e) {
+                ag[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], c[e], ag[i], 0, 0, 0);
+                au[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[e], c[e], au[i], 0, 0, 0);
+            }
         }
+    };
+    constexpr int AHEAD = MT == 1 ? 4 : MT == 2 ? 2 : 1; // steps requested together: MT = 1, all that a wave has up to K = 2048 (16 bits)
+    const int whole = K / STEP;
+    int s = wave;
+    for (; s + (AHEAD - 1) * NW < whole; s += NW * AHEAD) {
+        Raw a[AHEAD][2], b[AHEAD][2], c[AHEAD][2][MT];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if constexpr (sizeof(T) == 2) {
-                    const s16x8 cv = __builtin_bit_cast(s16x8, c[j][i]);
-                    ag[i] = mfma(__builtin_bit_cast(s16x8, a[j]), cv, ag[i], (T*)nullptr);
-                    au[i] = mfma(__builtin_bit_cast(s16x8, b[j]), cv, au[i], (T*)nullptr);
-                } else {
+            for (int t = 0; t < 2; ++t) {
+                const int k = (s + j * NW) * STEP + t * V;
+                a[j][t] = seq_raw<T, V>(pg + k);
+                b[j][t] = seq_raw<T, V>(pu + k);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        ag[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j][e], c[j][i][e], ag[i], 0, 0, 0);
-                        au[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j][e], c[j][i][e], au[i], 0, 0, 0);
-                    }
-                }
+                for (int i = 0; i < MT; ++i) c[j][t][i] = seq_raw<T, V>(px[i] + k);
             }
+        __builtin_amdgcn_sched_barrier(0);               // (all of them requested before the first is used)
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) multiply(a[j][t], b[j][t], c[j][t][i], i);
     }
+    auto read = [&](const T* at, int k) __attribute__((always_inline)) {         // zeros behind the row's end
+        if (kq + k + V <= K) return seq_raw<T, V>(at + k);
+        Raw v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v.v[e] = kq + k + e < K ? at[k + e] : (T)0.f;
+        return v;
+    };
+    for (; s * STEP < K; s += NW)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int k = s * STEP + t * V;
+            const Raw a = read(pg, k), b = read(pu, k);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) multiply(a, b, read(px[i], k), i);
+        }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll

@@ -1003,7 +1003,7 @@ def _seq_type(t, what, name):
 
 def _seq_same(t, like, shape, what, name, dtypes):
     """Checks a further tensor of a call: shape, type and device."""
-    if t is None:
+    if t is None or (t.shape == shape and t.dtype in dtypes and t.device == like.device):
         return
     if tuple(t.shape) != tuple(shape):
         raise RuntimeError("%s: %s must be %s, got %s" % (what, name, list(shape), list(t.shape)))
@@ -1019,14 +1019,15 @@ def _seq_ptr(t):
 
 def _seq_call(name, device, *args):
     """One entry of the library on `device` and its current stream."""
-    fn = getattr(_lib.load(), name)
+    fn = getattr(_lib._lib or _lib.load(), name)
     stream = torch._C._cuda_getCurrentRawStream(device.index)          # torch.cuda.current_stream(device).cuda_stream, without 2 us of Python
     if device.index == torch.cuda.current_device():
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
             rc = fn(*args, stream)
-    check(rc, name)
+    if rc:
+        check(rc, name)
 
 
 def _seq_rows(x):
@@ -1051,13 +1052,17 @@ def _once():
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _layer_norm_fwd(x, weight, bias, eps, want_stats):
     d = x.shape[-1]
     rows = x.numel() // d
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if want_stats else None
     if rows:
         xr, rs = _seq_rows(x)
@@ -1131,6 +1136,8 @@ def _scan_sizes(z, cu):
 
 
 def _scan_workspace(b, t, d, cu, z):
+    if cu is None and t <= 16:                           # (no segments: no workspace)
+        return None
     n = _lib.load().motif_gru_scan_ws_floats(b, t, d, int(cu is not None), _SEQ_DTYPES[z.dtype])
     if n < 0:
         raise RuntimeError("gru_scan: sizes %s outside what the kernels support (%d)" % (list(z.shape), n))
@@ -1139,7 +1146,7 @@ def _scan_workspace(b, t, d, cu, z):
 
 def _gru_scan_fwd(z, q, h0, cu):
     b, t, d, s = _scan_sizes(z, cu)
-    h = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    h = torch.empty_like(q, memory_format=torch.contiguous_format)
     last = torch.empty(s if cu is not None else b, d, dtype=torch.float32, device=q.device)
     if b * d == 0 or (t == 0 and cu is None):            # nothing to walk: the states stay what they were
         return h, last.copy_(h0) if h0 is not None else last.zero_()
@@ -1218,7 +1225,7 @@ def _gated_mlp_fwd(x, wg, wu, bg, bu, act, keep):
     if m:
         xr, rs = _seq_rows(x)
         args = (xr.data_ptr(), rs, wg.data_ptr(), wu.data_ptr())
-        ws = _mlp_workspace(_lib.load().motif_gated_mlp_ws_bytes(*args, m, k, f, code), x, k, f)
+        ws = _mlp_workspace(_lib.load().motif_gated_mlp_ws_bytes(*args, m, k, f, code), x, k, f) if m > 64 else None      # (few rows: no workspace)
         _seq_call("motif_gated_mlp_fwd", x.device, *args, _seq_ptr(bg), _seq_ptr(bu), h.data_ptr(), _seq_ptr(g), _seq_ptr(u), _seq_ptr(ws), m, k, f, act, code)
     return h, g, u
 
