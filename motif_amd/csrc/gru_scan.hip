@@ -333,15 +333,16 @@ __global__ __launch_bounds__(256) void gru_scan_empty_kernel(const int* __restri
 struct Plan { int V, TX, TY, R, groups, segs; long seg_rows; };
 
 // Vectors of 16 bytes, single values for rows shorter than that.  TY = 1 (a lane walks the whole sequence) where the
-// sequence is no longer than 16 rows or the channels alone give every CU two workgroups; else 32 time slots (8 with single values, whose
-// rows need more lanes to fill a cache line).  Segments: as many as give every CU four workgroups, none below two tiles.
+// sequence is no longer than 16 rows or the channels alone give every CU two workgroups; else 16 time slots, rows of 256 bytes (8 with single values, whose
+// rows need more lanes to fill a cache line).  Segments: as many as the chip holds workgroups of the second kernel at once -- three to a CU forward, four
+// backward, by their registers --, none below two tiles (65536 x 1024 bf16, forward: 74 us with 768 workgroups, 85 us with 1024).
 int vec_of(int dtype, long D) { const int V = 16 / seq_size(dtype); return D < V ? 1 : V; }
-Plan plan_of(int V, long B, long T, long D) {
+Plan plan_of(int V, long B, long T, long D, bool bwd) {
     Plan p;
     p.V = V;
     const long lanes = (D + V - 1) / V;
     const bool serial = T <= 16 || B * ((lanes + 255) / 256) >= 512;
-    p.TY = serial ? 1 : V > 1 ? 32 : 8;
+    p.TY = serial ? 1 : V > 1 ? 16 : 8;
     p.TX = 256 / p.TY;
     p.R = 4;
     p.groups = (int)((lanes + p.TX - 1) / p.TX);
@@ -349,7 +350,7 @@ Plan plan_of(int V, long B, long T, long D) {
     p.seg_rows = T;
     if (!serial) {
         const long tile = (long)p.TY * p.R, tiles = (T + tile - 1) / tile;
-        long segs = 1024 / (B * p.groups);
+        long segs = (bwd ? 1024 : 768) / (B * p.groups);
         segs = segs < 1 ? 1 : segs > 128 ? 128 : segs;
         const long per = segs < 2 ? tiles : (tiles + segs - 1) / segs < 2 ? 2 : (tiles + segs - 1) / segs;
         p.segs = (int)((tiles + per - 1) / per);
@@ -361,7 +362,7 @@ Plan plan_of(int V, long B, long T, long D) {
 template <typename T, int V, bool BWD, bool PACKED>
 void launch(const Plan& pl, const ScanArgs& a, hipStream_t s) {
     const unsigned grid = (unsigned)((long)a.B * pl.segs * pl.groups);
-    constexpr int TY = V > 1 ? 32 : 8, R = BWD ? 2 : 4;  // backward holds four tensors' rows
+    constexpr int TY = V > 1 ? 16 : 8, R = BWD ? 1 : 4;  // backward holds four tensors' rows
     if (pl.TY == 1) { gru_scan_kernel<T, V, 256, 1, R, BWD, PACKED><<<grid, 256, 0, s>>>(a); return; }
     if (pl.segs > 1) gru_scan_segments_kernel<T, V, 256 / TY, TY, BWD, PACKED><<<grid, 256, 0, s>>>(a);
     gru_scan_kernel<T, V, 256 / TY, TY, R, BWD, PACKED><<<grid, 256, 0, s>>>(a);
@@ -379,7 +380,7 @@ long cut_floats(const Plan& p, bool packed) { return packed && p.segs > 1 ? (p.s
 
 int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const float* empty_in, hipStream_t s) {
     const int V = vec_of(dtype, a.D);
-    const Plan pl = plan_of(V, a.B, a.T, a.D);
+    const Plan pl = plan_of(V, a.B, a.T, a.D, bwd);
     if ((long)a.B * pl.segs * pl.groups > 0x7fffffffL) return MOTIF_ELIMIT;
     if (pl.TY > 1) for (long stride : {a.zr, a.qr, a.dr, (long)a.D}) if (stride > 1L << 22) return MOTIF_ELIMIT;      // 128 rows x 4 bytes in 32 bits
     a.groups = pl.groups;
@@ -414,8 +415,13 @@ int check_sizes(long B, long T, long D, int S, const void* cu, int dtype) {
 extern "C" long motif_gru_scan_ws_floats(long B, long T, long D, int packed, int dtype) {
     const int rc = check_sizes(B, T, D, packed ? 1 : 0, packed ? (const void*)&B : nullptr, dtype);
     if (rc) return rc;
-    const Plan p = plan_of(vec_of(dtype, D), B, T, D);
-    return agg_floats(p, B, D) + cut_floats(p, packed) + (packed ? T : 0);
+    long need = 0;                                       // of either direction
+    for (bool bwd : {false, true}) {
+        const Plan p = plan_of(vec_of(dtype, D), B, T, D, bwd);
+        const long n = agg_floats(p, B, D) + cut_floats(p, packed);
+        need = n > need ? n : need;
+    }
+    return need + (packed ? T : 0);
 }
 
 extern "C" int motif_gru_scan_fwd(const void* z, long z_bs, long z_rs, const void* q, long q_bs, long q_rs, const float* h0, const int32_t* cu_seqlens, int S,
