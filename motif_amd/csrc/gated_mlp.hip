@@ -468,35 +468,54 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
                                                        void* dst, long plane, long pair, float* part, int rows, bool stream) {
     using O = std::conditional_t<sizeof(T) == 4, bf16_t, T>;
     __shared__ float sh[8][2][32][9];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.y * 256 + x * 8;
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c0 = blockIdx.y * 256 + x * 8, c = min(c0, ld - 8);
     const long r0 = (long)blockIdx.x * rows;
     float sg[8], su[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sg[e] = su[e] = 0.f;
-    if (c < ld) {
-#pragma unroll 2
-        for (int i = y; i < rows; i += 8) {
-            const long r = r0 + i;
-            if (r >= M) break;
-            float d[8], g[8], u[8];
-            if (c + 8 <= F) seq_load<T, 8>(dh + r * dhs + c, d);
-            else
+    // Every access is taken (rows behind the last do it again, lanes behind the last columns theirs, for no sum): the next row's requests then
+    // stay in flight while this one is computed and written.
+    struct Row { SeqRaw<T, 8> d; SeqRaw<float, 8> g, u; };
+    auto read = [&](Row& w, long r) __attribute__((always_inline)) {
+        const T* at = dh + r * dhs + c;
+        if (F >= 8) w.d = seq_raw<T, 8>(at - max(c + 8 - F, 0));      // a run that passes the row's end: the row's last eight values, moved below
+        else
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d[e] = c + e < F ? (float)dh[r * dhs + c + e] : 0.f;
-            seq_load<float, 8>(G + r * ld + c, g);
-            seq_load<float, 8>(U + r * ld + c, u);
+            for (int e = 0; e < 8; ++e) w.d.v[e] = c + e < F ? at[e] : (T)0.f;
+        w.g = seq_raw<float, 8>(G + r * ld + c);
+        w.u = seq_raw<float, 8>(U + r * ld + c);
+    };
+    const int move = F >= 8 ? max(c + 8 - F, 0) : 0;     // 0 but in the last run
+    Row now, next;
+    read(now, min(r0 + y, (long)M - 1));
+    for (int i = y; i < rows; i += 8) {
+        const long r = min(r0 + i, (long)M - 1);
+        const bool counts = r0 + i < M && c == c0;
+        read(next, min(r0 + min(i + 8, rows - 8 + y), (long)M - 1));
+        float g[8], u[8], d[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float v, dv;
-                gate_grad<sizeof(T) == 2>(g[e], act, v, dv);
-                g[e] = c + e < F ? d[e] * u[e] * dv : 0.f;
-                u[e] = c + e < F ? d[e] * v : 0.f;
-                sg[e] += g[e];
-                su[e] += u[e];
+        for (int e = 0; e < 8; ++e) d[e] = now.d[e];
+        if (move) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {                // d[e] = what stands at e + move (a run-time index would put the values into memory)
+                float t = 0.f;
+#pragma unroll
+                for (int k = e; k < 8; ++k) t = k == e + move ? now.d[k] : t;
+                d[e] = t;
             }
-            put8((T*)nullptr, dst, plane, r * ld + c, g, stream);
-            put8((T*)nullptr, (O*)dst + pair, plane, r * ld + c, u, stream);
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float v, dv;
+            gate_grad<sizeof(T) == 2>(now.g[e], act, v, dv);
+            g[e] = c + e < F ? d[e] * now.u[e] * dv : 0.f;
+            u[e] = c + e < F ? d[e] * v : 0.f;
+            sg[e] += counts ? g[e] : 0.f;
+            su[e] += counts ? u[e] : 0.f;
+        }
+        put8((T*)nullptr, dst, plane, r * ld + c, g, stream);
+        put8((T*)nullptr, (O*)dst + pair, plane, r * ld + c, u, stream);
+        now = next;
     }
     if (!part) return;
 #pragma unroll

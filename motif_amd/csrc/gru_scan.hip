@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void gru_scan_segments_kernel(ScanArgs p) {
     const Where at = where(p);
     if (at.seg == p.segs - 1) return;
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, first = (at.group * TX + tx) * V, c0 = min(first, p.D - V);
-    const bool on = first < p.D;                         // (the last lane of a row takes its last V channels: those it shares are written twice, alike)
+    const bool on = first < p.D;                         // (the last lanes of a row take its last V channels: those they share are written more than once, alike)
     const T* z = (const T*)p.z + at.b * p.zb + c0;
     const T* x = BWD ? (const T*)p.dh + at.b * p.db + c0 : (const T*)p.q + at.b * p.qb + c0;
     const long xr = BWD ? p.dr : p.qr;
@@ -143,11 +143,11 @@ __global__ __launch_bounds__(256) void gru_scan_segments_kernel(ScanArgs p) {
     int cut = 0;
     zero(A, 1.f);
     zero(H);
-    if (on) {
+    {
         Rows now, next;
         read(now, k0);
         for (long k = k0; k < k0 + run; k += 4) {
-            if (k + 4 < k0 + run) read(next, k + 4);
+            read(next, min(k + 4, k0 + run - 4));        // (always taken: the compiler counts the requests behind the one it waits for)
 #pragma unroll
             for (int r = 0; r < 4; ++r) compose<BWD, PACKED, V>(A, H, cut, now.z[r], now.x[r], now.f[r], BWD ? p.dlast : p.h0, c0, p.D);
             now = next;
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
     __shared__ typename S::Sums sums[2];
     const Where at = where(p);
     const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, first = (at.group * TX + tx) * V, c0 = min(first, p.D - V);
-    const bool on = first < p.D;                         // (the last lane of a row takes its last V channels: those it shares are written twice, alike)
+    // (the last lanes of a row take its last V channels: those they share are written more than once, alike)
     // Addresses: a uniform row of the tile, and a lane's offset from it in bytes (32 bits: the host bounds the strides where TY > 1).  Backward, time
     // runs down: slot TY - 1 has the tile's first rows.
     const int slot = (BWD ? TY - 1 - ty : ty) * R;
@@ -201,30 +201,35 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
     typedef SeqRaw<T, V> Raw;
     struct Rows { Raw z[R], q[R], d[BWD ? R : 1], h[BWD ? R : 1]; int f[R]; };
     auto row = [&](long k0, int r) __attribute__((always_inline)) { return BWD ? p.T - 1 - k0 - (TY * R - 1) + (R - 1 - r) : k0 + r; };
-    auto read = [&](Rows& w, long k0) __attribute__((always_inline)) {
+    // Whole tiles are read without a condition: the compiler then knows how many requests are younger than those it waits for, and the wait for a
+    // tile is none for the one requested behind it, nor for the stores between.
+    auto read = [&](Rows& w, long k0, bool whole) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const long k = k0 + ty * R + r, t = BWD ? p.T - 1 - k : k, t0 = row(k0, r);
-            w.z[r] = w.q[r] = Raw{};                     // no row: x -> x
-            if constexpr (BWD) w.d[r] = w.h[r] = Raw{};
-            if (PACKED) w.f[r] = 0;
-            if (on && k < k_end) {
+            if (!whole) {                                // no row: x -> x
+                w.z[r] = w.q[r] = Raw{};
+                if constexpr (BWD) w.d[r] = w.h[r] = Raw{};
+                if (PACKED) w.f[r] = 0;
+            }
+            if (whole || k < k_end) {
                 w.z[r] = seq_raw<T, V>((const T*)(z + t0 * p.zr * (long)sizeof(T) + oz));
-                if (!BWD || out0) w.q[r] = seq_raw<T, V>((const T*)(q + t0 * p.qr * (long)sizeof(T) + oq));
+                w.q[r] = seq_raw<T, V>((const T*)(q + t0 * p.qr * (long)sizeof(T) + oq));
                 if constexpr (BWD) {
                     w.d[r] = seq_raw<T, V>((const T*)(dh + t0 * p.dr * (long)sizeof(T) + od));
-                    if (out0 && t > 0) w.h[r] = seq_raw<T, V>((const T*)(hs + (t0 - 1) * p.D * (long)sizeof(T) + oo));
+                    w.h[r] = seq_raw<T, V>((const T*)(hs + (t0 - 1) * p.D * (long)sizeof(T) + (t > 0 ? oo : oo + (unsigned)p.D * (unsigned)sizeof(T))));
                 }
                 if (PACKED) w.f[r] = p.info[t];
             }
         }
     };
+    const long k_begin = at.seg * p.seg_rows, wholes = (k_end - k_begin) / (TY * R);
     Rows now, next;
-    read(now, at.seg * p.seg_rows);
+    if (wholes > 0) read(now, k_begin, true);
 
     float carry[V];
     zero(carry);                                         // (packed: a sequence's own state enters at its first row)
-    if (!PACKED && init && on) seq_load<float, V>(init + at.b * p.D + c0, carry);
+    if (!PACKED && init) seq_load<float, V>(init + at.b * p.D + c0, carry);
     int buf = 0;
     if (TY > 1 && at.seg > 0) {                          // the segments in front: slot ty composes a run of them, then the slots compose
         float A[V], H[V], in[V];
@@ -232,7 +237,7 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
         zero(A, 1.f);
         zero(H);
         const int per = (at.seg + TY - 1) / TY;
-        if (on) {
+        {
 #pragma unroll 2
             for (int s = ty * per; s < min(at.seg, (ty + 1) * per); ++s) {
                 float a[V], h[V];
@@ -250,8 +255,7 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
         S::template waves_apply<PACKED>(carry, in, sums[0], tx);
         buf = 1;
     }
-    for (long k0 = at.seg * p.seg_rows; k0 < k_end; k0 += TY * R) {
-        if (k0 + TY * R < k_end) read(next, k0 + TY * R);
+    auto tile = [&](const long k0, bool whole) __attribute__((always_inline)) {
         float h[V];
         if constexpr (TY > 1) {
             float A[V], H[V], in[V];
@@ -275,7 +279,7 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const long k = k0 + ty * R + r, t = BWD ? p.T - 1 - k : k, out = row(k0, r) * p.D * (long)sizeof(T);
-            if (!on || k >= k_end) continue;
+            if (!whole && k >= k_end) continue;
             const int f = PACKED ? now.f[r] : 0;
             const bool none = PACKED && f < 0, head = PACKED ? f >= 0 && (f & kFirst) : t == 0, tail = PACKED ? f >= 0 && (f & kLast) : t == p.T - 1;
             const long own = (PACKED ? (long)(f >> 2) : at.b) * p.D + c0;
@@ -306,7 +310,15 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
 #pragma unroll
             for (int v = 0; v < V; ++v) carry[v] = h[v];
         }
+    };
+    for (long i = 0; i < wholes; ++i) {
+        read(next, k_begin + min(i + 1, wholes - 1) * (TY * R), true);
+        tile(k_begin + i * (TY * R), true);
         now = next;
+    }
+    if (k_begin + wholes * (TY * R) < k_end) {
+        read(now, k_begin + wholes * (TY * R), false);
+        tile(k_begin + wholes * (TY * R), false);
     }
 }
 
@@ -362,7 +374,7 @@ Plan plan_of(int V, long B, long T, long D, bool bwd) {
 template <typename T, int V, bool BWD, bool PACKED>
 void launch(const Plan& pl, const ScanArgs& a, hipStream_t s) {
     const unsigned grid = (unsigned)((long)a.B * pl.segs * pl.groups);
-    constexpr int TY = V > 1 ? 16 : 8, R = BWD ? 1 : 4;  // backward holds four tensors' rows
+    constexpr int TY = V > 1 ? 16 : 8, R = BWD ? 1 : PACKED ? 2 : 4;      // registers: backward holds four tensors, packed rows their meaning and a second start
     if (pl.TY == 1) { gru_scan_kernel<T, V, 256, 1, R, BWD, PACKED><<<grid, 256, 0, s>>>(a); return; }
     if (pl.segs > 1) gru_scan_segments_kernel<T, V, 256 / TY, TY, BWD, PACKED><<<grid, 256, 0, s>>>(a);
     gru_scan_kernel<T, V, 256 / TY, TY, R, BWD, PACKED><<<grid, 256, 0, s>>>(a);
@@ -407,7 +419,7 @@ int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const 
 int check_sizes(long B, long T, long D, int S, const void* cu, int dtype) {
     if (B < 1 || T < 0 || D < 1 || !seq_dtype_ok(dtype)) return MOTIF_EINVAL;
     if (cu ? (B != 1 || S < 1) : T < 1) return MOTIF_EINVAL;
-    if (D > 0x3fffffffL || T > 0x7ffffff0L || B >= (1L << 29) || S >= (1 << 29)) return MOTIF_ELIMIT;
+    if (D > 0x0fffffffL || T > 0x7ffffff0L || B >= (1L << 29) || S >= (1 << 29)) return MOTIF_ELIMIT;
     return MOTIF_OK;
 }
 }  // namespace

@@ -47,18 +47,18 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* sh) {
 }
 
 // Run j of a lane: V columns from `c`.  Rows need not be whole runs: the run that would pass the row's end moves back onto the row's last V values,
-// of which `skip` belong to the run before -- they count for nothing in the sums and are written twice, alike.
+// and so do those wholly behind it.  What they share with runs before counts for nothing in the sums and is written more than once, alike.
+// No access depends on a lane or a row: in a loop whose loads and stores are all taken, the compiler knows how many are younger than the ones
+// it waits for, and the wait for the next row's values does not become a wait for this row's stores.
 template <int L, int V>
 struct Run {
     int c, skip;
-    bool on;
     __device__ __forceinline__ Run(int j, int lane, int D) {
         const int first = (j * L + lane) * V;
-        on = first < D;
         c = min(first, D - V);
         skip = first - c;
     }
-    __device__ __forceinline__ bool counts(int e) const { return on && e >= skip; }
+    __device__ __forceinline__ bool counts(int e) const { return e >= skip; }
 };
 
 // A lane's columns of a parameter; `none` where there is no parameter.
@@ -69,7 +69,7 @@ __device__ __forceinline__ void params(const void* p, int D, int pdt, int lane, 
         const Run<L, V> run(j, lane, D);
 #pragma unroll
         for (int e = 0; e < V; ++e) out[j][e] = none;
-        if (p && run.on) seq_param_vec<V>(p, run.c, pdt, out[j]);
+        if (p) seq_param_vec<V>(p, run.c, pdt, out[j]);
     }
 }
 
@@ -83,22 +83,18 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_fwd_kernel(const
     const long step = (long)gridDim.x * R;
     SeqRaw<T, V> next[NV];
     auto request = [&](long row) __attribute__((always_inline)) {
-        if (row >= rows) return;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const Run<L, V> run(j, lane, D);
-            if (run.on) next[j] = seq_raw<T, V>(x + row * xs + run.c);
-        }
+        for (int j = 0; j < NV; ++j) next[j] = seq_raw<T, V>(x + row * xs + Run<L, V>(j, lane, D).c);
     };
-#pragma unroll
-    for (int j = 0; j < NV; ++j) next[j] = SeqRaw<T, V>{};
-    long row = (long)blockIdx.x * R + threadIdx.x / L;
+    const long first = (long)blockIdx.x * R + threadIdx.x / L;
+    long row = min(first, rows - 1);                     // (a slot without a row of its own does the last one again)
     request(row);
     float wv[NV][V], bv[NV][V];
     params<L, V, NV>(w, D, pdt, lane, 1.f, wv);
     params<L, V, NV>(b, D, pdt, lane, 0.f, bv);
-    for (long base = (long)blockIdx.x * R; base < rows; base += step, row += step) {
-        const bool on = row < rows;
+    for (long base = (long)blockIdx.x * R, at = first; base < rows; base += step) {
+        at += step;
+        const long next_row = min(at, rows - 1);
         float v[NV][V];
         float s = 0.f;
 #pragma unroll
@@ -107,7 +103,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_fwd_kernel(const
 #pragma unroll
             for (int e = 0; e < V; ++e) { v[j][e] = next[j][e]; s += run.counts(e) ? v[j][e] : 0.f; }
         }
-        request(row + step);
+        request(next_row);
         const float mean = row_sum<L>(s, sh) / (float)D;
         float q = 0.f;
 #pragma unroll
@@ -117,17 +113,15 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_fwd_kernel(const
             for (int e = 0; e < V; ++e) { v[j][e] -= mean; q += run.counts(e) ? v[j][e] * v[j][e] : 0.f; }
         }
         const float r = 1.f / sqrtf(row_sum<L>(q, sh) / (float)D + eps);
-        if (!on) continue;                               // (rows of a workgroup end together where its lanes meet at barriers: R = 1)
         if (stats && lane == 0) { stats[2 * row] = mean; stats[2 * row + 1] = r; }
         T* yr = y + row * (long)D;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const Run<L, V> run(j, lane, D);
-            if (!run.on) continue;
 #pragma unroll
             for (int e = 0; e < V; ++e) v[j][e] = v[j][e] * r * wv[j][e] + bv[j][e];
-            seq_store<T, V>(yr + run.c, v[j], stream);
+            seq_store<T, V>(yr + Run<L, V>(j, lane, D).c, v[j], stream);
         }
+        row = next_row;
     }
 }
 
@@ -148,23 +142,22 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_bwd_kernel(const
     const long step = (long)gridDim.x * R;
     constexpr bool AHEAD = L < 1024;                     // 16 waves have 128 registers each: none to spare
     Raw xn[NV], dn[NV];                                  // the next row, requested while this one is summed
-    float mean_n = 0.f, r_n = 0.f;
+    float mean_n, r_n;
     auto request = [&](long row) __attribute__((always_inline)) {
-        if (row >= rows) return;
         mean_n = stats[2 * row];
         r_n = stats[2 * row + 1];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const Run<L, V> run(j, lane, D);
-            if (run.on) { xn[j] = seq_raw<T, V>(x + row * xs + run.c); dn[j] = seq_raw<T, V>(dy + row * dys + run.c); }
+            const int c = Run<L, V>(j, lane, D).c;
+            xn[j] = seq_raw<T, V>(x + row * xs + c);
+            dn[j] = seq_raw<T, V>(dy + row * dys + c);
         }
     };
-#pragma unroll
-    for (int j = 0; j < NV; ++j) xn[j] = dn[j] = Raw{};
-    if (AHEAD) request((long)blockIdx.x * R + slot);
-    for (long base = (long)blockIdx.x * R; base < rows; base += step) {
-        const long row = base + slot;
-        const bool on = row < rows;
+    long at = (long)blockIdx.x * R + slot;
+    if (AHEAD) request(min(at, rows - 1));
+    for (long base = (long)blockIdx.x * R; base < rows; base += step, at += step) {
+        const bool on = at < rows;                       // (a slot without a row of its own does the last one again, for no sum)
+        const long row = min(at, rows - 1);
         if (!AHEAD) request(row);
         const float mean = mean_n, r = r_n;
         float n[NV][V], g[NV][V];
@@ -176,34 +169,30 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void layer_norm_bwd_kernel(const
             for (int e = 0; e < V; ++e) {
                 n[j][e] = (xn[j][e] - mean) * r;
                 const float d = dn[j][e], gw = d * wv[j][e];
-                const bool counts = on && run.counts(e);
-                aw[j][e] += counts ? d * n[j][e] : 0.f;
-                ab[j][e] += counts ? d : 0.f;
+                const bool counts = run.counts(e);       // (in the row's own sums; a row done again counts for no column)
+                aw[j][e] += counts && on ? d * n[j][e] : 0.f;
+                ab[j][e] += counts && on ? d : 0.f;
                 s1 += counts ? gw : 0.f;
                 s2 += counts ? gw * n[j][e] : 0.f;
                 g[j][e] = gw;
             }
         }
-        if (AHEAD) request(row + step);
+        if (AHEAD) request(min(at + step, rows - 1));
         if (dx) {
             row_sum2<L>(s1, s2, sh);
             s1 *= inv; s2 *= inv;
-            if (on) {
-                T* xo = dx + row * (long)D;
+            T* xo = dx + row * (long)D;
 #pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const Run<L, V> run(j, lane, D);
-                    if (!run.on) continue;
-                    if constexpr (!AHEAD) {              // (from what was read: n and g of the first walk would not fit)
-                        seq_hold(xn[j]);
-                        seq_hold(dn[j]);
+            for (int j = 0; j < NV; ++j) {
+                if constexpr (!AHEAD) {                  // (from what was read: n and g of the first walk would not fit)
+                    seq_hold(xn[j]);
+                    seq_hold(dn[j]);
 #pragma unroll
-                        for (int e = 0; e < V; ++e) { n[j][e] = (xn[j][e] - mean) * r; g[j][e] = dn[j][e] * wv[j][e]; }
-                    }
-#pragma unroll
-                    for (int e = 0; e < V; ++e) g[j][e] = r * (g[j][e] - s1 - n[j][e] * s2);
-                    seq_store<T, V>(xo + run.c, g[j], stream);
+                    for (int e = 0; e < V; ++e) { n[j][e] = (xn[j][e] - mean) * r; g[j][e] = dn[j][e] * wv[j][e]; }
                 }
+#pragma unroll
+                for (int e = 0; e < V; ++e) g[j][e] = r * (g[j][e] - s1 - n[j][e] * s2);
+                seq_store<T, V>(xo + Run<L, V>(j, lane, D).c, g[j], stream);
             }
         }
     }
