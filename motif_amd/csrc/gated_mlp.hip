@@ -468,8 +468,9 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
                                                        void* dst, long plane, long pair, float* part, int rows, bool stream) {
     using O = std::conditional_t<sizeof(T) == 4, bf16_t, T>;
     __shared__ float sh[8][2][32][9];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c0 = blockIdx.y * 256 + x * 8, c = min(c0, ld - 8);
-    const long r0 = (long)blockIdx.x * rows;
+    const int cols = (ld + 255) / 256, cb = blockIdx.x % cols, rb = blockIdx.x / cols;      // neighbouring workgroups take neighbouring columns of the same rows
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c0 = cb * 256 + x * 8, c = min(c0, ld - 8);
+    const long r0 = (long)rb * rows;
     float sg[8], su[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sg[e] = su[e] = 0.f;
@@ -522,12 +523,12 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
     for (int e = 0; e < 8; ++e) { sh[y][0][x][e] = sg[e]; sh[y][1][x][e] = su[e]; }
     __syncthreads();
     for (int i = threadIdx.x; i < 512; i += 256) {
-        const int k = i >> 8, cx = i & 255, cc = blockIdx.y * 256 + cx;
+        const int k = i >> 8, cx = i & 255, cc = cb * 256 + cx;
         if (cc >= F) continue;
         float s = 0.f;
 #pragma unroll
         for (int q = 0; q < 8; ++q) s += sh[q][k][cx >> 3][cx & 7];
-        part[((long)blockIdx.x * 2 + k) * F + cc] = s;
+        part[((long)rb * 2 + k) * F + cc] = s;
     }
 }
 
@@ -836,7 +837,7 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
     seq_dispatch(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const int rows = grad_rows(M, F);
-        const dim3 grid(cdiv(M, rows), cdiv(b.dg.ld, 256));
+        const unsigned grid = (unsigned)((long)cdiv(M, rows) * cdiv(b.dg.ld, 256));
         gate_grad_kernel<T><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows, 4 * b.dg.plane * b.dg.n >= kSeqStream);
     });
     if (need_b) {
