@@ -40,3 +40,27 @@ class Linear(nn.Module):
         self.bias = nn.Parameter(torch.empty(cout))
         nn.init.kaiming_uniform_(self.weight, a=math.sqrt(5))
         nn.init.zeros_(self.bias)
+
+
+class LayerNorm(nn.Module):
+    """Same parameters / keys as nn.LayerNorm over the last axis; forward = ops.layer_norm.  Differentiable."""
+
+    def __init__(self, dim, eps=1e-5):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.bias = nn.Parameter(torch.zeros(dim))
+        self.eps = eps
+
+    def forward(self, x):
+        return ops.layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class GatedMLP(nn.Module):
+    """act(gate(x)) * up(x), two Linear layers of nn.Linear's keys (`gate.*`, `up.*`) in one kernel (ops.gated_mlp).  Differentiable."""
+
+    def __init__(self, cin, cout, act="silu"):
+        super().__init__()
+        self.gate, self.up, self.act = Linear(cin, cout), Linear(cin, cout), act
+
+    def forward(self, x):
+        return ops.gated_mlp(x, self.gate.weight, self.up.weight, self.gate.bias, self.up.bias, self.act)

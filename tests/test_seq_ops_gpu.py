@@ -642,3 +642,149 @@ def test_gradients_of_gradients_are_refused(ops):
     for y, leaf in ((ops.layer_norm(x), x), (ops.gru_scan(z, z.detach())[0], z), (ops.gated_mlp(x, w, w), x)):
         with pytest.raises(RuntimeError, match="differentiable once"):
             torch.autograd.grad(y.sum(), leaf, create_graph=True)
+
+
+# ------------------------------------------------------------------------------------------------------------------ together
+def block(ops, norm, mlp, out, x, h0, cu=None):
+    """A recurrent block over the frames of a clip, its gates from the normalised frame: norm -> gated projections -> scan -> add, norm."""
+    d = x.shape[-1]
+    f = mlp(norm(x))
+    h, last = ops.gru_scan(torch.sigmoid(f[..., :d]), torch.tanh(f[..., d:]), h0, cu_seqlens=cu)
+    return out(x + h), last
+
+
+def block_reference(norm, mlp, out, x, h0):
+    d = x.shape[-1]
+
+    def ln(m, v):
+        return torch.nn.functional.layer_norm(v, (d,), m.weight.double(), m.bias.double(), m.eps)
+    n = ln(norm, x.double())
+    g, u = n @ mlp.gate.weight.double().t() + mlp.gate.bias.double(), n @ mlp.up.weight.double().t() + mlp.up.bias.double()
+    f = torch.nn.functional.silu(g) * u
+    z, q, s, h = torch.sigmoid(f[..., :d]), torch.tanh(f[..., d:]), h0.double(), []
+    for t in range(x.shape[1]):
+        s = (1 - z[:, t]) * s + z[:, t] * q[:, t]
+        h.append(s)
+    return ln(out, x.double() + torch.stack(h, 1)), s
+
+
+def block_of(d, seed):
+    from motif_amd.models.modules.layers import GatedMLP, LayerNorm
+    torch.manual_seed(seed)
+    parts = [LayerNorm(d), GatedMLP(d, 2 * d), LayerNorm(d)]
+    with torch.no_grad():
+        for p in (p for m in parts for p in m.parameters()):
+            p.add_(0.1 * torch.randn_like(p))
+    return [m.cuda() for m in parts]
+
+
+def test_the_operators_together_as_a_recurrent_block_in_training(ops):
+    parts = block_of(64, 1)
+    x = torch.randn(3, 90, 64, generator=gen(1), device="cuda", requires_grad=True)
+    h0 = torch.randn(3, 64, generator=gen(2), device="cuda", requires_grad=True)
+    dy, dl = torch.randn(3, 90, 64, generator=gen(3), device="cuda"), torch.randn(3, 64, generator=gen(4), device="cuda")
+    leaves = [x, h0] + [p for m in parts for p in m.parameters()]
+    y, last = block(ops, *parts, x, h0)
+    got = torch.autograd.grad((y, last), leaves, (dy, dl))
+    yr, lr = block_reference(*parts, x, h0)
+    want = torch.autograd.grad((yr, lr), leaves, (dy.double(), dl.double()))
+    # five stages, each within a few hundred roundings of 2^-24 of values of order 1 (sums: of their terms' root sum of squares, at most 10 x the
+    # result's scale here): 2^-24 x 500 x 10
+    for a, b in zip((y, last) + got, (yr, lr) + want):
+        within(a, b, 5000 * F32 * (1 + b.abs().max()))
+
+
+def test_the_operators_together_stream_a_clip_and_replay_in_a_graph(ops):
+    """Serving: a clip at once, frame by frame with the state carried along, and frame by frame as the replay of one captured frame."""
+    for dtype, tol in ((torch.float32, 4000 * F32), (torch.bfloat16, 2.0 ** -4)):      # bf16: six roundings of 2^-8 on values up to 4
+        parts = [m.to(dtype) for m in block_of(96, 2)]
+        x = torch.randn(2, 12, 96, generator=gen(5), device="cuda").to(dtype)
+        h0 = torch.zeros(2, 96, device="cuda")
+        with torch.no_grad():
+            whole, last = block(ops, *parts, x, h0)
+            state, rows = h0, []
+            for t in range(12):
+                y, state = block(ops, *parts, x[:, t:t + 1], state)
+                rows.append(y)
+            within(torch.cat(rows, 1), whole, tol)
+            within(state, last, tol)
+            frame, held = x[:, :1].clone(), h0.clone()
+            graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.graph(graph, stream=side):
+                out, new = block(ops, *parts, frame, held)
+                held.copy_(new)
+            for t in range(12):
+                frame.copy_(x[:, t:t + 1])
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, rows[t]), (dtype, t)
+                block(ops, *parts, x, h0)                 # eager work between the replays
+            assert torch.equal(held, state)
+
+
+def test_the_operators_together_on_packed_clips(ops):
+    parts = block_of(64, 3)
+    bounds = [0, 7, 7, 30, 31]
+    cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+    x = torch.randn(31, 64, generator=gen(6), device="cuda")
+    h0 = torch.randn(4, 64, generator=gen(7), device="cuda")
+    with torch.no_grad():
+        y, last = block(ops, *parts, x, h0, cu)
+        for i, (lo, hi) in enumerate(zip(bounds, bounds[1:])):
+            if hi > lo:
+                yi, li = block(ops, *parts, x[None, lo:hi], h0[i:i + 1])
+                within(y[None, lo:hi], yi, 2000 * F32)
+                within(last[i:i + 1], li, 2000 * F32)
+            else:
+                assert torch.equal(last[i], h0[i])
+
+
+def test_two_streams_and_two_captured_graphs_share_nothing(ops):
+    """Workspaces belong to their call: two streams at once, and two graphs replayed in turn, give the bits of the calls alone."""
+    leaves = [[t.requires_grad_() for t in mlp_inputs(700, 200, 72, torch.float32, s, True)] for s in (1, 2)]
+    scans = [[t.requires_grad_() for t in scan_inputs((3000, 40), 3, torch.bfloat16, s)] for s in (1, 2)]
+    cu = torch.tensor([0, 1000, 1001, 2900], dtype=torch.int32, device="cuda")
+
+    def step(i):
+        h = ops.gated_mlp(*leaves[i])
+        s, last = ops.gru_scan(*scans[i], cu_seqlens=cu)
+        n = ops.layer_norm(leaves[i][0])
+        return [t.detach() for t in (h, s, last, n)] + list(torch.autograd.grad(h, leaves[i], torch.ones_like(h))) + \
+            list(torch.autograd.grad((s, last), scans[i], (torch.ones_like(s), torch.ones_like(last)))) + list(torch.autograd.grad(n, leaves[i][0], h.detach()[:, :1].expand_as(n)))
+    want = [[t.clone() for t in step(i)] for i in (0, 1)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for k in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i])), i
+    del got
+    graphs, held = [], []
+    for i, s in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            held.append(step(i))
+        graphs.append(g)
+    for k in range(3):
+        for t in held[0] + held[1]:
+            t.zero_()
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(held[i], want[i])), (k, i)
+        step(0)
+
+
+def test_gru_scan_bounds_behind_the_rows_end_with_them(ops):
+    z, q, h0 = scan_inputs((50, 24), 3, torch.float32, 31)
+    got = ops.gru_scan(z, q, h0, cu_seqlens=torch.tensor([0, 20, 70, 90], dtype=torch.int32, device="cuda"))
+    want = ops.gru_scan(z, q, h0, cu_seqlens=torch.tensor([0, 20, 50, 50], dtype=torch.int32, device="cuda"))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
