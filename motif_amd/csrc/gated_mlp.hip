@@ -663,18 +663,17 @@ void segments(GemmArgs& g, const Image& a, const Image& b0, const Image& b1) {
     }
 }
 
-// Tiles of 256 x 256 (C = 128) where they give every CU at least one, else of 128 x 128, of which a CU holds two.  The tiles behind the last whole round
-// of the chip are cut along the reduction so that their pieces fill it: the accumulators of a round are 64 MB, written and read again in about as long
-// as 24 units of a tile take (8192 x 2048 x 5632 bf16, weights' gradients: 352 tiles, 380 us in two rounds, 326 us with the second one cut in two).
+// The tiles behind the last whole round of the chip are cut along the reduction so that their pieces fill it: the accumulators of a round are 64 MB,
+// written and read again in about as long as 24 units of a tile take (8192 x 2048 x 5632 bf16, weights' gradients: 352 tiles, 380 us in two rounds,
+// 326 us with the second one cut in two).
 struct GemmPlan { bool big; int tiles_m, tiles_n, whole, pieces, units_per_piece; };
-GemmPlan gemm_plan(long M, long N, int halves, long units) {
+GemmPlan plan_with(bool big, long M, long N, int halves, long units) {
     GemmPlan p;
-    auto tiles_of = [&](int t) { return (long)cdiv(M, t) * cdiv(N, halves == 2 ? t / 2 : t); };
-    p.big = tiles_of(256) >= 256;
-    const int t = p.big ? 256 : 128;
-    const long tiles = tiles_of(t), slots = p.big ? 256 : 512, rest = tiles % slots;
+    p.big = big;
+    const int t = big ? 256 : 128;
     p.tiles_m = cdiv(M, t);
     p.tiles_n = cdiv(N, halves == 2 ? t / 2 : t);
+    const long tiles = (long)p.tiles_m * p.tiles_n, slots = big ? 256 : 512, rest = tiles % slots;
     long pieces = rest ? slots / rest : 1;
     if (pieces > units / 8) pieces = units / 8;
     if (pieces < 2 || units * (pieces - 1) < 24 * pieces) pieces = 1;
@@ -682,6 +681,22 @@ GemmPlan gemm_plan(long M, long N, int halves, long units) {
     p.pieces = (int)((units + p.units_per_piece - 1) / p.units_per_piece);
     p.whole = (int)(p.pieces > 1 ? tiles - rest : tiles);
     return p;
+}
+// Rounds of the chip that a plan takes, one of 512 tiles of 128 being half of one of 256 tiles of 256, and dearer for the same work: 8 %
+// in whole rounds, counted as 20 % (8192 x 2048 x 5632: 6 rounds of 256 take 374 us, 11 of 128 436 us).
+double rounds_of(const GemmPlan& p, long units) {
+    const long tiles = (long)p.tiles_m * p.tiles_n, slots = p.big ? 256 : 512;
+    const double r = p.pieces > 1 ? p.whole / slots + (double)p.units_per_piece / units + 24. / units : (double)cdiv(tiles, slots);
+    return p.big ? r : 0.6 * r;
+}
+// Tiles of 256 x 256 (C = 128) where they give every CU at least one and no fewer of 128 x 128, of which a CU holds two, end sooner (2048 x 2048 x
+// 5632 bf16: two rounds of 256, 97 us, or three of 128, 88 us; 8192 x 1024 x 4096: 131 or 140 us).  `keep`: under a reduction of up to 6 units the
+// epilogue, which then writes the projections too, is most of the time, and two tiles on a CU, the one in its products while the other writes, hide
+// it (57600 x 64 x 256 fp32: 91 us with tiles of 256, 82 us with 128; 16384 x 128 x 2048 bf16: 94 or 83 us; 8192 x 512 x 4096: 153 or 152 us).
+GemmPlan gemm_plan(long M, long N, int halves, long units, bool keep) {
+    const GemmPlan big = plan_with(true, M, N, halves, units), small = plan_with(false, M, N, halves, units);
+    const bool few = (long)big.tiles_m * big.tiles_n < 256;
+    return few || (keep && units <= 6) || rounds_of(small, units) < rounds_of(big, units) ? small : big;
 }
 long part_bytes(const GemmPlan& p) {
     const long cut = (long)p.tiles_m * p.tiles_n - p.whole;
@@ -746,7 +761,7 @@ int grad_rows(long M, long F) {
     while (rows > 8 && (long)cdiv(M, rows) * cdiv(F, 256) < 1024) rows /= 2;
     return rows;
 }
-GemmPlan fwd_plan(long M, long K, long F, int dtype) { return gemm_plan(M, F, 2, (long)(planes(dtype) == 3 ? 6 : 1) * units_of(K)); }
+GemmPlan fwd_plan(long M, long K, long F, int dtype, bool keep) { return gemm_plan(M, F, 2, (long)(planes(dtype) == 3 ? 6 : 1) * units_of(K), keep); }
 
 struct Backward { Inputs in; Image dg, du; float* bias_part; f32x4* part; GemmPlan dx, dw; };
 Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype, bool need_x, bool need_w, bool need_b) {
@@ -756,8 +771,8 @@ Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const vo
     char* p = (char*)ws.take(2L * 2 * n * M * ld);
     b.dg = {p, M * ld, ld, n};
     b.du = {p ? p + 2L * n * M * ld : nullptr, M * ld, ld, n};
-    if (need_x) b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * units_of(ld));
-    if (need_w) b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * units_of(M));
+    if (need_x) b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * units_of(ld), false);
+    if (need_w) b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * units_of(M), false);
     if (need_b) b.bias_part = (float*)ws.take(4L * cdiv(M, grad_rows(M, F)) * 2 * F);
     long part = need_x ? part_bytes(b.dx) : 0;           // the two products run one behind the other: one piece of memory serves both
     if (need_w && part_bytes(b.dw) > part) part = part_bytes(b.dw);
@@ -772,7 +787,8 @@ extern "C" long motif_gated_mlp_ws_bytes(const void* x, long x_rs, const void* w
     if (M <= kFewRows) return 0;
     Arena ws = {nullptr, 0};
     inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
-    ws.take(part_bytes(fwd_plan(M, K, F, dtype)));
+    const long p0 = part_bytes(fwd_plan(M, K, F, dtype, false)), p1 = part_bytes(fwd_plan(M, K, F, dtype, true));
+    ws.take(p0 > p1 ? p0 : p1);
     return ws.used;
 }
 
@@ -795,7 +811,7 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
     }
     Arena ws = {(char*)workspace, 0};
     const Inputs f = inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
-    const GemmPlan plan = fwd_plan(M, K, F, dtype);
+    const GemmPlan plan = fwd_plan(M, K, F, dtype, G != nullptr);
     f32x4* part = (f32x4*)ws.take(part_bytes(plan));
     if (ws.used && !workspace) return MOTIF_EINVAL;
     lay_out(f, true, true, x, x_rs, w_gate, w_up, M, K, F, dtype, s);
