@@ -172,12 +172,12 @@ def test_layer_norm_gives_the_same_bits_every_time_on_any_stream_and_in_a_graph(
 
     def step():
         y = ops.layer_norm(*leaves)
-        return (y,) + torch.autograd.grad(y, leaves, dy)
-    want = [t.detach().clone() for t in step()]
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+    want = [t.clone() for t in step()]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        other = [t.detach().clone() for t in step()]           # (no eager graph of these leaves lives into the capture)
+        other = step()                                   # (y is detached: no eager graph of these leaves lives into the capture)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(other, want))
     graph = torch.cuda.CUDAGraph()
@@ -185,7 +185,7 @@ def test_layer_norm_gives_the_same_bits_every_time_on_any_stream_and_in_a_graph(
         held = step()
     for k in range(3):
         for t in held:
-            t.detach().zero_()
+            t.zero_()
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want)), k
