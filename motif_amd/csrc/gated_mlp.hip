@@ -22,6 +22,8 @@ namespace {
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kSegs = 12;                                // dx in fp32: two pairs of operands, six products each
@@ -625,8 +627,227 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
     }
 }
 
+// ---- narrow layers -----------------------------------------------------------------------------------------------------------------------
+// K <= 64: a wave holds the weights of 32 columns of both projections in its registers and walks over blocks of 16 rows; neither a tile of the output nor
+// fp32's three parts pass through memory.  Four values of the reduction to a lane: one matrix instruction of 16 bits, four of fp32 (each takes one
+// value of every lane; which of the reduction's values those are is free as long as both operands agree).
+template <typename T>
+__device__ __forceinline__ f32x4 mfma4(const SeqRaw<T, 4>& a, const SeqRaw<T, 4>& b, f32x4 c) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    } else if constexpr (std::is_same_v<T, bf16_t>)
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ SeqRaw<T, 4> four(float a, float b, float c, float d) { return {{(T)a, (T)b, (T)c, (T)d}}; }
+
+// Forward, K a multiple of 4 and at most 16 KQ, F one of 8.  The weights are the instruction's rows, in the order that gives a lane eight neighbouring
+// columns of one row of the output; a run that would pass the last column is the last eight ones again, a row behind the last one the last, written
+// alike.
+template <typename T, int KQ>
+__global__ __launch_bounds__(256) void narrow_fwd_kernel(const T* __restrict__ x, long xs, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ bg, const T* __restrict__ bu,
+                                                         T* __restrict__ h, float* __restrict__ G, float* __restrict__ U, int M, int K, int F, int act, int walkers) {
+    const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
+    const int id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), runs = (F + 31) / 32, f0 = id % runs * 32, walker = id / runs;
+    if (walker >= walkers) return;
+    SeqRaw<T, 4> w[2][2][KQ];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < KQ; ++j) {
+            const int k = 16 * j + 4 * hi;
+            const long at = (long)(min(f0 + 8 * (lo >> 2), F - 8) + 4 * t + (lo & 3)) * K + min(k, K - 4);
+            w[0][t][j] = k < K ? seq_raw<T, 4>(wg + at) : four<T>(0.f, 0.f, 0.f, 0.f);
+            w[1][t][j] = k < K ? seq_raw<T, 4>(wu + at) : four<T>(0.f, 0.f, 0.f, 0.f);
+        }
+    const int c = min(f0 + 8 * hi, F - 8);
+    float b[2][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { b[0][e] = bg ? (float)bg[c + e] : 0.f; b[1][e] = bu ? (float)bu[c + e] : 0.f; }
+    SeqRaw<T, 4> next[KQ];
+    auto request = [&](int block) __attribute__((always_inline)) {
+        const T* at = x + (long)min(block * 16 + lo, M - 1) * xs;
+#pragma unroll
+        for (int j = 0; j < KQ; ++j) next[j] = seq_raw<T, 4>(at + min(16 * j + 4 * hi, K - 4));
+    };
+    const int blocks = (M + 15) / 16;
+    request(walker);
+    for (int block = walker; block < blocks; block += walkers) {
+        f32x4 a[2][2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) a[p][t] = f32x4{b[p][4 * t], b[p][4 * t + 1], b[p][4 * t + 2], b[p][4 * t + 3]};
+#pragma unroll
+        for (int j = 0; j < KQ; ++j) {
+            SeqRaw<T, 4> v = next[j];
+            if (16 * j + 4 * hi >= K) v = four<T>(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) a[p][t] = mfma4<T>(w[p][t][j], v, a[p][t]);
+        }
+        request(min(block + walkers, blocks - 1));
+        const long at = (long)min(block * 16 + lo, M - 1) * F + c;
+        float g[8], u[8], o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            g[e] = a[0][e >> 2][e & 3];
+            u[e] = a[1][e >> 2][e & 3];
+            o[e] = gate<sizeof(T) == 2>(g[e], act) * u[e];
+        }
+        seq_store<T, 8>(h + at, o);
+        if (G) { seq_store<float, 8>(G + at, g); seq_store<float, 8>(U + at, u); }
+    }
+}
+
+// Backward in one pass over dh, G and U: F a multiple of 8 up to 256, K one of 4 up to 16 KT.  A workgroup's eight waves take NC runs of 32 columns of 8 / NC
+// blocks of 16 rows.  A wave makes dG and dU of its rows and columns, with a row to a lane as dx needs them, and turns them over through LDS for the weights'
+// gradients, whose sums stay in its registers over all of its rows; the runs' shares of dx meet in LDS, in a fixed order.
+template <typename T, int KT, bool DX, bool DW>
+__global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x, long xs, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ dh, long dhs,
+                                                         const float* __restrict__ G, const float* __restrict__ U, T* __restrict__ dx, float* __restrict__ dw_part,
+                                                         float* __restrict__ db_part, int M, int K, int F, int act, int nc) {
+    __shared__ __attribute__((aligned(16))) float turn[8][2][32][20];              // [column][row]; 16-byte rows, writes of a wave on all banks
+    __shared__ __attribute__((aligned(16))) float shares[DX ? 2 : 1][8][DX ? KT * 4 : 1][68];
+    const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nr = 8 / nc, sub = wave / nc, f0 = wave % nc * 32, c = min(f0 + 8 * hi, F - 8);
+    const bool mine = f0 + 8 * hi < F;
+    SeqRaw<T, 4> w[DX ? 2 : 1][DX ? KT : 1][2];          // row k, four of the lane's eight columns
+    if constexpr (DX) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const long at = (long)(c + 4 * t + e) * K + min(16 * kt + lo, K - 1);
+                    w[0][kt][t].v[e] = mine ? wg[at] : (T)0.f;
+                    w[1][kt][t].v[e] = mine ? wu[at] : (T)0.f;
+                }
+    }
+    f32x4 dw[2][2][KT];
+    float db[2][2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            db[p][t] = 0.f;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) dw[p][t][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    SeqRaw<T, 8> nd;
+    SeqRaw<float, 8> ng, nu;
+    auto request = [&](int r0) __attribute__((always_inline)) {
+        const long r = min(r0 + lo, M - 1), at = r * F + c;
+        nd = seq_raw<T, 8>(dh + r * dhs + c);
+        ng = seq_raw<float, 8>(G + at);
+        nu = seq_raw<float, 8>(U + at);
+    };
+    const int step = (int)gridDim.x * nr * 16;
+    int buf = 0;
+    request((blockIdx.x * nr + sub) * 16);
+    for (int base = blockIdx.x * nr * 16; base < M; base += step) {
+        const int r0 = base + sub * 16;
+        SeqRaw<T, 4> xv[KT];                             // rows 4 hi .. + 3 of column lo
+        if constexpr (DW)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const T* at = x + (long)min(r0 + 4 * hi + e, M - 1) * xs;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) xv[kt].v[e] = at[min(16 * kt + lo, K - 1)];
+            }
+        const bool row = mine && r0 + lo < M;
+        float g[8], u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float v, d;
+            gate_grad<sizeof(T) == 2>(ng[e], act, v, d);
+            g[e] = row ? nd[e] * nu[e] * d : 0.f;
+            u[e] = row ? nd[e] * v : 0.f;
+            turn[wave][0][8 * hi + e][lo] = g[e];
+            turn[wave][1][8 * hi + e][lo] = u[e];
+        }
+        request(min(r0 + step, M - 1));
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();                 // (a wave's own part of `turn`; the LDS takes a wave's accesses in order)
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if constexpr (DX) {
+            SeqRaw<T, 4> og[2], ou[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                og[t] = four<T>(g[4 * t], g[4 * t + 1], g[4 * t + 2], g[4 * t + 3]);
+                ou[t] = four<T>(u[4 * t], u[4 * t + 1], u[4 * t + 2], u[4 * t + 3]);
+            }
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < 2; ++t) { a = mfma4<T>(w[0][kt][t], og[t], a); a = mfma4<T>(w[1][kt][t], ou[t], a); }
+                *(f32x4*)&shares[buf][wave][kt * 4 + hi][lo * 4] = a;
+            }
+        }
+        if constexpr (DW)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) xv[kt].v[e] = r0 + 4 * hi + e < M ? xv[kt].v[e] : (T)0.f;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const f32x4 v = *(const f32x4*)&turn[wave][p][16 * t + lo][4 * hi];
+                db[p][t] += (v[0] + v[1]) + (v[2] + v[3]);
+                const SeqRaw<T, 4> o = four<T>(v[0], v[1], v[2], v[3]);
+                if constexpr (DW)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) dw[p][t][kt] = mfma4<T>(o, xv[kt], dw[p][t][kt]);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if constexpr (DX) {
+            __syncthreads();                             // the other buffer's sums were taken before this
+            const int pairs = nr * 16 * KT * 8;
+            for (int i = 0; i < pairs; i += 512) {       // two values each; rows and columns behind the last: those again
+                const int q = min(i + (int)threadIdx.x, pairs - 1), m = min(q / (KT * 8), M - 1 - base), k = min(q % (KT * 8) * 2, K - 2);
+                float s[2] = {0.f, 0.f};
+                for (int n = 0; n < nc; ++n) {
+                    const float* at = &shares[buf][(m >> 4) * nc + n][k >> 2][(m & 15) * 4 + (k & 3)];
+                    s[0] += at[0];
+                    s[1] += at[1];
+                }
+                seq_store<T, 2>(dx + (long)(base + m) * K + k, s);
+            }
+            buf ^= 1;
+        }
+    }
+    const long slot = (long)blockIdx.x * nr + sub;
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float s = db[p][t];
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            const int f = f0 + 16 * t;
+            if (db_part && hi == 0 && f + lo < F) db_part[(slot * 2 + p) * F + f + lo] = s;
+            if constexpr (DW)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+                        if (f + 4 * hi + e < F && 16 * kt + lo < K) dw_part[((slot * 2 + p) * F + f + 4 * hi + e) * K + 16 * kt + lo] = dw[p][t][kt][e];
+        }
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 64;
+constexpr int kNarrowWaves = 8;                          // waves of narrow_fwd_kernel to a CU
 constexpr long kMostRows = 1L << 22;                    // offsets within a tile are 32 bits: 256 rows x this x 2 bytes
 int up8(long n) { return (int)((n + 7) & ~7L); }
 int units_of(long n) { return (int)((n + 63) / 64); }
@@ -735,6 +956,30 @@ void few_rows(const void* x, long xs, const void* wg, const void* wu, const void
     rows_kernel<T, MT><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
 }
 
+bool narrow(long K, long F) { return K <= 64 && K % 4 == 0 && F % 8 == 0; }
+bool narrow_bwd(long K, long F) { return narrow(K, F) && F <= 256; }
+int column_runs(long F) { return F > 128 ? 8 : F > 64 ? 4 : F > 32 ? 2 : 1; }       // of 32 columns, of a workgroup's eight waves
+int narrow_groups(long M, long F) {                      // one per CU; two blocks of rows each, so that the second is read while the first is computed
+    const long n = cdiv(M, 2 * 16 * (8 / column_runs(F)));
+    return (int)(n < 256 ? n : 256);
+}
+template <typename T>
+void narrow_fwd(const void* x, long xs, const void* wg, const void* wu, const void* bg, const void* bu, void* h, float* G, float* U, int M, int K, int F, int act, hipStream_t s) {
+    const int runs = (F + 31) / 32, blocks = (M + 15) / 16;
+    int walkers = 256 * kNarrowWaves / runs;
+    walkers = walkers < 1 ? 1 : walkers > blocks ? blocks : walkers;
+    const unsigned grid = (unsigned)(((long)runs * walkers + 3) / 4);
+    auto* kernel = K <= 32 ? narrow_fwd_kernel<T, 2> : narrow_fwd_kernel<T, 4>;
+    kernel<<<grid, 256, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, M, K, F, act, walkers);
+}
+template <typename T, int KT>
+void narrow_bwd(int grid, const void* x, long xs, const void* wg, const void* wu, const void* dh, long dhs, const float* G, const float* U, void* dx, float* dw_part, float* db_part,
+                int M, int K, int F, int act, hipStream_t s) {
+    auto* kernel = dx && dw_part ? narrow_bwd_kernel<T, KT, true, true> : dx ? narrow_bwd_kernel<T, KT, true, false>
+                 : dw_part ? narrow_bwd_kernel<T, KT, false, true> : narrow_bwd_kernel<T, KT, false, false>;
+    kernel<<<grid, 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)dh, dhs, G, U, (T*)dx, dw_part, db_part, M, K, F, act, column_runs(F));
+}
+
 // x, Wg and Wu as the products read them: as they lie, or laid out in the workspace.
 struct Inputs { Image x, wg, wu; bool lay_x, lay_w; };
 Inputs inputs_of(Arena& ws, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype) {
@@ -763,10 +1008,17 @@ int grad_rows(long M, long F) {
 }
 GemmPlan fwd_plan(long M, long K, long F, int dtype, bool keep) { return gemm_plan(M, F, 2, (long)(planes(dtype) == 3 ? 6 : 1) * units_of(K), keep); }
 
-struct Backward { Inputs in; Image dg, du; float* bias_part; f32x4* part; GemmPlan dx, dw; };
+struct Backward { Inputs in; Image dg, du; float* bias_part; f32x4* part; GemmPlan dx, dw; float* dw_part; bool one_pass; };
 Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype, bool need_x, bool need_w, bool need_b) {
     Backward b = {};
     const int n = planes(dtype), ld = up8(F);
+    if (narrow_bwd(K, F)) {
+        b.one_pass = true;
+        const long slots = (long)narrow_groups(M, F) * (8 / column_runs(F));
+        if (need_w) b.dw_part = (float*)ws.take(4 * slots * 2 * F * K);
+        if (need_b) b.bias_part = (float*)ws.take(4 * slots * 2 * F);
+        return b;
+    }
     b.in = inputs_of(ws, x, xs, wg, wu, M, K, F, dtype);
     char* p = (char*)ws.take(2L * 2 * n * M * ld);
     b.dg = {p, M * ld, ld, n};
@@ -784,7 +1036,7 @@ Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const vo
 extern "C" long motif_gated_mlp_ws_bytes(const void* x, long x_rs, const void* w_gate, const void* w_up, long M, long K, long F, int dtype) {
     const int rc = check_mlp(M, K, F, MOTIF_GATE_SILU, dtype);
     if (rc) return rc;
-    if (M <= kFewRows) return 0;
+    if (M <= kFewRows || narrow(K, F)) return 0;
     Arena ws = {nullptr, 0};
     inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
     const long p0 = part_bytes(fwd_plan(M, K, F, dtype, false)), p1 = part_bytes(fwd_plan(M, K, F, dtype, true));
@@ -806,6 +1058,11 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
             else if (M <= 32) few_rows<T, 2>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
             else few_rows<T, 4>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
         });
+        MOTIF_LAUNCH_CHECK();
+        return MOTIF_OK;
+    }
+    if (narrow(K, F)) {
+        seq_dispatch(dtype, [&](auto* t) { narrow_fwd<std::remove_pointer_t<decltype(t)>>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s); });
         MOTIF_LAUNCH_CHECK();
         return MOTIF_OK;
     }
@@ -844,11 +1101,23 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
     if (rc) return rc;
     const bool need_x = dx, need_w = dw_gate || dw_up, need_b = db_gate || db_up;
     if (need_w && (!dw_gate || !dw_up)) return MOTIF_EINVAL;
-    if (M < 1 || !x || !w_gate || !w_up || !G || !U || !dh || !workspace || x_rs < 0 || dh_rs < 0 || !(need_x || need_w || need_b)) return MOTIF_EINVAL;
+    if (M < 1 || !x || !w_gate || !w_up || !G || !U || !dh || x_rs < 0 || dh_rs < 0 || !(need_x || need_w || need_b)) return MOTIF_EINVAL;
     if (!seq_aligned(G, 16) || !seq_aligned(U, 16)) return MOTIF_EINVAL;
     hipStream_t s = (hipStream_t)stream;
     Arena ws = {(char*)workspace, 0};
     const Backward b = backward_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype, need_x, need_w, need_b);
+    if (ws.used && !workspace) return MOTIF_EINVAL;
+    if (b.one_pass) {
+        const int grid = narrow_groups(M, F), slots = grid * (8 / column_runs(F));
+        seq_dispatch(dtype, [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            if (K <= 32) narrow_bwd<T, 2>(grid, x, x_rs, w_gate, w_up, dh, dh_rs, G, U, dx, b.dw_part, b.bias_part, (int)M, (int)K, (int)F, act, s);
+            else narrow_bwd<T, 4>(grid, x, x_rs, w_gate, w_up, dh, dh_rs, G, U, dx, b.dw_part, b.bias_part, (int)M, (int)K, (int)F, act, s);
+        });
+        MOTIF_LAUNCH_CHECK();
+        const int r = need_w ? seq_colsum2(b.dw_part, slots, F * K, dw_gate, dw_up, dtype, s) : MOTIF_OK;
+        return r || !need_b ? r : seq_colsum2(b.bias_part, slots, F, db_gate, db_up, dtype, s);
+    }
     lay_out(b.in, need_w, need_x, x, x_rs, w_gate, w_up, M, K, F, dtype, s);
     seq_dispatch(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;

@@ -493,6 +493,52 @@ def test_gated_mlp_and_its_gradients(ops, dtype, M, K, F, act, bias):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M, K, F, act, bias", [(65, 4, 8, "silu", True), (1, 8, 16, "gelu", True), (66, 16, 24, "sigmoid", False), (100, 20, 40, "gelu", True),
+                                                (1000, 32, 64, "silu", True), (333, 36, 72, "silu", False), (1001, 60, 136, "gelu", True), (9001, 64, 248, "sigmoid", True),
+                                                (9000, 64, 256, "gelu", False), (700, 64, 264, "silu", True), (5003, 28, 96, "silu", True), (130, 64, 2064, "gelu", True)])
+def test_gated_mlp_of_narrow_layers(ops, dtype, M, K, F, act, bias):
+    """K up to 64: weights in registers, the backward pass in one; columns of less than a wave's 32, rows that end within a workgroup's share."""
+    mlp_check(ops, *mlp_inputs(M, K, F, dtype, M + K + F, bias), act)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["columns", "odd columns", "broadcast rows", "transposed", "one bias"])
+def test_gated_mlp_of_narrow_layers_takes_strided_inputs(ops, dtype, kind):
+    x, wg, wu, bg, bu = mlp_inputs(300, 48, 72, dtype, 3, True)
+    base = torch.randn(300, 160, generator=gen(4), device="cuda").to(dtype)
+    if kind == "columns":
+        x = base[:, 32:80]
+    elif kind == "odd columns":
+        x = base[:, 3:51]
+    elif kind == "broadcast rows":
+        x = base[:1, :48].expand(300, 48)
+    elif kind == "transposed":
+        x = torch.randn(48, 300, generator=gen(5), device="cuda").to(dtype).t()
+    else:
+        bu = None
+    mlp_check(ops, x, wg, wu, bg, bu, "gelu")
+
+
+def test_gated_mlp_of_narrow_layers_keeps_bad_rows_to_themselves(ops):
+    for dtype in DTYPES:
+        x, wg, wu, bg, bu = mlp_inputs(300, 36, 72, dtype, 6, True)
+        dh = torch.randn(300, 72, generator=gen(7), device="cuda").to(dtype)
+
+        def step(x, dh):
+            x = x.detach().requires_grad_()
+            h = ops.gated_mlp(x, wg.detach().requires_grad_(), wu, bg, bu)
+            return h.detach(), torch.autograd.grad(h, x, dh, retain_graph=True)[0]
+        want = step(x, dh)
+        bad, bad_dh = x.clone(), dh.clone()
+        bad[3, 7], bad[299, 35], bad_dh[17, 70] = math.inf, math.nan, math.nan
+        got = step(bad, bad_dh)
+        rest = [i for i in range(300) if i not in (3, 299, 17)]
+        assert all(torch.equal(a[rest], b[rest]) for a, b in zip(got, want))
+        assert not torch.isfinite(got[0][3]).all() and torch.isnan(got[0][299]).all() and torch.isnan(got[1][17]).all()
+        assert torch.equal(got[0][17], want[0][17])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_gated_mlp_in_large_tiles(ops, dtype):
     """Enough rows and columns for the 256 x 256 tiles in all three products, with edges in both axes."""
     mlp_check(ops, *mlp_inputs(4229, 4130, 2060, dtype, 1, True), "silu")
