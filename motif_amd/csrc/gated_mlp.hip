@@ -28,27 +28,71 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kSegs = 12;                                // dx in fp32: two pairs of operands, six products each
 
-// ---- activations.  FAST: v_exp_f32 and v_rcp_f32 as they are (relative error about 2^-21 at |g| = 8, behind a rounding to 8 or 11 bits) -------
+// ---- activations.  FAST: v_exp_f32 and v_rcp_f32 as they are (relative error about 2^-21 at |g| = 8, behind a rounding to 8 or 11 bits); else
+// expf and a reciprocal with a Newton step, one division's worth of accuracy at a third of its instructions ---------------------------------------
 template <bool FAST>
-__device__ __forceinline__ float sigm(float g) { return FAST ? __builtin_amdgcn_rcpf(1.f + __expf(-g)) : 1.f / (1.f + expf(-g)); }
-template <bool FAST>
-__device__ __forceinline__ float gate(float g, int act) {
-    if (act == MOTIF_GATE_SIGMOID) return sigm<FAST>(g);
-    if (act == MOTIF_GATE_SILU) return g * sigm<FAST>(g);
-    return 0.5f * g * (1.f + erff(g * 0.70710678f));
+__device__ __forceinline__ float reciprocal(float d) {  // finite d
+    const float t = __builtin_amdgcn_rcpf(d);
+    return FAST ? t : fmaf(t, fmaf(-d, t, 1.f), t);
 }
-// act(g) and its derivative
 template <bool FAST>
-__device__ __forceinline__ void gate_grad(float g, int act, float& v, float& d) {
+__device__ __forceinline__ float sigm(float g) {
+    const float e = FAST ? __expf(-g) : expf(-g);
+    return reciprocal<FAST>(1.f + (!FAST && e > 1e38f ? 1e38f : e));
+}
+// Phi(g) = erfc(-g / sqrt 2) / 2, and E = exp(-g^2 / 2).  erfc(x) exp(x^2) is smooth and falls like 1 / x: as t P(t) with t = 1 / (1 + 0.35 |g|), P of degree 8
+// fitted to the least relative error, it is off by 3.2e-8 over |g| <= 14 (below, E is 0).  No difference of near values on the negative side, and E serves
+// the derivative.
+template <bool FAST>
+__device__ __forceinline__ float normal_cdf(float g, float& E) {
+    const float t = reciprocal<FAST>(fmaf(0.35f, fminf(fabsf(g), 64.f), 1.f));
+    float p = -0.0291459057f;
+    p = fmaf(p, t, 0.143971592f);
+    p = fmaf(p, t, -0.255714029f);
+    p = fmaf(p, t, 0.159173936f);
+    p = fmaf(p, t, -0.0231096949f);
+    p = fmaf(p, t, 0.105507948f);
+    p = fmaf(p, t, 0.119832881f);
+    p = fmaf(p, t, 0.139861867f);
+    p = fmaf(p, t, 0.139621407f);
+    E = __expf(-0.5f * g * g);                           // (its error grows with g^2 as E falls: below 2^-26 of 1 everywhere)
+    const float q = E * (p * t);
+    return g < 0.f ? q : 1.f - q;
+}
+// v = act(g) and d = act'(g) of N values.  One branch for all of them: the values' chains of instructions then overlap.
+template <bool FAST, int N>
+__device__ __forceinline__ void gates(const float (&g)[N], int act, float (&v)[N]) {
     if (act == MOTIF_GATE_GELU) {
-        const float phi = 0.5f * (1.f + erff(g * 0.70710678f));
-        v = g * phi;
-        d = fmaf(g * 0.39894228f, FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g), phi);
-        return;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            float E;
+            v[e] = g[e] * normal_cdf<FAST>(g[e], E);
+        }
+    } else {
+        const bool silu = act == MOTIF_GATE_SILU;        // g s, or s
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = (silu ? g[e] : 1.f) * sigm<FAST>(g[e]);
     }
-    const float s = sigm<FAST>(g);
-    if (act == MOTIF_GATE_SIGMOID) { v = s; d = s * (1.f - s); }
-    else { v = g * s; d = s * fmaf(g, 1.f - s, 1.f); }
+}
+template <bool FAST, int N>
+__device__ __forceinline__ void gate_grads(const float (&g)[N], int act, float (&v)[N], float (&d)[N]) {
+    if (act == MOTIF_GATE_GELU) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            float E;
+            const float phi = normal_cdf<FAST>(g[e], E);
+            v[e] = g[e] * phi;
+            d[e] = fmaf(g[e] * 0.39894228f, E, phi);
+        }
+    } else {
+        const bool silu = act == MOTIF_GATE_SILU;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float s = sigm<FAST>(g[e]), m = silu ? g[e] : 1.f;
+            v[e] = m * s;
+            d[e] = s * fmaf(m, 1.f - s, silu ? 1.f : 0.f);
+        }
+    }
 }
 
 // ---- the matrix product ------------------------------------------------------------------------------------------------------------------
@@ -148,18 +192,6 @@ struct Operand {
     }
 };
 
-template <bool FAST, int ACT>
-__device__ __forceinline__ void gate4_as(const float (&g)[4], const float (&u)[4], float (&v)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = gate<FAST>(g[e], ACT) * u[e];
-}
-template <bool FAST>
-__device__ __forceinline__ void gate4(const float (&g)[4], const float (&u)[4], float (&v)[4], int act) {
-    if (act == MOTIF_GATE_SILU) gate4_as<FAST, MOTIF_GATE_SILU>(g, u, v);
-    else if (act == MOTIF_GATE_GELU) gate4_as<FAST, MOTIF_GATE_GELU>(g, u, v);
-    else gate4_as<FAST, MOTIF_GATE_SIGMOID>(g, u, v);
-}
-
 // Where a tile lies.  Workgroups are dealt to the eight XCDs in turn: each XCD takes a contiguous run of tiles, column by column within bands of 8 tile
 // rows, so that the tiles in flight on one XCD share their rows of both operands in its L2.
 template <int C, GemmMode MODE>
@@ -206,7 +238,9 @@ struct Store {
             float g[4], u[4], v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) { g[e] = o0[e] + bias[0][j][e]; u[e] = o1[e] + bias[1][j][e]; }
-            if (p.dtype == MOTIF_F32) gate4<false>(g, u, v, p.act); else gate4<true>(g, u, v, p.act);
+            if (p.dtype == MOTIF_F32) gates<false>(g, p.act, v); else gates<true>(g, p.act, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= u[e];
             store_as<4>(p.c0, (long)row * p.N + n, v, cnt, p.vec, p.dtype);
             if (p.g) {                                   // (their rows are padded to whole runs)
                 seq_store<float, 4>(p.g + row * p.ldg + n, g);
@@ -508,11 +542,13 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
             }
         }
 #pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = now.g[e];
+        float v[8], dv[8];
+        gate_grads<sizeof(T) == 2>(g, act, v, dv);
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float v, dv;
-            gate_grad<sizeof(T) == 2>(now.g[e], act, v, dv);
-            g[e] = c + e < F ? d[e] * now.u[e] * dv : 0.f;
-            u[e] = c + e < F ? d[e] * v : 0.f;
+            g[e] = c + e < F ? d[e] * now.u[e] * dv[e] : 0.f;
+            u[e] = c + e < F ? d[e] * v[e] : 0.f;
             sg[e] += counts ? g[e] : 0.f;
             su[e] += counts ? u[e] : 0.f;
         }
@@ -622,7 +658,9 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
         for (int w = 0; w < NW; ++w) { g += sh[w][0][m][i & 15]; u += sh[w][1][m][i & 15]; }
         if (bg) g += (float)bg[f];
         if (bu) u += (float)bu[f];
-        h[(long)m * F + f] = (T)(gate<sizeof(T) == 2>(g, act) * u);
+        float v[1];
+        gates<sizeof(T) == 2, 1>({g}, act, v);
+        h[(long)m * F + f] = (T)(v[0] * u);
         if (G) { G[m * ldg + f] = g; U[m * ldg + f] = u; }
     }
 }
@@ -631,13 +669,17 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
 // K <= 64: a wave holds the weights of 32 columns of both projections in its registers and walks over blocks of 16 rows; neither a tile of the output nor
 // fp32's three parts pass through memory.  Four values of the reduction to a lane: one matrix instruction of 16 bits, four of fp32 (each takes one
 // value of every lane; which of the reduction's values those are is free as long as both operands agree).
+// 57600 x 64 -> 2 x 256 fp32, gelu, training: forward 59 us (205 MB; the products of 64 x 512 fp32 alone 24 us, 103 us through the tiles and their three
+// parts), backward 100 + 11 us for the workgroups' sums (229 MB; products 48 us; 250 us through the tiles).  Of a SIMD's cycles in them the products
+// take 53 %, the activations and operands 25 %, waits the rest; making the next block's gradients between the products, starting a SIMD's two waves half a
+// block apart and serving one of them first each left the time as it was, so that the instructions of both kinds seem to share what they need.
+// The e-th of them; consecutive instructions should have accumulators of their own: one that adds to its predecessor's waits for it.
+template <typename T> constexpr int kFours = sizeof(T) == 4 ? 4 : 1;
 template <typename T>
-__device__ __forceinline__ f32x4 mfma4(const SeqRaw<T, 4>& a, const SeqRaw<T, 4>& b, f32x4 c) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
-        return c;
-    } else if constexpr (std::is_same_v<T, bf16_t>)
+__device__ __forceinline__ f32x4 mfma4(const SeqRaw<T, 4>& a, const SeqRaw<T, 4>& b, f32x4 c, int e) {
+    if constexpr (sizeof(T) == 4)
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    else if constexpr (std::is_same_v<T, bf16_t>)
         return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
@@ -648,7 +690,7 @@ __device__ __forceinline__ SeqRaw<T, 4> four(float a, float b, float c, float d)
 // Forward, K a multiple of 4 and at most 16 KQ, F one of 8.  The weights are the instruction's rows, in the order that gives a lane eight neighbouring
 // columns of one row of the output; a run that would pass the last column is the last eight ones again, a row behind the last one the last, written
 // alike.
-template <typename T, int KQ>
+template <typename T, int KQ, bool KEEP>
 __global__ __launch_bounds__(256) void narrow_fwd_kernel(const T* __restrict__ x, long xs, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ bg, const T* __restrict__ bu,
                                                          T* __restrict__ h, float* __restrict__ G, float* __restrict__ U, int M, int K, int F, int act, int walkers) {
     const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
@@ -687,9 +729,11 @@ __global__ __launch_bounds__(256) void narrow_fwd_kernel(const T* __restrict__ x
             SeqRaw<T, 4> v = next[j];
             if (16 * j + 4 * hi >= K) v = four<T>(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
+            for (int e = 0; e < kFours<T>; ++e)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) a[p][t] = mfma4<T>(w[p][t][j], v, a[p][t]);
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) a[p][t] = mfma4<T>(w[p][t][j], v, a[p][t], e);
         }
         request(min(block + walkers, blocks - 1));
         const long at = (long)min(block * 16 + lo, M - 1) * F + c;
@@ -698,10 +742,12 @@ __global__ __launch_bounds__(256) void narrow_fwd_kernel(const T* __restrict__ x
         for (int e = 0; e < 8; ++e) {
             g[e] = a[0][e >> 2][e & 3];
             u[e] = a[1][e >> 2][e & 3];
-            o[e] = gate<sizeof(T) == 2>(g[e], act) * u[e];
         }
+        gates<sizeof(T) == 2>(g, act, o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] *= u[e];
         seq_store<T, 8>(h + at, o);
-        if (G) { seq_store<float, 8>(G + at, g); seq_store<float, 8>(U + at, u); }
+        if (KEEP) { seq_store<float, 8>(G + at, g); seq_store<float, 8>(U + at, u); }
     }
 }
 
@@ -761,14 +807,15 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) xv[kt].v[e] = at[min(16 * kt + lo, K - 1)];
             }
-        const bool row = mine && r0 + lo < M;
-        float g[8], u[8];
+        const unsigned keep = mine && r0 + lo < M ? ~0u : 0u;      // (as bits: a choice between values would become a branch around their making)
+        float g[8], u[8], v[8], d[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = ng[e];
+        gate_grads<sizeof(T) == 2>(g, act, v, d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float v, d;
-            gate_grad<sizeof(T) == 2>(ng[e], act, v, d);
-            g[e] = row ? nd[e] * nu[e] * d : 0.f;
-            u[e] = row ? nd[e] * v : 0.f;
+            g[e] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, nd[e] * nu[e] * d[e]) & keep);
+            u[e] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, nd[e] * v[e]) & keep);
             turn[wave][0][8 * hi + e][lo] = g[e];
             turn[wave][1][8 * hi + e][lo] = u[e];
         }
@@ -783,13 +830,17 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
                 og[t] = four<T>(g[4 * t], g[4 * t + 1], g[4 * t + 2], g[4 * t + 3]);
                 ou[t] = four<T>(u[4 * t], u[4 * t + 1], u[4 * t + 2], u[4 * t + 3]);
             }
+            f32x4 a[KT];
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            for (int kt = 0; kt < KT; ++kt) a[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int t = 0; t < 2; ++t) { a = mfma4<T>(w[0][kt][t], og[t], a); a = mfma4<T>(w[1][kt][t], ou[t], a); }
-                *(f32x4*)&shares[buf][wave][kt * 4 + hi][lo * 4] = a;
-            }
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 2 * kFours<T>; ++e)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) a[kt] = mfma4<T>(w[e & 1][kt][t], e & 1 ? ou[t] : og[t], a[kt], e >> 1);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) *(f32x4*)&shares[buf][wave][kt * 4 + hi][lo * 4] = a[kt];
         }
         if constexpr (DW)
 #pragma unroll
@@ -805,7 +856,9 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
                 const SeqRaw<T, 4> o = four<T>(v[0], v[1], v[2], v[3]);
                 if constexpr (DW)
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) dw[p][t][kt] = mfma4<T>(o, xv[kt], dw[p][t][kt]);
+                    for (int e = 0; e < kFours<T>; ++e)
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) dw[p][t][kt] = mfma4<T>(o, xv[kt], dw[p][t][kt], e);
             }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -847,7 +900,9 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 64;
-constexpr int kNarrowWaves = 8;                          // waves of narrow_fwd_kernel to a CU
+// Waves of narrow_fwd_kernel to a CU: more hide more of the reads, until their writes get in each other's way (57600 x 64 -> 2 x 1024 bf16: 88 us with 8, 83 with 12;
+// with kept projections 200 and 206).
+int narrow_waves(bool keep) { return keep ? 8 : 12; }
 constexpr long kMostRows = 1L << 22;                    // offsets within a tile are 32 bits: 256 rows x this x 2 bytes
 int up8(long n) { return (int)((n + 7) & ~7L); }
 int units_of(long n) { return (int)((n + 63) / 64); }
@@ -966,10 +1021,10 @@ int narrow_groups(long M, long F) {                      // one per CU; two bloc
 template <typename T>
 void narrow_fwd(const void* x, long xs, const void* wg, const void* wu, const void* bg, const void* bu, void* h, float* G, float* U, int M, int K, int F, int act, hipStream_t s) {
     const int runs = (F + 31) / 32, blocks = (M + 15) / 16;
-    int walkers = 256 * kNarrowWaves / runs;
+    int walkers = 256 * narrow_waves(G != nullptr) / runs;
     walkers = walkers < 1 ? 1 : walkers > blocks ? blocks : walkers;
     const unsigned grid = (unsigned)(((long)runs * walkers + 3) / 4);
-    auto* kernel = K <= 32 ? narrow_fwd_kernel<T, 2> : narrow_fwd_kernel<T, 4>;
+    auto* kernel = K <= 32 ? G ? narrow_fwd_kernel<T, 2, true> : narrow_fwd_kernel<T, 2, false> : G ? narrow_fwd_kernel<T, 4, true> : narrow_fwd_kernel<T, 4, false>;
     kernel<<<grid, 256, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, M, K, F, act, walkers);
 }
 template <typename T, int KT>
