@@ -323,9 +323,16 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
 }
 
 // Packed rows: what each row is.  cu [S + 1] need not be sound for memory's sake: an owner is always one of the S sequences, and a sequence that
-// would pass the last row ends there.
-__global__ __launch_bounds__(256) void gru_scan_rows_kernel(const int* __restrict__ cu, int S, int rows, int* __restrict__ info) {
+// would pass the last row ends there.  The workgroups behind those of the rows take an empty sequence each: its state, which no row carries, is
+// out = in (or 0).
+__global__ __launch_bounds__(256) void gru_scan_rows_kernel(const int* __restrict__ cu, int S, int rows, int* __restrict__ info, int D, const float* __restrict__ in, float* __restrict__ out) {
     const long t = (long)blockIdx.x * 256 + threadIdx.x;
+    const int empty = blockIdx.x - (rows + 255) / 256;
+    if (empty >= 0) {
+        if (min(cu[empty + 1], rows) > cu[empty]) return;
+        for (long c = threadIdx.x; c < D; c += 256) out[(long)empty * D + c] = in ? in[(long)empty * D + c] : 0.f;
+        return;
+    }
     if (t >= rows) return;
     int lo = 0, hi = S + 1;                              // the first bound behind t
     while (lo < hi) {
@@ -335,12 +342,6 @@ __global__ __launch_bounds__(256) void gru_scan_rows_kernel(const int* __restric
     const int s = lo - 1;
     if (s < 0 || s >= S) { info[t] = -1; return; }
     info[t] = (s << 2) | (cu[s] == t ? kFirst : 0) | (min(cu[s + 1], rows) == t + 1 ? kLast : 0);
-}
-// ... and an empty sequence's state, which no row carries: out = in (or 0).
-__global__ __launch_bounds__(256) void gru_scan_empty_kernel(const int* __restrict__ cu, int rows, int D, const float* __restrict__ in, float* __restrict__ out) {
-    const int s = blockIdx.x;
-    if (min(cu[s + 1], rows) > cu[s]) return;
-    for (long c = threadIdx.x; c < D; c += 256) out[(long)s * D + c] = in ? in[(long)s * D + c] : 0.f;
 }
 
 struct Plan { int V, TX, TY, R, groups, segs; long seg_rows; };
@@ -404,8 +405,8 @@ int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const 
     if (cu) {
         a.cuts = (int*)(ws + agg_floats(pl, a.B, a.D));
         int* info = (int*)(ws + agg_floats(pl, a.B, a.D) + cut_floats(pl, true));
-        if (a.T > 0) gru_scan_rows_kernel<<<cdiv(a.T, 256), 256, 0, s>>>(cu, S, (int)a.T, info);
-        if (a.state) gru_scan_empty_kernel<<<S, 256, 0, s>>>(cu, (int)a.T, a.D, empty_in, a.state);
+        const unsigned grid = (unsigned)cdiv(a.T, 256) + (a.state ? S : 0);
+        if (grid) gru_scan_rows_kernel<<<grid, 256, 0, s>>>(cu, S, (int)a.T, info, a.D, empty_in, a.state);
         a.info = info;
     }
     if (a.T > 0)
