@@ -8,6 +8,8 @@
 // cancellation), and the backward pass takes dx and the parameters' sums from the same read: a workgroup walks over rows with its lanes'
 // columns fixed, keeps the sums of its columns in registers (fp32) and writes them once; seq_colsum2 adds the workgroups' sums in a fixed
 // order.  No atomics: the same bits every time.
+// Measured (training): 16384 x 4096 bf16 50 us forward (268 MB, 5.4 TB/s; one workgroup per row and outputs through the caches: 69) and 77 + 5 back
+// (403 MB, 5.2 TB/s); 57600 x 64 fp32 8 and 13 + 4; 4099 x 1001 fp16 8 and 15 + 4; 16 x 1024 bf16 3.5, a launch.
 #include "seq_common.h"
 
 namespace {

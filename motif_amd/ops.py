@@ -992,7 +992,7 @@ def frames_f32_to_u8(frames, round_half_even=True, swap_rb=True):
 # ----------------------------------------------------------------------------------------- sequence operators
 # Token-major tensors [..., D], the last axis dense, fp32, bf16 or fp16; statistics, sums and states fp32.  They work on the device and the
 # current stream of their tensors, allocate what they need per call (nothing is shared between calls, streams or captured graphs) and are
-# differentiable once.
+# differentiable once.  Into a HIP graph a backward pass can be captured as any of torch's: while no eager graph of the same leaves lives.
 _SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -1188,9 +1188,9 @@ class _GruScan(torch.autograd.Function):
 def gru_scan(z, q, h0=None, cu_seqlens=None):
     """gru_update along whole sequences, for gates that do not read the state: h_t = (1 - z_t) h_{t-1} + z_t q_t, channel by channel.
 
-    z, q: [B, T, D], fp32 / bf16 / fp16, any batch and row strides; h0: fp32 [B, D] (None: zeros).  Returns (h like q, the last states fp32 [B, D]);
+    z (a gate: 0 .. 1), q: [B, T, D], fp32 / bf16 / fp16, any batch and row strides; h0: fp32 [B, D] (None: zeros).  Returns (h like q, the last states fp32 [B, D]);
     the states can be handed to the next call: a sequence may come in pieces, down to single rows.  With cu_seqlens -- int32 [S + 1] on the device,
-    not decreasing, within 0 .. T -- z and q are [T, D] with S sequences packed one behind the other, h0 and the last states [S, D]; an empty
+    not decreasing from 0 on; what lies behind T counts as T -- z and q are [T, D] with S sequences packed one behind the other, h0 and the last states [S, D]; an empty
     sequence keeps its state, and rows that no sequence covers come out as zeros, whatever they hold.  Differentiable in z, q and h0."""
     what = "gru_scan"
     _seq_type(q, what, "q")
@@ -1267,7 +1267,7 @@ def gated_mlp(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
     """Gated feed-forward block act(x w_gate^T + b_gate) * (x w_up^T + b_up) in one kernel; act: "silu", "gelu" (exact) or "sigmoid".
 
     x [..., K], w_gate / w_up [F, K] (nn.Linear's layout), b_gate / b_up [F], all fp32, bf16 or fp16; K, F <= 65536, at most 2^22 rows.  Sums are
-    fp32; fp32 data keep fp32's accuracy on the matrix cores (three exact bf16 parts of every operand; an infinite operand makes its outputs NaN).
+    fp32; fp32 data keep fp32's accuracy on the matrix cores (fp32 instructions, or three exact bf16 parts of every operand; an infinite operand may make its outputs NaN).
     With gradients the two projections are kept in fp32 (8 bytes per output value).  Differentiable in all tensors."""
     what = "gated_mlp"
     _seq_type(x, what, "x")
