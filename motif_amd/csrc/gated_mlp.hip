@@ -15,7 +15,8 @@
 // dU are rounded once, to be operands of the matrix cores.
 // Up to 64 rows the forward pass is bound by reading the weights (rows_kernel); layers of up to 64 inputs hold theirs in registers (narrow_*_kernel).
 // Measured, 8192 x 2048 -> 2 x 5632 bf16: forward 313 us (1.21 PFLOP/s; the library's product of that size alone 352), 400 with G and U written
-// besides (369 MB); dG and dU 161 (646 MB, 4.0 TB/s), dx 278 (1.36 PFLOP/s; the library 291), dWg and dWu 296 + 16 (1.21 PFLOP/s; 356).
+// besides (369 MB); dG and dU 147 (646 MB, 4.4 TB/s; past the caches: in them they would push out
+// what the products read, 4 % of an fp32 backward pass), dx 278 (1.36 PFLOP/s; the library 291), dWg and dWu 296 + 16 (1.21 PFLOP/s; 356).
 // Sums over rows and over the pieces of a split reduction are taken in a fixed order: no atomics, the same bits every time.
 #include "seq_common.h"
 
@@ -1058,12 +1059,9 @@ void lay_out(const Inputs& f, bool need_x, bool need_w, const void* x, long xs, 
     });
 }
 
-// Rows of a workgroup of gate_grad_kernel: 64, fewer where that would leave less than four workgroups per CU.
-int grad_rows(long M, long F) {
-    int rows = 64;
-    while (rows > 8 && (long)cdiv(M, rows) * cdiv(F, 256) < 1024) rows /= 2;
-    return rows;
-}
+// Rows of a workgroup of gate_grad_kernel: 16 -- the last round of many short workgroups leaves little of the chip idle (8192 x 5632 bf16 from memory: 147 us,
+// 161 with 64 rows, whose column sums cost 5 us less; whole backward passes 0 to 2 % shorter) --, 8 where that would leave less than four per CU.
+int grad_rows(long M, long F) { return (long)cdiv(M, 16) * cdiv(F, 256) < 1024 ? 8 : 16; }
 GemmPlan fwd_plan(long M, long K, long F, int dtype, bool keep) { return gemm_plan(M, F, 2, (long)(planes(dtype) == 3 ? 6 : 1) * units_of(K), keep); }
 
 struct Backward { Inputs in; Image dg, du; float* bias_part; f32x4* part; GemmPlan dx, dw; float* dw_part; bool one_pass; };
