@@ -31,17 +31,19 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kSegs = 12;                                // dx in fp32: two pairs of operands, six products each
 
-// ---- activations.  FAST: v_exp_f32 and v_rcp_f32 as they are (relative error about 2^-21 at |g| = 8, behind a rounding to 8 or 11 bits); else
+// ---- activations.  FAST: v_exp_f32 and v_rcp_f32 as they are (relative error 2^-24 (|g| + 4), behind a rounding to 8 or 11 bits); else
 // expf and a reciprocal with a Newton step, one division's worth of accuracy at a third of its instructions ---------------------------------------
 template <bool FAST>
 __device__ __forceinline__ float reciprocal(float d) {  // finite d
     const float t = __builtin_amdgcn_rcpf(d);
     return FAST ? t : fmaf(t, fmaf(-d, t, 1.f), t);
 }
+// s = 1 / (1 + exp(-g)) and `rest` = 1 - s, both from e = exp(-|g|): neither passes a type's range, nor is one a difference from 1.
 template <bool FAST>
-__device__ __forceinline__ float sigm(float g) {
-    const float e = FAST ? __expf(-g) : expf(-g);
-    return reciprocal<FAST>(1.f + (!FAST && e > 1e38f ? 1e38f : e));
+__device__ __forceinline__ float sigm(float g, float& rest) {
+    const float e = FAST ? __expf(-fabsf(g)) : expf(-fabsf(g)), t = reciprocal<FAST>(1.f + e), u = e * t;
+    rest = g < 0.f ? t : u;
+    return g < 0.f ? u : t;
 }
 // Phi(g) = erfc(-g / sqrt 2) / 2, and E = exp(-g^2 / 2).  erfc(x) exp(x^2) is smooth and falls like 1 / x: as t P(t) with t = 1 / (1 + 0.35 |g|), P of degree 8
 // fitted to the least relative error, it is off by 3.2e-8 over |g| <= 14 (below, E is 0).  No difference of near values on the negative side, and E serves
@@ -74,7 +76,10 @@ __device__ __forceinline__ void gates(const float (&g)[N], int act, float (&v)[N
     } else {
         const bool silu = act == MOTIF_GATE_SILU;        // g s, or s
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = (silu ? g[e] : 1.f) * sigm<FAST>(g[e]);
+        for (int e = 0; e < N; ++e) {
+            float rest;
+            v[e] = (silu ? g[e] : 1.f) * sigm<FAST>(g[e], rest);
+        }
     }
 }
 template <bool FAST, int N>
@@ -91,9 +96,10 @@ __device__ __forceinline__ void gate_grads(const float (&g)[N], int act, float (
         const bool silu = act == MOTIF_GATE_SILU;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const float s = sigm<FAST>(g[e]), m = silu ? g[e] : 1.f;
+            float rest;
+            const float s = sigm<FAST>(g[e], rest), m = silu ? g[e] : 1.f;
             v[e] = m * s;
-            d[e] = s * fmaf(m, 1.f - s, silu ? 1.f : 0.f);
+            d[e] = s * fmaf(m, rest, silu ? 1.f : 0.f);
         }
     }
 }

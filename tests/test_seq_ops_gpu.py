@@ -419,11 +419,11 @@ def test_gru_scan_gives_the_same_bits_every_time_on_any_stream_and_in_a_graph(op
 
 # ------------------------------------------------------------------------------------------------------------------ gated_mlp
 def gate_reference(g, act):
-    s = torch.sigmoid(g)
+    s, rest = torch.sigmoid(g), torch.sigmoid(-g)          # 1 - s: not as a difference, which is 0 from g = 37 on
     if act == "sigmoid":
-        return s, s * (1 - s)
+        return s, s * rest
     if act == "silu":
-        return g * s, s * (1 + g * (1 - s))
+        return g * s, s * (1 + g * rest)
     phi = 0.5 * (1 + torch.erf(g / math.sqrt(2)))
     return g * phi, phi + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
 
@@ -598,6 +598,30 @@ def test_gated_mlp_of_fp32_spans_its_magnitudes(ops):
     # the sigmoid moves by its own derivative over G's error, and by its relative error where it is small (underflows: below 1e-38)
     lo, hi = torch.sigmoid(G - eG), torch.sigmoid(G + eG)
     within(h, s * U, 1.01 * ((hi - lo) * U.abs() + (16 + 2 * G.abs().clamp_max(100)) * F32 * (s * U).abs() + (7 * 64 + 64) * F32 * size * hi) + 1e-37 * U.abs() + 1e-38)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M, K", [(16, 128), (100, 128), (16, 8), (100, 8)])
+def test_gated_mlp_gates_far_from_zero(ops, dtype, act, M, K):
+    """Gates of up to 1e30 (fp16: 6e4) through each kind of kernel: G is column 0 of x, U column 1.  The activations and their derivatives are 0, 1 or g
+    there: to the type's rounding, and to 1e-30 where they underflow."""
+    values = [0.0, 20.0, 60.0, 90.0, 200.0, 6e4] + ([] if dtype == torch.float16 else [1e10, 1e30])
+    g = torch.tensor([s * v for v in values for s in (1, -1)], device="cuda")
+    x = torch.zeros(M, K, device="cuda", dtype=dtype)
+    x[:, 0] = g[torch.arange(M, device="cuda") % len(g)].to(dtype)
+    x[:, 1] = 1
+    wg, wu = torch.zeros(16, K, device="cuda", dtype=dtype), torch.zeros(16, K, device="cuda", dtype=dtype)
+    wg[:, 0], wu[:, 1] = 1, 1
+    x.requires_grad_()
+    h = ops.gated_mlp(x, wg, wu, act=act)
+    dx, = torch.autograd.grad(h, x, torch.full_like(h, 1 / 16))
+    v, d = gate_reference(x[:, 0].detach().double(), act)
+    within(h, v[:, None].expand(M, 16), half_step(dtype, v[:, None]) + 200 * F32 * v[:, None].abs() + 1e-30)
+    # one rounding of dG and dU to operands, sums of 16 alike (exact), one of dx; dG is d / 16, dU v / 16
+    tol = lambda t: 2.01 * half_step(dtype, t) + 16 * 2.01 * half_step(dtype, t / 16) + 200 * F32 * t.abs() + 1e-30  # noqa: E731
+    within(dx[:, 0], d, tol(d))
+    within(dx[:, 1], v, tol(v))
 
 
 def test_gated_mlp_gradient_against_differences(ops):
