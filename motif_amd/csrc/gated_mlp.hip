@@ -13,7 +13,7 @@
 // whose rows are not whole 16-byte pieces are laid out first (layout_kernel).
 // G and U are kept in fp32 for the backward pass: rounded to the data's type they would add an error of their own to every gradient; dG and
 // dU are rounded once, to be operands of the matrix cores.
-// Up to 64 rows the forward pass is bound by reading the weights (rows_kernel); layers of up to 64 inputs hold theirs in registers (narrow_*_kernel).
+// Up to 64 rows the forward pass is bound by reading the weights (rows_kernel, which small products share); layers of up to 64 inputs hold theirs in registers (narrow_*_kernel).
 // Measured, 8192 x 2048 -> 2 x 5632 bf16: forward 313 us (1.21 PFLOP/s; the library's product of that size alone 352), 400 with G and U written
 // besides (369 MB); dG and dU 147 (646 MB, 4.4 TB/s; past the caches: in them they would push out
 // what the products read, 4 % of an fp32 backward pass), dx 278 (1.36 PFLOP/s; the library 291), dWg and dWu 296 + 16 (1.21 PFLOP/s; 356).
@@ -579,8 +579,8 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
     }
 }
 
-// ---- few rows ----------------------------------------------------------------------------------------------------------------------------
-// Up to 16 MT rows: a workgroup takes 16 columns of both projections, its 8 waves share the reduction, each lane reads 32 bytes of a weight row at a time
+// ---- few rows, small products -------------------------------------------------------------------------------------------------------------
+// 16 MT rows to a workgroup, which takes 16 columns of both projections; its 8 waves share the reduction, each lane reads 32 bytes of a weight row at a time
 // (16 rows x 128 bytes: whole cache lines) straight into the matrix instruction's operands -- which of the reduction's values a lane holds is free as
 // long as both operands agree --; the waves' sums meet in LDS in a fixed order.  Bound by the weights' bytes.  fp32 runs on the fp32 matrix instruction.
 // One row through 2048 -> 2 x 5632 bf16: 11.4 us, of which the 46 MB take 7.5 at the rate of a long read.
@@ -590,14 +590,14 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
     constexpr int V = 16 / sizeof(T), STEP = 8 * V, NW = 8;
     __shared__ float sh[NW][2][16 * MT][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = lane & 15, kq = (lane >> 4) * 2 * V;
-    const int f0 = blockIdx.x * 16, fr = min(f0 + lo, F - 1);
+    const int f0 = blockIdx.x * 16, fr = min(f0 + lo, F - 1), m0 = blockIdx.y * 16 * MT;
     const T* pg = wg + (long)fr * K + kq;
     const T* pu = wu + (long)fr * K + kq;
     const T* px[MT];
     f32x4 ag[MT], au[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        px[i] = x + (long)min(i * 16 + lo, M - 1) * xs + kq;
+        px[i] = x + (long)min(m0 + i * 16 + lo, M - 1) * xs + kq;
         ag[i] = au[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     typedef SeqRaw<T, V> Raw;
@@ -661,11 +661,11 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
         }
     __syncthreads();
     for (int i = threadIdx.x; i < 256 * MT; i += 512) {
-        const int m = i >> 4, f = f0 + (i & 15);
+        const int row = i >> 4, m = m0 + row, f = f0 + (i & 15);
         if (m >= M || f >= F) continue;
         float g = 0.f, u = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { g += sh[w][0][m][i & 15]; u += sh[w][1][m][i & 15]; }
+        for (int w = 0; w < NW; ++w) { g += sh[w][0][row][i & 15]; u += sh[w][1][row][i & 15]; }
         if (bg) g += (float)bg[f];
         if (bu) u += (float)bu[f];
         float v[1];
@@ -910,6 +910,15 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 64;
+// Products for rows_kernel: up to 64 rows, and beyond them what its workgroups of 64 rows x 16 columns have done in two rounds of the chip -- four where the
+// tiles' operands would have to be laid out first -- and 2^19 steps of a workgroup; the tiles of so small a product leave most CUs idle.  bf16, this
+// kernel or tiles: 256 x 1024 -> 2 x 1024 (256 workgroups) 9 or 18 us, 512 x 256 -> 2 x 1024 (512) 8 or 9, 512 x 1024 -> 2 x 1024 (512, 2^19 steps) 13
+// or 13, 1024 x 512 -> 2 x 1024 (1024) 15 or 11; fp32: 512 x 256 -> 2 x 1024 12 or 29, 2048 x 128 -> 2 x 512 (1024) 12 or 23, 257 x 1000 -> 2 x 2729
+// (855, 1.6 x 2^19) 65 or 61, 8192 x 72 -> 2 x 512 (4096) 51 or 30.
+bool few(long M, long K, long F, bool laid_out) {
+    const long groups = (long)cdiv(F, 16) * cdiv(M, 64);
+    return M <= kFewRows || (groups <= (laid_out ? 1024 : 512) && groups * K <= 1L << 19);
+}
 // Waves of narrow_fwd_kernel to a CU: more hide more of the reads, until their writes get in each other's way (57600 x 64 -> 2 x 1024 bf16: 88 us with 8, 83 with 12;
 // with kept projections 200 and 206).
 int narrow_waves(bool keep) { return keep ? 8 : 12; }
@@ -1018,7 +1027,7 @@ int check_mlp(long M, long K, long F, int act, int dtype) {
 
 template <typename T, int MT>
 void few_rows(const void* x, long xs, const void* wg, const void* wu, const void* bg, const void* bu, void* h, float* G, float* U, int M, int K, int F, int act, hipStream_t s) {
-    rows_kernel<T, MT><<<cdiv(F, 16), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
+    rows_kernel<T, MT><<<dim3(cdiv(F, 16), cdiv(M, 16 * MT)), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
 }
 
 bool narrow(long K, long F) { return K <= 64 && K % 4 == 0 && F % 8 == 0; }
@@ -1100,7 +1109,8 @@ extern "C" long motif_gated_mlp_ws_bytes(const void* x, long x_rs, const void* w
     if (rc) return rc;
     if (M <= kFewRows || narrow(K, F)) return 0;
     Arena ws = {nullptr, 0};
-    inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+    const Inputs f = inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+    if (few(M, K, F, f.lay_x || f.lay_w)) return 0;
     const long p0 = part_bytes(fwd_plan(M, K, F, dtype, false)), p1 = part_bytes(fwd_plan(M, K, F, dtype, true));
     ws.take(p0 > p1 ? p0 : p1);
     return ws.used;
@@ -1113,7 +1123,14 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
     if (M == 0) return MOTIF_OK;
     if (!x || !w_gate || !w_up || !h || x_rs < 0 || !G != !U) return MOTIF_EINVAL;
     hipStream_t s = (hipStream_t)stream;
-    if (M <= kFewRows) {
+    if (M > kFewRows && narrow(K, F)) {
+        seq_dispatch(dtype, [&](auto* t) { narrow_fwd<std::remove_pointer_t<decltype(t)>>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s); });
+        MOTIF_LAUNCH_CHECK();
+        return MOTIF_OK;
+    }
+    Arena ws = {(char*)workspace, 0};
+    const Inputs f = inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+    if (few(M, K, F, f.lay_x || f.lay_w)) {
         seq_dispatch(dtype, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
             if (M <= 16) few_rows<T, 1>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);
@@ -1123,13 +1140,6 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
         MOTIF_LAUNCH_CHECK();
         return MOTIF_OK;
     }
-    if (narrow(K, F)) {
-        seq_dispatch(dtype, [&](auto* t) { narrow_fwd<std::remove_pointer_t<decltype(t)>>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s); });
-        MOTIF_LAUNCH_CHECK();
-        return MOTIF_OK;
-    }
-    Arena ws = {(char*)workspace, 0};
-    const Inputs f = inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
     const GemmPlan plan = fwd_plan(M, K, F, dtype, G != nullptr);
     f32x4* part = (f32x4*)ws.take(part_bytes(plan));
     if (ws.used && !workspace) return MOTIF_EINVAL;

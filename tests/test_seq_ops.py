@@ -55,7 +55,7 @@ def test_gated_mlp_refuses_bad_arguments_before_it_launches(lib):
         return lib.motif_gated_mlp_fwd(x, rs, wg, wu, None, None, h, G, U, ws, M, K, F, act, dt, None)
     assert fwd(x=None) == fwd(wg=None) == fwd(wu=None) == fwd(h=None) == fwd(M=-1) == fwd(K=0) == fwd(F=0) == fwd(act=3) == fwd(act=-1) == fwd(dt=5) == fwd(rs=-1) == EINVAL
     assert fwd(G=P) == fwd(U=P) == EINVAL                # both or neither
-    assert fwd(dt=0, K=128, rs=128, ws=None) == fwd(K=65, rs=65, ws=None) == EINVAL      # operands to be laid out need a workspace
+    assert fwd(M=5000, F=1024, dt=0, K=128, rs=128, ws=None) == fwd(M=5000, F=1024, K=65, rs=65, ws=None) == EINVAL      # operands to be laid out need a workspace
     assert fwd(K=65537) == fwd(F=65537) == fwd(M=(1 << 22) + 1) == ELIMIT
     assert fwd(x=None, M=0) == 0
     def bwd(G=P, dh=P, dx=P, dwg=P, dwu=P, ws=P, M=100):
@@ -63,7 +63,8 @@ def test_gated_mlp_refuses_bad_arguments_before_it_launches(lib):
     assert bwd(G=None) == bwd(dh=None) == bwd(dwg=None) == bwd(dwu=None) == bwd(ws=None) == bwd(M=0) == bwd(dx=None, dwg=None, dwu=None) == bwd(G=P + 4) == EINVAL
     ws = lib.motif_gated_mlp_ws_bytes
     assert ws(P, 64, P, P, 64, 64, 64, 0) == 0           # few rows: none
-    assert ws(P, 128, P, P, 65, 128, 64, 0) >= 3 * 2 * (65 + 128) * 128
+    assert ws(P, 128, P, P, 5000, 128, 1024, 0) >= 3 * 2 * (5000 + 2048) * 128
+    assert ws(P, 128, P, P, 100, 128, 64, 0) == 0         # small products: none
     assert ws(P, 64, P, P, 65, 64, 64, 0) == 0           # narrow layers: none
     assert ws(P, 64, P, P, 100, 70000, 64, 1) == ELIMIT
 

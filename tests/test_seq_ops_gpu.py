@@ -539,6 +539,54 @@ def test_gated_mlp_of_narrow_layers_keeps_bad_rows_to_themselves(ops):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M, K, F, act, bias", [(4200, 72, 264, "silu", True), (5000, 100, 300, "gelu", True), (1030, 1003, 517, "sigmoid", False), (1100, 1000, 770, "silu", True),
+                                                (2050, 504, 1001, "gelu", True), (4097, 136, 1000, "sigmoid", True), (1500, 333, 1030, "silu", False), (300, 2056, 1224, "silu", True)])
+def test_gated_mlp_in_tiles_with_edges(ops, dtype, M, K, F, act, bias):
+    """Products that are too large for 64 rows to a workgroup, small enough for 128 x 128 tiles: ends inside a tile in every axis, operands as they lie and
+    laid out."""
+    mlp_check(ops, *mlp_inputs(M, K, F, dtype, M + K + F, bias), act)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M, K, F, act, bias", [(65, 1024, 1024, "silu", True), (200, 300, 333, "gelu", True), (1000, 136, 72, "sigmoid", True), (513, 72, 520, "silu", False),
+                                                (129, 2048, 31, "gelu", True), (4000, 66, 9, "silu", True)])
+def test_gated_mlp_of_small_products(ops, dtype, M, K, F, act, bias):
+    """Workgroups of 64 rows beyond the first 64, the last ones part empty."""
+    mlp_check(ops, *mlp_inputs(M, K, F, dtype, M + K + F, bias), act)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["columns", "odd columns", "transposed", "one bias"])
+def test_gated_mlp_in_tiles_takes_strided_inputs(ops, dtype, kind):
+    x, wg, wu, bg, bu = mlp_inputs(4200, 96, 264, dtype, 3, True)
+    base = torch.randn(4200, 160, generator=gen(4), device="cuda").to(dtype)
+    if kind == "columns":
+        x = base[:, 32:128]
+    elif kind == "odd columns":
+        x = base[:, 3:99]
+    elif kind == "transposed":
+        x = torch.randn(96, 4200, generator=gen(5), device="cuda").to(dtype).t()
+    else:
+        bg = None
+    mlp_check(ops, x, wg, wu, bg, bu, "silu")
+
+
+def test_gated_mlp_in_tiles_keeps_bad_rows_to_themselves_and_spans_fp32s_magnitudes(ops):
+    x, wg, wu, bg, bu = mlp_inputs(4200, 128, 264, torch.float32, 6, True)
+    want = ops.gated_mlp(x, wg, wu, bg, bu)
+    bad = x.clone()
+    bad[3, 7], bad[4199, 127] = math.inf, math.nan
+    got = ops.gated_mlp(bad, wg, wu, bg, bu)
+    assert torch.equal(got[4:4199], want[4:4199]) and torch.equal(got[:3], want[:3])
+    assert not torch.isfinite(got[3]).all() and torch.isnan(got[4199]).all()
+    # the three parts carry 24 bits at any exponent: h is s U, whose relative error c(128) times the terms' sum does not depend on the scale
+    x = x * torch.logspace(-20, 15, 4200, device="cuda")[:, None]
+    u = ops.gated_mlp(x, torch.zeros_like(wg), wu, act="sigmoid")
+    X, W = x.double(), wu.double()
+    within(u, 0.5 * (X @ W.t()), 0.5 * 1.01 * ((6 * 128 + 64) * F32 + 3 * 2.0 ** -23) * (X.abs() @ W.abs().t()) + 4 * F32 * (X @ W.t()).abs())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_gated_mlp_in_large_tiles(ops, dtype):
     """Enough rows and columns for the 256 x 256 tiles in all three products, with edges in both axes."""
     mlp_check(ops, *mlp_inputs(4229, 4130, 2060, dtype, 1, True), "silu")
