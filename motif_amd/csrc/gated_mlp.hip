@@ -124,7 +124,7 @@ struct GemmArgs {
     long ldg;
     const void *bias0, *bias1;
     f32x4* part;                                         // pieces' accumulators: [tile - whole][piece][accumulator][thread]
-    int act, dtype, vec;                                 // vec: rows of the outputs allow runs of four values
+    int act, dtype;
 };
 
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c, bf16_t*) {
@@ -146,18 +146,18 @@ __device__ __forceinline__ void to_lds(unsigned lds, const void* own) {
 __device__ u32x4 g_zeros;                                // what lies behind the end of a reduction
 
 template <typename T, typename O, int N>
-__device__ __forceinline__ void store_run(void* p, long at, const float (&v)[N], int n, bool vec) {      // n of N values; whole aligned runs as one store
+__device__ __forceinline__ void store_run(void* p, long at, const float (&v)[N], int n) {      // n of N values; whole runs as one store, at any address
     O* o = (O*)p + at;
-    if (vec && n == N) seq_store<O, N>(o, v);
+    if (n == N) seq_store<O, N>(o, v);
     else
 #pragma unroll
         for (int i = 0; i < N; ++i) if (i < n) o[i] = (O)v[i];
 }
 template <int N>
-__device__ __forceinline__ void store_as(void* p, long at, const float (&v)[N], int n, bool vec, int dtype) {
-    if (dtype == MOTIF_F32) store_run<float, float, N>(p, at, v, n, vec);
-    else if (dtype == MOTIF_BF16) store_run<bf16_t, bf16_t, N>(p, at, v, n, vec);
-    else store_run<f16_t, f16_t, N>(p, at, v, n, vec);
+__device__ __forceinline__ void store_as(void* p, long at, const float (&v)[N], int n, int dtype) {
+    if (dtype == MOTIF_F32) store_run<float, float, N>(p, at, v, n);
+    else if (dtype == MOTIF_BF16) store_run<bf16_t, bf16_t, N>(p, at, v, n);
+    else store_run<f16_t, f16_t, N>(p, at, v, n);
 }
 
 // One operand of a tile: two blocks of C rows (of the output), 64 of the reduction deep, 128 C bytes each.  A wave requests two pieces of 1 KB of
@@ -250,7 +250,7 @@ struct Store {
             if (p.dtype == MOTIF_F32) gates<false>(g, p.act, v); else gates<true>(g, p.act, v);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] *= u[e];
-            store_as<4>(p.c0, (long)row * p.N + n, v, cnt, p.vec, p.dtype);
+            store_as<4>(p.c0, (long)row * p.N + n, v, cnt, p.dtype);
             if (p.g) {                                   // (their rows are padded to whole runs)
                 seq_store<float, 4>(p.g + row * p.ldg + n, g);
                 seq_store<float, 4>(p.u + row * p.ldg + n, u);
@@ -264,7 +264,7 @@ struct Store {
                 if (row >= rows || cnt <= 0) continue;
                 const f32x4& o = h ? o1 : o0;
                 const float v[4] = {o[0], o[1], o[2], o[3]};
-                store_as<4>(MODE == ONE || h == 0 ? p.c0 : p.c1, (long)row * cols + col, v, cnt, p.vec, p.dtype);
+                store_as<4>(MODE == ONE || h == 0 ? p.c0 : p.c1, (long)row * cols + col, v, cnt, p.dtype);
             }
         }
     }
@@ -1152,7 +1152,6 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
     g.M = (int)M; g.N = (int)F;
     g.c0 = h; g.g = G; g.u = U; g.ldg = up8(F); g.bias0 = b_gate; g.bias1 = b_up;
     g.act = act; g.dtype = dtype;
-    g.vec = F % 4 == 0 && seq_aligned(h, 16);
     g.part = part;
     gemm_dtype<GATED>(dtype, plan, g, s);
     MOTIF_LAUNCH_CHECK();
@@ -1211,7 +1210,6 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         g.M = (int)M; g.N = (int)K; g.wb = up8(K);
         g.c0 = dx; g.dtype = dtype;
         g.part = b.part;
-        g.vec = K % 4 == 0 && seq_aligned(dx, 16);
         gemm_dtype<ONE>(dtype, b.dx, g, s);
     }
     if (need_w) {
@@ -1223,7 +1221,6 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         g.M = (int)K; g.N = (int)F; g.wa = up8(K); g.wb = b.dg.ld;
         g.c0 = dw_gate; g.c1 = dw_up; g.dtype = dtype;
         g.part = b.part;
-        g.vec = K % 4 == 0 && seq_aligned(dw_gate, 16) && seq_aligned(dw_up, 16);
         gemm_dtype<TWO>(dtype, b.dw, g, s);
     }
     MOTIF_LAUNCH_CHECK();
