@@ -906,3 +906,60 @@ def test_gru_scan_bounds_behind_the_rows_end_with_them(ops):
     got = ops.gru_scan(z, q, h0, cu_seqlens=torch.tensor([0, 20, 70, 90], dtype=torch.int32, device="cuda"))
     want = ops.gru_scan(z, q, h0, cu_seqlens=torch.tensor([0, 20, 50, 50], dtype=torch.int32, device="cuda"))
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ------------------------------------------------------------------------------------------------------------------ unusual calls
+def test_one_tensor_in_several_places_and_broadcast_parameters(ops):
+    """x as both weights, the gate as its own candidate, a weight of one value for all columns, a row for all rows: gradients add up over the places."""
+    a = torch.randn(70, 64, generator=gen(41), device="cuda").mul_(0.125).requires_grad_()
+    g, = torch.autograd.grad(ops.gated_mlp(a, a, a).sum(), a)
+    b = a.detach().double().requires_grad_()
+    p = b @ b.t()
+    want, = torch.autograd.grad((torch.nn.functional.silu(p) * p).sum(), b)
+    # products of 64 terms below 2 in sum, three roundings on the way, sums of 2 x 70: within 2000 x 2^-24 of the largest gradient
+    within(g, want, 2000 * F32 * want.abs().max())
+    z = torch.rand(2, 50, 8, generator=gen(42), device="cuda").requires_grad_()
+    h, last = ops.gru_scan(z, z)
+    g, = torch.autograd.grad(h.sum() + last.sum(), z)
+    d = z.detach().double().requires_grad_()
+    s, total = torch.zeros(2, 8, device="cuda", dtype=torch.float64), 0
+    for t in range(50):
+        s = (1 - d[:, t]) * s + d[:, t] * d[:, t]
+        total = total + s.sum()
+    want, = torch.autograd.grad(total + s.sum(), d)
+    within(g, want, 1000 * F32 * (1 + want.abs().max()))
+    x, w = torch.randn(1, 64, generator=gen(43), device="cuda").requires_grad_(), torch.ones(1, device="cuda", requires_grad=True)
+    got = torch.autograd.grad(ops.layer_norm(x.expand(5, 64), w.expand(64)).square().sum(), (x, w))
+    x2, w2 = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    n = (x2 - x2.mean()) / (x2.var(unbiased=False) + 1e-5).sqrt()
+    want = torch.autograd.grad((n.expand(5, 64) * w2).square().sum(), (x2, w2))
+    # dx is a difference of terms of order 2 n / sigma (5 rows): absolute, to 100 roundings of their size
+    within(got[0], want[0], 100 * F32 * 5 * 2 * float(n.detach().abs().max()) ** 2 * torch.ones_like(want[0]))
+    within(got[1], want[1], 100 * F32 * want[1].abs())
+
+
+def test_offsets_beyond_32_bits(ops):
+    rows, d = 3 << 20, 1024                              # 3.2e9 values
+    x = torch.zeros(rows, d, device="cuda", dtype=torch.bfloat16)
+    x[-1] = torch.arange(d, device="cuda").bfloat16()
+    with torch.no_grad():
+        y = ops.layer_norm(x)
+        assert torch.equal(y[-1], ops.layer_norm(x[-1:].clone())[0]) and not y[:-1].any()
+        del y
+        z = torch.full_like(x, 0.5)
+        h, last = ops.gru_scan(z, x.fill_(1), cu_seqlens=torch.tensor([0, rows - 5, rows], dtype=torch.int32, device="cuda"))
+        assert (h[rows - 6] == 1).all() and (h[rows - 5] == 0.5).all() and (last[1] == 1 - 2.0 ** -5).all()
+        del h, z, x
+        x = torch.randn(4 << 20, 64, generator=gen(44), device="cuda").bfloat16()
+        wg, wu = (torch.randn(1024, 64, generator=gen(45 + i), device="cuda").mul_(0.125).bfloat16() for i in (0, 1))
+        y = ops.gated_mlp(x, wg, wu)                     # narrow: 4.3e9 outputs
+        assert torch.equal(y[-100:], ops.gated_mlp(x[-100:].clone(), wg, wu))
+        del y, x
+        x = torch.randn(2 << 20, 1032, generator=gen(47), device="cuda", dtype=torch.bfloat16)[:, :1024]
+        wg, wu = (torch.randn(1040, 1024, generator=gen(48 + i), device="cuda").mul_(2.0 ** -5).bfloat16() for i in (0, 1))
+        y = ops.gated_mlp(x, wg, wu)                     # tiles: 2.2e9 inputs and outputs
+        p, q = (x[-100:].double() @ w.double().t() for w in (wg, wu))
+        size = x[-100:].double().abs() @ wg.double().abs().t(), x[-100:].double().abs() @ wu.double().abs().t()
+        v = torch.nn.functional.silu(p)
+        c = (1024 + 64) * F32
+        within(y[-100:], v * q, half_step(torch.bfloat16, v * q) + 1.01 * (1.13 * c * size[0] * q.abs() + c * size[1] * v.abs()) + (20 + 2 * p.abs()) * F32 * (v * q).abs())
