@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
 // (16 rows x 128 bytes: whole cache lines) straight into the matrix instruction's operands -- which of the reduction's values a lane holds is free as
 // long as both operands agree --; the waves' sums meet in LDS in a fixed order.  Bound by the weights' bytes.  fp32 runs on the fp32 matrix instruction.
 // One row through 2048 -> 2 x 5632 bf16: 11.4 us, of which the 46 MB take 7.5 at the rate of a long read.
-template <typename T, int MT>
+template <typename T, int MT, bool STEPS>
 __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long xs, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ bg, const T* __restrict__ bu,
                                                    T* __restrict__ h, float* __restrict__ G, float* __restrict__ U, long ldg, int M, int K, int F, int act) {
     constexpr int V = 16 / sizeof(T), STEP = 8 * V, NW = 8;
@@ -614,28 +614,54 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
             }
         }
     };
-    constexpr int AHEAD = MT == 1 ? 4 : MT == 2 ? 2 : 1; // steps requested together: MT = 1, all that a wave has up to K = 2048 (16 bits)
+    // Steps requested together -- MT = 1, all that a wave has up to K = 2048 (16 bits) -- by two workgroups to a CU, or a step ahead by one.
     const int whole = K / STEP;
     int s = wave;
-    for (; s + (AHEAD - 1) * NW < whole; s += NW * AHEAD) {
-        Raw a[AHEAD][2], b[AHEAD][2], c[AHEAD][2][MT];
+    if constexpr (!STEPS) {
+        constexpr int AHEAD = MT == 1 ? 4 : MT == 2 ? 2 : 1;
+        for (; s + (AHEAD - 1) * NW < whole; s += NW * AHEAD) {
+            Raw a[AHEAD][2], b[AHEAD][2], c[AHEAD][2][MT];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
+            for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int k = (s + j * NW) * STEP + t * V;
+                    a[j][t] = seq_raw<T, V>(pg + k);
+                    b[j][t] = seq_raw<T, V>(pu + k);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) c[j][t][i] = seq_raw<T, V>(px[i] + k);
+                }
+            __builtin_amdgcn_sched_barrier(0);               // (all of them requested before the first is used)
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) multiply(a[j][t], b[j][t], c[j][t][i], i);
+        }
+    } else if (s < whole) {
+        struct Step { Raw a[2], b[2], c[2][MT]; };
+        auto request = [&](Step& w, int step) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int k = (s + j * NW) * STEP + t * V;
-                a[j][t] = seq_raw<T, V>(pg + k);
-                b[j][t] = seq_raw<T, V>(pu + k);
+                const int k = step * STEP + t * V;
+                w.a[t] = seq_raw<T, V>(pg + k);
+                w.b[t] = seq_raw<T, V>(pu + k);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) c[j][t][i] = seq_raw<T, V>(px[i] + k);
+                for (int i = 0; i < MT; ++i) w.c[t][i] = seq_raw<T, V>(px[i] + k);
             }
-        __builtin_amdgcn_sched_barrier(0);               // (all of them requested before the first is used)
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
+        };
+        Step now, next;
+        request(now, s);
+        for (; s < whole; s += NW) {
+            request(next, min(s + NW, whole - 1));
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) multiply(a[j][t], b[j][t], c[j][t][i], i);
+                for (int i = 0; i < MT; ++i) multiply(now.a[t], now.b[t], now.c[t][i], i);
+            now = next;
+        }
     }
     auto read = [&](const T* at, int k) __attribute__((always_inline)) {         // zeros behind the row's end
         if (kq + k + V <= K) return seq_raw<T, V>(at + k);
@@ -910,14 +936,15 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 64;
-// Products for rows_kernel: up to 64 rows, and beyond them what its workgroups of 64 rows x 16 columns have done in two rounds of the chip -- four where the
+// Products for rows_kernel: up to 64 rows (fp32: 128), and beyond them what its workgroups of 64 rows x 16 columns have done in two rounds of the chip -- four where the
 // tiles' operands would have to be laid out first -- and 2^19 steps of a workgroup; the tiles of so small a product leave most CUs idle.  bf16, this
 // kernel or tiles: 256 x 1024 -> 2 x 1024 (256 workgroups) 9 or 18 us, 512 x 256 -> 2 x 1024 (512) 8 or 9, 512 x 1024 -> 2 x 1024 (512, 2^19 steps) 13
 // or 13, 1024 x 512 -> 2 x 1024 (1024) 15 or 11; fp32: 512 x 256 -> 2 x 1024 12 or 29, 2048 x 128 -> 2 x 512 (1024) 12 or 23, 257 x 1000 -> 2 x 2729
-// (855, 1.6 x 2^19) 65 or 61, 8192 x 72 -> 2 x 512 (4096) 51 or 30.
-bool few(long M, long K, long F, bool laid_out) {
+// (855, 1.6 x 2^19) 65 or 61, 8192 x 72 -> 2 x 512 (4096) 51 or 30.  fp32 up to 128 rows whatever the size, whose weights would be laid out for little: 128 x
+// 4096 -> 2 x 8192 198 or 293, 128 x 2048 -> 2 x 5632 82 or 98; 192 x 2048 -> 2 x 5632 134 or 126.
+bool few(long M, long K, long F, int dtype, bool laid_out) {
     const long groups = (long)cdiv(F, 16) * cdiv(M, 64);
-    return M <= kFewRows || (groups <= (laid_out ? 1024 : 512) && groups * K <= 1L << 19);
+    return M <= (dtype == MOTIF_F32 ? 2 * kFewRows : kFewRows) || (groups <= (laid_out ? 1024 : 512) && groups * K <= 1L << 19);
 }
 // Waves of narrow_fwd_kernel to a CU: more hide more of the reads, until their writes get in each other's way (57600 x 64 -> 2 x 1024 bf16: 88 us with 8, 83 with 12;
 // with kept projections 200 and 206).
@@ -1027,7 +1054,11 @@ int check_mlp(long M, long K, long F, int act, int dtype) {
 
 template <typename T, int MT>
 void few_rows(const void* x, long xs, const void* wg, const void* wu, const void* bg, const void* bu, void* h, float* G, float* U, int M, int K, int F, int act, hipStream_t s) {
-    rows_kernel<T, MT><<<dim3(cdiv(F, 16), cdiv(M, 16 * MT)), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
+    // fp32 from 17 rows on multiplies a long row's steps for long enough to cover the next one's requests alone (64 rows, 4096 -> 2 x 8192: 102 us, 133 with
+    // steps together; 1024 -> 2 x 1024 18 and 19; 512 -> 2 x 2048 13 and 11; bf16 4096 -> 2 x 8192 55 and 47).
+    auto* kernel = rows_kernel<T, MT, false>;
+    if constexpr (sizeof(T) == 4 && MT > 1) if (K >= 1024) kernel = rows_kernel<T, MT, true>;
+    kernel<<<dim3(cdiv(F, 16), cdiv(M, 16 * MT)), 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, (T*)h, G, U, up8(F), M, K, F, act);
 }
 
 bool narrow(long K, long F) { return K <= 64 && K % 4 == 0 && F % 8 == 0; }
@@ -1110,7 +1141,7 @@ extern "C" long motif_gated_mlp_ws_bytes(const void* x, long x_rs, const void* w
     if (M <= kFewRows || narrow(K, F)) return 0;
     Arena ws = {nullptr, 0};
     const Inputs f = inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
-    if (few(M, K, F, f.lay_x || f.lay_w)) return 0;
+    if (few(M, K, F, dtype, f.lay_x || f.lay_w)) return 0;
     const long p0 = part_bytes(fwd_plan(M, K, F, dtype, false)), p1 = part_bytes(fwd_plan(M, K, F, dtype, true));
     ws.take(p0 > p1 ? p0 : p1);
     return ws.used;
@@ -1130,7 +1161,7 @@ extern "C" int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate,
     }
     Arena ws = {(char*)workspace, 0};
     const Inputs f = inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
-    if (few(M, K, F, f.lay_x || f.lay_w)) {
+    if (few(M, K, F, dtype, f.lay_x || f.lay_w)) {
         seq_dispatch(dtype, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
             if (M <= 16) few_rows<T, 1>(x, x_rs, w_gate, w_up, b_gate, b_up, h, G, U, (int)M, (int)K, (int)F, act, s);

@@ -549,9 +549,10 @@ def test_gated_mlp_in_tiles_with_edges(ops, dtype, M, K, F, act, bias):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M, K, F, act, bias", [(65, 1024, 1024, "silu", True), (200, 300, 333, "gelu", True), (1000, 136, 72, "sigmoid", True), (513, 72, 520, "silu", False),
-                                                (129, 2048, 31, "gelu", True), (4000, 66, 9, "silu", True)])
+                                                (129, 2048, 31, "gelu", True), (4000, 66, 9, "silu", True), (20, 1030, 47, "silu", True),
+                                                (33, 1500, 100, "gelu", True), (128, 1111, 72, "sigmoid", False), (64, 1280, 33, "silu", True)])
 def test_gated_mlp_of_small_products(ops, dtype, M, K, F, act, bias):
-    """Workgroups of 64 rows beyond the first 64, the last ones part empty."""
+    """Workgroups of 64 rows beyond the first 64, the last ones part empty; long rows, whose steps fp32 requests one ahead."""
     mlp_check(ops, *mlp_inputs(M, K, F, dtype, M + K + F, bias), act)
 
 
