@@ -1021,7 +1021,7 @@ def _seq_call(name, device, *args):
     """One entry of the library on `device` and its current stream."""
     fn = getattr(_lib._lib or _lib.load(), name)
     stream = torch._C._cuda_getCurrentRawStream(device.index)          # torch.cuda.current_stream(device).cuda_stream, without 2 us of Python
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
@@ -1063,7 +1063,7 @@ def _layer_norm_fwd(x, weight, bias, eps, want_stats):
     d = x.shape[-1]
     rows = x.numel() // d
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if want_stats else None
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
     if rows:
         xr, rs = _seq_rows(x)
         p = weight if weight is not None else bias
@@ -1087,14 +1087,13 @@ class _LayerNorm(torch.autograd.Function):
         d = x.shape[-1]
         rows = x.numel() // d
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw, db = (torch.empty(d, dtype=ctx.param_dtype, device=x.device) if need else None for need in (need_w, need_b))
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+        dw = x.new_empty(d, dtype=ctx.param_dtype) if need_w else None
+        db = x.new_empty(d, dtype=ctx.param_dtype) if need_b else None
         if rows:
             xr, xs = _seq_rows(x)
             dyr, ds = _seq_rows(dy)
-            ws = None
-            if need_w or need_b:
-                ws = torch.empty(_lib.load().motif_layer_norm_bwd_ws_floats(rows, d), dtype=torch.float32, device=x.device)
+            ws = stats.new_empty(_lib._lib.motif_layer_norm_bwd_ws_floats(rows, d)) if need_w or need_b else None
             _seq_call("motif_layer_norm_bwd", x.device, xr.data_ptr(), xs, dyr.data_ptr(), ds, _seq_ptr(weight), stats.data_ptr(), _seq_ptr(dx),
                       _seq_ptr(dw), _seq_ptr(db), _seq_ptr(ws), rows, d, _SEQ_DTYPES[x.dtype], _SEQ_DTYPES[ctx.param_dtype])
         else:
@@ -1171,8 +1170,9 @@ class _GruScan(torch.autograd.Function):
         z, q, h0, cu, h = ctx.saved_tensors
         b, t, d, s = _scan_sizes(z, cu)
         need_z, need_q, need_h, _ = ctx.needs_input_grad
-        dz, dq = (torch.empty(q.shape, dtype=q.dtype, device=q.device) if need else None for need in (need_z, need_q))
-        dh0 = torch.empty(dlast.shape, dtype=torch.float32, device=q.device) if need_h else None
+        dz = torch.empty_like(h) if need_z else None     # (h is dense)
+        dq = torch.empty_like(h) if need_q else None
+        dh0 = torch.empty_like(dlast, memory_format=torch.contiguous_format) if need_h else None
         if b * d == 0 or (t == 0 and cu is None):
             return dz, dq, dlast.clone() if need_h else None, None
         zt, zb, zr = _scan_strides(z)
@@ -1221,7 +1221,8 @@ def _gated_mlp_fwd(x, wg, wu, bg, bu, act, keep):
     f, k = wg.shape
     m, code = x.numel() // k, _SEQ_DTYPES[x.dtype]
     h = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
-    g, u = (torch.empty(m, (f + 7) & ~7, dtype=torch.float32, device=x.device) for _ in range(2)) if keep else (None, None)
+    g = x.new_empty((m, (f + 7) & ~7), dtype=torch.float32) if keep else None
+    u = torch.empty_like(g) if keep else None
     if m:
         xr, rs = _seq_rows(x)
         args = (xr.data_ptr(), rs, wg.data_ptr(), wu.data_ptr())
@@ -1245,15 +1246,15 @@ class _GatedMlp(torch.autograd.Function):
         f, k = wg.shape
         m, code = x.numel() // k, _SEQ_DTYPES[x.dtype]
         need_x, need_wg, need_wu, need_bg, need_bu, _ = ctx.needs_input_grad
-        new = lambda shape, need: torch.empty(shape, dtype=x.dtype, device=x.device) if need else None  # noqa: E731
-        dx = new(x.shape, need_x)
-        dwg, dwu = (new((f, k), need_wg or need_wu) for _ in range(2))
-        dbg, dbu = new((f,), need_bg), new((f,), need_bu)
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+        dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_wg or need_wu else (None, None)      # (dense, as the weights)
+        dbg = x.new_empty(f) if need_bg else None
+        dbu = x.new_empty(f) if need_bu else None
         if m:
             xr, xs = _seq_rows(x)
             dr, ds = _seq_rows(dh)
             args = (xr.data_ptr(), xs, wg.data_ptr(), wu.data_ptr())
-            ws = _mlp_workspace(_lib.load().motif_gated_mlp_bwd_ws_bytes(*args, m, k, f, code, need_x, dwg is not None, need_bg or need_bu), x, k, f)
+            ws = _mlp_workspace(_lib._lib.motif_gated_mlp_bwd_ws_bytes(*args, m, k, f, code, need_x, dwg is not None, need_bg or need_bu), x, k, f)
             _seq_call("motif_gated_mlp_bwd", x.device, *args, g.data_ptr(), u.data_ptr(), dr.data_ptr(), ds,
                       _seq_ptr(dx), _seq_ptr(dwg), _seq_ptr(dwu), _seq_ptr(dbg), _seq_ptr(dbu), _seq_ptr(ws), m, k, f, ctx.act, code)
         else:
