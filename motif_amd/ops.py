@@ -8,6 +8,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import MotifConvDesc, check
@@ -992,7 +993,7 @@ def frames_f32_to_u8(frames, round_half_even=True, swap_rb=True):
 # ----------------------------------------------------------------------------------------- sequence operators
 # Token-major tensors [..., D], the last axis dense, fp32, bf16 or fp16; statistics, sums and states fp32.  They work on the device and the
 # current stream of their tensors, allocate what they need per call (nothing is shared between calls, streams or captured graphs) and are
-# differentiable once.  Into a HIP graph a backward pass can be captured as any of torch's: while no eager graph of the same leaves lives.
+# differentiable once, backwards (forward mode is refused).  Into a HIP graph a backward pass can be captured as any of torch's: while no eager graph of the same leaves lives.
 _SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -1049,6 +1050,15 @@ def _once():
     """A backward pass that is itself recorded (create_graph=True) would record nothing of what the library computes."""
     if torch.is_grad_enabled():
         raise RuntimeError("motif_amd's sequence operators are differentiable once: their gradients cannot be differentiated (create_graph=True)")
+
+
+def _no_tangents(what, *tensors):
+    """Forward-mode differentiation (torch.autograd.forward_ad, torch.func.jvp) would take an output without a tangent for one whose tangent is zero."""
+    if forward_ad._current_level < 0:                    # outside any dual_level(): no tensor has a tangent
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("%s: has no forward-mode derivative (an input carries a tangent)" % what)
 
 
 def _wants_grad(*tensors):
@@ -1117,6 +1127,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise RuntimeError("%s: the last axis must hold 1 to %d values, got shape %s" % (what, LAYER_NORM_MAX, list(x.shape)))
     _seq_same(weight, x, (d,), what, "weight", (x.dtype, torch.float32))
     _seq_same(bias, x, (d,), what, "bias", (x.dtype, torch.float32) if weight is None else (weight.dtype,))
+    _no_tangents(what, x, weight, bias)
     require_device(x, "layer_norm needs CUDA(ROCm) tensors")
     if _wants_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight if weight is None else _c(weight), bias if bias is None else _c(bias), float(eps))
@@ -1200,6 +1211,7 @@ def gru_scan(z, q, h0=None, cu_seqlens=None):
     if cu_seqlens is not None and (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.device != q.device):
         raise RuntimeError("%s: cu_seqlens must be int32 [S + 1], S >= 1, on %s, got %s %s on %s" % (what, q.device, cu_seqlens.dtype, list(cu_seqlens.shape), cu_seqlens.device))
     _seq_same(h0, q, (q.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1, q.shape[-1]), what, "h0", (torch.float32,))
+    _no_tangents(what, z, q, h0)
     require_device(q, "gru_scan needs CUDA(ROCm) tensors")
     h0 = None if h0 is None else _c(h0)
     cu = None if cu_seqlens is None else _c(cu_seqlens)
@@ -1283,6 +1295,7 @@ def gated_mlp(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
     _seq_same(w_up, x, w_gate.shape, what, "w_up", (x.dtype,))
     _seq_same(b_gate, x, (f,), what, "b_gate", (x.dtype,))
     _seq_same(b_up, x, (f,), what, "b_up", (x.dtype,))
+    _no_tangents(what, x, w_gate, w_up, b_gate, b_up)
     require_device(x, "gated_mlp needs CUDA(ROCm) tensors")
     params = [None if p is None else _c(p) for p in (w_gate, w_up, b_gate, b_up)]
     if _wants_grad(x, *params):

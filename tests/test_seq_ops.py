@@ -104,3 +104,25 @@ def test_the_modules_hold_torchs_parameters(ops):
     for module in (n, m):
         with pytest.raises(RuntimeError, match="CUDA"):
             module(torch.zeros(2, 24))
+
+
+def test_forward_mode_is_refused_wherever_a_tangent_comes_in(ops):
+    """An output without a tangent counts as one whose derivative is zero: a silent wrong answer."""
+    from torch.autograd import forward_ad
+    calls = ((lambda x, w, b: ops.layer_norm(x, w, b), ((4, 8), (8,), (8,))),
+             (lambda z, q, h0: ops.gru_scan(z, q, h0), ((2, 3, 8), (2, 3, 8), (2, 8))),
+             (lambda x, wg, wu, bg, bu: ops.gated_mlp(x, wg, wu, bg, bu), ((4, 8), (5, 8), (5, 8), (5,), (5,))))
+    for call, shapes in calls:
+        tensors = [torch.zeros(s) for s in shapes]
+        for i in range(len(tensors)):
+            with forward_ad.dual_level():
+                duals = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(tensors)]
+                for mode in (torch.enable_grad, torch.no_grad):
+                    with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                        call(*duals)
+                with pytest.raises(RuntimeError, match="CUDA"):          # no tangent: as outside
+                    call(*tensors)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(call, tuple(tensors), tuple(torch.ones_like(t) for t in tensors))
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call(*tensors)
