@@ -461,13 +461,16 @@ __global__ __launch_bounds__(1024) void join_kernel(GemmArgs p) {
 
 // ---- laying operands out -----------------------------------------------------------------------------------------------------------------
 // fp32 as three bf16 parts of 8 bits each, by truncation: x = p0 + p1 + p2 exactly (but for what is below bf16's smallest number).  An infinity or
-// NaN has no further parts: their differences would make other NaNs of it.
+// NaN has no further parts: their differences would make other NaNs of it.  An infinite operand multiplies every part of the other one, and times a
+// part of 0 -- 1, 0.5, any value of few bits has such parts -- it would be a NaN where the product is infinite: a second or third part that comes out as
+// 0 is bf16's smallest normal number of x's sign instead, 2^-36 of x at most (hence only from 2^-90 on: an infinity times less may come out as a NaN).
 __device__ __forceinline__ void split3(float x, bf16_t (&out)[3]) {
     float r = x;
+    const unsigned least = fabsf(x) >= 0x1p-90f ? (__builtin_bit_cast(unsigned, x) & 0x80000000u) | 0x00800000u : 0u;
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
         const unsigned top = __builtin_bit_cast(unsigned, r) & 0xffff0000u;
-        out[i] = __builtin_bit_cast(bf16_t, (unsigned short)(top >> 16));
+        out[i] = __builtin_bit_cast(bf16_t, (unsigned short)((i && top << 1 == 0 ? least : top) >> 16));
         r = (top & 0x7f800000u) == 0x7f800000u ? 0.f : r - __builtin_bit_cast(float, top);
     }
     // a NaN whose payload lies in the lower half only must not become an infinity

@@ -1280,7 +1280,7 @@ def gated_mlp(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
     """Gated feed-forward block act(x w_gate^T + b_gate) * (x w_up^T + b_up) in one kernel; act: "silu", "gelu" (exact) or "sigmoid".
 
     x [..., K], w_gate / w_up [F, K] (nn.Linear's layout), b_gate / b_up [F], all fp32, bf16 or fp16; K, F <= 65536, at most 2^22 rows.  Sums are
-    fp32; fp32 data keep fp32's accuracy on the matrix cores (fp32 instructions, or three exact bf16 parts of every operand; an infinite operand may make its outputs NaN).
+    fp32; fp32 data keep fp32's accuracy on the matrix cores (fp32 instructions, or three exact bf16 parts of every operand; an infinite operand beside one of less than 2^-90 may make its outputs NaN).
     With gradients the two projections are kept in fp32 (8 bytes per output value).  Differentiable in all tensors."""
     what = "gated_mlp"
     _seq_type(x, what, "x")

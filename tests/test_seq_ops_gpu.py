@@ -964,3 +964,40 @@ def test_offsets_beyond_32_bits(ops):
         v = torch.nn.functional.silu(p)
         c = (1024 + 64) * F32
         within(y[-100:], v * q, half_step(torch.bfloat16, v * q) + 1.01 * (1.13 * c * size[0] * q.abs() + c * size[1] * v.abs()) + (20 + 2 * p.abs()) * F32 * (v * q).abs())
+
+
+# ------------------------------------------------------------------------------------------------------------------ infinities and ranges
+def same_kind(got, want):
+    """Infinite, with its sign, or NaN where the 64-bit result is; finite where it is."""
+    got, want = got.detach().double().cpu(), want.double().cpu()
+    for kind in (torch.isnan, lambda t: t == math.inf, lambda t: t == -math.inf):
+        bad = kind(got) != kind(want)
+        assert not bad.any(), (int(bad.sum()), bad.numel(), got[bad][:4], want[bad][:4])
+
+
+@pytest.mark.parametrize("M, K, F", [(40, 200, 600), (500, 64, 96), (2050, 200, 600)], ids=["few rows", "narrow", "tiles"])
+def test_gated_mlp_of_fp32_infinities_come_out_as_they_would_in_fp32(ops, M, K, F):
+    """Whatever the number of rows: an infinite value among finite ones, beside weights of many bits and of few (their lower parts are 0) and of none."""
+    x, wg, wu, bg, bu = mlp_inputs(M, K, F, torch.float32, 31, True)
+    for w in (wg, wu):
+        w[::3] = w[::3].bfloat16().float()
+        w[1::9] = torch.exp2(torch.floor(torch.log2(w[1::9].abs()))) * w[1::9].sign()
+    wu[2, 7] = wg[4, 7] = 0.0
+    x[3, 7], x[M - 1, K - 1], x[17, 0], x[17, 1] = math.inf, -math.inf, math.inf, -math.inf
+    dh = torch.randn(M, F, generator=gen(32), device="cuda")
+    dh[5, 11], dh[M - 2, F - 1] = math.inf, -math.inf
+    for act in ("silu", "gelu", "sigmoid"):
+        leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+        h = ops.gated_mlp(*leaves, bg, bu, act=act)
+        X, WG, WU, DH = (t.double().cpu() for t in (x, wg, wu, dh))
+        G, U = X @ WG.t() + bg.double().cpu(), X @ WU.t() + bu.double().cpu()
+        v, dv = gate_reference(G, act)
+        same_kind(h, v * U)
+        assert torch.isfinite(h[:3]).all() and torch.isinf(h[3]).any()
+        # backward from what the activations give for finite gates; infinite ones have derivatives of inf - inf and 0 x inf
+        finite = torch.isfinite(G).all(1) & torch.isfinite(U).all(1)
+        rows = finite.nonzero()[:, 0]
+        dx, = torch.autograd.grad(h, leaves[:1], dh)
+        dG, dU = (DH * U * dv)[rows], (DH * v)[rows]
+        same_kind(dx[rows.cuda()], dG @ WG + dU @ WU)
+        assert not torch.isfinite(dx[5]).all()
