@@ -470,7 +470,7 @@ __device__ __forceinline__ void split3(float x, bf16_t (&out)[3]) {
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
         const unsigned top = __builtin_bit_cast(unsigned, r) & 0xffff0000u;
-        out[i] = __builtin_bit_cast(bf16_t, (unsigned short)((i && top << 1 == 0 ? least : top) >> 16));
+        out[i] = __builtin_bit_cast(bf16_t, (unsigned short)((i && __builtin_bit_cast(float, top) == 0.f ? least : top) >> 16));
         r = (top & 0x7f800000u) == 0x7f800000u ? 0.f : r - __builtin_bit_cast(float, top);
     }
     // a NaN whose payload lies in the lower half only must not become an infinity
