@@ -434,7 +434,8 @@ long motif_gated_mlp_ws_bytes(const void* x, long x_rs, const void* w_gate, cons
 int motif_gated_mlp_fwd(const void* x, long x_rs, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* h, float* G, float* U,
                         void* workspace, long M, long K, long F, int act, int dtype, void* stream);
 /* Its backward pass from G and U: dx [M, K] dense (may be NULL), dw_gate and dw_up [F, K] (both or neither), db_gate / db_up [F] (either may be
- * NULL).  workspace: motif_gated_mlp_bwd_ws_bytes bytes for the same inputs and the gradients that are wanted. */
+ * NULL).  16-bit types round the projections' gradients to their type once, as operands (fp16: times a power of two where their range asks for it).
+ * workspace: motif_gated_mlp_bwd_ws_bytes bytes for the same inputs and the gradients that are wanted. */
 long motif_gated_mlp_bwd_ws_bytes(const void* x, long x_rs, const void* w_gate, const void* w_up, long M, long K, long F, int dtype, int need_x, int need_w, int need_b);
 int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate, const void* w_up, const float* G, const float* U, const void* dh, long dh_rs,
                         void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* workspace, long M, long K, long F, int act, int dtype, void* stream);

@@ -12,7 +12,9 @@
 // split exactly into three bf16 parts, and the six products that reach fp32's last place are six segments of the reduction.  Operands
 // whose rows are not whole 16-byte pieces are laid out first (layout_kernel).
 // G and U are kept in fp32 for the backward pass: rounded to the data's type they would add an error of their own to every gradient; dG and
-// dU are rounded once, to be operands of the matrix cores.
+// dU are rounded once, to be operands of the matrix cores: to 8 bits (bf16) or 11 (fp16), which makes the 16-bit gradients' rms error 1.4 times what fp32
+// operands would leave (the outputs' own rounding is the rest); fp32 keeps all their bits.  fp16 ends at 65504 and loses bits below 2^-14, where the
+// gradients need not: see scale_of.
 // Up to 64 rows the forward pass is bound by reading the weights (rows_kernel, which small products share); layers of up to 64 inputs hold theirs in registers (narrow_*_kernel).
 // Measured, 8192 x 2048 -> 2 x 5632 bf16: forward 313 us (1.21 PFLOP/s; the library's product of that size alone 352), 400 with G and U written
 // besides (369 MB); dG and dU 147 (646 MB, 4.4 TB/s; past the caches: in them they would push out
@@ -124,6 +126,7 @@ struct GemmArgs {
     long ldg;
     const void *bias0, *bias1;
     f32x4* part;                                         // pieces' accumulators: [tile - whole][piece][accumulator][thread]
+    const float* up;                                     // ONE, TWO: what the outputs are multiplied by; null: 1
     int act, dtype;
 };
 
@@ -222,13 +225,14 @@ struct Store {
     const GemmArgs& p;
     const Tile<C, MODE>& t;
     int m, c, lo, hi;                                    // this wave's first row of A and column of a half; of a fragment: the lane's place
-    float bias[2][2][4];                                 // GATED: [half][j]
+    float bias[2][2][4], up;                             // GATED: [half][j]
     __device__ __forceinline__ Store(const GemmArgs& p_, const Tile<C, MODE>& t_, int wave, int lane) : p(p_), t(t_) {
         constexpr int WN = C / 32;
         m = t.m0 + wave / WN * C;
         c = wave % WN * 32;
         lo = lane & 15;
         hi = (lane >> 4) * 4;
+        up = MODE != GATED && p.up ? *p.up : 1.f;
         if constexpr (MODE == GATED) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
@@ -263,7 +267,7 @@ struct Store {
                 const int rows = MODE == ONE ? p.M : p.N, cols = MODE == ONE ? p.N : p.M, cnt = min(4, cols - col);
                 if (row >= rows || cnt <= 0) continue;
                 const f32x4& o = h ? o1 : o0;
-                const float v[4] = {o[0], o[1], o[2], o[3]};
+                const float v[4] = {o[0] * up, o[1] * up, o[2] * up, o[3] * up};
                 store_as<4>(MODE == ONE || h == 0 ? p.c0 : p.c1, (long)row * cols + col, v, cnt, p.dtype);
             }
         }
@@ -509,14 +513,56 @@ __global__ __launch_bounds__(256) void layout_kernel(const T* __restrict__ src, 
     }
 }
 
+// fp16: dG and dU are made and rounded as they are; where their largest finite value (`peak`) then passes fp16's range, or lies so low that what is 2^-10 of
+// it no longer has all of its bits, they are made again times a power of two that takes the peak to 2^14 .. 2^15, and the products are multiplied by its
+// reciprocal in fp32.  A gradient comes out infinite only where it is, and a small one keeps its bits.  Every workgroup writes its peak; the launch that
+// makes them again reads all of them and ends at once if there is nothing to do: 4 to 9 us (training passes: 1337 x 1000 -> 2 x 2730 114 -> 120 us, 57600 x 64 -> 2 x 256 96 -> 101,
+// 8192 x 2048 -> 2 x 5632 1165 -> 1173; made again: 136, 148).
+template <typename T> constexpr bool kRanged = std::is_same_v<T, f16_t>;
+__device__ __forceinline__ float peak_of(float peak, const float (&g)[8], const float (&u)[8]) {
+    float most = 0.f;                                    // (fmaxf passes NaN by)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(fmaxf(most, fabsf(g[e])), fabsf(u[e]));
+    if (most < HUGE_VALF) return fmaxf(peak, most);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (fabsf(g[e]) < HUGE_VALF) peak = fmaxf(peak, fabsf(g[e]));
+        if (fabsf(u[e]) < HUGE_VALF) peak = fmaxf(peak, fabsf(u[e]));
+    }
+    return peak;
+}
+template <int WAVES>
+__device__ __forceinline__ float peak_in_workgroup(float peak, float* sh) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = peak;
+    __syncthreads();
+    peak = sh[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) peak = fmaxf(peak, sh[i]);
+    return peak;
+}
+// The power of two, from the n peaks that the first launch wrote; its reciprocal to peaks[n].
+template <int WAVES>
+__device__ __forceinline__ float scale_of(float* peaks, int n, float* sh) {
+    float peak = 0.f;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += WAVES * 64) peak = fmaxf(peak, peaks[i]);
+    peak = peak_in_workgroup<WAVES>(peak, sh);
+    int e = 0;
+    if (peak > 65504.f || (peak > 0.f && peak < 0x1p-4f)) e = max(-100, min(100, 14 + 127 - (int)(__builtin_bit_cast(unsigned, peak) >> 23)));
+    if (blockIdx.x == 0 && threadIdx.x == 0) peaks[n] = __builtin_bit_cast(float, (unsigned)(127 - e) << 23);
+    return __builtin_bit_cast(float, (unsigned)(127 + e) << 23);
+}
+
 // dG and dU: [rows][ld], ld = F rounded up to 8 (G and U have it too), zeros behind F; fp32: three planes.  dU lies `pair` elements behind dG.
 // A workgroup takes 256 columns x `rows` rows, eight columns per thread, and sums its columns over its rows (part [row blocks][2][F], may be null).
-template <typename T>
-__global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh, long dhs, const float* __restrict__ G, const float* __restrict__ U, int M, int F, int ld, int act,
-                                                       void* dst, long plane, long pair, float* part, int rows, bool stream) {
+// `id`: the workgroup's place, one of `blocks`.  AGAIN: a workgroup takes several, times scale_of.
+template <typename T, bool AGAIN>
+__device__ __forceinline__ void gate_grad_block(const int id, const float scale, float& peak, float (&sh)[8][2][32][9], const T* __restrict__ dh, long dhs, const float* __restrict__ G,
+                                                const float* __restrict__ U, int M, int F, int ld, int act, void* dst, long plane, long pair, float* part, int rows, bool stream) {
     using O = std::conditional_t<sizeof(T) == 4, bf16_t, T>;
-    __shared__ float sh[8][2][32][9];
-    const int cols = (ld + 255) / 256, cb = blockIdx.x % cols, rb = blockIdx.x / cols;      // neighbouring workgroups take neighbouring columns of the same rows
+    const int cols = (ld + 255) / 256, cb = id % cols, rb = id / cols;      // neighbouring workgroups take neighbouring columns of the same rows
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c0 = cb * 256 + x * 8, c = min(c0, ld - 8);
     const long r0 = (long)rb * rows;
     float sg[8], su[8];
@@ -563,12 +609,14 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
             u[e] = c + e < F ? d[e] * v[e] : 0.f;
             sg[e] += counts ? g[e] : 0.f;
             su[e] += counts ? u[e] : 0.f;
+            if constexpr (AGAIN) { g[e] *= scale; u[e] *= scale; }
         }
+        if constexpr (kRanged<T> && !AGAIN) peak = peak_of(peak, g, u);
         put8((T*)nullptr, dst, plane, r * ld + c, g, stream);
         put8((T*)nullptr, (O*)dst + pair, plane, r * ld + c, u, stream);
         now = next;
     }
-    if (!part) return;
+    if (AGAIN || !part) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e) { sh[y][0][x][e] = sg[e]; sh[y][1][x][e] = su[e]; }
     __syncthreads();
@@ -579,6 +627,23 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh
 #pragma unroll
         for (int q = 0; q < 8; ++q) s += sh[q][k][cx >> 3][cx & 7];
         part[((long)rb * 2 + k) * F + cc] = s;
+    }
+}
+template <typename T, bool AGAIN>
+__global__ __launch_bounds__(256) void gate_grad_kernel(const T* __restrict__ dh, long dhs, const float* __restrict__ G, const float* __restrict__ U, int M, int F, int ld, int act,
+                                                       void* dst, long plane, long pair, float* part, int rows, bool stream, float* peaks, int blocks) {
+    __shared__ float sh[8][2][32][9], waves[4];
+    float peak = 0.f;
+    if constexpr (!AGAIN) {
+        gate_grad_block<T, false>(blockIdx.x, 1.f, peak, sh, dh, dhs, G, U, M, F, ld, act, dst, plane, pair, part, rows, stream);
+        if constexpr (kRanged<T>) {
+            peak = peak_in_workgroup<4>(peak, waves);
+            if (threadIdx.x == 0) peaks[blockIdx.x] = peak;
+        }
+    } else {
+        const float scale = scale_of<4>(peaks, blocks, waves);
+        if (scale == 1.f) return;
+        for (int id = blockIdx.x; id < blocks; id += gridDim.x) gate_grad_block<T, true>(id, scale, peak, sh, dh, dhs, G, U, M, F, ld, act, dst, plane, pair, part, rows, stream);
     }
 }
 
@@ -796,7 +861,14 @@ __global__ __launch_bounds__(256) void narrow_fwd_kernel(const T* __restrict__ x
 template <typename T, int KT, bool DX, bool DW>
 __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x, long xs, const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ dh, long dhs,
                                                          const float* __restrict__ G, const float* __restrict__ U, T* __restrict__ dx, float* __restrict__ dw_part,
-                                                         float* __restrict__ db_part, int M, int K, int F, int act, int nc) {
+                                                         float* __restrict__ db_part, int M, int K, int F, int act, int nc, float* peaks, bool again) {
+    __shared__ float waves[8];
+    float scale = 1.f, peak = 0.f;                       // fp16: see scale_of
+    if constexpr (kRanged<T>) if (again) {
+        scale = scale_of<8>(peaks, gridDim.x, waves);
+        if (scale == 1.f) return;
+    }
+    const float up = 1.f / scale;
     __shared__ __attribute__((aligned(16))) float turn[8][2][32][20];              // [column][row]; 16-byte rows, writes of a wave on all banks
     __shared__ __attribute__((aligned(16))) float shares[DX ? 2 : 1][8][DX ? KT * 4 : 1][68];
     const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -855,9 +927,11 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
         for (int e = 0; e < 8; ++e) {
             g[e] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, nd[e] * nu[e] * d[e]) & keep);
             u[e] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, nd[e] * v[e]) & keep);
+            if constexpr (kRanged<T>) { g[e] *= scale; u[e] *= scale; }
             turn[wave][0][8 * hi + e][lo] = g[e];
             turn[wave][1][8 * hi + e][lo] = u[e];
         }
+        if constexpr (kRanged<T>) peak = peak_of(peak, g, u);
         request(min(r0 + step, M - 1));
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();                 // (a wave's own part of `turn`; the LDS takes a wave's accesses in order)
@@ -913,6 +987,7 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
                     s[0] += at[0];
                     s[1] += at[1];
                 }
+                if constexpr (kRanged<T>) { s[0] *= up; s[1] *= up; }
                 seq_store<T, 2>(dx + (long)(base + m) * K + k, s);
             }
             buf ^= 1;
@@ -923,7 +998,7 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
     for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            float s = db[p][t];
+            float s = db[p][t] * up;
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
             const int f = f0 + 16 * t;
@@ -933,8 +1008,12 @@ __global__ __launch_bounds__(512) void narrow_bwd_kernel(const T* __restrict__ x
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int kt = 0; kt < KT; ++kt)
-                        if (f + 4 * hi + e < F && 16 * kt + lo < K) dw_part[((slot * 2 + p) * F + f + 4 * hi + e) * K + 16 * kt + lo] = dw[p][t][kt][e];
+                        if (f + 4 * hi + e < F && 16 * kt + lo < K) dw_part[((slot * 2 + p) * F + f + 4 * hi + e) * K + 16 * kt + lo] = dw[p][t][kt][e] * up;
         }
+    if constexpr (kRanged<T>) if (!again) {
+        peak = peak_in_workgroup<8>(peak, waves);
+        if (threadIdx.x == 0) peaks[blockIdx.x] = peak;
+    }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------------
@@ -1082,10 +1161,12 @@ void narrow_fwd(const void* x, long xs, const void* wg, const void* wu, const vo
 }
 template <typename T, int KT>
 void narrow_bwd(int grid, const void* x, long xs, const void* wg, const void* wu, const void* dh, long dhs, const float* G, const float* U, void* dx, float* dw_part, float* db_part,
-                int M, int K, int F, int act, hipStream_t s) {
+                float* peaks, int M, int K, int F, int act, hipStream_t s) {
     auto* kernel = dx && dw_part ? narrow_bwd_kernel<T, KT, true, true> : dx ? narrow_bwd_kernel<T, KT, true, false>
                  : dw_part ? narrow_bwd_kernel<T, KT, false, true> : narrow_bwd_kernel<T, KT, false, false>;
-    kernel<<<grid, 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)dh, dhs, G, U, (T*)dx, dw_part, db_part, M, K, F, act, column_runs(F));
+    for (bool again : {false, true})
+        if (!again || (kRanged<T> && (dx || dw_part)))
+            kernel<<<grid, 512, 0, s>>>((const T*)x, xs, (const T*)wg, (const T*)wu, (const T*)dh, dhs, G, U, (T*)dx, dw_part, db_part, M, K, F, act, column_runs(F), peaks, again);
 }
 
 // x, Wg and Wu as the products read them: as they lie, or laid out in the workspace.
@@ -1113,7 +1194,8 @@ void lay_out(const Inputs& f, bool need_x, bool need_w, const void* x, long xs, 
 int grad_rows(long M, long F) { return (long)cdiv(M, 16) * cdiv(F, 256) < 1024 ? 8 : 16; }
 GemmPlan fwd_plan(long M, long K, long F, int dtype, bool keep) { return gemm_plan(M, F, 2, (long)(planes(dtype) == 3 ? 6 : 1) * units_of(K), keep); }
 
-struct Backward { Inputs in; Image dg, du; float* bias_part; f32x4* part; GemmPlan dx, dw; float* dw_part; bool one_pass; };
+int grad_blocks(long M, long F) { return (int)((long)cdiv(M, grad_rows(M, F)) * cdiv(up8(F), 256)); }
+struct Backward { Inputs in; Image dg, du; float *bias_part, *peaks; f32x4* part; GemmPlan dx, dw; float* dw_part; bool one_pass; };
 Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const void* wu, long M, long K, long F, int dtype, bool need_x, bool need_w, bool need_b) {
     Backward b = {};
     const int n = planes(dtype), ld = up8(F);
@@ -1122,6 +1204,7 @@ Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const vo
         const long slots = (long)narrow_groups(M, F) * (8 / column_runs(F));
         if (need_w) b.dw_part = (float*)ws.take(4 * slots * 2 * F * K);
         if (need_b) b.bias_part = (float*)ws.take(4 * slots * 2 * F);
+        if (dtype == MOTIF_F16) b.peaks = (float*)ws.take(4 * (narrow_groups(M, F) + 1));
         return b;
     }
     b.in = inputs_of(ws, x, xs, wg, wu, M, K, F, dtype);
@@ -1131,6 +1214,7 @@ Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const vo
     if (need_x) b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * units_of(ld), false);
     if (need_w) b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * units_of(M), false);
     if (need_b) b.bias_part = (float*)ws.take(4L * cdiv(M, grad_rows(M, F)) * 2 * F);
+    if (dtype == MOTIF_F16) b.peaks = (float*)ws.take(4L * (grad_blocks(M, F) + 1));
     long part = need_x ? part_bytes(b.dx) : 0;           // the two products run one behind the other: one piece of memory serves both
     if (need_w && part_bytes(b.dw) > part) part = part_bytes(b.dw);
     if (part) b.part = (f32x4*)ws.take(part);
@@ -1216,8 +1300,8 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         const int grid = narrow_groups(M, F), slots = grid * (8 / column_runs(F));
         seq_dispatch(dtype, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            if (K <= 32) narrow_bwd<T, 2>(grid, x, x_rs, w_gate, w_up, dh, dh_rs, G, U, dx, b.dw_part, b.bias_part, (int)M, (int)K, (int)F, act, s);
-            else narrow_bwd<T, 4>(grid, x, x_rs, w_gate, w_up, dh, dh_rs, G, U, dx, b.dw_part, b.bias_part, (int)M, (int)K, (int)F, act, s);
+            if (K <= 32) narrow_bwd<T, 2>(grid, x, x_rs, w_gate, w_up, dh, dh_rs, G, U, dx, b.dw_part, b.bias_part, b.peaks, (int)M, (int)K, (int)F, act, s);
+            else narrow_bwd<T, 4>(grid, x, x_rs, w_gate, w_up, dh, dh_rs, G, U, dx, b.dw_part, b.bias_part, b.peaks, (int)M, (int)K, (int)F, act, s);
         });
         MOTIF_LAUNCH_CHECK();
         const int r = need_w ? seq_colsum2(b.dw_part, slots, F * K, dw_gate, dw_up, dtype, s) : MOTIF_OK;
@@ -1227,8 +1311,13 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
     seq_dispatch(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const int rows = grad_rows(M, F);
-        const unsigned grid = (unsigned)((long)cdiv(M, rows) * cdiv(b.dg.ld, 256));
-        gate_grad_kernel<T><<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows, 4 * b.dg.plane * b.dg.n >= kSeqStream);
+        const int blocks = grad_blocks(M, F);
+        auto launch = [&](auto* kernel, int grid) {
+            kernel<<<grid, 256, 0, s>>>((const T*)dh, dh_rs, G, U, (int)M, (int)F, b.dg.ld, act, (void*)b.dg.p, b.dg.plane, b.dg.plane * b.dg.n, b.bias_part, rows, 4 * b.dg.plane * b.dg.n >= kSeqStream,
+                                        b.peaks, blocks);
+        };
+        launch(gate_grad_kernel<T, false>, blocks);
+        if constexpr (kRanged<T>) if (need_x || need_w) launch(gate_grad_kernel<T, true>, blocks < 256 ? blocks : 256);
     });
     if (need_b) {
         const int r = seq_colsum2(b.bias_part, cdiv(M, grad_rows(M, F)), F, db_gate, db_up, dtype, s);
@@ -1243,6 +1332,7 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         g.units = units_of(b.dg.ld);
         g.M = (int)M; g.N = (int)K; g.wb = up8(K);
         g.c0 = dx; g.dtype = dtype;
+        g.up = b.peaks ? b.peaks + grad_blocks(M, F) : nullptr;
         g.part = b.part;
         gemm_dtype<ONE>(dtype, b.dx, g, s);
     }
@@ -1254,6 +1344,7 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
         g.units = units_of(M);
         g.M = (int)K; g.N = (int)F; g.wa = up8(K); g.wb = b.dg.ld;
         g.c0 = dw_gate; g.c1 = dw_up; g.dtype = dtype;
+        g.up = b.peaks ? b.peaks + grad_blocks(M, F) : nullptr;
         g.part = b.part;
         gemm_dtype<TWO>(dtype, b.dw, g, s);
     }

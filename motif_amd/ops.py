@@ -1281,7 +1281,9 @@ def gated_mlp(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
 
     x [..., K], w_gate / w_up [F, K] (nn.Linear's layout), b_gate / b_up [F], all fp32, bf16 or fp16; K, F <= 65536, at most 2^22 rows.  Sums are
     fp32; fp32 data keep fp32's accuracy on the matrix cores (fp32 instructions, or three exact bf16 parts of every operand; an infinite operand beside one of less than 2^-90 may make its outputs NaN).
-    With gradients the two projections are kept in fp32 (8 bytes per output value).  Differentiable in all tensors."""
+    With gradients the two projections are kept in fp32 (8 bytes per output value).  Backward, 16-bit types round the gradients of the projections to
+    x's type once, as operands of the matrix cores; in fp16 they are scaled by a power of two where their range asks for it, so that gradients are infinite only
+    where their own value is.  Differentiable in all tensors."""
     what = "gated_mlp"
     _seq_type(x, what, "x")
     if act not in _GATES:

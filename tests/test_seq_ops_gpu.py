@@ -1001,3 +1001,102 @@ def test_gated_mlp_of_fp32_infinities_come_out_as_they_would_in_fp32(ops, M, K, 
         dG, dU = (DH * U * dv)[rows], (DH * v)[rows]
         same_kind(dx[rows.cuda()], dG @ WG + dU @ WU)
         assert not torch.isfinite(dx[5]).all()
+
+
+def mlp_ranges_check(ops, x, wg, wu, dh, act):
+    """mlp_check's bounds of dx, dWg and dWu for fp16 gradients of any size.  dG and dU are rounded once: by 2^-11 of their value, and of no less than
+    2^-14 where their largest value P lies in 2^-4 .. 65504, of no less than 2^-28 P elsewhere (a power of two takes P to 2^14 and more)."""
+    M, K, F = x.shape[0], x.shape[1], wg.shape[0]
+    leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+    h = ops.gated_mlp(*leaves, act=act)
+    got = torch.autograd.grad(h, leaves, dh)
+    X, WG, WU, DH = (t.double() for t in (x, wg, wu, dh))
+    G, U = X @ WG.t(), X @ WU.t()
+    c = lambda n: (n + 64) * F32  # noqa: E731
+    eG, eU = c(K) * (X.abs() @ WG.abs().t()), c(K) * (X.abs() @ WU.abs().t())
+    v, dv = gate_reference(G, act)
+    rel = (16 + 2 * G.abs()) * F32
+    ev = 1.13 * eG + rel * v.abs() + (16 * F32 * G.abs() if act == "gelu" else 0)
+    edv = eG + rel * (dv.abs() + 1)
+    dG, dU = DH * U * dv, DH * v
+    edG = DH.abs() * (eU * dv.abs() + edv * U.abs() + eU * edv) + 4 * F32 * dG.abs()
+    edU = DH.abs() * ev + 4 * F32 * dU.abs()
+    peak = max(float(dG.abs().max()), float(dU.abs().max()))
+    least = 2.0 ** -14 if 2.0 ** -4 <= peak <= 65504 else 2.0 ** -28 * peak
+    step = lambda t: 2.0 ** -11 * t.clamp_min(least)  # noqa: E731
+    rG, rU = edG + 1.01 * step(dG.abs() + edG), edU + 1.01 * step(dU.abs() + edU)
+    want = [dG @ WG + dU @ WU, dG.t() @ X, dU.t() @ X]
+    tol = [rG @ WG.abs() + rU @ WU.abs() + c(2 * F) * (dG.abs() @ WG.abs() + dU.abs() @ WU.abs())]
+    tol += [r.t() @ X.abs() + c(M) * (d.abs().t() @ X.abs()) for d, r in ((dG, rG), (dU, rU))]
+    sizes = []
+    for a, w, t in zip(got, want, tol):
+        t = half_step(torch.float16, w) + 1.01 * t
+        inside, outside = w.abs() + t < 65504, w.abs() - t > 65520
+        within(torch.where(inside, a.double(), 0), torch.where(inside, w, 0), t)
+        assert torch.equal(a[outside].double(), torch.sign(w[outside]) * math.inf), "gradients that do not fit are infinite"
+        sizes.append(float(inside.double().mean()))
+    return peak, sizes
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("M, K, F", [(40, 200, 600), (2050, 200, 600), (1500, 333, 1030), (700, 64, 96), (1000, 20, 256)])
+def test_gated_mlp_of_fp16_gradients_of_any_size(ops, M, K, F, act):
+    """The products dh U and dh act(G) pass fp16's range, or lie below its normal numbers, where the gradients made of them do not: in tiles, in the
+    narrow layers' one pass."""
+    g = gen(M + K + F)
+    n = lambda *s, scale=1.0: (torch.randn(*s, generator=g, device="cuda") * scale).half()  # noqa: E731
+    # (x, weights, dh): G and U of about 1 to 30; peaks beyond 65504 with finite dx, with finite dW; far below 2^-4
+    for x, w, dh, finite in ((2.0 ** 11, 2.0 ** -6, 8192.0, 0), (2.0 ** -9, 2.0 ** 14, 8192.0, 1), (1.0, 1.0, 2.0 ** -17, 0), (1.0, 1.0, 2.0 ** -11, 1)):
+        peak, sizes = mlp_ranges_check(ops, n(M, K, scale=x), n(F, K, scale=w * K ** -0.5), n(F, K, scale=w * K ** -0.5), n(M, F, scale=dh), act)
+        assert (peak > 65504) == (dh > 1) and sizes[finite] > 0.99, (peak, sizes)
+    # one gradient far above the others: they keep what fp16 numbers beside it keep
+    dh = n(M, F, scale=2.0 ** -6)
+    dh[3, 5] = 60000.0
+    mlp_ranges_check(ops, n(M, K, scale=4.0), n(F, K, scale=4 * K ** -0.5), n(F, K, scale=K ** -0.5), dh, act)
+
+
+def test_gated_mlp_of_fp16_bad_gradients_stay_in_their_rows(ops):
+    """An infinite or NaN gradient is no measure of the others, and biases are summed from what was not rounded."""
+    for M, K, F in ((300, 136, 200), (300, 36, 72)):
+        x, wg, wu, bg, bu = mlp_inputs(M, K, F, torch.float16, 6, True)
+        dh = torch.randn(M, F, generator=gen(7), device="cuda").half()
+
+        def step(dh):
+            leaves = [t.detach().requires_grad_() for t in (x, bg, bu)]
+            return torch.autograd.grad(ops.gated_mlp(leaves[0], wg, wu, *leaves[1:]), leaves, dh)
+        want = step(dh)
+        bad = dh.clone()
+        bad[3, 7], bad[299, 35] = math.inf, math.nan
+        got = step(bad)
+        rest = [i for i in range(300) if i not in (3, 299)]
+        assert torch.equal(got[0][rest], want[0][rest]) and not torch.isfinite(got[0][3]).all() and torch.isnan(got[0][299]).all()
+        keep = [f for f in range(F) if f not in (7, 35)]
+        assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got[1:], want[1:]))
+
+
+def test_gated_mlp_of_fp16_gradients_of_any_size_in_a_graph(ops):
+    """The same captured step serves gradients of every size: what they need is found on the device."""
+    for M, K, F in ((300, 136, 200), (300, 36, 72)):
+        leaves = [t.requires_grad_() for t in mlp_inputs(M, K, F, torch.float16, 8, True)]
+        dh = torch.randn(M, F, generator=gen(9), device="cuda").half()
+
+        def step():
+            h = ops.gated_mlp(*leaves)
+            return (h.detach(),) + torch.autograd.grad(h, leaves, dh)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = step()
+        for scale in (1.0, 2.0 ** -18, 20000.0, 1.0, 2.0 ** -10):
+            with torch.no_grad():
+                dh.copy_(torch.randn(M, F, generator=gen(10), device="cuda") * scale)
+            for t in held:
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(held, step())), scale
+            torch.cuda.synchronize()
