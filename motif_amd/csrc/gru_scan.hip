@@ -33,7 +33,7 @@ struct ScanArgs {
     const int* info;                                     // packed rows: owner << 2 | last << 1 | first, -1: no sequence's row.  null: B sequences of T rows
     long zb, zr, qb, qr, db, dr;                         // batch and row strides of z, q, dh; h, out0 and out1 are dense
     long T, seg_rows;
-    int B, D, groups, segs;
+    int B, D, groups, segs;                              // groups: workgroups that share a batch's channels, TY = 1: lanes
     bool stream;
 };
 
@@ -184,9 +184,11 @@ template <typename T, int V, int TX, int TY, int R, bool BWD, bool PACKED>
 __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
     using S = Slots<V, TX, TY>;
     __shared__ typename S::Sums sums[2];
-    const Where at = where(p);
-    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, first = (at.group * TX + tx) * V, c0 = min(first, p.D - V);
-    // (the last lanes of a row take its last V channels: those they share are written more than once, alike)
+    // TY = 1: the lanes of all batches one behind the other, `groups` to a batch (host: below 2^32 in all; those behind the last do its work again, and write alike)
+    const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
+    const unsigned n = min(blockIdx.x * 256u + threadIdx.x, (unsigned)p.B * (unsigned)p.groups - 1u);
+    const Where at = TY == 1 ? Where{(int)(n % (unsigned)p.groups), 0, (long)(n / (unsigned)p.groups)} : where(p);
+    const int c0 = min((TY == 1 ? at.group : at.group * TX + tx) * V, p.D - V);      // (the last lanes of a row take its last V channels: those they share are written more than once, alike)
     // Addresses: a uniform row of the tile, and a lane's offset from it in bytes (32 bits: the host bounds the strides where TY > 1).  Backward, time
     // runs down: slot TY - 1 has the tile's first rows.
     const int slot = (BWD ? TY - 1 - ty : ty) * R;
@@ -348,11 +350,15 @@ __global__ __launch_bounds__(256) void gru_scan_rows_kernel(const int* __restric
     info[t] = (s << 2) | (cu[s] == t ? kFirst : 0) | (min(cu[s + 1], rows) == t + 1 ? kLast : 0);
 }
 
-struct Plan { int V, TX, TY, R, groups, segs; long seg_rows; };
+struct Plan { int V, TX, TY, R, groups, segs; long seg_rows, workgroups; };
+constexpr long kMostGroups = (1L << 24) - 1;             // a grid holds less than 2^32 threads
 
-// Vectors of 16 bytes, single values for rows shorter than that.  TY = 1 (a lane walks the whole sequence) where the
-// sequence is no longer than 16 rows or the channels alone give every CU two workgroups; else 16 time slots, rows of 256 bytes (8 with single values, whose
-// rows need more lanes to fill a cache line).  Segments: as many as the chip holds workgroups of the second kernel at once -- three to a CU forward, four
+// Vectors of 16 bytes, single values for rows shorter than that.  TY = 1 (a lane walks the whole sequence, the lanes of all batches side by side) where the
+// sequence is no longer than 16 rows or the channels alone would give every CU 16 workgroups of time slots; else 16 time slots, rows of 256 bytes (8 with single
+// values, whose rows need more lanes to fill a cache line).  What counts are lanes that hold channels (training steps, us, slots or lanes): 512 x 8192 x 16 bf16, two
+// lanes to a batch, 1495 or 8950; 512 x 4096 x 64 738 or 6190; 300 x 1000 x 1000 fp16 1530 or 2025; at the bound 512 x 24 x 1024 81 or 45, 512 x 100 x 1024 213 or 226,
+// 512 x 2000 x 1000 fp32 11200 or 7730; 20000 x 100 x 8 fp32 337 or 205.  Rows of 64 lanes and more start at a multiple of 16, whole 256 bytes.
+// Segments: as many as the chip holds workgroups of the second kernel at once -- three to a CU forward, four
 // backward, by their registers --, none below two tiles (65536 x 1024 bf16, forward: 74 us with 768 workgroups, 85 us with 1024; backward:
 // 212 with 768, 166 with 1024, 184 with 768 of two rows a slot).
 int vec_of(int dtype, long D) { const int V = 16 / seq_size(dtype); return D < V ? 1 : V; }
@@ -360,27 +366,33 @@ Plan plan_of(int V, long B, long T, long D, bool bwd) {
     Plan p;
     p.V = V;
     const long lanes = (D + V - 1) / V;
-    const bool serial = T <= 16 || B * ((lanes + 255) / 256) >= 512;
-    p.TY = serial ? 1 : V > 1 ? 16 : 8;
+    p.TY = V > 1 ? 16 : 8;
     p.TX = 256 / p.TY;
     p.R = 4;
-    p.groups = (int)((lanes + p.TX - 1) / p.TX);
     p.segs = 1;
     p.seg_rows = T;
-    if (!serial) {
-        const long tile = (long)p.TY * p.R, tiles = (T + tile - 1) / tile;
-        long segs = (bwd ? 1024 : 768) / (B * p.groups);
-        segs = segs < 1 ? 1 : segs > 128 ? 128 : segs;
-        const long per = segs < 2 ? tiles : (tiles + segs - 1) / segs < 2 ? 2 : (tiles + segs - 1) / segs;
-        p.segs = (int)((tiles + per - 1) / per);
-        p.seg_rows = per * tile;
+    const long groups = (lanes + p.TX - 1) / p.TX;
+    if (T <= 16 || B * groups * p.TX >= 256 * 256) {
+        p.TY = 1;
+        p.TX = 256;
+        p.groups = (int)(lanes < 64 ? lanes : (lanes + 15) / 16 * 16);
+        p.workgroups = (B * p.groups + 255) / 256;
+        return p;
     }
+    p.groups = (int)groups;
+    const long tile = (long)p.TY * p.R, tiles = (T + tile - 1) / tile;
+    long segs = (bwd ? 1024 : 768) / (B * groups);
+    segs = segs < 1 ? 1 : segs > 128 ? 128 : segs;
+    const long per = segs < 2 ? tiles : (tiles + segs - 1) / segs < 2 ? 2 : (tiles + segs - 1) / segs;
+    p.segs = (int)((tiles + per - 1) / per);
+    p.seg_rows = per * tile;
+    p.workgroups = B * p.segs * groups;
     return p;
 }
 
 template <typename T, int V, bool BWD, bool PACKED>
 void launch(const Plan& pl, const ScanArgs& a, hipStream_t s) {
-    const unsigned grid = (unsigned)((long)a.B * pl.segs * pl.groups);
+    const unsigned grid = (unsigned)pl.workgroups;
     constexpr int TY = V > 1 ? 16 : 8, R = BWD ? 1 : PACKED ? 2 : 4;      // registers: backward holds four tensors, packed rows their meaning and a second start
     if (pl.TY == 1) { gru_scan_kernel<T, V, 256, 1, R, BWD, PACKED><<<grid, 256, 0, s>>>(a); return; }
     if (pl.segs > 1) gru_scan_segments_kernel<T, V, 256 / TY, TY, BWD, PACKED><<<grid, 256, 0, s>>>(a);
@@ -400,7 +412,7 @@ long cut_floats(const Plan& p, bool packed) { return packed && p.segs > 1 ? (p.s
 int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const float* empty_in, hipStream_t s) {
     const int V = vec_of(dtype, a.D);
     const Plan pl = plan_of(V, a.B, a.T, a.D, bwd);
-    if ((long)a.B * pl.segs * pl.groups > 0x7fffffffL) return MOTIF_ELIMIT;
+    if (pl.workgroups > kMostGroups) return MOTIF_ELIMIT;
     if (pl.TY > 1) for (long stride : {a.zr, a.qr, a.dr, (long)a.D}) if (stride > 1L << 22) return MOTIF_ELIMIT;      // 128 rows x 4 bytes in 32 bits
     a.groups = pl.groups;
     a.segs = pl.segs;

@@ -126,3 +126,14 @@ def test_forward_mode_is_refused_wherever_a_tangent_comes_in(ops):
             torch.func.jvp(call, tuple(tensors), tuple(torch.ones_like(t) for t in tensors))
         with pytest.raises(RuntimeError, match="CUDA"):
             call(*tensors)
+
+
+def test_gru_scan_gives_time_slots_to_few_channels_whatever_their_number_of_batches(lib):
+    """Long sequences are walked by one lane per channel only where channels are many; a workspace (of segments) means time slots.  What a grid cannot hold is
+    refused."""
+    ws = lib.motif_gru_scan_ws_floats
+    for B in (1, 100, 511, 512):                          # (beyond, one segment to a batch fills the chip)
+        assert ws(B, 8192, 16, 0, 1) > 0, B
+    assert ws(512, 65536, 1024, 0, 1) == 0 and ws(1, 4096, 1 << 20, 0, 0) == 0
+    fwd = lambda B, T, D: lib.motif_gru_scan_fwd(P, T * D, D, P, T * D, D, None, None, 0, P, P, P, B, T, D, 0, None)  # noqa: E731
+    assert fwd(1 << 25, 1, 1024) == fwd((1 << 29) - 1, 2, 40) == ELIMIT

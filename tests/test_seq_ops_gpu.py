@@ -1100,3 +1100,15 @@ def test_gated_mlp_of_fp16_gradients_of_any_size_in_a_graph(ops):
             torch.cuda.synchronize()
             assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(held, step())), scale
             torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B, T, D", [(512, 300, 16), (511, 300, 16), (512, 130, 64), (4097, 16, 8), (70000, 1, 3), (20000, 20, 3), (20000, 20, 8), (700, 33, 1000), (520, 18, 1020),
+                                     (3000, 7, 257), (257, 100, 1024), (1000, 70, 200)])
+def test_gru_scan_of_many_batches(ops, dtype, B, T, D):
+    """Many sequences of few channels: time slots, or lanes of several batches in one wave; runs that end within a batch's last lanes."""
+    z, q, h0 = scan_inputs((B, T, D), B, dtype, B + T + D)
+    scan_check(ops, z, q, h0)
+    # as a slice of a larger tensor, time first: batch strides that differ from one another's
+    big, _, _ = scan_inputs((T, B, D + 5), B, dtype, 3)
+    scan_check(ops, big[..., 3:3 + D].transpose(0, 1), q, None)
