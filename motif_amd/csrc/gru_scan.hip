@@ -329,14 +329,16 @@ __global__ __launch_bounds__(256) void gru_scan_kernel(ScanArgs p) {
 }
 
 // Packed rows: what each row is.  cu [S + 1] need not be sound for memory's sake: an owner is always one of the S sequences, and a sequence that
-// would pass the last row ends there.  The workgroups behind those of the rows take an empty sequence each: its state, which no row carries, is
-// out = in (or 0).
+// would pass the last row ends there, one that would begin before the first row begins with it.  The workgroups behind those of the rows share the empty
+// sequences: their states, which no row carries, are out = in (or 0).
 __global__ __launch_bounds__(256) void gru_scan_rows_kernel(const int* __restrict__ cu, int S, int rows, int* __restrict__ info, int D, const float* __restrict__ in, float* __restrict__ out) {
     const long t = (long)blockIdx.x * 256 + threadIdx.x;
-    const int empty = blockIdx.x - (rows + 255) / 256;
-    if (empty >= 0) {
-        if (min(cu[empty + 1], rows) > cu[empty]) return;
-        for (long c = threadIdx.x; c < D; c += 256) out[(long)empty * D + c] = in ? in[(long)empty * D + c] : 0.f;
+    const int row_groups = (rows + 255) / 256;
+    if ((int)blockIdx.x >= row_groups) {
+        for (int s = blockIdx.x - row_groups; s < S; s += gridDim.x - row_groups) {
+            if (min(cu[s + 1], rows) > max(cu[s], 0)) continue;
+            for (long c = threadIdx.x; c < D; c += 256) out[(long)s * D + c] = in ? in[(long)s * D + c] : 0.f;
+        }
         return;
     }
     if (t >= rows) return;
@@ -347,11 +349,12 @@ __global__ __launch_bounds__(256) void gru_scan_rows_kernel(const int* __restric
     }
     const int s = lo - 1;
     if (s < 0 || s >= S) { info[t] = -1; return; }
-    info[t] = (s << 2) | (cu[s] == t ? kFirst : 0) | (min(cu[s + 1], rows) == t + 1 ? kLast : 0);
+    info[t] = (s << 2) | (max(cu[s], 0) == t ? kFirst : 0) | (min(cu[s + 1], rows) == t + 1 ? kLast : 0);
 }
 
 struct Plan { int V, TX, TY, R, groups, segs; long seg_rows, workgroups; };
 constexpr long kMostGroups = (1L << 24) - 1;             // a grid holds less than 2^32 threads
+constexpr int kEmptyGroups = 1 << 20;                    // of the empty sequences, besides those of up to 2^31 rows
 
 // Vectors of 16 bytes, single values for rows shorter than that.  TY = 1 (a lane walks the whole sequence, the lanes of all batches side by side) where the
 // sequence is no longer than 16 rows or the channels alone would give every CU 16 workgroups of time slots; else 16 time slots, rows of 256 bytes (8 with single
@@ -422,7 +425,7 @@ int run(bool bwd, int dtype, ScanArgs a, const int* cu, int S, float* ws, const 
     if (cu) {
         a.cuts = (int*)(ws + agg_floats(pl, a.B, a.D));
         int* info = (int*)(ws + agg_floats(pl, a.B, a.D) + cut_floats(pl, true));
-        const unsigned grid = (unsigned)cdiv(a.T, 256) + (a.state ? S : 0);
+        const unsigned grid = (unsigned)cdiv(a.T, 256) + (a.state ? S < kEmptyGroups ? S : kEmptyGroups : 0);
         if (grid) gru_scan_rows_kernel<<<grid, 256, 0, s>>>(cu, S, (int)a.T, info, a.D, empty_in, a.state);
         a.info = info;
     }

@@ -1201,7 +1201,7 @@ def gru_scan(z, q, h0=None, cu_seqlens=None):
 
     z (a gate: 0 .. 1), q: [B, T, D], fp32 / bf16 / fp16, any batch and row strides; h0: fp32 [B, D] (None: zeros).  Returns (h like q, the last states fp32 [B, D]);
     the states can be handed to the next call: a sequence may come in pieces, down to single rows.  With cu_seqlens -- int32 [S + 1] on the device,
-    not decreasing from 0 on; what lies behind T counts as T -- z and q are [T, D] with S sequences packed one behind the other, h0 and the last states [S, D]; an empty
+    not decreasing; what lies before 0 counts as 0, behind T as T -- z and q are [T, D] with S sequences packed one behind the other, h0 and the last states [S, D]; an empty
     sequence keeps its state, and rows that no sequence covers come out as zeros, whatever they hold.  Differentiable in z, q and h0."""
     what = "gru_scan"
     _seq_type(q, what, "q")

@@ -1112,3 +1112,25 @@ def test_gru_scan_of_many_batches(ops, dtype, B, T, D):
     # as a slice of a larger tensor, time first: batch strides that differ from one another's
     big, _, _ = scan_inputs((T, B, D + 5), B, dtype, 3)
     scan_check(ops, big[..., 3:3 + D].transpose(0, 1), q, None)
+
+
+def test_gru_scan_of_very_many_packed_sequences_and_of_bounds_before_the_first_row(ops):
+    """More sequences than a grid holds workgroups, nearly all of them empty; and bounds below 0, which count as 0."""
+    S, T, D = 17 << 20, 40, 2
+    cu = torch.zeros(S + 1, dtype=torch.int32, device="cuda")
+    cu[5:], cu[S // 2:], cu[S:] = 7, 30, 38
+    z, q, _ = scan_inputs((T, D), 1, torch.float32, 51)
+    h0 = torch.randn(S, D, generator=gen(52), device="cuda")
+    with torch.no_grad():
+        h, last = ops.gru_scan(z, q, h0, cu_seqlens=cu)
+        rows = [4, S // 2 - 1, S - 1]                    # 0 .. 6, 7 .. 29, 30 .. 37
+        want, end = ops.gru_scan(z, q, h0[rows].contiguous(), cu_seqlens=torch.tensor([0, 7, 30, 38], dtype=torch.int32, device="cuda"))
+        assert torch.equal(h, want) and torch.equal(last[rows], end)
+        keep = torch.ones(S, dtype=torch.bool, device="cuda")
+        keep[rows] = False
+        assert torch.equal(last[keep], h0[keep])
+        del keep, last
+        h0 = h0[:4].contiguous()
+        got = ops.gru_scan(z, q, h0, cu_seqlens=torch.tensor([-9, -3, 12, 12, 40], dtype=torch.int32, device="cuda"))
+        want = ops.gru_scan(z, q, h0, cu_seqlens=torch.tensor([0, 0, 12, 12, 40], dtype=torch.int32, device="cuda"))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
