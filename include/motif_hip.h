@@ -440,6 +440,10 @@ long motif_gated_mlp_bwd_ws_bytes(const void* x, long x_rs, const void* w_gate, 
 int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate, const void* w_up, const float* G, const float* U, const void* dh, long dh_rs,
                         void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* workspace, long M, long K, long F, int act, int dtype, void* stream);
 
+/* Which tiles a product of these calls runs in: 256 or 128 rows a tile, 0 where another kernel takes it (few rows, small products, narrow layers).  product: 0
+ * forward, 1 forward with G and U, 2 dx, 3 the weights' gradients.  For tests and measurements: it launches nothing. */
+int motif_gated_mlp_tile(const void* x, long x_rs, const void* w_gate, const void* w_up, long M, long K, long F, int dtype, int product);
+
 #ifdef __cplusplus
 }
 #endif

@@ -83,6 +83,7 @@ _SIGS = {
     "motif_gated_mlp_ws_bytes": (c_long, [P, c_long, P, P, c_long, c_long, c_long, c_int]),
     "motif_gated_mlp_fwd": (c_int, [P, c_long, P, P, P, P, P, P, P, P, c_long, c_long, c_long, c_int, c_int, P]),
     "motif_gated_mlp_bwd_ws_bytes": (c_long, [P, c_long, P, P, c_long, c_long, c_long, c_int, c_int, c_int, c_int]),
+    "motif_gated_mlp_tile": (c_int, [P, c_long, P, P, c_long, c_long, c_long, c_int, c_int]),
     "motif_gated_mlp_bwd": (c_int, [P, c_long, P, P, P, P, P, c_long, P, P, P, P, P, P, c_long, c_long, c_long, c_int, c_int, P]),
 }
 ABI_VERSION = 9          # include/motif_hip.h / api.hip: motif_abi_version()

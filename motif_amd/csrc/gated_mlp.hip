@@ -1192,7 +1192,10 @@ void lay_out(const Inputs& f, bool need_x, bool need_w, const void* x, long xs, 
 // Rows of a workgroup of gate_grad_kernel: 16 -- the last round of many short workgroups leaves little of the chip idle (8192 x 5632 bf16 from memory: 147 us,
 // 161 with 64 rows, whose column sums cost 5 us less; whole backward passes 0 to 2 % shorter) --, 8 where that would leave less than four per CU.
 int grad_rows(long M, long F) { return (long)cdiv(M, 16) * cdiv(F, 256) < 1024 ? 8 : 16; }
-GemmPlan fwd_plan(long M, long K, long F, int dtype, bool keep) { return gemm_plan(M, F, 2, (long)(planes(dtype) == 3 ? 6 : 1) * units_of(K), keep); }
+long products(int dtype) { return planes(dtype) == 3 ? 6 : 1; }
+GemmPlan fwd_plan(long M, long K, long F, int dtype, bool keep) { return gemm_plan(M, F, 2, products(dtype) * units_of(K), keep); }
+GemmPlan dx_plan(long M, long K, long F, int dtype) { return gemm_plan(M, K, 1, 2 * products(dtype) * units_of(F), false); }
+GemmPlan dw_plan(long M, long K, long F, int dtype) { return gemm_plan(K, F, 2, products(dtype) * units_of(M), false); }
 
 int grad_blocks(long M, long F) { return (int)((long)cdiv(M, grad_rows(M, F)) * cdiv(up8(F), 256)); }
 struct Backward { Inputs in; Image dg, du; float *bias_part, *peaks; f32x4* part; GemmPlan dx, dw; float* dw_part; bool one_pass; };
@@ -1211,8 +1214,8 @@ Backward backward_of(Arena& ws, const void* x, long xs, const void* wg, const vo
     char* p = (char*)ws.take(2L * 2 * n * M * ld);
     b.dg = {p, M * ld, ld, n};
     b.du = {p ? p + 2L * n * M * ld : nullptr, M * ld, ld, n};
-    if (need_x) b.dx = gemm_plan(M, K, 1, (long)(n == 3 ? 12 : 2) * units_of(ld), false);
-    if (need_w) b.dw = gemm_plan(K, F, 2, (long)(n == 3 ? 6 : 1) * units_of(M), false);
+    if (need_x) b.dx = dx_plan(M, K, F, dtype);
+    if (need_w) b.dw = dw_plan(M, K, F, dtype);
     if (need_b) b.bias_part = (float*)ws.take(4L * cdiv(M, grad_rows(M, F)) * 2 * F);
     if (dtype == MOTIF_F16) b.peaks = (float*)ws.take(4L * (grad_blocks(M, F) + 1));
     long part = need_x ? part_bytes(b.dx) : 0;           // the two products run one behind the other: one piece of memory serves both
@@ -1350,4 +1353,17 @@ extern "C" int motif_gated_mlp_bwd(const void* x, long x_rs, const void* w_gate,
     }
     MOTIF_LAUNCH_CHECK();
     return MOTIF_OK;
+}
+
+extern "C" int motif_gated_mlp_tile(const void* x, long x_rs, const void* w_gate, const void* w_up, long M, long K, long F, int dtype, int product) {
+    const int rc = check_mlp(M, K, F, MOTIF_GATE_SILU, dtype);
+    if (rc || product < 0 || product > 3) return rc ? rc : MOTIF_EINVAL;
+    if (product < 2) {
+        Arena ws = {nullptr, 0};
+        const Inputs f = inputs_of(ws, x, x_rs, w_gate, w_up, M, K, F, dtype);
+        if ((M > kFewRows && narrow(K, F)) || few(M, K, F, dtype, f.lay_x || f.lay_w)) return 0;
+        return fwd_plan(M, K, F, dtype, product == 1).big ? 256 : 128;
+    }
+    if (narrow_bwd(K, F)) return 0;
+    return (product == 2 ? dx_plan(M, K, F, dtype) : dw_plan(M, K, F, dtype)).big ? 256 : 128;
 }

@@ -1134,3 +1134,71 @@ def test_gru_scan_of_very_many_packed_sequences_and_of_bounds_before_the_first_r
         got = ops.gru_scan(z, q, h0, cu_seqlens=torch.tensor([-9, -3, 12, 12, 40], dtype=torch.int32, device="cuda"))
         want = ops.gru_scan(z, q, h0, cu_seqlens=torch.tensor([0, 0, 12, 12, 40], dtype=torch.int32, device="cuda"))
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------------------------ every tile of every type
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M, K, F, act, bias", [(8190, 2040, 5624, "silu", False), (1100, 2040, 4088, "gelu", True), (1100, 2041, 4085, "sigmoid", True)])
+def test_gated_mlp_weights_gradients_in_large_tiles(ops, dtype, M, K, F, act, bias):
+    """The 256 x 256 tiles of the weights' gradients in every type: ends inside a tile on every axis, operands as they lie and laid out, whole and cut along the
+    reduction (8190: 352 tiles, 96 behind the last whole round of the chip)."""
+    from motif_amd import _lib
+    x, wg, wu, bg, bu = mlp_inputs(M, K, F, dtype, 61, bias)
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    tile = [_lib.load().motif_gated_mlp_tile(x.data_ptr(), K, wg.data_ptr(), wu.data_ptr(), M, K, F, code, product) for product in range(4)]
+    assert tile[3] == 256 and (M < 8190 or tile == [256] * 4), tile
+    mlp_check(ops, x, wg, wu, bg, bu, act)
+
+
+def one_hot_rows(rows, cols, place, value):
+    t = torch.zeros(rows, cols, device="cuda")
+    t[torch.arange(rows, device="cuda"), place] = value
+    return t
+
+
+# A product of two 24-bit values as six of the nine products of their 8-bit parts: with p1 < 2^-7 and p2 < 2^-15 of a value's leading power of two (truncation), the
+# three that are left out are below 2 x 2^-22 + 2^-30 of the product of both powers, that is, of the product; the six are exact (16 bits) and added with up to
+# two roundings' worth each (2 x 2^-24, whether the matrix cores round or truncate).  Any one of the six left out instead misses by up to 2^-14 or 2^-15.
+SIX = 2.0 ** -21 + 2.0 ** -30 + 12 * F32
+
+
+@pytest.mark.parametrize("M, K, F, tile", [(2050, 200, 600, 128), (1030, 1003, 517, 128), (4229, 4130, 2060, 256), (8190, 600, 5624, 256)])
+def test_gated_mlp_of_fp32_in_tiles_holds_all_of_a_products_bits(ops, M, K, F, tile):
+    """Sums of one product each (the others are 0), so that what is off is a product's own error: every part of every product has to be there, forward, in dx and in
+    the weights' gradients."""
+    from motif_amd import _lib
+    g = gen(62)
+    size = lambda *s: (torch.rand(*s, generator=g, device="cuda") + 1) * torch.exp2(torch.randint(-3, 4, s, generator=g, device="cuda").float())  # noqa: E731
+    sign = lambda *s: torch.randint(0, 2, s, generator=g, device="cuda").float() * 2 - 1  # noqa: E731
+    place = torch.randint(0, K, (M,), generator=g, device="cuda")
+    value = size(M) * sign(M)
+    x, w = one_hot_rows(M, K, place, value), size(F, K)
+    for product in range(4):
+        assert _lib.load().motif_gated_mlp_tile(x.data_ptr(), K, w.data_ptr(), w.data_ptr(), M, K, F, 0, product) in ((tile, 128) if product else (tile,))
+    V, W = value.double(), w.double()
+    exact = V[:, None] * W.t()[place]
+    zero, one = torch.zeros_like(w), torch.ones(F, device="cuda")
+    # h = U / 2 (sigmoid(0) is 1 / 2), and h = silu(G) of gates of 64 and more, where it is G (1 - exp(-64)), times u = 1 (8 roundings of the activation)
+    within(ops.gated_mlp(x, zero, w, act="sigmoid"), exact / 2, SIX * exact.abs() / 2)
+    within(ops.gated_mlp(x.abs() * 4096, w, zero, None, one, act="silu"), 4096 * exact.abs(), (SIX + 8 * F32) * 4096 * exact.abs())
+    # backward with one gradient to a row and to a column: dU = dh / 2, dG = dh U / 4 (act sigmoid at 0), every entry of dx = dU Wu, of dWu and dWg one product
+    n = min(M, F)
+    column = torch.randperm(F, generator=g, device="cuda")[:n]
+    dvalue = size(n) * sign(n)
+    dh = torch.zeros(M, F, device="cuda")
+    dh[torch.arange(n, device="cuda"), column] = dvalue
+    dense, wg, wu = size(M, K) * sign(M, K), zero.clone().requires_grad_(), w.clone().requires_grad_()
+    xl = dense.clone().requires_grad_()
+    bias = torch.full((F,), 1.5, device="cuda")            # (U for dG: x is dense here, and x wu would be a sum)
+    D, X = dvalue.double(), dense.double()
+    h = ops.gated_mlp(xl, wg, wu, None, None, act="sigmoid")
+    dx, dwu = torch.autograd.grad(h, (xl, wu), dh)
+    want = torch.zeros(M, K, dtype=torch.float64, device="cuda")
+    want[:n] = D[:, None] / 2 * W[column]
+    within(dx, want, SIX * want.abs())
+    want = torch.zeros(F, K, dtype=torch.float64, device="cuda")
+    want[column] = D[:, None] / 2 * X[:n]
+    within(dwu, want, SIX * want.abs())
+    dwg, = torch.autograd.grad(ops.gated_mlp(dense, wg, zero, None, bias, act="sigmoid"), (wg,), dh)
+    want[column] = D[:, None] * 0.375 * X[:n]             # dh x 1.5 x 1 / 4: a rounding or two
+    within(dwg, want, (SIX + 4 * F32) * want.abs())
