@@ -1202,3 +1202,27 @@ def test_gated_mlp_of_fp32_in_tiles_holds_all_of_a_products_bits(ops, M, K, F, t
     dwg, = torch.autograd.grad(ops.gated_mlp(dense, wg, zero, None, bias, act="sigmoid"), (wg,), dh)
     want[column] = D[:, None] * 0.375 * X[:n]             # dh x 1.5 x 1 / 4: a rounding or two
     within(dwg, want, (SIX + 4 * F32) * want.abs())
+
+
+@pytest.mark.parametrize("M, K", [(64, 128), (2100, 200), (3000, 32)], ids=["few rows", "tiles", "narrow"])
+def test_gated_mlp_of_fp32_gelu_keeps_its_digits_on_the_negative_side(ops, M, K):
+    """gelu(g) and its derivative relative to their own size down to g = -12.  E = exp(-g^2 / 2): the square, its product with log2 e and that constant are rounded, 2.4 x 2^-24 of
+    an exponent of g^2 / 2, and E itself to 2 x 2^-24.  The fit is off by 6.2e-8 (1.1 x 2^-24), its eight steps, reciprocal and products by 16 x 2^-24 more."""
+    F = 600 if M == 2100 else 64
+    g = -torch.rand(M, generator=gen(71), device="cuda") * 12
+    x = torch.zeros(M, K, device="cuda")
+    x[:, 0] = g
+    wg, zero = torch.zeros(F, K, device="cuda"), torch.zeros(F, K, device="cuda")
+    wg[:, 0] = 1
+    one = torch.ones(F, device="cuda")
+    x.requires_grad_()
+    h = ops.gated_mlp(x, wg, zero, None, one, act="gelu")
+    dh = torch.zeros(M, F, device="cuda")
+    dh[:, 5] = 1
+    dx, = torch.autograd.grad(h, x, dh)
+    G = g.double()
+    phi, pdf = torch.special.erfc(-G / math.sqrt(2)) / 2, torch.exp(-0.5 * G * G) / math.sqrt(2 * math.pi)
+    rel = (1.2 * G * G + 2 + 18) * F32
+    within(h, (G * phi)[:, None].expand(M, F), (rel * (G * phi).abs())[:, None])
+    six = (2.0 ** -21 if M == 2100 else 0) + 8 * F32       # dx: one product with 1
+    within(dx[:, 0], phi + G * pdf, (rel + six) * (phi + (G * pdf).abs()))
