@@ -1226,3 +1226,29 @@ def test_gated_mlp_of_fp32_gelu_keeps_its_digits_on_the_negative_side(ops, M, K)
     within(h, (G * phi)[:, None].expand(M, F), (rel * (G * phi).abs())[:, None])
     six = (2.0 ** -21 if M == 2100 else 0) + 8 * F32       # dx: one product with 1
     within(dx[:, 0], phi + G * pdf, (rel + six) * (phi + (G * pdf).abs()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [3, 24, 300, 512, 1000, 4097])
+def test_layer_norm_bits_do_not_depend_on_strides_and_alignment(ops, dtype, D):
+    """Which lane holds which column follows from D alone: the same rows give the same bits, output and all gradients, wherever they lie."""
+    rows = 37
+    g = gen(D)
+    base = torch.randn(2 * rows, D + 64, generator=g, device="cuda").to(dtype)
+    w, b = torch.randn(D, generator=g, device="cuda").to(dtype), torch.randn(D, generator=g, device="cuda").to(dtype)
+    dbase = torch.randn(2 * rows, D + 64, generator=g, device="cuda").to(dtype)
+    flat = torch.randn(rows * D + 1, generator=g, device="cuda").to(dtype)
+    layouts = {"columns": lambda t: t[:rows, 32:32 + D], "odd columns": lambda t: t[:rows, 3:3 + D], "every second row": lambda t: t[::2, :D], "last columns": lambda t: t[rows:, 64:],
+               "misaligned": lambda t: flat[1:].view(rows, D), "transposed": lambda t: t[:rows, :D].t().contiguous().t(), "one row for all": lambda t: t[:1, 5:5 + D].expand(rows, D)}
+
+    def step(x, dy, w, b):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = ops.layer_norm(*leaves)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+    for name, view in layouts.items():
+        x, dy = view(base), view(dbase)
+        want = step(x.clone(memory_format=torch.contiguous_format), dy.clone(memory_format=torch.contiguous_format), w, b)
+        odd = torch.cat([w[:1], w, b])                   # parameters at odd addresses
+        for got in (step(x, dy, w, b), step(x, dy, odd[1:1 + D], odd[1 + D:])):
+            for part, p, q in zip(("y", "dx", "dw", "db"), got, want):
+                assert torch.equal(p, q), (name, part)
