@@ -1,8 +1,9 @@
 """Tensor-level wrappers over the C ABI (include/motif_hip.h).
 
 PyTorch is plumbing here: it owns device memory and the stream; every computation below is a
-hand-written HIP kernel in libmotif_hip.so.  All tensors must be CUDA (ROCm) fp32; there is no CPU or
-eager fallback -- a missing library or a non-GPU tensor raises.
+hand-written HIP kernel in libmotif_hip.so.  All tensors must be CUDA (ROCm) fp32 (the sequence operators
+at the end also take bf16 and fp16, and have gradients); there is no CPU or eager fallback -- a missing
+library or a non-GPU tensor raises.
 """
 import ctypes
 import os
@@ -1118,7 +1119,7 @@ LAYER_NORM_MAX = 16384
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last axis: (x - mean) / sqrt(var + eps) * weight + bias.  x [..., D] fp32 / bf16 / fp16 with D <= 16384, any
-    strides (a copy is made only where the rows have no common stride or the last axis is not dense); weight / bias [D] of x's type or fp32.
+    strides (a copy is made only where the rows have no common stride or the last axis is not dense); weight / bias [D] of x's type or fp32, both of one type.
     Differentiable in x, weight and bias.  (instance_norm is the planar counterpart: statistics over a channel's plane.)"""
     what = "layer_norm"
     _seq_type(x, what, "x")
@@ -1199,10 +1200,12 @@ class _GruScan(torch.autograd.Function):
 def gru_scan(z, q, h0=None, cu_seqlens=None):
     """gru_update along whole sequences, for gates that do not read the state: h_t = (1 - z_t) h_{t-1} + z_t q_t, channel by channel.
 
-    z (a gate: 0 .. 1), q: [B, T, D], fp32 / bf16 / fp16, any batch and row strides; h0: fp32 [B, D] (None: zeros).  Returns (h like q, the last states fp32 [B, D]);
-    the states can be handed to the next call: a sequence may come in pieces, down to single rows.  With cu_seqlens -- int32 [S + 1] on the device,
+    z (a gate, 0 .. 1: of others the product over a run of rows can pass fp32's range, and NaN come out where the state is finite), q: [B, T, D],
+    fp32 / bf16 / fp16, any batch and row strides; h0: fp32 [B, D] (None: zeros).  Returns (h like q, the last states fp32 [B, D]); the states can be
+    handed to the next call: a sequence may come in pieces, down to single rows.  With cu_seqlens -- int32 [S + 1] on the device,
     not decreasing; what lies before 0 counts as 0, behind T as T -- z and q are [T, D] with S sequences packed one behind the other, h0 and the last states [S, D]; an empty
-    sequence keeps its state, and rows that no sequence covers come out as zeros, whatever they hold.  Differentiable in z, q and h0."""
+    sequence keeps its state, and rows that no sequence covers come out as zeros, whatever they hold.  Differentiable in z, q and h0: dz = g (q - h_{t-1}) takes
+    the states from h as it was returned, rounded to q's type (fp32 copies of them would be 4 bytes per value more to write and read)."""
     what = "gru_scan"
     _seq_type(q, what, "q")
     if q.dim() != (3 if cu_seqlens is None else 2):
@@ -1279,8 +1282,9 @@ class _GatedMlp(torch.autograd.Function):
 def gated_mlp(x, w_gate, w_up, b_gate=None, b_up=None, act="silu"):
     """Gated feed-forward block act(x w_gate^T + b_gate) * (x w_up^T + b_up) in one kernel; act: "silu", "gelu" (exact) or "sigmoid".
 
-    x [..., K], w_gate / w_up [F, K] (nn.Linear's layout), b_gate / b_up [F], all fp32, bf16 or fp16; K, F <= 65536, at most 2^22 rows.  Sums are
-    fp32; fp32 data keep fp32's accuracy on the matrix cores (fp32 instructions, or three exact bf16 parts of every operand; an infinite operand beside one of less than 2^-90 may make its outputs NaN).
+    x [..., K], w_gate / w_up [F, K] (nn.Linear's layout), b_gate / b_up [F], all of one type, fp32, bf16 or fp16 (autocast changes none of them);
+    K, F <= 65536, at most 2^22 rows.  Sums are fp32; fp32 data keep fp32's accuracy on the matrix cores (fp32 instructions, or three exact bf16 parts of
+    every operand, whose products are off by 2^-24 rms, 2^-21 at most; an infinite operand beside one of less than 2^-90 may make its outputs NaN).
     With gradients the two projections are kept in fp32 (8 bytes per output value).  Backward, 16-bit types round the gradients of the projections to
     x's type once, as operands of the matrix cores; in fp16 they are scaled by a power of two where their range asks for it, so that gradients are infinite only
     where their own value is.  Differentiable in all tensors."""
