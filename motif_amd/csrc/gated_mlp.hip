@@ -774,8 +774,8 @@ __global__ __launch_bounds__(512) void rows_kernel(const T* __restrict__ x, long
 // K <= 64: a wave holds the weights of 32 columns of both projections in its registers and walks over blocks of 16 rows; neither a tile of the output nor
 // fp32's three parts pass through memory.  Four values of the reduction to a lane: one matrix instruction of 16 bits, four of fp32 (each takes one
 // value of every lane; which of the reduction's values those are is free as long as both operands agree).
-// 57600 x 64 -> 2 x 256 fp32, gelu, training: forward 59 us (205 MB; the products of 64 x 512 fp32 alone 24 us, 103 us through the tiles and their three
-// parts), backward 100 + 11 us for the workgroups' sums (229 MB; products 48 us; 250 us through the tiles).  Of a SIMD's cycles in them the products
+// 57600 x 64 -> 2 x 256 fp32, gelu, training: forward 71 us (64 at least; 205 MB; the products of 64 x 512 fp32 alone 24 us, 103 us through the tiles and their three
+// parts), backward 103 + 11 us for the workgroups' sums (229 MB; products 48 us; 250 us through the tiles).  Of a SIMD's cycles in them the products
 // take 53 %, the activations and operands 25 %, waits the rest; making the next block's gradients between the products, starting a SIMD's two waves half a
 // block apart and serving one of them first each left the time as it was, so that the instructions of both kinds seem to share what they need.
 // The e-th of them; consecutive instructions should have accumulators of their own: one that adds to its predecessor's waits for it.
@@ -856,7 +856,8 @@ __global__ __launch_bounds__(256) void narrow_fwd_kernel(const T* __restrict__ x
     }
 }
 
-// Backward in one pass over dh, G and U: F a multiple of 8 up to 256, K one of 4 up to 16 KT.  A workgroup's eight waves take NC runs of 32 columns of 8 / NC
+// Backward in one pass over dh, G and U: F a multiple of 8 up to 256, which is what a workgroup's eight waves hold in columns (training steps of 57600 x 64 fp32: 2 x 256 159 us,
+// through the tiles 2 x 264 433, 2 x 512 570, 2 x 1024 1062), K one of 4 up to 16 KT.  A workgroup's eight waves take NC runs of 32 columns of 8 / NC
 // blocks of 16 rows.  A wave makes dG and dU of its rows and columns, with a row to a lane as dx needs them, and turns them over through LDS for the weights'
 // gradients, whose sums stay in its registers over all of its rows; the runs' shares of dx meet in LDS, in a fixed order.
 template <typename T, int KT, bool DX, bool DW>

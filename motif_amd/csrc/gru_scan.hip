@@ -15,9 +15,9 @@
 // channels are few, a sequence is cut into segments: a first kernel reads what the composition needs and writes every segment's (A, H), and each
 // segment's workgroup then composes those before it, in a fixed order -- the cost is a second read of half the inputs.  The states, A and H are
 // fp32.  No atomics: the same bits every time.
-// Measured: 65536 x 1024 bf16 50 + 71 us forward (two reads, then two reads and a write: 5.4 and 5.7 TB/s), 44 + 166 back (4.8 TB/s in the second);
-// 7 x 3686400 fp32, one lane per four channels, 61 (310 MB, 5.1 TB/s); 20011 x 771 fp16 in 37 sequences 5 + 21 + 46 and 5 + 22 + 78: three tiles to a
-// workgroup do not hide their first reads.  Where z leaves 0 .. 1 far enough for a run's A to pass fp32's range, the split form gives NaN even
+// Measured: 65536 x 1024 bf16 51 + 71 us forward (two reads, then two reads and a write: 5.3 and 5.7 TB/s), 43 + 176 back (4.6 TB/s in the second);
+// 7 x 3686400 fp32, one lane per four channels, 64 (310 MB, 4.9 TB/s) and 114 back (619 MB, 5.4 TB/s; forward 54 in a row of its own calls); 20011 x 771 fp16 in 37 sequences
+// 4 + 22 + 46 and 4 + 22 + 78: three tiles to a workgroup do not hide their first reads.  Where z leaves 0 .. 1 far enough for a run's A to pass fp32's range, the split form gives NaN even
 // where the state itself stays finite.
 #include "seq_common.h"
 
@@ -361,8 +361,8 @@ constexpr int kEmptyGroups = 1 << 20;                    // of the empty sequenc
 // values, whose rows need more lanes to fill a cache line).  What counts are lanes that hold channels (training steps, us, slots or lanes): 512 x 8192 x 16 bf16, two
 // lanes to a batch, 1495 or 8950; 512 x 4096 x 64 738 or 6190; 300 x 1000 x 1000 fp16 1530 or 2025; at the bound 512 x 24 x 1024 81 or 45, 512 x 100 x 1024 213 or 226,
 // 512 x 2000 x 1000 fp32 11200 or 7730; 20000 x 100 x 8 fp32 337 or 205.  Rows of 64 lanes and more start at a multiple of 16, whole 256 bytes.
-// Segments: as many as the chip holds workgroups of the second kernel at once -- three to a CU forward, four
-// backward, by their registers --, none below two tiles (65536 x 1024 bf16, forward: 74 us with 768 workgroups, 85 us with 1024; backward:
+// Segments: forward as many as the chip holds workgroups of the second kernel at once, three to a CU (145 registers); backward 1024, which are held at once in fp32 (116 registers,
+// four to a CU) and two rounds of two to a CU in 16 bits (170); none below two tiles (65536 x 1024 bf16, forward: 74 us with 768 workgroups, 85 us with 1024; backward:
 // 212 with 768, 166 with 1024, 184 with 768 of two rows a slot).
 int vec_of(int dtype, long D) { const int V = 16 / seq_size(dtype); return D < V ? 1 : V; }
 Plan plan_of(int V, long B, long T, long D, bool bwd) {

@@ -9,7 +9,9 @@
 // columns fixed, keeps the sums of its columns in registers (fp32) and writes them once; seq_colsum2 adds the workgroups' sums in a fixed
 // order.  No atomics: the same bits every time.
 // Measured (training): 16384 x 4096 bf16 50 us forward (268 MB, 5.4 TB/s; one workgroup per row and outputs through the caches: 69) and 77 + 5 back
-// (403 MB, 5.2 TB/s); 57600 x 64 fp32 8 and 13 + 4; 4099 x 1001 fp16 8 and 15 + 4; 16 x 1024 bf16 3.5, a launch.
+// (403 MB, 5.2 TB/s); 57600 x 64 fp32 8 and 13 + 4; 4099 x 1001 fp16 8 and 15 + 4; 16 x 1024 bf16 3.5, a launch.  Beyond 4096 columns 1024 lanes share a row, with 128 registers
+// each: backward no row is requested ahead, and from 8193 columns on the weights, both sums and both inputs of 16 columns do not fit (20 bytes a lane go through scratch in 16 bits,
+// 52 in fp32): 4096 x 16384 bf16 65 and 140 (134 MB a tensor, 2.9 TB/s back), fp32 101 and 203.
 #include "seq_common.h"
 
 namespace {
@@ -268,8 +270,8 @@ void with_layout(int D, F&& f) {
     else if (D <= 256 * 16) with_values<T, 256>(D, f);
     else with_values<T, 1024>(D, f);
 }
-// Workgroups: as many as their registers let the chip hold at once, each with a share of the rows (backward: 150 registers at 16 values a lane, three
-// workgroups of 256 to a CU; a fourth share would be a round of its own).
+// Workgroups: as many as their registers let the chip hold at once, each with a share of the rows (backward: 138 to 146 registers at 16 values of 16 bits a lane, three
+// workgroups of 256 to a CU; a fourth share would be a round of its own.  fp32, up to 171, holds two).
 int groups_of(long rows, int D, long most) {
     const long want = cdiv(rows, D <= 256 ? 16 : D <= 1024 ? 4 : 1);
     return (int)(want < most ? want : most);
