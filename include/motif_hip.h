@@ -410,7 +410,8 @@ int motif_layer_norm_bwd(const void* x, long x_rs, const void* dy, long dy_rs, c
  * channel.  Either B sequences of T rows -- z, q [B, T, D] with batch and row strides (_bs, _rs; the last axis dense), cu_seqlens NULL, h0 /
  * h_last [B, D] --, or S sequences packed one behind the other -- z, q [T, D], B = 1, cu_seqlens [S + 1] on the device, sequence s = rows
  * cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (empty ones keep their state), h0 / h_last [S, D]; rows that no sequence covers come out as zeros,
- * whatever they hold, and a bound (they do not decrease) below 0 or behind row T counts as 0 or T.  h0 NULL: zeros.  z in 0 .. 1.  h dense; h_last may be NULL.  States are fp32.  workspace: motif_gru_scan_ws_floats floats (of type
+ * whatever they hold, and a bound (they do not decrease) below 0 or behind row T counts as 0 or T.  h0 NULL: zeros.  z in 0 .. 1.  B < 2^29, and B rows of D hold
+ * less than 2^32 vectors of 16 bytes.  h dense; h_last may be NULL.  States are fp32.  workspace: motif_gru_scan_ws_floats floats (of type
  * dtype's call; NULL where that is 0, always so for T <= 16 without cu_seqlens), no clearing needed.  The result does not depend on timing: no atomics. */
 long motif_gru_scan_ws_floats(long B, long T, long D, int packed, int dtype);
 int motif_gru_scan_fwd(const void* z, long z_bs, long z_rs, const void* q, long q_bs, long q_rs, const float* h0, const int32_t* cu_seqlens, int S,
